@@ -23,7 +23,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 # EFA_B200_LIB names another build of the same library (a debug build, say); the default is the one beside this file.
 LIB_PATH = os.environ.get("EFA_B200_LIB") or os.path.join(_HERE, "libefa_b200.so")
 
-F32, F16 = 0, 1
+F32, F16, E4M3 = 0, 1, 2
 MODE_ATTN, MODE_ATTN_TILED, MODE_MEGATRON, MODE_SYNC, MODE_OVERLAP, MODE_STREAM, MODE_COMM = range(7)
 MODE_NAMES = ("attn", "attn_tiled", "megatron", "sync", "overlap", "stream", "comm")
 REDUCE_NCCL, REDUCE_P2P, REDUCE_NVLS, REDUCE_PULL = 0, 1, 2, 3
@@ -81,6 +81,25 @@ class FlashPlan(C.Structure):
                 ("stage_step", C.c_int)]
 
 
+class PagedCache(C.Structure):
+    """efa_paged_cache: pages of keys and values. ``paged_cache`` makes one of tensors and keeps them alive."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_exp", C.c_void_p), ("v_exp", C.c_void_p),
+                ("num_pages", C.c_int), ("page_size", C.c_int), ("H_kv", C.c_int), ("d_h", C.c_int), ("dtype", C.c_int),
+                ("page_stride", C.c_int64)]
+
+
+class PagedBatch(C.Structure):
+    """efa_paged_batch: a ragged batch over a paged cache. ``paged_batch`` makes one of tensors and keeps them alive."""
+    _fields_ = [("q_start", C.c_void_p), ("kv_len", C.c_void_p), ("pages", C.c_void_p),
+                ("num_seqs", C.c_int), ("max_pages", C.c_int), ("tokens", C.c_int), ("max_q", C.c_int), ("max_kv", C.c_int)]
+
+
+class PagedAttentionParams(C.Structure):
+    """efa_paged_attention_params; strides in elements, 0 = dense."""
+    _fields_ = [("H_q", C.c_int), ("causal", C.c_int), ("scale", C.c_float),
+                ("q_head_stride", C.c_int64), ("q_token_stride", C.c_int64), ("o_token_stride", C.c_int64)]
+
+
 class StreamGroup(C.Structure):
     """efa_stream_group: tiles [first_tile, first_tile + ntiles) share one projection and one AllReduce."""
     _fields_ = [("first_tile", C.c_int), ("ntiles", C.c_int)]
@@ -108,6 +127,13 @@ _SIGNATURES = {
     "efa_convert_f32_to_f16": (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
     "efa_project_f16": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p]),
     "efa_compute_qkv_f16": (C.c_int, [C.c_void_p] * 7 + [C.c_int] * 4 + [C.c_void_p]),
+    "efa_paged_check": (C.c_char_p, [C.POINTER(PagedCache), C.POINTER(PagedBatch)]),
+    "efa_paged_attention_check": (C.c_char_p, [C.POINTER(PagedCache), C.POINTER(PagedBatch), C.POINTER(PagedAttentionParams)]),
+    "efa_paged_attention_workspace": (C.c_size_t, [C.POINTER(PagedCache), C.POINTER(PagedBatch), C.POINTER(PagedAttentionParams)]),
+    "efa_cache_write": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.POINTER(PagedCache), C.POINTER(PagedBatch), C.c_void_p]),
+    "efa_cache_read": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.POINTER(PagedCache), C.POINTER(PagedBatch), C.c_void_p]),
+    "efa_paged_attention": (C.c_int, [C.c_void_p, C.c_void_p, C.POINTER(PagedCache), C.POINTER(PagedBatch),
+                                      C.POINTER(PagedAttentionParams), C.c_void_p, C.c_size_t, C.c_void_p]),
     "efa_kernel_status": (C.c_int, [C.POINTER(C.c_int)]),
     "efa_kernel_status_reset": (C.c_int, []),
     "efa_mode_name": (C.c_char_p, [C.c_int]),
@@ -304,6 +330,87 @@ def compute_qkv(X, W_q, W_k, W_v, Qh, Kh, Vh, S: int, d: int, H_local: int, d_h:
     """compute_qkv (attn_main.cu:127-153) on fp16 data: Q/K/V = X @ W per head, written fp16 head-major."""
     _check(lib().efa_compute_qkv_f16(_ptr(X), _ptr(W_q), _ptr(W_k), _ptr(W_v), _ptr(Qh), _ptr(Kh), _ptr(Vh),
                                      S, d, H_local, d_h, _stream(stream)), "compute_qkv")
+
+
+# ------------------------------------------------------------------------------------------------
+# Paged key/value cache
+# ------------------------------------------------------------------------------------------------
+def paged_cache(k, v, k_exp=None, v_exp=None) -> PagedCache:
+    """A cache of tensors ``[num_pages][H_kv][page_size][d_h]``: fp16, or 8-bit codes (uint8 or float8_e4m3fn) with
+    ``k_exp``, ``v_exp`` uint8 ``[num_pages][H_kv][page_size]``. Pages may lie apart (a stride of the first dimension), the rest is dense."""
+    if k.dim() != 4 or v.shape != k.shape or v.stride() != k.stride() or v.dtype != k.dtype:
+        raise EfaError("paged_cache: k and v must be [num_pages][H_kv][page_size][d_h], alike in shape, strides and type")
+    pages, heads, size, d_h = k.shape
+    dtype = {2: F16, 1: E4M3}.get(k.element_size()) if str(k.dtype) in ("torch.float16", "torch.uint8", "torch.float8_e4m3fn") else None
+    if dtype is None:
+        raise EfaError(f"paged_cache: {k.dtype} is neither fp16 nor 8-bit codes")
+    if tuple(k.stride()[1:]) != (size * d_h, d_h, 1):
+        raise EfaError("paged_cache: a page must be dense")
+    for e in (k_exp, v_exp):
+        if (dtype == E4M3) != (e is not None):
+            raise EfaError("paged_cache: 8-bit codes come with k_exp and v_exp, fp16 without")
+        if e is not None and (tuple(e.shape) != (pages, heads, size) or str(e.dtype) != "torch.uint8" or not e.is_contiguous()):
+            raise EfaError("paged_cache: exponents must be dense uint8 [num_pages][H_kv][page_size]")
+    c = PagedCache(_ptr(k), _ptr(v), _ptr(k_exp), _ptr(v_exp), pages, size, heads, d_h, dtype, k.stride(0) if pages > 1 else 0)
+    c.tensors = (k, v, k_exp, v_exp)
+    return c
+
+
+def paged_batch(q_start, kv_len, pages, tokens: int, max_q: int, max_kv: int) -> PagedBatch:
+    """A ragged batch of int32 tensors: ``q_start [num_seqs + 1]``, ``kv_len [num_seqs]``, ``pages [num_seqs][max_pages]``, whose contents
+    are read when the kernels run. ``tokens``: rows of the row tensors; ``max_q``, ``max_kv``: no chunk and no sequence is longer."""
+    n = kv_len.numel()
+    if any(str(x.dtype) != "torch.int32" or not x.is_contiguous() for x in (q_start, kv_len, pages)):
+        raise EfaError("paged_batch: q_start, kv_len and pages must be dense int32 tensors")
+    if q_start.numel() != n + 1 or pages.dim() != 2 or pages.shape[0] != n:
+        raise EfaError("paged_batch: q_start must be [num_seqs + 1], kv_len [num_seqs], pages [num_seqs][max_pages]")
+    b = PagedBatch(_ptr(q_start), _ptr(kv_len), _ptr(pages), n, pages.shape[1], tokens, max_q, max_kv)
+    b.tensors = (q_start, kv_len, pages)
+    return b
+
+
+def paged_attention_params(H_q: int, d_h: int, causal: int = 1, scale: Optional[float] = None, q_head_stride: int = 0,
+                           q_token_stride: int = 0, o_token_stride: int = 0) -> PagedAttentionParams:
+    """Scale 1/sqrt(d_h) unless given; strides in elements, 0 = dense (Q ``[H_q][tokens][d_h]``, O ``[tokens][H_q * d_h]``)."""
+    return PagedAttentionParams(H_q, int(bool(causal)), d_h ** -0.5 if scale is None else scale, q_head_stride, q_token_stride, o_token_stride)
+
+
+def paged_check(cache: PagedCache, batch: PagedBatch, ap: Optional[PagedAttentionParams] = None) -> Optional[str]:
+    """None if calls on them (with ``ap``: paged_attention) are legal, else the reason. Host arithmetic."""
+    if ap is None:
+        why = lib().efa_paged_check(C.byref(cache), C.byref(batch))
+    else:
+        why = lib().efa_paged_attention_check(C.byref(cache), C.byref(batch), C.byref(ap))
+    return None if why is None else why.decode()
+
+
+def cache_write(K, V, cache: PagedCache, batch: PagedBatch, stream=None, head_stride: int = 0, token_stride: int = 0) -> None:
+    """Rows of the batch's chunks (fp16 ``[H_kv][tokens][d_h]``, or with strides in elements) into their pages, rounded to
+    8 bits with an exponent per row where the cache is e4m3. Asynchronous on ``stream``."""
+    _check(lib().efa_cache_write(_ptr(K), _ptr(V), head_stride, token_stride, cache, batch, _stream(stream)), "cache_write")
+
+
+def cache_read(K, V, cache: PagedCache, batch: PagedBatch, stream=None, head_stride: int = 0, token_stride: int = 0) -> None:
+    """The inverse of cache_write: the last keys and values of each sequence into fp16 rows."""
+    _check(lib().efa_cache_read(_ptr(K), _ptr(V), head_stride, token_stride, cache, batch, _stream(stream)), "cache_read")
+
+
+def paged_attention_workspace(cache: PagedCache, batch: PagedBatch, ap: PagedAttentionParams) -> int:
+    """Bytes of workspace that paged_attention needs for these sizes (0: none)."""
+    why = paged_check(cache, batch, ap)
+    if why is not None:
+        raise EfaError(f"paged_attention_workspace: {why}")
+    return lib().efa_paged_attention_workspace(C.byref(cache), C.byref(batch), C.byref(ap))
+
+
+def paged_attention(Q, O, cache: PagedCache, batch: PagedBatch, ap: PagedAttentionParams, workspace=None, stream=None,
+                    workspace_bytes: Optional[int] = None) -> None:
+    """Attention of the batch's chunks over the cache, which holds their own keys already: O ``[tokens][H_q * d_h]`` fp16.
+    ``workspace``: a tensor of at least paged_attention_workspace bytes (or an address, with ``workspace_bytes``), not used by any
+    other call until this one is done. Asynchronous on ``stream``."""
+    if workspace_bytes is None:
+        workspace_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    _check(lib().efa_paged_attention(_ptr(Q), _ptr(O), cache, batch, ap, _ptr(workspace), workspace_bytes, _stream(stream)), "paged_attention")
 
 
 def kernel_status() -> Sequence[int]:

@@ -2,6 +2,7 @@
 #include "fa_fwd_sm100.cuh"
 #include "host_util.h"
 #include "nvls_reduce.h"
+#include "paged_attention.h"
 #include "runtime.h"
 
 #include <cuda_fp16.h>
@@ -83,6 +84,45 @@ extern "C" int efa_compute_qkv_f16(const void* X, const void* W_q, const void* W
     const void* W[3] = {W_q, W_k, W_v};
     void* out[3] = {Qh, Kh, Vh};
     return project_heads_f16(X, W, out, S, d, H_local, d_h, (cudaStream_t)stream);
+}
+
+extern "C" const char* efa_paged_check(const efa_paged_cache* cache, const efa_paged_batch* batch)
+{
+    if (!cache || !batch) return "null argument";
+    return paged_check(*cache, *batch);
+}
+
+extern "C" const char* efa_paged_attention_check(const efa_paged_cache* cache, const efa_paged_batch* batch, const efa_paged_attention_params* p)
+{
+    if (!cache || !batch || !p) return "null argument";
+    return paged_attention_check(*cache, *batch, *p);
+}
+
+extern "C" size_t efa_paged_attention_workspace(const efa_paged_cache* cache, const efa_paged_batch* batch, const efa_paged_attention_params* p)
+{
+    if (!cache || !batch || !p || paged_attention_check(*cache, *batch, *p)) return 0;
+    return paged_attention_bytes(*cache, *batch, *p);
+}
+
+extern "C" int efa_cache_write(const void* K, const void* V, int64_t head_stride, int64_t token_stride,
+                               const efa_paged_cache* cache, const efa_paged_batch* batch, void* stream)
+{
+    if (!K || !V || !cache || !batch) { set_error("efa_cache_write: null argument"); return 2; }
+    return cache_write(K, V, head_stride, token_stride, *cache, *batch, (cudaStream_t)stream);
+}
+
+extern "C" int efa_cache_read(void* K, void* V, int64_t head_stride, int64_t token_stride,
+                              const efa_paged_cache* cache, const efa_paged_batch* batch, void* stream)
+{
+    if (!K || !V || !cache || !batch) { set_error("efa_cache_read: null argument"); return 2; }
+    return cache_read(K, V, head_stride, token_stride, *cache, *batch, (cudaStream_t)stream);
+}
+
+extern "C" int efa_paged_attention(const void* Q, void* O, const efa_paged_cache* cache, const efa_paged_batch* batch,
+                                   const efa_paged_attention_params* p, void* workspace, size_t workspace_bytes, void* stream)
+{
+    if (!Q || !O || !cache || !batch || !p) { set_error("efa_paged_attention: null argument"); return 2; }
+    return paged_attention(Q, O, *cache, *batch, *p, workspace, workspace_bytes, (cudaStream_t)stream);
 }
 
 extern "C" int efa_kernel_status(int* out4)

@@ -1,0 +1,200 @@
+// What the kernels of the paged key/value cache share: the cache and the ragged batch as they see them, where a key lies,
+// and how work is laid out over the GPU when only the device knows the lengths.
+//
+// Everything that comes from device memory (lengths, page numbers) is brought into range before it is used as an index: a call whose
+// lengths or pages are wrong stays inside its buffers and reports it in the status word.
+#pragma once
+
+#include "sm100_ptx.cuh"
+
+namespace efa {
+
+struct PagedArgs {
+    uint8_t* k;             // [num_pages][H_kv][page][d_h], fp16 or e4m3
+    uint8_t* v;
+    uint8_t* k_exp;         // [num_pages][H_kv][page], e4m3 only: 127 + exponent of a row
+    uint8_t* v_exp;
+    const int* q_start;     // [num_seqs + 1]
+    const int* kv_len;      // [num_seqs]
+    const int* pages;       // [num_seqs][max_pages]
+    int num_seqs, max_pages, tokens, max_q, kv_cap /* min(max_kv, what a row of `pages` holds) */;
+    int num_pages, page_shift, H_kv;
+    long long page_stride;  // bytes from a page of k or v to the next
+    int* status;
+};
+
+// The first thing that is wrong stays in the status word (code, sequence, site).
+__device__ __forceinline__ void paged_report(const PagedArgs& c, int code, int seq, int site)
+{
+    if (c.status != nullptr && atomicCAS(c.status, 0, code) == 0) {
+        c.status[1] = seq;
+        c.status[2] = site;
+    }
+}
+
+struct PagedSeq { int row0, n, kv; };      // first row of the chunk, its rows, keys in the cache (the chunk's included)
+
+template <bool REPORT = false>
+__device__ __forceinline__ PagedSeq paged_seq(const PagedArgs& c, int b, int site = 0)
+{
+    const int s0 = c.q_start[b], s1 = c.q_start[b + 1], kv = c.kv_len[b];
+    PagedSeq s;
+    s.row0 = min(max(s0, 0), c.tokens);
+    s.n = min(min(max(s1, s.row0), c.tokens) - s.row0, c.max_q);
+    s.kv = min(max(kv, 0), c.kv_cap);
+    if (REPORT && (s.row0 != s0 || s.n != s1 - s0 || s.kv != kv)) paged_report(c, KS_BAD_LENGTH, b, site);
+    return s;
+}
+
+// The page that holds key `key` (below kv_cap) of sequence b; -1, and a report, if there is no such page.
+__device__ __forceinline__ int paged_page(const PagedArgs& c, int b, int key, int site)
+{
+    const int page = c.pages[(long long)b * c.max_pages + (key >> c.page_shift)];
+    if ((unsigned)page < (unsigned)c.num_pages) return page;
+    paged_report(c, KS_BAD_PAGE, b, site);
+    return -1;
+}
+
+// ---------------------------------------------------------------------------------------------
+// e4m3 with an exponent per row: value = code * 2^(byte - 127). The writer's exponents are -24 to 8, for which every value is an fp16
+// exactly (a code has four significant bits; 2^-24 is fp16's smallest step).
+// ---------------------------------------------------------------------------------------------
+__device__ __forceinline__ float exp_byte_f32(unsigned byte) { return __uint_as_float(byte << 23); }     // byte 0, which nothing is stored with, as 0
+
+// 2^(byte - 127) twice as fp16; beyond fp16's range 0 or 2^15.
+__device__ __forceinline__ uint32_t exp_byte_f16x2(unsigned byte)
+{
+    const int e = (int)byte - 127;
+    const uint32_t h = e >= -14 ? (uint32_t)(min(e, 15) + 15) << 10 : e >= -24 ? 1u << (e + 24) : 0u;
+    return h | h << 16;
+}
+
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two)
+{
+    uint32_t r;
+    asm("{\n.reg .b16 x;\ncvt.u16.u32 x, %1;\ncvt.rn.f16x2.e4m3x2 %0, x;\n}\n" : "=r"(r) : "r"(two));
+    return r;
+}
+
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b)
+{
+    uint32_t r;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+
+// Halves of x that are infinite or NaN as a mask.
+__device__ __forceinline__ uint32_t nonfinite_f16x2(uint32_t x)
+{
+    return __vcmpeq2(x & 0x7c007c00u, 0x7c007c00u);
+}
+
+// ---------------------------------------------------------------------------------------------
+// Work over the GPU
+// ---------------------------------------------------------------------------------------------
+// An item is a tile of rows of one sequence and kv head: the rows (token, query head of the group) in that order, `tile` of them
+// at a time, so that all heads of a group, and several tokens, share what is loaded of the keys. Its keys are units of
+// `unit` keys, as many as its last row sees. All units of all items in a row (heads outermost) are cut into as many equal parts as there are
+// blocks: no length of any sequence leaves an SM idle. An item that a cut goes through is merged afterwards (paged_merge_kernel).
+struct PagedShape {
+    int G, causal, tile, unit, max_tiles;   // query heads per kv head; rows of a tile; keys of a unit; tiles of the longest chunk
+};
+
+__device__ __forceinline__ int paged_tiles(const PagedShape& w, const PagedSeq& s) { return (s.n * w.G + w.tile - 1) / w.tile; }
+
+// Keys that row r of a sequence (token r / G) sees: below this. Not above kv; at most 0: none.
+__device__ __forceinline__ int paged_visible(const PagedShape& w, const PagedSeq& s, int r)
+{
+    return w.causal ? s.kv - s.n + r / w.G + 1 : s.kv;
+}
+
+// One unit at least: rows that see nothing are written as well.
+__device__ __forceinline__ int paged_units(const PagedShape& w, const PagedSeq& s, int rt)
+{
+    const int last = min((rt + 1) * w.tile, s.n * w.G) - 1;
+    return max(1, (paged_visible(w, s, last) + w.unit - 1) / w.unit);
+}
+
+// A place in the row of units.
+struct PagedAt { int h, b, rt, off /* units of the item ahead of it */; };
+
+__device__ __forceinline__ void paged_next(const PagedArgs& c, const PagedShape& w, PagedAt& at)
+{
+    at.off = 0;
+    at.rt++;
+    while (at.h < c.H_kv) {
+        if (at.rt < paged_tiles(w, paged_seq(c, at.b))) return;
+        at.rt = 0;
+        if (++at.b == c.num_seqs) { at.b = 0; at.h++; }
+    }
+}
+
+struct PagedScratch { int warp_sum[32]; int total; PagedAt at; };
+
+// The units [begin, end) of block `part` of `parts` and the place of the first, found by all THREADS threads of a block together. false: there are fewer units
+// than parts, and none for this one.
+template <int THREADS>
+__device__ bool paged_part(const PagedArgs& c, const PagedShape& w, int part, int parts, PagedScratch& s, int& begin, int& end, PagedAt& at)
+{
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int entries = c.num_seqs * w.max_tiles, per = (entries + THREADS - 1) / THREADS;
+    const int e0 = min(tid * per, entries), e1 = min(e0 + per, entries);
+    int sum = 0;
+    for (int e = e0; e < e1; ) {
+        const int b = e / w.max_tiles, rt0 = e - b * w.max_tiles;
+        const PagedSeq q = paged_seq(c, b);
+        const int stop = min(paged_tiles(w, q), rt0 + e1 - e);
+        for (int rt = rt0; rt < stop; rt++) sum += paged_units(w, q, rt);
+        e = (b + 1) * w.max_tiles;
+    }
+    int before = sum;
+    #pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+        const int o = __shfl_up_sync(0xffffffffu, before, d);
+        if (lane >= d) before += o;
+    }
+    if (lane == 31) s.warp_sum[warp] = before;
+    __syncthreads();
+    int total = 0;
+    #pragma unroll
+    for (int i = 0; i < THREADS / 32; i++) {
+        if (i < warp) before += s.warp_sum[i];
+        total += s.warp_sum[i];
+    }
+    before -= sum;
+    const long long all = (long long)total * c.H_kv;
+    parts = (int)min(all, (long long)parts);                // no part without a unit
+    if (part >= parts) return false;
+    begin = (int)(all * part / parts);
+    end = (int)(all * (part + 1) / parts);
+    const int h = begin / total, rest = begin - h * total;
+    if (rest >= before && rest < before + sum) {
+        int left = rest - before;
+        for (int e = e0; e < e1; ) {
+            const int b = e / w.max_tiles, rt0 = e - b * w.max_tiles;
+            const PagedSeq q = paged_seq(c, b);
+            const int stop = min(paged_tiles(w, q), rt0 + e1 - e);
+            for (int rt = rt0; rt < stop; rt++) {
+                const int n = paged_units(w, q, rt);
+                if (left < n) { s.at = PagedAt{h, b, rt, left}; e = entries; break; }
+                left -= n;
+            }
+            if (e < entries) e = (b + 1) * w.max_tiles;
+        }
+    }
+    __syncthreads();
+    at = s.at;
+    return true;
+}
+
+// Where blocks leave their shares of items that a cut goes through: per block two places (its first item, and its last where that is
+// another), each `tile` rows of (maximum in the log2 domain, denominator) and of O without the division; and what the first unit of a block
+// belongs to.
+struct PagedCut { int item_begin /* of all units */, units, begin /* the block's own first unit */, h, b, rt, pad0, pad1; };
+struct PagedParts {
+    PagedCut* cut;      // [parts]
+    float2* ml;         // [parts][2][tile]
+    float* o;           // [parts][2][tile][d_h]
+};
+
+}  // namespace efa

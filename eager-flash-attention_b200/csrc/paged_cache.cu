@@ -1,0 +1,331 @@
+// The paged key/value cache: rows of keys and values into pages and out of them, the checks of its arguments, and which kernel an attention
+// over it takes. fp16, or e4m3 with an exponent per row (token and head): of a row x with largest finite magnitude `top`
+//     e = max(-24, smallest e with top <= 448 * 2^e),   code = x * 2^-e on the e4m3 grid, ties to even,   value = code * 2^e.
+// A power of two costs no accuracy (a code has its four significant bits wherever it stands) and buys exactness: every value is an fp16, in
+// the scores the exponents multiply fp32 numbers, and one rounding is all that the cache adds. With e = 8 codes end at 240: 256 * 2^8 is no fp16.
+#include "paged_attention.h"
+#include "paged_kernels.cuh"
+
+#include <cuda_fp8.h>
+
+#include <algorithm>
+#include <climits>
+#include <cmath>
+
+namespace efa {
+
+namespace {
+
+constexpr int PC_THREADS = 256;
+constexpr int PC_HEADS = 4;          // heads that a thread moves at a time: what it has in flight
+
+struct PagedRows {
+    __half* k;
+    __half* v;
+    long long head, token;           // strides in elements
+};
+
+// The sequence that a row belongs to: the last b with q_start[b] <= row. -1: none.
+__device__ __forceinline__ int sequence_of(const PagedArgs& c, int row)
+{
+    int lo = 0, hi = c.num_seqs;                           // q_start[lo] <= row < q_start[hi], if anywhere
+    if (row < c.q_start[0] || row >= c.q_start[hi]) return -1;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (c.q_start[mid] <= row) lo = mid; else hi = mid;
+    }
+    return lo;
+}
+
+// Eight fp16 of a row of LANES * 8, spread over LANES lanes, to eight codes; the row's exponent byte.
+template <int LANES>
+__device__ __forceinline__ uint2 to_e4m3(const uint4& x, unsigned& byte)
+{
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+    uint32_t top2 = 0;
+    #pragma unroll
+    for (int i = 0; i < 4; i++) top2 = __vmaxu2(top2, w[i] & 0x7fff7fffu & ~nonfinite_f16x2(w[i]));
+    uint32_t top = max(top2 & 0xffffu, top2 >> 16);        // magnitudes of fp16 order like their bits
+    #pragma unroll
+    for (int d = 1; d < LANES; d *= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+    const uint32_t bits = __float_as_uint(__half2float(__ushort_as_half((unsigned short)top)));
+    const int e = max(-24, (int)(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0));     // 448 = 1.75 * 2^8
+    byte = (unsigned)(e + 127);
+    const float scale = __uint_as_float((unsigned)(127 - e) << 23), most = e == 8 ? 240.f : 448.f;
+    uint32_t code[4];
+    #pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        float2 y = make_float2(fminf(fmaxf(f.x * scale, -most), most), fminf(fmaxf(f.y * scale, -most), most));
+        const uint32_t bad = nonfinite_f16x2(w[i]);        // e4m3 has no infinity: stored as NaN
+        if (bad & 0xffffu) y.x = NAN;
+        if (bad >> 16) y.y = NAN;
+        code[i] = __nv_cvt_float2_to_fp8x2(y, __NV_SATFINITE, __NV_E4M3);
+    }
+    return make_uint2(code[0] | code[1] << 16, code[2] | code[3] << 16);
+}
+
+__device__ __forceinline__ uint4 from_e4m3(const uint2& x, unsigned byte)
+{
+    const uint32_t s = exp_byte_f16x2(byte);
+    return make_uint4(mul_f16x2(e4m3x2_to_f16x2(x.x & 0xffffu), s), mul_f16x2(e4m3x2_to_f16x2(x.x >> 16), s),
+                      mul_f16x2(e4m3x2_to_f16x2(x.y & 0xffffu), s), mul_f16x2(e4m3x2_to_f16x2(x.y >> 16), s));
+}
+
+// Rows into pages (READ: out of them). A row of a head is D / 8 lanes of 16 bytes fp16; a warp takes the 256 / D rows that it holds of one token range and up to
+// PC_HEADS heads of K and V at a time. HBM-bound for prompts, a chain of three loads (lengths, page, row) for single tokens.
+template <int D, bool F8, bool READ>
+__global__ void __launch_bounds__(PC_THREADS)
+paged_move_kernel(const PagedArgs c, const PagedRows rows)
+{
+    constexpr int LANES = D / 8, PER_WARP = 32 / LANES;
+    pdl_wait();
+    pdl_trigger();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int sub = lane % LANES;
+    const int row = (blockIdx.x * (PC_THREADS / 32) + warp) * PER_WARP + lane / LANES;
+    const int h0 = blockIdx.y * PC_HEADS;
+    const bool there = row < c.tokens;
+    const long long at = (long long)row * rows.token + sub * 8;
+
+    uint4 k[PC_HEADS], v[PC_HEADS];
+    if constexpr (!READ) {                                 // asked for ahead of the search for their place
+        #pragma unroll
+        for (int i = 0; i < PC_HEADS; i++)
+            if (there && h0 + i < c.H_kv) {
+                k[i] = *reinterpret_cast<const uint4*>(rows.k + (h0 + i) * rows.head + at);
+                v[i] = *reinterpret_cast<const uint4*>(rows.v + (h0 + i) * rows.head + at);
+            } else k[i] = v[i] = make_uint4(0u, 0u, 0u, 0u);
+    }
+    int page = -1, slot = 0;
+    bool owned = false;                                    // a row of some sequence
+    if (there) {
+        const int b = sequence_of(c, row);
+        if (b >= 0) {
+            const PagedSeq q = sub == 0 && h0 == 0 ? paged_seq<true>(c, b, 50) : paged_seq(c, b);
+            const int i = row - q.row0, position = q.kv - q.n + i;
+            owned = i >= 0 && i < q.n;
+            if (owned && position >= 0) {
+                page = paged_page(c, b, position, 50);
+                slot = position & ((1 << c.page_shift) - 1);
+            }
+        }
+    }
+    #pragma unroll
+    for (int i = 0; i < PC_HEADS; i++) {
+        const int h = h0 + i;
+        if (h >= c.H_kv) break;
+        const int in_page = (h << c.page_shift) + slot;
+        const long long to = (long long)max(page, 0) * c.page_stride + ((long long)in_page * D + sub * 8) * (F8 ? 1 : 2);
+        const long long e = ((long long)max(page, 0) * c.H_kv << c.page_shift) + in_page;
+        if constexpr (READ) {
+            uint4 x = make_uint4(0u, 0u, 0u, 0u), y = x;
+            if (page >= 0) {
+                if constexpr (F8) {
+                    x = from_e4m3(*reinterpret_cast<const uint2*>(c.k + to), c.k_exp[e]);
+                    y = from_e4m3(*reinterpret_cast<const uint2*>(c.v + to), c.v_exp[e]);
+                } else {
+                    x = *reinterpret_cast<const uint4*>(c.k + to);
+                    y = *reinterpret_cast<const uint4*>(c.v + to);
+                }
+            }
+            if (owned) {
+                *reinterpret_cast<uint4*>(rows.k + h * rows.head + at) = x;
+                *reinterpret_cast<uint4*>(rows.v + h * rows.head + at) = y;
+            }
+        } else if constexpr (F8) {
+            unsigned bk, bv;                               // all lanes of the warp: the row's maximum goes through shuffles
+            const uint2 x = to_e4m3<LANES>(k[i], bk), y = to_e4m3<LANES>(v[i], bv);
+            if (page >= 0) {
+                *reinterpret_cast<uint2*>(c.k + to) = x;
+                *reinterpret_cast<uint2*>(c.v + to) = y;
+                if (sub == 0) { c.k_exp[e] = (uint8_t)bk; c.v_exp[e] = (uint8_t)bv; }
+            }
+        } else if (page >= 0) {
+            *reinterpret_cast<uint4*>(c.k + to) = k[i];
+            *reinterpret_cast<uint4*>(c.v + to) = v[i];
+        }
+    }
+}
+
+PagedArgs device_args(const efa_paged_cache& c, const efa_paged_batch& b)
+{
+    PagedArgs a{};
+    a.k = static_cast<uint8_t*>(c.k); a.v = static_cast<uint8_t*>(c.v);
+    a.k_exp = c.k_exp; a.v_exp = c.v_exp;
+    a.q_start = b.q_start; a.kv_len = b.kv_len; a.pages = b.pages;
+    a.num_seqs = b.num_seqs; a.max_pages = b.max_pages; a.tokens = b.tokens; a.max_q = b.max_q;
+    a.kv_cap = (int)std::min<long long>(b.max_kv, (long long)b.max_pages * c.page_size);
+    a.num_pages = c.num_pages; a.H_kv = c.H_kv;
+    while ((1 << a.page_shift) < c.page_size) a.page_shift++;
+    const long long per_page = (long long)c.H_kv * c.page_size * c.d_h;
+    a.page_stride = (c.page_stride ? c.page_stride : per_page) * (c.dtype == EFA_F16 ? 2 : 1);
+    return a;
+}
+
+// Memory that the kernels may use: a call on another device's tensors, or the host's, is refused here and not found out by the GPU.
+int check_memory(const char* what, const void* const* p, int n)
+{
+    int dev = -1;
+    EFA_CUDA(cudaGetDevice(&dev));
+    for (int i = 0; i < n; i++) {
+        if (!p[i]) continue;
+        cudaPointerAttributes attr;
+        EFA_CUDA(cudaPointerGetAttributes(&attr, p[i]));
+        if (attr.type == cudaMemoryTypeUnregistered) { set_error("%s: argument %d is not memory that a GPU can use", what, i); return 2; }
+        if (attr.type == cudaMemoryTypeDevice && attr.device != dev) {
+            set_error("%s: argument %d is memory of device %d, the current device is %d", what, i, attr.device, dev);
+            return 2;
+        }
+    }
+    return 0;
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+const char* check_rows(const efa_paged_cache& c, const efa_paged_batch& b, long long& head, long long& token)
+{
+    if (head == 0 && token == 0) { token = c.d_h; head = (long long)b.tokens * c.d_h; return nullptr; }
+    if (head < c.d_h || token < c.d_h || head % 8 || token % 8) return "paged: row strides must be multiples of 8 and at least d_h";
+    if (token < (c.H_kv - 1) * head + c.d_h && head < (b.tokens - 1) * token + c.d_h) return "paged: rows of these strides overlap";
+    return nullptr;
+}
+
+template <int D, bool F8>
+int launch_move(bool read, const PagedArgs& a, const PagedRows& rows, cudaStream_t stream)
+{
+    const int per_block = PC_THREADS / 32 * (256 / D);
+    const dim3 grid((a.tokens + per_block - 1) / per_block, (a.H_kv + PC_HEADS - 1) / PC_HEADS);
+    EFA_CUDA(read ? paged_launch(paged_move_kernel<D, F8, true>, grid, PC_THREADS, 0, stream, a, rows)
+                  : paged_launch(paged_move_kernel<D, F8, false>, grid, PC_THREADS, 0, stream, a, rows));
+    return 0;
+}
+
+int move_rows(const char* what, bool read, const void* K, const void* V, long long head, long long token, const efa_paged_cache& c,
+              const efa_paged_batch& b, cudaStream_t stream)
+{
+    if (const char* why = paged_check(c, b)) { set_error("%s: %s", what, why); return 2; }
+    if (const char* why = check_rows(c, b, head, token)) { set_error("%s: %s", what, why); return 2; }
+    if (!aligned16(K) || !aligned16(V)) { set_error("%s: K and V must be 16-byte aligned", what); return 2; }
+    if (b.num_seqs == 0 || b.tokens == 0) return 0;
+    const void* const mem[] = {K, V, c.k, c.v, c.k_exp, c.v_exp, b.q_start, b.kv_len, b.pages};
+    if (int rc = check_memory(what, mem, 9)) return rc;
+    PagedArgs a = device_args(c, b);
+    a.status = kernel_status_word();
+    const PagedRows rows{static_cast<__half*>(const_cast<void*>(K)), static_cast<__half*>(const_cast<void*>(V)), head, token};
+    const bool f8 = c.dtype == EFA_E4M3;
+    switch (c.d_h) {
+        case 16:  return f8 ? launch_move<16, true>(read, a, rows, stream) : launch_move<16, false>(read, a, rows, stream);
+        case 32:  return f8 ? launch_move<32, true>(read, a, rows, stream) : launch_move<32, false>(read, a, rows, stream);
+        case 64:  return f8 ? launch_move<64, true>(read, a, rows, stream) : launch_move<64, false>(read, a, rows, stream);
+        default:  return f8 ? launch_move<128, true>(read, a, rows, stream) : launch_move<128, false>(read, a, rows, stream);
+    }
+}
+
+struct PagedPlan { PagedShape w; int blocks; bool cut; size_t cut_bytes, ml_bytes, o_bytes; };
+
+PagedPlan plan_attention(const efa_paged_cache& c, const efa_paged_batch& b, const efa_paged_attention_params& p)
+{
+    PagedPlan plan{};
+    const int G = p.H_q / c.H_kv;
+    const long long rows = (long long)b.max_q * G, kv_cap = std::min<long long>(b.max_kv, (long long)b.max_pages * c.page_size);
+    const int tile = paged_rows_tile((int)std::min<long long>(rows, INT_MAX));
+    plan.w = PagedShape{G, p.causal ? 1 : 0, tile, PAGED_ROWS_UNIT, (int)((rows + tile - 1) / tile)};
+    const long long items = (long long)b.num_seqs * c.H_kv * plan.w.max_tiles, units = std::max<long long>(1, (kv_cap + PAGED_ROWS_UNIT - 1) / PAGED_ROWS_UNIT);
+    const int parts = device_sms() * paged_rows_blocks_per_sm(c.d_h, c.dtype == EFA_E4M3);
+    plan.cut = units > 8 && items > 0;
+    plan.blocks = (int)std::min<long long>(plan.cut ? std::min<long long>(parts, items * units) : items, INT_MAX);
+    if (plan.cut) {
+        plan.cut_bytes = ((size_t)plan.blocks * sizeof(PagedCut) + 255) / 256 * 256;
+        plan.ml_bytes = (size_t)plan.blocks * 2 * tile * sizeof(float2);
+        plan.o_bytes = (size_t)plan.blocks * 2 * tile * c.d_h * sizeof(float);
+    }
+    return plan;
+}
+
+}  // namespace
+
+const char* paged_check(const efa_paged_cache& c, const efa_paged_batch& b)
+{
+    if (c.dtype != EFA_F16 && c.dtype != EFA_E4M3) return "paged: the cache must be EFA_F16 or EFA_E4M3";
+    if (c.d_h != 16 && c.d_h != 32 && c.d_h != 64 && c.d_h != 128) return "paged: d_h must be 16, 32, 64 or 128";
+    if (c.page_size < 16 || c.page_size > 256 || (c.page_size & (c.page_size - 1))) return "paged: page_size must be 16, 32, 64, 128 or 256";
+    if (c.H_kv < 1 || c.H_kv > 65535) return "paged: H_kv must be positive";
+    if (c.num_pages < 1) return "paged: num_pages must be positive";
+    if (!c.k || !c.v || !aligned16(c.k) || !aligned16(c.v)) return "paged: k and v must be 16-byte aligned memory";
+    if (c.dtype == EFA_E4M3 && (!c.k_exp || !c.v_exp || !aligned16(c.k_exp) || !aligned16(c.v_exp))) return "paged: an e4m3 cache needs k_exp and v_exp, 16-byte aligned";
+    if (c.page_stride != 0 && (c.page_stride < (long long)c.H_kv * c.page_size * c.d_h || c.page_stride % 16)) return "paged: page_stride must be 0 or a multiple of 16 that holds a page";
+    if (b.num_seqs < 0 || b.tokens < 0 || b.max_q < 0 || b.max_kv < 0) return "paged: negative size";
+    if (b.max_pages < 1) return "paged: max_pages must be positive";
+    if (!b.q_start || !b.kv_len || !b.pages) return "paged: q_start, kv_len and pages must not be null";
+    if ((long long)b.num_seqs * b.max_pages > INT_MAX || (long long)c.H_kv * c.page_size * c.d_h > INT_MAX) return "paged: sizes too large";
+    return nullptr;
+}
+
+const char* paged_attention_check(const efa_paged_cache& c, const efa_paged_batch& b, const efa_paged_attention_params& p)
+{
+    if (const char* why = paged_check(c, b)) return why;
+    if (p.H_q < 1 || p.H_q % c.H_kv) return "paged: H_q must be a positive multiple of H_kv";
+    if (!std::isfinite(p.scale)) return "paged: scale must be finite";
+    if (p.q_head_stride || p.q_token_stride) {
+        if (p.q_head_stride < c.d_h || p.q_token_stride < c.d_h || p.q_head_stride % 8 || p.q_token_stride % 8) return "paged: row strides must be multiples of 8 and at least d_h";
+    }
+    if (p.o_token_stride != 0 && (p.o_token_stride < (long long)p.H_q * c.d_h || p.o_token_stride % 8)) return "paged: o_token_stride must be 0 or a multiple of 8 that holds H_q * d_h";
+    const long long rows = (long long)b.max_q * (p.H_q / c.H_kv), units = ((long long)b.max_kv + 63) / 64 + 1;
+    if (rows > INT_MAX / 2 || (double)b.num_seqs * c.H_kv * ((double)rows / 16 + 1) * (double)units > (double)INT_MAX) return "paged: sizes too large";
+    return nullptr;
+}
+
+size_t paged_attention_bytes(const efa_paged_cache& c, const efa_paged_batch& b, const efa_paged_attention_params& p)
+{
+    const PagedPlan plan = plan_attention(c, b, p);
+    return plan.cut_bytes + plan.ml_bytes + plan.o_bytes;
+}
+
+int cache_write(const void* K, const void* V, long long head_stride, long long token_stride, const efa_paged_cache& c, const efa_paged_batch& b, cudaStream_t stream)
+{
+    return move_rows("cache_write", false, K, V, head_stride, token_stride, c, b, stream);
+}
+
+int cache_read(void* K, void* V, long long head_stride, long long token_stride, const efa_paged_cache& c, const efa_paged_batch& b, cudaStream_t stream)
+{
+    return move_rows("cache_read", true, K, V, head_stride, token_stride, c, b, stream);
+}
+
+int paged_attention(const void* Q, void* O, const efa_paged_cache& c, const efa_paged_batch& b, const efa_paged_attention_params& p,
+                    void* workspace, size_t workspace_bytes, cudaStream_t stream)
+{
+    if (const char* why = paged_attention_check(c, b, p)) { set_error("paged_attention: %s", why); return 2; }
+    if (!aligned16(Q) || !aligned16(O)) { set_error("paged_attention: Q and O must be 16-byte aligned"); return 2; }
+    if (b.num_seqs == 0 || b.tokens == 0 || b.max_q == 0) return 0;
+    const PagedPlan plan = plan_attention(c, b, p);
+    const size_t need = plan.cut_bytes + plan.ml_bytes + plan.o_bytes;
+    if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace))) {
+        set_error("paged_attention: needs a workspace of %zu bytes, 16-byte aligned (got %zu)", need, workspace ? workspace_bytes : 0);
+        return 2;
+    }
+    const void* const mem[] = {Q, O, c.k, c.v, c.k_exp, c.v_exp, b.q_start, b.kv_len, b.pages, need ? workspace : nullptr};
+    if (int rc = check_memory("paged_attention", mem, 10)) return rc;
+    PagedArgs args = device_args(c, b);
+    args.status = kernel_status_word();
+    PagedAttnArgs a{};
+    a.Q = static_cast<const __half*>(Q);
+    a.O = static_cast<__half*>(O);
+    const bool dense = p.q_head_stride == 0 && p.q_token_stride == 0;
+    a.q_head = dense ? (long long)b.tokens * c.d_h : p.q_head_stride;
+    a.q_token = dense ? c.d_h : p.q_token_stride;
+    a.o_token = p.o_token_stride ? p.o_token_stride : (long long)p.H_q * c.d_h;
+    a.scale_log2e = p.scale * 1.4426950408889634f;
+    a.w = plan.w;
+    if (plan.cut) {
+        uint8_t* at = static_cast<uint8_t*>(workspace);
+        a.parts.cut = reinterpret_cast<PagedCut*>(at);
+        a.parts.ml = reinterpret_cast<float2*>(at + plan.cut_bytes);
+        a.parts.o = reinterpret_cast<float*>(at + plan.cut_bytes + plan.ml_bytes);
+    }
+    if (int rc = paged_rows_launch(args, a, c.d_h, c.dtype == EFA_E4M3, plan.blocks, stream)) return rc;
+    if (!plan.cut || plan.blocks < 2) return 0;
+    return paged_merge_launch(args, a, c.d_h, plan.blocks, (int)std::min<long long>(plan.w.tile, (long long)b.max_q * plan.w.G), stream);
+}
+
+}  // namespace efa

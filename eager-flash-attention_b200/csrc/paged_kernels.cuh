@@ -1,0 +1,34 @@
+// Launch arguments of the attention kernels over the paged cache, and their launchers.
+#pragma once
+
+#include "host_util.h"
+#include "paged_args.cuh"
+
+namespace efa {
+
+struct PagedAttnArgs {
+    const __half* Q;
+    __half* O;
+    long long q_head, q_token, o_token;     // strides in elements
+    float scale_log2e;
+    PagedShape w;
+    PagedParts parts;                       // all null: nothing is cut, one block per item
+};
+
+// mma.sync over tiles of up to 64 rows (paged_rows_sm100.cu).
+int paged_rows_tile(int rows);              // rows of a tile for chunks of up to `rows` rows (tokens x heads of a group)
+constexpr int PAGED_ROWS_UNIT = 64;
+int paged_rows_blocks_per_sm(int d_h, bool f8);
+int paged_rows_launch(const PagedArgs& c, const PagedAttnArgs& a, int d_h, bool f8, int blocks, cudaStream_t stream);
+
+// Merge of the items that the cuts of `blocks` parts go through.
+int paged_merge_launch(const PagedArgs& c, const PagedAttnArgs& a, int d_h, int blocks, int most_rows, cudaStream_t stream);
+
+// A launch like launch_early's (host_util.h) of a kernel whose name the caller has as a value.
+template <class... P, class... A>
+cudaError_t paged_launch(void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem, cudaStream_t stream, const A&... args)
+{
+    return launch_kernel(true, 1, kernel, grid, threads, smem, stream, args...);
+}
+
+}  // namespace efa

@@ -1,0 +1,515 @@
+// Attention of few rows over the paged cache: the next token of each sequence, or some tokens, of all query heads that share a kv head
+// (up to 64 rows to a tile; longer chunks as several tiles). For row i over the keys j it sees, with s_ij = scale * log2(e) * q_i . k_j,
+//     m_i = max_j s_ij,  l_i = sum_j 2^(s_ij - m_i),  O_i = sum_j 2^(s_ij - m_i) v_j / l_i
+// in one pass: m, l and O of what has been seen are rescaled when m grows.
+//
+// Few rows do little with each key that they load, so it is the loading that takes the time: every key and value comes from memory once per
+// group of heads, and the blocks' work is a contiguous share of all keys of all sequences (paged_part), whatever their lengths.
+// A block is four warps in teams: WM warps of 16 rows each share a team's keys, 4 / WM teams take 16 * WM keys each of a unit of 64 keys. A team has a
+// ring of stages in shared memory that its warps fill with asynchronous 16-byte copies and wait for by themselves, so no barrier of
+// the block is in the loop. The products are mma.sync m16n8k16: a tile of 16 rows is what there is, and tcgen05's least 64 rows would need the
+// softmax to cross tensor memory for nothing.
+//
+// fp16 keys reach the registers by ldmatrix. Codes of e4m3 are read as 16 bytes of a key per thread and converted there (exactly): the order of
+// the head's elements in Q K^T, and that of O's columns, is then each thread's own, and Q's fragments and the stores follow it. The exponents of keys
+// multiply the scores; those of values multiply the converted values, which is exact too.
+#include "paged_kernels.cuh"
+#include "fa_args.cuh"
+
+namespace efa {
+
+namespace {
+
+constexpr int PR_THREADS = 128;
+
+template <int D, bool F8, int WM>
+struct RowsCfg {
+    static constexpr int TEAMS = 4 / WM, TILE = 16 * WM, KS = 16 * WM;       // a team's keys of a unit
+    static constexpr int RB = D * (F8 ? 1 : 2);                               // bytes of a key
+    static constexpr int STAGE = 2 * KS * RB + (F8 ? 2 * KS : 0);             // of a team
+    static constexpr int UNIT_BYTES = TEAMS * STAGE;
+    static constexpr int STAGES = UNIT_BYTES >= 32768 ? 3 : UNIT_BYTES >= 16384 ? 6 : 8;
+    static constexpr int RING = STAGES * UNIT_BYTES;
+    static constexpr int OPITCH = D + 4;
+    static constexpr int MERGE = 4 * 16 * OPITCH * 4 + 4 * 16 * 8;            // four warps' O, and (m, l)
+    static constexpr int SMEM = RING > MERGE ? RING : MERGE;
+};
+
+// Where 16-byte chunk c of key r of a stage lies. Rows of 128 bytes or more: chunk ^ f(r), f one to one on 0..7, so that eight rows' equal chunks (ldmatrix)
+// lie in eight different bank groups; f(2p) and f(2p+1) differ in bit 2 (two keys x four chunks, a phase of the e4m3 key loads), and f(0), f(2), f(4),
+// f(6) above bit 0 (two chunks x four keys, a phase of its value loads). Shorter rows: the same over lines of 128 bytes.
+template <int RB>
+__device__ __forceinline__ int rows_swizzled(int r, int c)
+{
+    if constexpr (RB >= 128) return r * RB + ((c ^ ((r & 7) ^ ((r & 1) << 2))) << 4);
+    if constexpr (RB == 64) return (r >> 1) * 128 + ((((r & 1) * 4 + c) ^ ((0x6530 >> (4 * ((r >> 1) & 3))) & 7)) << 4);
+    if constexpr (RB == 32) return (r >> 2) * 128 + ((((r & 3) * 2 + c) ^ ((r >> 2) & 1)) << 4);
+    return r * RB + (c << 4);
+}
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" :: "n"(N) : "memory"); }
+
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4])
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4])
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// BYTES (2 to 16) of shared memory as words.
+template <int BYTES>
+__device__ __forceinline__ void load_words(uint32_t addr, uint32_t (&w)[4])
+{
+    if constexpr (BYTES == 16) asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr) : "memory");
+    if constexpr (BYTES == 8) asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr) : "memory");
+    if constexpr (BYTES == 4) asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[0]) : "r"(addr) : "memory");
+    if constexpr (BYTES == 2) asm volatile("{\n.reg .b16 x;\nld.shared.b16 x, [%1];\ncvt.u32.u16 %0, x;\n}\n" : "=r"(w[0]) : "r"(addr) : "memory");
+}
+
+__device__ __forceinline__ unsigned load_byte(uint32_t addr)
+{
+    uint32_t x;
+    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(x) : "r"(addr) : "memory");
+    return x;
+}
+
+template <int D, bool F8, int WM>
+__global__ void __launch_bounds__(PR_THREADS, 2)
+paged_rows_kernel(const PagedArgs c, const PagedAttnArgs a)
+{
+    using C = RowsCfg<D, F8, WM>;
+    constexpr int RB = C::RB, KS = C::KS, NT = D / 8, KSTEPS = D / 16;
+    constexpr int EB = D / 4 < 16 ? D / 4 : 16;            // e4m3: bytes of a key that a thread reads at a time
+    constexpr int VB = D / 8;                              // e4m3: bytes of a value row that a thread reads, its columns of O
+
+    extern __shared__ __align__(128) uint8_t smem_rows[];
+    __shared__ PagedScratch scratch;
+
+    const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+    const int g = lane >> 2, t = lane & 3;                 // row pair and column pair of the fragments
+    const int team = warp / WM, mrow = warp % WM;
+
+    pdl_wait();
+    pdl_trigger();
+
+    int begin = 0, end = 1;
+    PagedAt at;
+    const bool cut = a.parts.cut != nullptr;
+    if (cut) {
+        const bool any = paged_part<PR_THREADS>(c, a.w, blockIdx.x, gridDim.x, scratch, begin, end, at);
+        if (tid == 0) {
+            PagedCut here{};
+            if (any) here = PagedCut{begin - at.off, paged_units(a.w, paged_seq<true>(c, at.b, 51), at.rt), begin, at.h, at.b, at.rt, 0, 0};
+            a.parts.cut[blockIdx.x] = here;
+        }
+        if (!any) return;
+    } else {
+        const int per = c.H_kv * a.w.max_tiles, b = blockIdx.x / per, rest = blockIdx.x - b * per;
+        at = PagedAt{rest % c.H_kv, b, rest / c.H_kv, 0};
+        const PagedSeq q = paged_seq(c, b);
+        if (tid == 0 && rest == 0) paged_seq<true>(c, b, 51);
+        if (at.rt >= paged_tiles(a.w, q)) return;
+        end = paged_units(a.w, q, at.rt);
+    }
+
+    const uint32_t ring = smem_u32(smem_rows) + team * C::STAGE;       // stage s of this team: + s * UNIT_BYTES
+
+    bool first = true;
+    for (int left = end - begin; left > 0; paged_next(c, a.w, at), first = false) {
+        const PagedSeq q = paged_seq(c, at.b);
+        const int units = paged_units(a.w, q, at.rt);
+        const int u_lo = at.off, u_hi = min(units, at.off + left);
+        left -= u_hi - u_lo;
+        const bool whole = u_hi - u_lo == units;
+        const int rows = min(C::TILE, q.n * a.w.G - at.rt * C::TILE), r0 = at.rt * C::TILE;      // of the item
+
+        // ---- the asynchronous copies of a unit: this warp's 16 keys of the team's
+        int page_of = 0, page_from = u_lo - 32;            // lane l: page of this warp's keys in unit page_from + l
+        auto load = [&](int u) {
+            if (u < u_hi) {
+                if (u - page_from >= 32) {
+                    page_from = u;
+                    const int key = (u + lane) * PAGED_ROWS_UNIT + team * KS + mrow * 16;
+                    page_of = key < q.kv && u + lane < u_hi ? paged_page(c, at.b, key, 52) : -1;
+                }
+                const int page = __shfl_sync(0xffffffffu, page_of, u - page_from);
+                const int key = u * PAGED_ROWS_UNIT + team * KS + mrow * 16;
+                const int there = page >= 0 ? q.kv - key : 0;                     // keys that exist
+                const uint32_t dst = ring + ((u - u_lo) % C::STAGES) * C::UNIT_BYTES;
+                const int row = (at.h << c.page_shift) + (key & ((1 << c.page_shift) - 1));
+                const long long src = (long long)max(page, 0) * c.page_stride + (long long)row * RB;
+                #pragma unroll
+                for (int i = 0; i < (RB + 31) / 32; i++) {
+                    const int idx = i * 32 + lane, r = idx / (RB / 16), ch = idx % (RB / 16);
+                    if (RB < 32 && idx >= RB) break;
+                    const uint32_t to = dst + rows_swizzled<RB>(mrow * 16 + r, ch);
+                    copy16(to, c.k + src + idx * 16, r < there);
+                    copy16(to + KS * RB, c.v + src + idx * 16, r < there);
+                }
+                if (F8 && lane < 2) {
+                    const long long e = ((long long)max(page, 0) * c.H_kv << c.page_shift) + row;
+                    copy16(dst + 2 * KS * RB + lane * KS + mrow * 16, (lane ? c.v_exp : c.k_exp) + e, there > 0);
+                }
+            }
+            copy_commit();
+        };
+        #pragma unroll
+        for (int i = 0; i < C::STAGES - 1; i++) load(u_lo + i);
+
+        // ---- Q fragments: rows g and g + 8 of this warp's 16
+        uint32_t qf[KSTEPS][4];
+        int sees[2];                                       // keys below this
+        #pragma unroll
+        for (int half = 0; half < 2; half++) {
+            const int rr = mrow * 16 + g + half * 8, r = r0 + rr;
+            const bool valid = rr < rows;
+            sees[half] = valid ? paged_visible(a.w, q, r) : q.kv;
+            const int token = valid ? r / a.w.G : 0;
+            const __half* src = a.Q + (long long)(at.h * a.w.G + (valid ? r - token * a.w.G : 0)) * a.q_head + (long long)(q.row0 + token) * a.q_token;
+            #pragma unroll
+            for (int s = 0; s < KSTEPS; s++) {
+                if constexpr (F8) {
+                    const int col = (t + 4 * (s / (EB / 4))) * EB + (s % (EB / 4)) * 4;
+                    const uint2 x = valid ? *reinterpret_cast<const uint2*>(src + col) : make_uint2(0u, 0u);
+                    qf[s][half] = x.x;
+                    qf[s][2 + half] = x.y;
+                } else {
+                    qf[s][half] = valid ? *reinterpret_cast<const uint32_t*>(src + s * 16 + t * 2) : 0u;
+                    qf[s][2 + half] = valid ? *reinterpret_cast<const uint32_t*>(src + s * 16 + t * 2 + 8) : 0u;
+                }
+            }
+        }
+        // Keys that every row of this warp sees need no mask.
+        const int all_see = __reduce_min_sync(0xffffffffu, min(min(sees[0], sees[1]), q.kv));
+
+        float o[NT][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+        #pragma unroll
+        for (int j = 0; j < NT; j++) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+        bool poison = false;                               // a value that some row does not see is not finite
+
+        for (int u = u_lo; u < u_hi; u++) {
+            copy_wait<C::STAGES - 2>();
+            if constexpr (WM == 1) __syncwarp();
+            else asm volatile("bar.sync %0, %1;" :: "r"(1 + team), "n"(32 * WM) : "memory");
+            load(u + C::STAGES - 1);
+            const uint32_t sk = ring + ((u - u_lo) % C::STAGES) * C::UNIT_BYTES, sv = sk + KS * RB, se = sv + KS * RB;
+            #pragma unroll 1
+            for (int blk = 0; blk < WM; blk++) {
+                const int key0 = u * PAGED_ROWS_UNIT + team * KS + blk * 16;
+                if (key0 >= q.kv) break;
+                // ---- S = Q K^T, 16 rows x 16 keys
+                float s[2][4] = {};
+                if constexpr (F8) {
+                    #pragma unroll
+                    for (int nt = 0; nt < 2; nt++)
+                        #pragma unroll
+                        for (int i = 0; i < D / (4 * EB); i++) {
+                            uint32_t w[4];
+                            const int byte = (t + 4 * i) * EB;
+                            load_words<EB>(sk + rows_swizzled<RB>(blk * 16 + nt * 8 + g, byte >> 4) + (byte & 15), w);
+                            #pragma unroll
+                            for (int x = 0; x < EB / 4; x++)
+                                mma16816(s[nt], qf[i * (EB / 4) + x], e4m3x2_to_f16x2(w[x] & 0xffffu), e4m3x2_to_f16x2(w[x] >> 16));
+                        }
+                } else {
+                    #pragma unroll
+                    for (int st = 0; st < KSTEPS; st++) {
+                        uint32_t w[4];
+                        ldsm4(sk + rows_swizzled<RB>(blk * 16 + (lane & 7) + ((lane >> 4) << 3), st * 2 + ((lane >> 3) & 1)), w);
+                        mma16816(s[0], qf[st], w[0], w[1]);
+                        mma16816(s[1], qf[st], w[2], w[3]);
+                    }
+                }
+                // ---- softmax; this thread has keys key0 + nt * 8 + t * 2 + {0, 1} of rows g (s[.][0..1]) and g + 8
+                const bool masked = key0 + 16 > all_see;
+                uint32_t vexp[2][2];
+                #pragma unroll
+                for (int nt = 0; nt < 2; nt++)
+                    #pragma unroll
+                    for (int x = 0; x < 2; x++) {
+                        float f = a.scale_log2e;
+                        if constexpr (F8) {
+                            const int kk = blk * 16 + nt * 8 + t * 2 + x;
+                            f *= exp_byte_f32(load_byte(se + kk));
+                            vexp[nt][x] = exp_byte_f16x2(load_byte(se + KS + kk));
+                        }
+                        #pragma unroll
+                        for (int half = 0; half < 2; half++) {
+                            float& e = s[nt][half * 2 + x];
+                            e *= f;
+                            if (masked && key0 + nt * 8 + t * 2 + x >= min(sees[half], q.kv)) e = -INFINITY;
+                        }
+                    }
+                float off[2], alpha[2];
+                #pragma unroll
+                for (int half = 0; half < 2; half++) {
+                    float mx = fmaxf(fmaxf(s[0][half * 2], s[0][half * 2 + 1]), fmaxf(s[1][half * 2], s[1][half * 2 + 1]));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                    mx = fmaxf(mx, m[half]);
+                    off[half] = mx == -INFINITY ? 0.f : mx;
+                    alpha[half] = m[half] == mx ? 1.f : ex2(m[half] - off[half]);
+                    m[half] = mx;
+                }
+                if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
+                    #pragma unroll
+                    for (int j = 0; j < NT; j++) { o[j][0] *= alpha[0]; o[j][1] *= alpha[0]; o[j][2] *= alpha[1]; o[j][3] *= alpha[1]; }
+                    l[0] *= alpha[0];
+                    l[1] *= alpha[1];
+                }
+                uint32_t p[4];
+                #pragma unroll
+                for (int nt = 0; nt < 2; nt++)
+                    #pragma unroll
+                    for (int half = 0; half < 2; half++) {
+                        const float p0 = ex2(s[nt][half * 2] - off[half]), p1 = ex2(s[nt][half * 2 + 1] - off[half]);
+                        l[half] += p0 + p1;
+                        p[nt * 2 + half] = pack_f16x2(p0, p1);
+                    }
+                // ---- O += P V. A masked weight is 0, and 0 times what is not finite is not 0: such values are left out here and, for the rows that
+                // do see them, put in at the end.
+                auto clean = [&](uint32_t (&w)[4]) {
+                    #pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const uint32_t bad = nonfinite_f16x2(w[i]);
+                        poison |= bad != 0;
+                        w[i] &= ~bad;
+                    }
+                };
+                if constexpr (F8) {
+                    uint32_t w[4][4];                      // keys t * 2, t * 2 + 1, t * 2 + 8, t * 2 + 9
+                    #pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        load_words<VB>(sv + rows_swizzled<RB>(blk * 16 + (i >> 1) * 8 + t * 2 + (i & 1), (g * VB) >> 4) + ((g * VB) & 15), w[i]);
+                    #pragma unroll
+                    for (int j = 0; j < NT; j += 2) {
+                        uint32_t h[4];
+                        #pragma unroll
+                        for (int i = 0; i < 4; i++) h[i] = mul_f16x2(e4m3x2_to_f16x2((w[i][j >> 2] >> ((j & 2) * 8)) & 0xffffu), vexp[i >> 1][i & 1]);
+                        if (masked) clean(h);
+                        mma16816(o[j], p, __byte_perm(h[0], h[1], 0x5410), __byte_perm(h[2], h[3], 0x5410));
+                        mma16816(o[j + 1], p, __byte_perm(h[0], h[1], 0x7632), __byte_perm(h[2], h[3], 0x7632));
+                    }
+                } else {
+                    #pragma unroll
+                    for (int j = 0; j < NT; j += 2) {
+                        uint32_t w[4];
+                        ldsm4_t(sv + rows_swizzled<RB>(blk * 16 + (lane & 7) + (((lane >> 3) & 1) << 3), j + (lane >> 4)), w);
+                        if (masked) clean(w);
+                        mma16816(o[j], p, w[0], w[1]);
+                        mma16816(o[j + 1], p, w[2], w[3]);
+                    }
+                }
+            }
+        }
+        copy_wait<0>();
+
+        // Column of O that o[j][.] with column pair x (0, 1) is.
+        auto column = [&](int j, int x) { return F8 ? (t * 2 + x) * VB + j : j * 8 + t * 2 + x; };
+        if (__any_sync(0xffffffffu, poison)) {
+            // Rare: the values that are not finite, of keys that some row of the warp does not see, for the rows that see them.
+            for (int u = max(u_lo, max(all_see, 0) / PAGED_ROWS_UNIT); u < u_hi; u++)
+                for (int x = 0; x < KS; x++) {
+                    const int key = u * PAGED_ROWS_UNIT + team * KS + x;
+                    if (key >= q.kv || (key | 15) < all_see) continue;
+                    const int page = paged_page(c, at.b, key, 52);
+                    if (page < 0) continue;
+                    const int row = (at.h << c.page_shift) + (key & ((1 << c.page_shift) - 1));
+                    const uint8_t* src = c.v + (long long)page * c.page_stride + (long long)row * RB;
+                    for (int half = 0; half < 2; half++) {
+                        if (key >= sees[half]) continue;
+                        #pragma unroll
+                        for (int j = 0; j < NT; j++)
+                            #pragma unroll
+                            for (int y = 0; y < 2; y++) {
+                                float v;
+                                if constexpr (F8) v = (src[column(j, y)] & 0x7f) == 0x7f ? NAN : 0.f;
+                                else v = __half2float(reinterpret_cast<const __half*>(src)[column(j, y)]);
+                                if (!isfinite(v)) o[j][half * 2 + y] += v;
+                            }
+                    }
+                }
+        }
+
+        // ---- the warps' results, merged through shared memory (the ring has been read by now)
+        #pragma unroll
+        for (int half = 0; half < 2; half++) {
+            l[half] += __shfl_xor_sync(0xffffffffu, l[half], 1);
+            l[half] += __shfl_xor_sync(0xffffffffu, l[half], 2);
+        }
+        __syncthreads();
+        float* so = reinterpret_cast<float*>(smem_rows);                               // [4][16][OPITCH]
+        float2* sml = reinterpret_cast<float2*>(so + 4 * 16 * C::OPITCH);              // [4][16]
+        #pragma unroll
+        for (int half = 0; half < 2; half++) {
+            const int rr = warp * 16 + g + half * 8;
+            if (t == 0) sml[rr] = make_float2(m[half], l[half]);
+            float* dst = so + rr * C::OPITCH;
+            #pragma unroll
+            for (int j = 0; j < NT; j++) { dst[column(j, 0)] = o[j][half * 2]; dst[column(j, 1)] = o[j][half * 2 + 1]; }
+        }
+        __syncthreads();
+        const int place = (int)blockIdx.x * 2 + (first ? 0 : 1);
+        for (int e = tid; e < rows * (D / 8); e += PR_THREADS) {
+            const int rr = e / (D / 8), col = (e % (D / 8)) * 8;
+            float top = -INFINITY, sum = 0.f, acc[8] = {};
+            #pragma unroll
+            for (int i = 0; i < C::TEAMS; i++) top = fmaxf(top, sml[i * C::TILE + rr].x);
+            #pragma unroll
+            for (int i = 0; i < C::TEAMS; i++) {
+                const float2 ml = sml[i * C::TILE + rr];
+                const float w = ml.x == top ? 1.f : ex2(ml.x - top);
+                sum += w * ml.y;
+                const float* src = so + (i * C::TILE + rr) * C::OPITCH + col;
+                #pragma unroll
+                for (int x = 0; x < 8; x++) acc[x] += w * src[x];
+            }
+            if (whole) {
+                const int r = r0 + rr, token = r / a.w.G;
+                const bool none = paged_visible(a.w, q, r) <= 0;                       // nothing to see: zeros
+                const float inv = none ? 0.f : 1.f / sum;
+                uint4 out;
+                uint32_t* w = &out.x;
+                #pragma unroll
+                for (int x = 0; x < 4; x++) w[x] = none ? 0u : pack_f16x2(acc[2 * x] * inv, acc[2 * x + 1] * inv);
+                *reinterpret_cast<uint4*>(a.O + (long long)(q.row0 + token) * a.o_token + (long long)(at.h * a.w.G + r - token * a.w.G) * D + col) = out;
+            } else {
+                const long long slot = (long long)place * C::TILE + rr;
+                float4* dst = reinterpret_cast<float4*>(a.parts.o + slot * D + col);
+                dst[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+                dst[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+                if (col == 0) a.parts.ml[slot] = make_float2(top, sum);
+            }
+        }
+        __syncthreads();
+        if (left <= 0) break;
+    }
+}
+
+// Merge of what the blocks left of the items that a cut goes through (PagedCut), over the pieces i of an item:
+//     O = sum_i 2^(m_i - max m) O_i / sum_i 2^(m_i - max m) l_i.
+// Block (x, y) looks at the cut ahead of part x + 1: if it is the first in its item it merges the item's rows 4y .. 4y + 3, a warp each.
+template <int D>
+__global__ void __launch_bounds__(128)
+paged_merge_kernel(const PagedArgs c, const PagedAttnArgs a, int parts)
+{
+    pdl_wait();
+    pdl_trigger();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int part = blockIdx.x + 1;
+    const PagedCut here = a.parts.cut[part];
+    const int ahead = a.parts.cut[part - 1].begin;         // where the part before it begins
+    if (here.begin <= here.item_begin || ahead > here.item_begin) return;     // not inside an item, or not the first in it
+    const PagedSeq q = paged_seq(c, here.b);
+    const int rr = blockIdx.y * 4 + warp, r = here.rt * a.w.tile + rr;
+    if (rr >= a.w.tile || r >= q.n * a.w.G) return;
+    const int stop = here.item_begin + here.units;         // unit behind the item
+    const int sees = min(paged_visible(a.w, q, r), q.kv);
+
+    // Pieces: part - 1 (its last item, unless it begins with it), then the first item of part, part + 1, ...
+    const int first_place = (part - 1) * 2 + (ahead < here.item_begin ? 1 : 0);
+    auto place_of = [&](int i) { return i == 0 ? first_place : (part - 1 + i) * 2; };
+    auto exists = [&](int i) -> bool { return i == 0 || (part - 1 + i < parts && a.parts.cut[part - 1 + i].begin < stop && a.parts.cut[part - 1 + i].units > 0); };
+    float top = -INFINITY;
+    int n = 0;
+    for (int i0 = 0; ; i0 += 32) {
+        const bool is = exists(i0 + lane);
+        const float m = is ? a.parts.ml[(long long)place_of(i0 + lane) * a.w.tile + rr].x : -INFINITY;
+        float mx = m;
+        #pragma unroll
+        for (int d = 16; d > 0; d /= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+        top = fmaxf(top, mx);
+        const int here_n = __popc(__ballot_sync(0xffffffffu, is));
+        n += here_n;
+        if (here_n < 32) break;
+    }
+    constexpr int COLS = D >= 128 ? 4 : D >= 64 ? 2 : 1;   // columns of a lane
+    const int col = lane * COLS;
+    float acc[COLS] = {}, sum = 0.f;
+    if (col < D || D >= 32) {
+        for (int i = 0; i < n; i++) {
+            const long long slot = (long long)place_of(i) * a.w.tile + rr;
+            const float2 ml = a.parts.ml[slot];
+            const float w = ml.x == top ? 1.f : ex2(ml.x - top);
+            sum += w * ml.y;
+            const float* src = a.parts.o + slot * D + col;
+            if (col < D) {
+                #pragma unroll
+                for (int x = 0; x < COLS; x++) acc[x] += w * src[x];
+            }
+        }
+    }
+    if (col >= D) return;
+    const int token = r / a.w.G;
+    __half* dst = a.O + (long long)(q.row0 + token) * a.o_token + (long long)(here.h * a.w.G + r - token * a.w.G) * D + col;
+    #pragma unroll
+    for (int x = 0; x < COLS; x++) dst[x] = __float2half_rn(sees <= 0 ? 0.f : acc[x] / sum);
+}
+
+template <int D, bool F8, int WM>
+int launch_rows(const PagedArgs& c, const PagedAttnArgs& a, int blocks, cudaStream_t stream)
+{
+    using C = RowsCfg<D, F8, WM>;
+    static bool configured[64] = {};
+    int dev = 0;
+    EFA_CUDA(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64 || !configured[dev]) {
+        EFA_CUDA(cudaFuncSetAttribute(paged_rows_kernel<D, F8, WM>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+        if (dev >= 0 && dev < 64) configured[dev] = true;
+    }
+    EFA_CUDA(paged_launch(paged_rows_kernel<D, F8, WM>, dim3(blocks), PR_THREADS, C::SMEM, stream, c, a));
+    return 0;
+}
+
+template <int D, bool F8>
+int launch_rows(const PagedArgs& c, const PagedAttnArgs& a, int blocks, cudaStream_t stream)
+{
+    switch (a.w.tile) {
+        case 16: return launch_rows<D, F8, 1>(c, a, blocks, stream);
+        case 32: return launch_rows<D, F8, 2>(c, a, blocks, stream);
+        default: return launch_rows<D, F8, 4>(c, a, blocks, stream);
+    }
+}
+
+}  // namespace
+
+int paged_rows_tile(int rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+
+int paged_rows_blocks_per_sm(int d_h, bool f8) { (void)d_h; (void)f8; return 2; }
+
+int paged_rows_launch(const PagedArgs& c, const PagedAttnArgs& a, int d_h, bool f8, int blocks, cudaStream_t stream)
+{
+    switch (d_h) {
+        case 16:  return f8 ? launch_rows<16, true>(c, a, blocks, stream) : launch_rows<16, false>(c, a, blocks, stream);
+        case 32:  return f8 ? launch_rows<32, true>(c, a, blocks, stream) : launch_rows<32, false>(c, a, blocks, stream);
+        case 64:  return f8 ? launch_rows<64, true>(c, a, blocks, stream) : launch_rows<64, false>(c, a, blocks, stream);
+        default:  return f8 ? launch_rows<128, true>(c, a, blocks, stream) : launch_rows<128, false>(c, a, blocks, stream);
+    }
+}
+
+int paged_merge_launch(const PagedArgs& c, const PagedAttnArgs& a, int d_h, int blocks, int most_rows, cudaStream_t stream)
+{
+    const dim3 grid(blocks - 1, (most_rows + 3) / 4);
+    switch (d_h) {
+        case 16:  EFA_CUDA(paged_launch(paged_merge_kernel<16>, grid, 128, 0, stream, c, a, blocks)); break;
+        case 32:  EFA_CUDA(paged_launch(paged_merge_kernel<32>, grid, 128, 0, stream, c, a, blocks)); break;
+        case 64:  EFA_CUDA(paged_launch(paged_merge_kernel<64>, grid, 128, 0, stream, c, a, blocks)); break;
+        default:  EFA_CUDA(paged_launch(paged_merge_kernel<128>, grid, 128, 0, stream, c, a, blocks)); break;
+    }
+    return 0;
+}
+
+}  // namespace efa

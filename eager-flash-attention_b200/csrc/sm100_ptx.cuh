@@ -19,6 +19,8 @@ constexpr unsigned long long kWaitLimitNs = 2000000000ull;   // 2 s per wait, th
 enum KernelStatus : int {
     KS_OK = 0,
     KS_WAIT_TIMEOUT = 1,
+    KS_BAD_PAGE = 2,          // a page table entry outside the pool; spare words: sequence, site
+    KS_BAD_LENGTH = 3,        // lengths of a batch outside its buffers or bounds
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p)

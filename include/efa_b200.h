@@ -27,6 +27,7 @@ extern "C" {
 /* Element types of O / output buffers. */
 #define EFA_F32 0
 #define EFA_F16 1
+#define EFA_E4M3 2   /* of a paged cache: 8-bit floating point with an exponent per row */
 
 int         efa_abi_version(void);
 const char* efa_last_error(void);
@@ -141,8 +142,84 @@ int efa_project_f16(const void* O_tile, const void* W_O, void* out,
 int efa_compute_qkv_f16(const void* X, const void* W_q, const void* W_k, const void* W_v,
                         void* Qh, void* Kh, void* Vh, int S, int d, int H_local, int d_h, void* stream);
 
-/* Status word written by kernels whose bounded waits ran out: out4 = {code, block, site, 0};
- * code 0 = no kernel reported a problem since the last efa_kernel_status_reset(). */
+/* ------------------------------------------------------------------------------------------
+ * Paged key/value cache
+ * ------------------------------------------------------------------------------------------ */
+
+/* Keys and values of past tokens, kept in pages that any sequence may own, and attention of new tokens over them: what serving a model
+ * needs beside the block, whose K and V are whole sequences (the reference has no cache, hence no counterpart for what follows).
+ *
+ * k, v: [num_pages][H_kv][page_size][d_h], 16-byte aligned, fp16 (EFA_F16) or e4m3 (EFA_E4M3); page_stride: elements from a page to the next,
+ * 0 = dense. page_size: 16, 32, 64, 128 or 256; d_h: 16, 32, 64 or 128.
+ * k_exp, v_exp (e4m3 only, else NULL): [num_pages][H_kv][page_size], a byte per row; value = code * 2^(byte - 127). efa_cache_write stores bytes of
+ * 103 to 135, for which every value is an fp16 exactly; of other bytes nothing is promised. */
+typedef struct efa_paged_cache {
+    void*    k;
+    void*    v;
+    uint8_t* k_exp;
+    uint8_t* v_exp;
+    int      num_pages, page_size, H_kv, d_h, dtype;
+    int64_t  page_stride;
+} efa_paged_cache;
+
+/* A ragged batch. Sequence b has kv_len[b] keys in the cache; key j is row j % page_size of page pages[b * max_pages + j / page_size]. The last
+ * n_b = q_start[b + 1] - q_start[b] of them are its chunk (the new tokens), and belong to rows q_start[b] ... of the row tensors, which
+ * have `tokens` rows to a head. Row i of a chunk stands at position kv_len[b] - n_b + i; one at a negative position (n_b > kv_len[b]) has no place in
+ * the cache and no key to see. Rows of no sequence (before q_start[0], from q_start[num_seqs] on) are neither read nor written.
+ * The three arrays are device memory, read when the kernels run: a captured graph follows their contents. The host gives
+ * bounds: max_q >= every n_b, max_kv >= every kv_len[b]; tight ones choose faster kernels. Lengths outside the bounds or the
+ * buffers, and page numbers outside the pool where a key lies, are reported by efa_kernel_status (code 3 and 2, sequence, site); the call then stays
+ * inside its buffers: lengths are cut to the bounds, keys of a missing page read as zeros and are not written.
+ * Sequences may share pages; a page that efa_cache_write writes to in one call should belong to one sequence. */
+typedef struct efa_paged_batch {
+    const int* q_start;     /* [num_seqs + 1] */
+    const int* kv_len;      /* [num_seqs] */
+    const int* pages;       /* [num_seqs][max_pages] */
+    int        num_seqs, max_pages, tokens, max_q, max_kv;
+} efa_paged_batch;
+
+/* NULL when a call on this cache and batch is legal, else a static description. */
+const char* efa_paged_check(const efa_paged_cache* cache, const efa_paged_batch* batch);
+
+/* Rows K, V (fp16) of the batch's chunks into their pages. Element (head, row, x) at head * head_stride + row * token_stride + x; both strides 0:
+ * [H_kv][tokens][d_h], as efa_compute_qkv_f16 writes them. Strides are multiples of 8, K and V 16-byte aligned.
+ * e4m3: per row the smallest exponent e >= -24 with max |x| <= 448 * 2^e, codes x * 2^-e rounded to nearest, ties to even (with e = 8 cut at
+ * 240, as 256 * 2^8 is no fp16); infinities and NaN are stored as NaN and do not count for the maximum. Asynchronous on `stream`. The first call of
+ * these entry points on a device must come before any stream capture (the status word is allocated then). */
+int efa_cache_write(const void* K, const void* V, int64_t head_stride, int64_t token_stride,
+                    const efa_paged_cache* cache, const efa_paged_batch* batch, void* stream);
+
+/* The inverse: the last n_b keys and values of every sequence into rows K, V (fp16; exact). With q_start counting whole sequences it lays them out
+ * as efa_flash_attn_tc_forward takes them. Rows without a place in the cache become zeros. */
+int efa_cache_read(void* K, void* V, int64_t head_stride, int64_t token_stride,
+                   const efa_paged_cache* cache, const efa_paged_batch* batch, void* stream);
+
+/* H_q: query heads, a multiple of H_kv; query head h sees kv head h / (H_q / H_kv). causal: row i of a chunk sees the keys up to its own
+ * position, else all kv_len[b]. Strides in elements: Q's both 0 = [H_q][tokens][d_h]; o_token_stride 0 = H_q * d_h. */
+typedef struct efa_paged_attention_params {
+    int     H_q;
+    int     causal;
+    float   scale;          /* softmax scale, 1/sqrt(d_h) */
+    int64_t q_head_stride, q_token_stride, o_token_stride;
+} efa_paged_attention_params;
+
+const char* efa_paged_attention_check(const efa_paged_cache* cache, const efa_paged_batch* batch, const efa_paged_attention_params* p);
+
+/* Bytes of workspace that efa_paged_attention needs for these sizes on the current device (may be 0). Host arithmetic only. */
+size_t efa_paged_attention_workspace(const efa_paged_cache* cache, const efa_paged_batch* batch, const efa_paged_attention_params* p);
+
+/* Attention of the chunks over the cache, the chunk's own keys included (efa_cache_write first): O[row][h * d_h + x], fp16, what
+ * efa_project_f16 takes. Scores, maxima, sums and O are accumulated in fp32; the softmax weights are rounded to fp16 for their product with V.
+ * A row that sees no key becomes zeros. Values that are not finite reach only the rows that see them.
+ * workspace: 16-byte aligned device memory that no other call uses until this one is done (two captured graphs that may run
+ * side by side need one each); its contents do not matter before and after. Equal calls give equal bits; the bits of a sequence
+ * may depend on the lengths of the others, by the fp32 order in which parts of long sequences are added. Asynchronous on `stream`. */
+int efa_paged_attention(const void* Q, void* O, const efa_paged_cache* cache, const efa_paged_batch* batch,
+                        const efa_paged_attention_params* p, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Status word written by kernels whose bounded waits ran out, or that found lengths or pages of a paged batch wrong: out4 = {code, block, site, 0};
+ * code 0 = no kernel reported a problem since the last efa_kernel_status_reset(), 1 = a wait ran out, 2 = a page outside the pool, 3 = a
+ * length outside its bounds (2, 3: the sequence in place of the block; site 50 = write or read, 51, 52 = attention). */
 int efa_kernel_status(int* out4);
 int efa_kernel_status_reset(void);
 

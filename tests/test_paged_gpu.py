@@ -1,0 +1,476 @@
+"""The paged key/value cache on a GPU: writing, reading back and attention against the definitions in 64 bits."""
+import math
+
+import pytest
+import torch
+
+from paged_helpers import Batch, Pool, attention_ref, check_attention, decode, encode, fill_random
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def clean_status(pkg, torch_cuda):
+    pkg.kernel_status_reset()
+    yield
+    torch.cuda.synchronize()
+    pkg.kernel_status_reset()
+
+
+def _rows(seed, *shape, spread=1.0):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    return (spread * torch.randn(*shape, generator=gen, device="cuda")).half()
+
+
+def _attend(pkg, q, pool, batch, causal=1, scale=None, out=None, stream=None):
+    H_q, tokens, d = q.shape
+    ap = pkg.paged_attention_params(H_q, d, causal, scale)
+    O = torch.full((tokens, H_q * d), 777.0, dtype=torch.float16, device="cuda") if out is None else out
+    size = pkg.paged_attention_workspace(pool.cache, batch.batch, ap)
+    ws = torch.full((size,), 0xFF, dtype=torch.uint8, device="cuda") if size else None      # NaN wherever it is read before it is written
+    pkg.paged_attention(q, O, pool.cache, batch.batch, ap, ws, stream)
+    torch.cuda.synchronize()
+    return O
+
+
+# ---- write and read ----------------------------------------------------------------------------------------------------------------------
+RAGGED = [([1], [1]), ([37, 5, 64], [37, 1, 0]), ([300, 1, 129, 0, 17], [300, 1, 64, 0, 16])]
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("d", [16, 32, 64, 128])
+@pytest.mark.parametrize("H,page,lens", [(1, 16, 0), (3, 64, 1), (8, 32, 2), (5, 256, 2)])
+def test_rows_go_to_their_pages_and_come_back(pkg, bits, d, H, page, lens):
+    kv, q = RAGGED[lens]
+    batch = Batch(pkg, kv, q, page, seed=d + H, extra_rows=3)
+    pool = Pool(pkg, batch.num_pages, H, page, d, bits, fill=0xA5)
+    before = [x.clone() for x in (pool.k, pool.v)]
+    K, V = _rows(1, H, batch.tokens, d), _rows(2, H, batch.tokens, d, spread=30)
+    pkg.cache_write(K, V, pool.cache, batch.batch)
+    for name, rows, was in (("k", K, before[0]), ("v", V, before[1])):
+        want = was.clone()
+        for b, n in enumerate(q):
+            if n == 0:
+                continue
+            page_of, slot = (x.cuda() for x in batch.places(b, kv[b] - n, kv[b]))
+            x = rows[:, batch.starts[b]:batch.starts[b] + n]
+            if bits == 8:
+                code, byte = encode(x)
+                want[page_of, :, slot] = code.transpose(0, 1)
+                assert torch.equal(getattr(pool, name + "_exp")[page_of, :, slot], byte.transpose(0, 1))
+            else:
+                want[page_of, :, slot] = x.transpose(0, 1)
+        assert torch.equal(getattr(pool, name).view(torch.uint8), want.view(torch.uint8))           # all other slots are as they were
+    Ko, Vo = torch.full_like(K, 5), torch.full_like(V, 6)
+    pkg.cache_read(Ko, Vo, pool.cache, batch.batch)
+    torch.cuda.synchronize()
+    last = batch.starts[-1]
+    for got, rows, mark in ((Ko, K, 5), (Vo, V, 6)):
+        want = rows[:, :last] if bits == 16 else decode(*encode(rows[:, :last])).half()
+        assert torch.equal(got[:, :last], want)
+        assert torch.all(got[:, last:] == mark)                            # rows of no sequence are left alone
+    assert pkg.kernel_status()[0] == 0
+
+
+def test_codes_of_rows_of_every_size(pkg):
+    """Rows from the smallest fp16 to the largest, on ties and grid points, with zeros, infinities and NaN among them."""
+    d, rows = 64, []
+    gen = torch.Generator().manual_seed(3)
+    for e in range(-24, 16):
+        for _ in range(3):
+            rows.append(torch.randn(d, generator=gen).double() * 2.0 ** e)
+    for e in range(-24, 7):                                                # grid points and the middles between them, below one top of 448 * 2^e
+        g = torch.arange(0, d).double() * 2.0 ** (e - 3)
+        g[0] = 448 * 2.0 ** e
+        rows.append(g)
+        rows.append(-g - 2.0 ** (e - 4))
+    for top in (65504.0, 61440.0, 57344.0, 57376.0, 448.0, 448.25, 2.0 ** -24, 0.0):
+        x = torch.linspace(-1, 1, d).double() * top
+        x[5] = top
+        rows.append(x)
+    special = torch.randn(d, generator=gen).double()
+    special[3], special[9], special[11] = math.inf, -math.inf, math.nan
+    rows += [special, torch.full((d,), math.nan).double(), torch.full((d,), -math.inf).double()]
+    x = torch.stack(rows).half()
+    x = torch.where(torch.isinf(x) & torch.isfinite(torch.stack(rows)), torch.full_like(x, 65504), x).cuda()[None]
+    n = x.shape[1]
+    batch = Batch(pkg, [n], [n], 16)
+    pool = Pool(pkg, batch.num_pages, 1, 16, d, 8)
+    pkg.cache_write(x, -x, pool.cache, batch.batch)
+    torch.cuda.synchronize()
+    page, slot = (p.cuda() for p in batch.places(0, 0, n))
+    code, byte = encode(x[0])
+    assert torch.equal(pool.k_exp[page, 0, slot], byte) and torch.equal(pool.v_exp[page, 0, slot], byte)
+    nan = torch.isnan(decode(code, byte))
+    got, neg = pool.k[page, 0, slot], pool.v[page, 0, slot]
+    assert torch.equal(torch.isnan(decode(got, byte)), nan) and torch.equal(torch.isnan(decode(neg, byte)), nan)
+    assert torch.equal(got[~nan], code[~nan]) and torch.equal(neg[~nan], code[~nan] ^ 128)
+    value = decode(code, byte)[~nan]
+    assert torch.equal(value.half().double(), value)                       # exact as fp16
+    Ko, Vo = torch.empty_like(x), torch.empty_like(x)
+    pkg.cache_read(Ko, Vo, pool.cache, batch.batch)
+    torch.cuda.synchronize()
+    assert torch.equal(Ko[0][~nan].double(), value) and torch.equal(Vo[0][~nan].double(), -value) and bool(torch.isnan(Ko[0][nan]).all())
+    # half a step of three bits behind the first: 2^-4 of a value above the smallest normal code
+    keep = ~nan & (x[0].double().abs() >= 2.0 ** -6 * torch.exp2(byte.double() - 127)[:, None])
+    assert float(((decode(code, byte) - x[0].double()).abs() / x[0].double().abs())[keep].max()) <= 2.0 ** -4
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+def test_strides_of_rows_and_pages(pkg, bits):
+    H, d, page = 3, 64, 32
+    batch = Batch(pkg, [70, 33], [70, 2], page)
+    pool = Pool(pkg, batch.num_pages, H, page, d, bits, gap=48)
+    dense = Pool(pkg, batch.num_pages, H, page, d, bits)
+    K, V = _rows(1, H, batch.tokens, d), _rows(2, H, batch.tokens, d)
+    pkg.cache_write(K, V, dense.cache, batch.batch)
+    wide = torch.zeros(2, batch.tokens, H, d + 8, dtype=torch.float16, device="cuda")      # token by token, heads side by side
+    wide[0, :, :, :d], wide[1, :, :, :d] = K.transpose(0, 1), V.transpose(0, 1)
+    pkg.cache_write(wide[0], wide[1], pool.cache, batch.batch, head_stride=d + 8, token_stride=H * (d + 8))
+    out = torch.full_like(wide, 9)
+    pkg.cache_read(out[0], out[1], pool.cache, batch.batch, head_stride=d + 8, token_stride=H * (d + 8))
+    Ko, Vo = torch.empty_like(K), torch.empty_like(V)
+    pkg.cache_read(Ko, Vo, dense.cache, batch.batch)
+    torch.cuda.synchronize()
+    assert torch.equal(out[0, :, :, :d].transpose(0, 1), Ko) and torch.equal(out[1, :, :, :d].transpose(0, 1), Vo) and torch.all(out[..., d:] == 9)
+    fill_random(pool, batch, 5)
+    fill_random(dense, batch, 5)
+    q = _rows(3, 6, batch.tokens, d)
+    want = _attend(pkg, q, dense, batch)
+    ap = pkg.paged_attention_params(6, d, q_head_stride=d + 8, q_token_stride=6 * (d + 8), o_token_stride=6 * d + 16)
+    qw = torch.zeros(batch.tokens, 6, d + 8, dtype=torch.float16, device="cuda")
+    qw[..., :d] = q.transpose(0, 1)
+    O = torch.full((batch.tokens, 6 * d + 16), 9.0, dtype=torch.float16, device="cuda")
+    ws = torch.empty(max(16, pkg.paged_attention_workspace(pool.cache, batch.batch, ap)), dtype=torch.uint8, device="cuda")
+    pkg.paged_attention(qw, O, pool.cache, batch.batch, ap, ws)
+    torch.cuda.synchronize()
+    assert torch.equal(O[:, :6 * d], want) and torch.all(O[:, 6 * d:] == 9)
+
+
+# ---- attention ---------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("d", [16, 32, 64, 128])
+@pytest.mark.parametrize("H,G,page,kv,q", [
+    (1, 1, 16, [1], [1]),                                                    # one key
+    (2, 1, 16, [129, 64, 17, 65], [1, 1, 1, 1]),                             # single tokens
+    (2, 8, 64, [1000, 1, 63], [1, 1, 1]),                                    # a group of heads, blocks that share a long sequence
+    (1, 7, 32, [515, 2051, 96], [1, 2, 0]),                                  # odd groups, a sequence without a chunk
+    (3, 4, 16, [700, 90, 333], [4, 7, 1]),                                   # several tokens: 28 rows
+    (2, 3, 128, [400, 77], [17, 20]),                                        # 60 rows
+    (2, 2, 32, [300, 700, 33], [130, 33, 33]),                               # more than one tile, chunks from the first token on
+    (1, 1, 256, [900], [700])])
+def test_attention_of_a_chunk(pkg, bits, d, H, G, page, kv, q):
+    batch = Batch(pkg, kv, q, page, seed=G, extra_rows=2)
+    pool = Pool(pkg, batch.num_pages, H, page, d, bits)                      # NaN wherever nothing is put
+    fill_random(pool, batch, d + G)
+    Q = _rows(7, H * G, batch.tokens, d, spread=2)
+    for causal in (1, 0):
+        O = _attend(pkg, Q, pool, batch, causal)
+        check_attention(O, Q, pool, batch, d ** -0.5, causal)
+        assert torch.all(O[batch.starts[-1]:] == 777)
+        assert torch.equal(O, _attend(pkg, Q, pool, batch, causal))          # the same bits again
+    assert pkg.kernel_status()[0] == 0
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("d,H,G,kv,q", [(128, 2, 4, [9000, 1, 4097], [1, 1, 1]), (64, 1, 1, [20000], [3]), (128, 1, 8, [5000, 300], [40, 300]), (32, 4, 2, [3000], [257])])
+def test_attention_over_long_sequences(pkg, bits, d, H, G, kv, q):
+    batch = Batch(pkg, kv, q, 64, seed=1)
+    pool = Pool(pkg, batch.num_pages, H, 64, d, bits)
+    fill_random(pool, batch, 3)
+    Q = _rows(9, H * G, batch.tokens, d, spread=3)
+    check_attention(_attend(pkg, Q, pool, batch), Q, pool, batch, d ** -0.5, 1)
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+def test_scores_that_rise_and_fall(pkg, bits):
+    """Maxima that move by far more than fp16 holds, up and down the keys."""
+    d, n = 64, 1500
+    batch = Batch(pkg, [n, n], [1, 5], 16)
+    pool = Pool(pkg, batch.num_pages, 1, 16, d, bits)
+    K, V = _rows(1, 1, n, d), _rows(2, 1, n, d)
+    K[:, :, 0] = torch.linspace(-90, 90, n).cuda()
+    for b in range(2):
+        pool.put(batch, b, "k", K if b == 0 else K.flip(1))
+        pool.put(batch, b, "v", V)
+    Q = _rows(3, 2, batch.tokens, d)
+    Q[:, :, 0] = 12
+    check_attention(_attend(pkg, Q, pool, batch), Q, pool, batch, d ** -0.5, 1)
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("long", [0, 1])
+def test_rows_that_see_nothing_are_zeros(pkg, bits, long):
+    kv, q = [0, 3, 200, 1], [4, 8, 5, 1]
+    if long:
+        kv, q = kv + [3000], q + [1]
+    batch = Batch(pkg, kv, q, 16)
+    pool = Pool(pkg, batch.num_pages, 2, 16, 64, bits)
+    fill_random(pool, batch, 1)
+    Q = _rows(1, 6, batch.tokens, 64)
+    O = _attend(pkg, Q, pool, batch)
+    assert torch.all(O[:4] == 0) and torch.all(O[4:9] == 0)
+    check_attention(O, Q, pool, batch, 64 ** -0.5, 1)
+    O = _attend(pkg, Q, pool, batch, causal=0)
+    assert torch.all(O[:4] == 0)
+    check_attention(O, Q, pool, batch, 64 ** -0.5, 0)
+    assert pkg.kernel_status()[0] == 0
+    # their rows have no place in the cache either
+    K, V = _rows(2, 2, batch.tokens, 64), _rows(3, 2, batch.tokens, 64)
+    was = pool.k.clone()
+    only = Batch(pkg, [0, 3], [4, 8], 16)
+    only.dev[2].copy_(torch.tensor(batch.table, dtype=torch.int32)[:2, :only.width])
+    pkg.cache_write(K, V, pool.cache, only.batch, head_stride=batch.tokens * 64, token_stride=64)
+    Ko = torch.full((2, only.tokens, 64), 3.0, dtype=torch.float16, device="cuda")
+    Vo = Ko.clone()
+    pkg.cache_read(Ko, Vo, pool.cache, only.batch)
+    torch.cuda.synchronize()
+    assert torch.all(Ko[:, :9] == 0) and torch.all(Vo[:, :9] == 0) and torch.all(Ko[:, 9:12] != 3)
+    page, slot = (x.cuda() for x in batch.places(1, 0, 3))
+    now = pool.k.clone()
+    now[page, :, slot] = was[page, :, slot]
+    assert torch.equal(now.view(torch.uint8), was.view(torch.uint8)) and pkg.kernel_status()[0] == 0
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("d", [16, 64, 128])
+@pytest.mark.parametrize("kv,q,G", [([40, 700], [9, 6], 2), ([333, 64], [140, 64], 1), ([1500], [300], 4)])
+def test_values_that_are_not_finite_reach_only_the_rows_that_see_them(pkg, bits, d, kv, q, G):
+    batch = Batch(pkg, kv, q, 32)
+    pool = Pool(pkg, batch.num_pages, 2, 32, d, bits)
+    fill_random(pool, batch, 2)
+    for b, (n, m) in enumerate(zip(kv, q)):
+        V = pool.values(batch, b, "v").clone()
+        for i, key in enumerate((n - m // 2, n - 2, n - 1)):
+            V[i % 2, key, (5 * i + b) % d] = (math.nan, math.inf, -math.inf)[i] if bits == 16 else math.nan
+        if bits == 8:
+            V = torch.where(torch.isfinite(V), V, torch.full_like(V, math.nan))
+        pool.put(batch, b, "v", V)
+        K = pool.values(batch, b, "k").clone()
+        K[1, n - 1, 3] = math.nan                                             # the last token's key: its own row alone
+        pool.put(batch, b, "k", K)
+    Q = _rows(4, 2 * G, batch.tokens, d)
+    O = _attend(pkg, Q, pool, batch)
+    for b, (n, m) in enumerate(zip(kv, q)):
+        lo = batch.starts[b]
+        got = O[lo:lo + m].reshape(m, 2 * G, d).transpose(0, 1).double()
+        K, V = pool.values(batch, b, "k"), pool.values(batch, b, "v")
+        ref, tol = attention_ref(Q[:, lo:lo + m - 1].double(), K[:, :-1], V[:, :-1], m - 1, n - 1, d ** -0.5, 1)
+        assert torch.equal(torch.isfinite(got[:, :-1]), torch.isfinite(ref))
+        assert bool(((got[:, :-1] - ref).abs().nan_to_num() <= tol).all())
+        assert bool(torch.isnan(got[G:, -1]).all())                          # a score that is NaN
+
+
+def test_keys_without_finite_scores(pkg):
+    """All scores -inf: no weight is defined, as in the formula. An infinite key that a row does not see leaves it alone."""
+    batch = Batch(pkg, [20], [3], 16)
+    pool = Pool(pkg, batch.num_pages, 1, 16, 16, 16)
+    fill_random(pool, batch, 1)
+    K = pool.values(batch, 0, "k").clone()
+    K[0, 18:, 0] = -math.inf
+    pool.put(batch, 0, "k", K)
+    Q = torch.ones(1, 3, 16, dtype=torch.float16, device="cuda")
+    O = _attend(pkg, Q, pool, batch)
+    V = pool.values(batch, 0, "v")
+    ref, tol = attention_ref(Q.double(), K[:, :18], V[:, :18], 1, 18, 0.25, 0)
+    assert bool(((O.double()[None] - ref[:, :1]).abs() <= tol[:, :1]).all())  # -inf weighs nothing
+    K[0, :, 0] = -math.inf
+    pool.put(batch, 0, "k", K)
+    assert bool(torch.isnan(_attend(pkg, Q, pool, batch)).all())
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("q", [[1, 1, 1], [40, 100, 3]])
+def test_wrong_pages_and_lengths_are_reported(pkg, bits, q):
+    """... and the call stays inside its buffers, with the other sequences as they should be."""
+    kv = [600, 700, 64]
+    batch = Batch(pkg, kv, q, 32)
+    pool = Pool(pkg, batch.num_pages, 2, 32, 64, bits)
+    fill_random(pool, batch, 1)
+    Q = _rows(4, 4, batch.tokens, 64)
+    K, V = _rows(5, 2, batch.tokens, 64), _rows(6, 2, batch.tokens, 64)
+    for wrong in (-1, batch.num_pages, 1 << 30, -(1 << 31)):
+        was = [x.clone() for x in (pool.k, pool.v)]
+        good = batch.dev[2][1, 21].item()
+        batch.dev[2][1, 21] = wrong
+        O = _attend(pkg, Q, pool, batch)
+        assert pkg.kernel_status()[:2] == (2, 1)
+        pkg.kernel_status_reset()
+        check_attention(O, Q, pool, batch, 0.125, 1, skip=(1,))
+        assert bool(torch.isfinite(O).all())
+        pkg.cache_write(K, V, pool.cache, batch.batch)
+        torch.cuda.synchronize()
+        assert pkg.kernel_status()[:2] == (2, 1)
+        pkg.kernel_status_reset()
+        Ko, Vo = torch.full_like(K, 5), torch.full_like(V, 5)
+        pkg.cache_read(Ko, Vo, pool.cache, batch.batch)
+        torch.cuda.synchronize()
+        assert pkg.kernel_status()[:2] == (2, 1)
+        pkg.kernel_status_reset()
+        lo = batch.starts[2] - min(q[1], 700 - 21 * 32)
+        assert torch.all(Ko[:, lo:batch.starts[2]] == 0) and torch.all(Vo[:, lo:batch.starts[2]] == 0)
+        assert torch.equal(Ko[:, batch.starts[2]:], K[:, batch.starts[2]:] if bits == 16 else decode(*encode(K[:, batch.starts[2]:])).half())
+        batch.dev[2][1, 21] = good
+        for x, y in zip((pool.k, pool.v), was):
+            x.copy_(y)
+    for which, index, value in ((1, 1, 701), (1, 1, -5), (0, 1, 1 << 30), (0, 2, -7), (0, 3, batch.tokens + 1)):
+        x = batch.dev[which]
+        good = x[index].item()
+        x[index] = value
+        _attend(pkg, Q, pool, batch)
+        assert pkg.kernel_status()[0] == 3, (which, index, value)
+        pkg.kernel_status_reset()
+        pkg.cache_write(K, V, pool.cache, batch.batch)
+        pkg.cache_read(torch.empty_like(K), torch.empty_like(V), pool.cache, batch.batch)
+        torch.cuda.synchronize()
+        pkg.kernel_status_reset()
+        x[index] = good
+
+
+def test_a_captured_call_follows_lengths_and_pages(pkg):
+    """The arrays of a batch are read when the graph runs; two graphs with a workspace each run side by side."""
+    kv, q = [1500, 40, 900, 2], [1, 1, 1, 1]
+    batch = Batch(pkg, kv, q, 16, max_kv=2000, width=125, spare=300)
+    pool = Pool(pkg, batch.num_pages, 2, 16, 128, 8)
+    fill_random(pool, batch, 1)
+    Q = _rows(4, 8, batch.tokens, 128)
+    K, V = _rows(5, 2, batch.tokens, 128), _rows(6, 2, batch.tokens, 128)
+    _attend(pkg, Q, pool, batch)                                             # the first call comes before any capture
+    ap = pkg.paged_attention_params(8, 128)
+    size = pkg.paged_attention_workspace(pool.cache, batch.batch, ap)
+    graphs, outs, streams, keep = [], [], [], []
+    for i in range(2):
+        stream = torch.cuda.Stream()
+        O, ws, q_i = torch.zeros(batch.tokens, 1024, dtype=torch.float16, device="cuda"), torch.empty(size, dtype=torch.uint8, device="cuda"), Q * (i + 1)
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            pkg.paged_attention(q_i, O, pool.cache, batch.batch, ap, ws, stream=stream)
+        graphs.append(graph), outs.append(O), streams.append(stream), keep.append((ws, q_i))
+    for step in range(3):
+        if step == 1:                                                        # one more token each
+            batch.kv = [n + 1 for n in batch.kv]
+            free = [p for p in range(batch.num_pages) if not any(p in row for row in batch.table)]
+            for b, n in enumerate(batch.kv):
+                if (n - 1) % 16 == 0:
+                    batch.table[b][(n - 1) // 16] = free.pop()
+            batch.dev[1].copy_(torch.tensor(batch.kv, dtype=torch.int32))
+            batch.dev[2].copy_(torch.tensor(batch.table, dtype=torch.int32))
+            pkg.cache_write(K, V, pool.cache, batch.batch)
+        if step == 2:                                                        # other lengths altogether
+            batch.kv = [3, 0, 1999, 64]
+            held = list(range(batch.num_pages))
+            batch.table = [[held.pop() for _ in range(125)] for _ in range(4)] if batch.num_pages >= 500 else [[held[(31 * b + i) % len(held)] for i in range(125)] for b in range(4)]
+            batch.dev[1].copy_(torch.tensor(batch.kv, dtype=torch.int32))
+            batch.dev[2].copy_(torch.tensor(batch.table, dtype=torch.int32))
+            pool.k.fill_(0x31), pool.v.fill_(0x29), pool.k_exp.fill_(120), pool.v_exp.fill_(125)
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for i in range(2):
+            check_attention(outs[i], Q * (i + 1), pool, batch, 128 ** -0.5, 1)
+    assert pkg.kernel_status()[0] == 0
+
+
+def test_streams_of_the_caller(pkg):
+    """Write, attention and read on a stream of their own, behind one another without a wait of the host."""
+    stream = torch.cuda.Stream()
+    batch = Batch(pkg, [4000, 100], [4000, 100], 64)
+    for bits in (16, 8):
+        pool = Pool(pkg, batch.num_pages, 4, 64, 128, bits)
+        K, V, Q = _rows(1, 4, batch.tokens, 128), _rows(2, 4, batch.tokens, 128), _rows(3, 4, batch.tokens, 128)
+        torch.cuda.synchronize()
+        pkg.cache_write(K, V, pool.cache, batch.batch, stream=stream)
+        O = _attend(pkg, Q, pool, batch, stream=stream)
+        check_attention(O, Q, pool, batch, 128 ** -0.5, 1)
+
+
+def test_memory_of_the_host_is_refused(pkg):
+    batch = Batch(pkg, [20], [2], 16)
+    pool = Pool(pkg, batch.num_pages, 1, 16, 64, 16)
+    host = torch.zeros(1, 2, 64, dtype=torch.float16)
+    with pytest.raises(pkg.EfaError, match="memory"):
+        pkg.cache_write(host, host, pool.cache, batch.batch)
+    lens = pkg.paged_batch(*(x.cpu() for x in batch.dev), batch.tokens, 2, 20)
+    with pytest.raises(pkg.EfaError, match="memory"):
+        pkg.paged_attention(host.cuda(), torch.zeros(2, 64, dtype=torch.float16, device="cuda"), pool.cache, lens, pkg.paged_attention_params(1, 64))
+
+
+def test_pages_far_into_a_large_pool(pkg):
+    """Offsets of more than 32 bits, in elements and in bytes."""
+    H, page, d = 8, 64, 128
+    for bits, pages in ((16, 70000), (8, 140000)):
+        batch = Batch(pkg, [700, 130], [5, 130], page)
+        far = [[pages - 1 - 17 * (b * batch.width + i) for i in range(batch.width)] for b in range(2)]
+        batch.table, batch.num_pages = far, pages
+        batch.dev[2].copy_(torch.tensor(far, dtype=torch.int32))
+        pool = Pool(pkg, pages, H, page, d, bits)
+        assert pool.k.numel() * (1 if bits == 8 else 2) > 1 << 33
+        fill_random(pool, batch, 1)
+        K, V, Q = _rows(1, H, batch.tokens, d), _rows(2, H, batch.tokens, d), _rows(3, 2 * H, batch.tokens, d)
+        pkg.cache_write(K, V, pool.cache, batch.batch)
+        Ko, Vo = torch.empty_like(K), torch.empty_like(V)
+        pkg.cache_read(Ko, Vo, pool.cache, batch.batch)
+        torch.cuda.synchronize()
+        assert torch.equal(Ko, K if bits == 16 else decode(*encode(K)).half())
+        check_attention(_attend(pkg, Q, pool, batch), Q, pool, batch, d ** -0.5, 1)
+        del pool
+        torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("d_h", [64, 128])
+def test_a_serving_step_end_to_end(pkg, bits, d_h):
+    """Projections, cache, attention and output projection as a server chains them: a prompt, then tokens; against the whole in 64 bits, and against
+    attention over the contiguous keys that the cache gives back."""
+    H, page, tokens = 4, 32, 192
+    d = H * d_h
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    W = [(torch.randn(H, d, d_h, generator=gen, device="cuda") / d ** 0.5).half() for _ in range(3)]
+    W_O = (torch.randn(d, d, generator=gen, device="cuda") / d ** 0.5).half()
+    total = tokens + 64
+    X = torch.randn(total, d, generator=gen, device="cuda").half()
+    pages = -(-total // page)
+    pool = Pool(pkg, pages + 2, H, page, d_h, bits)
+    order = torch.randperm(pages + 2, generator=torch.Generator().manual_seed(2))[:pages].int().cuda()[None].contiguous()
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    outs, at = [], 0
+    for n in (tokens, 64):                                                   # the projections take 64 rows at a time
+        x = X[at:at + n]
+        Qh, Kh, Vh = (torch.empty(H, n, d_h, dtype=torch.float16, device="cuda") for _ in range(3))
+        O, out = (torch.empty(n, d, dtype=torch.float16, device="cuda") for _ in range(2))
+        batch = pkg.paged_batch(i32(0, n), i32(at + n), order, n, n, total)
+        ap = pkg.paged_attention_params(H, d_h)
+        ws = torch.empty(max(16, pkg.paged_attention_workspace(pool.cache, batch, ap)), dtype=torch.uint8, device="cuda")
+        pkg.compute_qkv(x, *W, Qh, Kh, Vh, n, d, H, d_h)
+        pkg.cache_write(Kh, Vh, pool.cache, batch)
+        pkg.paged_attention(Qh, O, pool.cache, batch, ap, ws)
+        pkg.project(O, W_O, out, n, d, d)
+        outs.append((Qh, O, out))
+        at += n
+    whole = pkg.paged_batch(i32(0, total), i32(total), order, total, total, total)
+    K, V = (torch.empty(H, total, d_h, dtype=torch.float16, device="cuda") for _ in range(2))
+    pkg.cache_read(K, V, pool.cache, whole)
+    Q = torch.cat([o[0] for o in outs], 1)
+    O = torch.cat([o[1] for o in outs])
+    torch.cuda.synchronize()
+    ref, tol = attention_ref(Q.double(), K.double(), V.double(), total, total, d_h ** -0.5, 1)
+    ref, tol = (x.transpose(0, 1).reshape(total, d) for x in (ref, tol))
+    assert bool(((O.double() - ref).abs() <= tol).all())
+    contiguous = torch.empty_like(O)
+    fp = pkg.make_params(total, d, H, 64, causal=1).flash_tc
+    pkg.flash_attn_tc_forward(Q, K, V, contiguous, None, 0, total, fp)
+    torch.cuda.synchronize()
+    assert float((contiguous.double() - O.double()).abs().max()) <= 2e-3     # both hold the framework's own gate
+    out = torch.cat([o[2] for o in outs]).double()
+    want = O.double() @ W_O.double()
+    size = O.double().abs() @ W_O.double().abs()
+    assert bool(((out - want).abs() <= 2.0 ** -11 * want.abs() + d * 2.0 ** -23 * size + 2.0 ** -25).all())
+    if bits == 16:                                                           # the cache adds nothing: the block itself
+        k64, v64, q64 = (torch.stack([X.double() @ w[h].double() for h in range(H)]) for w in (W[1], W[2], W[0]))
+        block, _ = attention_ref(q64, k64, v64, total, total, d_h ** -0.5, 1)
+        block = block.transpose(0, 1).reshape(total, d) @ W_O.double()
+        assert float((out - block).abs().max()) <= 1e-2 * float(block.abs().max())
+    assert pkg.kernel_status()[0] == 0
