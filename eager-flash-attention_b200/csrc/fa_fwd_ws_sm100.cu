@@ -47,6 +47,7 @@
 #include "fa_fwd_sm100.cuh"
 #include "fa_args.cuh"
 #include "host_util.h"
+#include "paged_kernels.cuh"
 #include "sm100_ptx.cuh"
 
 #include <algorithm>
@@ -780,6 +781,8 @@ int launch_form(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap&
     return out_f16 ? launch_form<D, true>(tq, tk, tv, a, reserve_sms, stream) : launch_form<D, false>(tq, tk, tv, a, reserve_sms, stream);
 }
 
+#include "paged_chunk.cuh"
+
 template <int D>
 void ring_of(FaPlan& plan, bool halves)
 {
@@ -831,6 +834,16 @@ int fa_forward_ws(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMa
 }
 
 int fa_ws_kv_box_rows() { return WS_BN; }
+
+int paged_chunk_launch(const PagedArgs& c, const PagedAttnArgs& a, int d_h, bool f8, int blocks, cudaStream_t stream)
+{
+    switch (d_h) {
+        case 16:  return f8 ? launch_paged_chunk<16, true>(c, a, blocks, stream) : launch_paged_chunk<16, false>(c, a, blocks, stream);
+        case 32:  return f8 ? launch_paged_chunk<32, true>(c, a, blocks, stream) : launch_paged_chunk<32, false>(c, a, blocks, stream);
+        case 64:  return f8 ? launch_paged_chunk<64, true>(c, a, blocks, stream) : launch_paged_chunk<64, false>(c, a, blocks, stream);
+        default:  return f8 ? launch_paged_chunk<128, true>(c, a, blocks, stream) : launch_paged_chunk<128, false>(c, a, blocks, stream);
+    }
+}
 
 
 namespace {

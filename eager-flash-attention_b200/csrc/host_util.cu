@@ -208,4 +208,21 @@ int make_tmap_f32(CUtensorMap* out, const void* base, int rank, const unsigned l
     return make_tmap(out, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4u, base, rank, dims, strides_bytes, box);
 }
 
+int make_tmap_pages(CUtensorMap* out, const void* base, unsigned elem_bytes, int d_h, unsigned long long page_rows, unsigned long long pages,
+                    unsigned long long page_bytes, unsigned cols, unsigned rows, bool plain)
+{
+    const DriverApi* api = driver_api();
+    if (!api) return 1;
+    const unsigned inner = cols * elem_bytes;
+    if (!plain && inner != 128 && inner != 64 && inner != 32) { set_error("make_tmap_pages: inner box of %u bytes has no swizzle mode", inner); return 1; }
+    const CUtensorMapSwizzle swz = plain ? CU_TENSOR_MAP_SWIZZLE_NONE : inner == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : inner == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                         : CU_TENSOR_MAP_SWIZZLE_32B;
+    const cuuint64_t dims[3] = {(cuuint64_t)d_h, page_rows, pages}, strides[2] = {(cuuint64_t)d_h * elem_bytes, page_bytes};
+    const cuuint32_t box[3] = {cols, rows, 1}, step[3] = {1, 1, 1};
+    const CUresult r = api->cuTensorMapEncodeTiled(out, elem_bytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base),
+                                                   dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, swz, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return check_cu(r, "cuTensorMapEncodeTiled", __FILE__, __LINE__);
+}
+
 }  // namespace efa

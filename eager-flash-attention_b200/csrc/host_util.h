@@ -117,5 +117,9 @@ int make_tmap_f16(CUtensorMap* out, const void* base, int rank,
 // The same over fp32 data.
 int make_tmap_f32(CUtensorMap* out, const void* base, int rank, const unsigned long long* dims,
                   const unsigned long long* strides_bytes, const unsigned* box);
+// Map over the pages of a cache, (column, row of the page, page), elements of one or two bytes, boxes of `cols` x `rows` x 1. plain: without a
+// swizzle. Boxes at a page from `pages` on read as zeros.
+int make_tmap_pages(CUtensorMap* out, const void* base, unsigned elem_bytes, int d_h, unsigned long long page_rows, unsigned long long pages,
+                    unsigned long long page_bytes, unsigned cols, unsigned rows, bool plain);
 
 }  // namespace efa

@@ -222,18 +222,20 @@ int move_rows(const char* what, bool read, const void* K, const void* V, long lo
     }
 }
 
-struct PagedPlan { PagedShape w; int blocks; bool cut; size_t cut_bytes, ml_bytes, o_bytes; };
+struct PagedPlan { PagedShape w; int blocks; bool cut, chunk; size_t cut_bytes, ml_bytes, o_bytes; };
 
 PagedPlan plan_attention(const efa_paged_cache& c, const efa_paged_batch& b, const efa_paged_attention_params& p)
 {
     PagedPlan plan{};
     const int G = p.H_q / c.H_kv;
     const long long rows = (long long)b.max_q * G, kv_cap = std::min<long long>(b.max_kv, (long long)b.max_pages * c.page_size);
-    const int tile = paged_rows_tile((int)std::min<long long>(rows, INT_MAX));
-    plan.w = PagedShape{G, p.causal ? 1 : 0, tile, PAGED_ROWS_UNIT, (int)((rows + tile - 1) / tile)};
-    const long long items = (long long)b.num_seqs * c.H_kv * plan.w.max_tiles, units = std::max<long long>(1, (kv_cap + PAGED_ROWS_UNIT - 1) / PAGED_ROWS_UNIT);
-    const int parts = device_sms() * paged_rows_blocks_per_sm(c.d_h, c.dtype == EFA_E4M3);
-    plan.cut = units > 8 && items > 0;
+    // Rows for which the keys' way to the SM is the time go to the kernel of small tiles, more to the tensor cores' tiles of 256.
+    plan.chunk = rows > 64;
+    const int tile = plan.chunk ? PAGED_CHUNK_TILE : paged_rows_tile((int)rows), unit = plan.chunk ? PAGED_CHUNK_UNIT : PAGED_ROWS_UNIT;
+    plan.w = PagedShape{G, p.causal ? 1 : 0, tile, unit, (int)((rows + tile - 1) / tile)};
+    const long long items = (long long)b.num_seqs * c.H_kv * plan.w.max_tiles, units = std::max<long long>(1, (kv_cap + unit - 1) / unit);
+    const int parts = device_sms() * (plan.chunk ? 1 : paged_rows_blocks_per_sm(c.d_h, c.dtype == EFA_E4M3));
+    plan.cut = plan.chunk || units > 8;
     plan.blocks = (int)std::min<long long>(plan.cut ? std::min<long long>(parts, items * units) : items, INT_MAX);
     if (plan.cut) {
         plan.cut_bytes = ((size_t)plan.blocks * sizeof(PagedCut) + 255) / 256 * 256;
@@ -316,6 +318,7 @@ int paged_attention(const void* Q, void* O, const efa_paged_cache& c, const efa_
     a.q_token = dense ? c.d_h : p.q_token_stride;
     a.o_token = p.o_token_stride ? p.o_token_stride : (long long)p.H_q * c.d_h;
     a.scale_log2e = p.scale * 1.4426950408889634f;
+    a.rescale_above = c.d_h >= 64 ? 8.f : 0.f;             // as the attention over contiguous keys has it
     a.w = plan.w;
     if (plan.cut) {
         uint8_t* at = static_cast<uint8_t*>(workspace);
@@ -323,7 +326,8 @@ int paged_attention(const void* Q, void* O, const efa_paged_cache& c, const efa_
         a.parts.ml = reinterpret_cast<float2*>(at + plan.cut_bytes);
         a.parts.o = reinterpret_cast<float*>(at + plan.cut_bytes + plan.ml_bytes);
     }
-    if (int rc = paged_rows_launch(args, a, c.d_h, c.dtype == EFA_E4M3, plan.blocks, stream)) return rc;
+    const bool f8 = c.dtype == EFA_E4M3;
+    if (int rc = plan.chunk ? paged_chunk_launch(args, a, c.d_h, f8, plan.blocks, stream) : paged_rows_launch(args, a, c.d_h, f8, plan.blocks, stream)) return rc;
     if (!plan.cut || plan.blocks < 2) return 0;
     return paged_merge_launch(args, a, c.d_h, plan.blocks, (int)std::min<long long>(plan.w.tile, (long long)b.max_q * plan.w.G), stream);
 }

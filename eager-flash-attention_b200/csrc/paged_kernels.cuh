@@ -10,7 +10,7 @@ struct PagedAttnArgs {
     const __half* Q;
     __half* O;
     long long q_head, q_token, o_token;     // strides in elements
-    float scale_log2e;
+    float scale_log2e, rescale_above;       // log2 units by which a maximum may outgrow the exponent offset in use (paged_chunk_kernel)
     PagedShape w;
     PagedParts parts;                       // all null: nothing is cut, one block per item
 };
@@ -20,6 +20,10 @@ int paged_rows_tile(int rows);              // rows of a tile for chunks of up t
 constexpr int PAGED_ROWS_UNIT = 64;
 int paged_rows_blocks_per_sm(int d_h, bool f8);
 int paged_rows_launch(const PagedArgs& c, const PagedAttnArgs& a, int d_h, bool f8, int blocks, cudaStream_t stream);
+
+// tcgen05 over tiles of 256 rows (paged_chunk.cuh). Always cuts.
+constexpr int PAGED_CHUNK_TILE = 256, PAGED_CHUNK_UNIT = 128;
+int paged_chunk_launch(const PagedArgs& c, const PagedAttnArgs& a, int d_h, bool f8, int blocks, cudaStream_t stream);
 
 // Merge of the items that the cuts of `blocks` parts go through.
 int paged_merge_launch(const PagedArgs& c, const PagedAttnArgs& a, int d_h, int blocks, int most_rows, cudaStream_t stream);
