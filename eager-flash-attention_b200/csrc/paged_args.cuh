@@ -76,6 +76,11 @@ __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two)
     return r;
 }
 
+__device__ __forceinline__ void e4m3x4_to_f16x4(uint32_t four, uint32_t& lo, uint32_t& hi)
+{
+    asm("{\n.reg .b16 x, y;\nmov.b32 {x, y}, %2;\ncvt.rn.f16x2.e4m3x2 %0, x;\ncvt.rn.f16x2.e4m3x2 %1, y;\n}\n" : "=r"(lo), "=r"(hi) : "r"(four));
+}
+
 __device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b)
 {
     uint32_t r;
@@ -94,18 +99,19 @@ __device__ __forceinline__ uint32_t nonfinite_f16x2(uint32_t x)
 // ---------------------------------------------------------------------------------------------
 // An item is a tile of rows of one sequence and kv head: the rows (token, query head of the group) in that order, `tile` of them
 // at a time, so that all heads of a group, and several tokens, share what is loaded of the keys. Its keys are units of
-// `unit` keys, as many as its last row sees. All units of all items in a row (heads outermost) are cut into as many equal parts as there are
-// blocks: no length of any sequence leaves an SM idle. An item that a cut goes through is merged afterwards (paged_merge_kernel).
+// `unit` keys, as many as its last row sees, and its weight is its units plus `extra` for what an item costs besides them. All items
+// in a row (heads outermost) are cut into as many shares of equal weight as there are blocks: no length of any sequence leaves an SM idle.
+// An item that a cut goes through is merged afterwards (paged_merge_kernel).
 struct PagedShape {
-    int G, causal, tile, unit, max_tiles;   // query heads per kv head; rows of a tile; keys of a unit; tiles of the longest chunk
+    int G, causal, tile, unit, extra, max_tiles;   // query heads per kv head; rows of a tile; keys of a unit; ...; tiles of the longest chunk
 };
 
-__device__ __forceinline__ int paged_tiles(const PagedShape& w, const PagedSeq& s) { return (s.n * w.G + w.tile - 1) / w.tile; }
+__device__ __forceinline__ int paged_tiles(const PagedShape& w, const PagedSeq& s) { return (int)((unsigned)(s.n * w.G + w.tile - 1) / (unsigned)w.tile); }
 
 // Keys that row r of a sequence (token r / G) sees: below this. Not above kv; at most 0: none.
 __device__ __forceinline__ int paged_visible(const PagedShape& w, const PagedSeq& s, int r)
 {
-    return w.causal ? s.kv - s.n + r / w.G + 1 : s.kv;
+    return w.causal ? s.kv - s.n + (int)((unsigned)r / (unsigned)w.G) + 1 : s.kv;
 }
 
 // One unit at least: rows that see nothing are written as well.
@@ -115,8 +121,8 @@ __device__ __forceinline__ int paged_units(const PagedShape& w, const PagedSeq& 
     return max(1, (paged_visible(w, s, last) + w.unit - 1) / w.unit);
 }
 
-// A place in the row of units.
-struct PagedAt { int h, b, rt, off /* units of the item ahead of it */; };
+// A place in the row of items; off: weight of the item ahead of it.
+struct PagedAt { int h, b, rt, off; };
 
 __device__ __forceinline__ void paged_next(const PagedArgs& c, const PagedShape& w, PagedAt& at)
 {
@@ -129,22 +135,37 @@ __device__ __forceinline__ void paged_next(const PagedArgs& c, const PagedShape&
     }
 }
 
-struct PagedScratch { int warp_sum[32]; int total; PagedAt at; };
+// The units [u_lo, u_hi) of the item at `at` that a share with `left` weight from there on has (perhaps none); takes them off `left`.
+struct PagedPiece { PagedSeq q; int h, b, rt, units, u_lo, u_hi; };
+__device__ __forceinline__ PagedPiece paged_piece(const PagedArgs& c, const PagedShape& w, const PagedAt& at, int& left)
+{
+    PagedPiece p;
+    p.q = paged_seq(c, at.b);
+    p.h = at.h; p.b = at.b; p.rt = at.rt;
+    p.units = paged_units(w, p.q, at.rt);
+    const int take = min(p.units + w.extra - at.off, left);
+    p.u_lo = max(0, at.off - w.extra);
+    p.u_hi = max(0, at.off + take - w.extra);
+    left -= take;
+    return p;
+}
 
-// The units [begin, end) of block `part` of `parts` and the place of the first, found by all THREADS threads of a block together. false: there are fewer units
-// than parts, and none for this one.
+struct PagedScratch { int warp_sum[32]; PagedAt at; };
+
+// The weight of share `part` of `parts` and where it begins, found by all THREADS threads of a block together; 0: there is less weight
+// than shares, and none for this one.
 template <int THREADS>
-__device__ bool paged_part(const PagedArgs& c, const PagedShape& w, int part, int parts, PagedScratch& s, int& begin, int& end, PagedAt& at)
+__device__ int paged_part(const PagedArgs& c, const PagedShape& w, int part, int parts, PagedScratch& s, PagedAt& at)
 {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int entries = c.num_seqs * w.max_tiles, per = (entries + THREADS - 1) / THREADS;
+    const int entries = c.num_seqs * w.max_tiles, per = (int)((unsigned)(entries + THREADS - 1) / THREADS);
     const int e0 = min(tid * per, entries), e1 = min(e0 + per, entries);
     int sum = 0;
     for (int e = e0; e < e1; ) {
-        const int b = e / w.max_tiles, rt0 = e - b * w.max_tiles;
+        const int b = (int)((unsigned)e / (unsigned)w.max_tiles), rt0 = e - b * w.max_tiles;
         const PagedSeq q = paged_seq(c, b);
         const int stop = min(paged_tiles(w, q), rt0 + e1 - e);
-        for (int rt = rt0; rt < stop; rt++) sum += paged_units(w, q, rt);
+        for (int rt = rt0; rt < stop; rt++) sum += paged_units(w, q, rt) + w.extra;
         e = (b + 1) * w.max_tiles;
     }
     int before = sum;
@@ -162,20 +183,20 @@ __device__ bool paged_part(const PagedArgs& c, const PagedShape& w, int part, in
         total += s.warp_sum[i];
     }
     before -= sum;
-    const long long all = (long long)total * c.H_kv;
-    parts = (int)min(all, (long long)parts);                // no part without a unit
-    if (part >= parts) return false;
-    begin = (int)(all * part / parts);
-    end = (int)(all * (part + 1) / parts);
-    const int h = begin / total, rest = begin - h * total;
+    const unsigned all = (unsigned)total * (unsigned)c.H_kv;        // below 2^31 (paged_attention_check)
+    parts = (int)min(all, (unsigned)parts);
+    if (part >= parts) return 0;
+    const unsigned each = all / (unsigned)parts, more = all - each * (unsigned)parts;        // the first `more` shares have one more
+    const unsigned begin = (unsigned)part * each + min((unsigned)part, more);
+    const int h = (int)(begin / (unsigned)total), rest = (int)begin - h * total;
     if (rest >= before && rest < before + sum) {
         int left = rest - before;
         for (int e = e0; e < e1; ) {
-            const int b = e / w.max_tiles, rt0 = e - b * w.max_tiles;
+            const int b = (int)((unsigned)e / (unsigned)w.max_tiles), rt0 = e - b * w.max_tiles;
             const PagedSeq q = paged_seq(c, b);
             const int stop = min(paged_tiles(w, q), rt0 + e1 - e);
             for (int rt = rt0; rt < stop; rt++) {
-                const int n = paged_units(w, q, rt);
+                const int n = paged_units(w, q, rt) + w.extra;
                 if (left < n) { s.at = PagedAt{h, b, rt, left}; e = entries; break; }
                 left -= n;
             }
@@ -184,17 +205,17 @@ __device__ bool paged_part(const PagedArgs& c, const PagedShape& w, int part, in
     }
     __syncthreads();
     at = s.at;
-    return true;
+    return (int)each + ((unsigned)part < more ? 1 : 0);
 }
 
-// Where blocks leave their shares of items that a cut goes through: per block two places (its first item, and its last where that is
-// another), each `tile` rows of (maximum in the log2 domain, denominator) and of O without the division; and what the first unit of a block
-// belongs to.
-struct PagedCut { int item_begin /* of all units */, units, begin /* the block's own first unit */, h, b, rt, pad0, pad1; };
+// Where blocks leave their pieces of items that a cut goes through: two places a block, one for the item that its share begins with and one
+// for the other (the last). A place is `tile` rows of (maximum in the log2 domain, denominator), and of O without the division as [d_h / 4][tile] float4, so that
+// neighbouring rows lie side by side for writer and reader.
+struct PagedCut { int h, b, rt, off /* units of that item ahead of the share */, units /* 0: no share */, pad0, pad1, pad2; };
 struct PagedParts {
-    PagedCut* cut;      // [parts]
+    PagedCut* cut;      // [parts]: what each share begins with
     float2* ml;         // [parts][2][tile]
-    float* o;           // [parts][2][tile][d_h]
+    float4* o;          // [parts][2][d_h / 4][tile]
 };
 
 }  // namespace efa

@@ -232,7 +232,7 @@ PagedPlan plan_attention(const efa_paged_cache& c, const efa_paged_batch& b, con
     // Rows for which the keys' way to the SM is the time go to the kernel of small tiles, more to the tensor cores' tiles of 256.
     plan.chunk = rows > 64;
     const int tile = plan.chunk ? PAGED_CHUNK_TILE : paged_rows_tile((int)rows), unit = plan.chunk ? PAGED_CHUNK_UNIT : PAGED_ROWS_UNIT;
-    plan.w = PagedShape{G, p.causal ? 1 : 0, tile, unit, (int)((rows + tile - 1) / tile)};
+    plan.w = PagedShape{G, p.causal ? 1 : 0, tile, unit, plan.chunk ? PAGED_CHUNK_EXTRA : PAGED_ROWS_EXTRA, (int)((rows + tile - 1) / tile)};
     const long long items = (long long)b.num_seqs * c.H_kv * plan.w.max_tiles, units = std::max<long long>(1, (kv_cap + unit - 1) / unit);
     const int parts = device_sms() * (plan.chunk ? 1 : paged_rows_blocks_per_sm(c.d_h, c.dtype == EFA_E4M3));
     plan.cut = plan.chunk || units > 8;
@@ -268,12 +268,12 @@ const char* paged_attention_check(const efa_paged_cache& c, const efa_paged_batc
 {
     if (const char* why = paged_check(c, b)) return why;
     if (p.H_q < 1 || p.H_q % c.H_kv) return "paged: H_q must be a positive multiple of H_kv";
-    if (!std::isfinite(p.scale)) return "paged: scale must be finite";
+    if (!std::isfinite(p.scale) || p.scale <= 0.f) return "paged: scale must be positive and finite";
     if (p.q_head_stride || p.q_token_stride) {
         if (p.q_head_stride < c.d_h || p.q_token_stride < c.d_h || p.q_head_stride % 8 || p.q_token_stride % 8) return "paged: row strides must be multiples of 8 and at least d_h";
     }
     if (p.o_token_stride != 0 && (p.o_token_stride < (long long)p.H_q * c.d_h || p.o_token_stride % 8)) return "paged: o_token_stride must be 0 or a multiple of 8 that holds H_q * d_h";
-    const long long rows = (long long)b.max_q * (p.H_q / c.H_kv), units = ((long long)b.max_kv + 63) / 64 + 1;
+    const long long rows = (long long)b.max_q * (p.H_q / c.H_kv), units = ((long long)b.max_kv + 63) / 64 + 8;
     if (rows > INT_MAX / 2 || (double)b.num_seqs * c.H_kv * ((double)rows / 16 + 1) * (double)units > (double)INT_MAX) return "paged: sizes too large";
     return nullptr;
 }
@@ -324,7 +324,7 @@ int paged_attention(const void* Q, void* O, const efa_paged_cache& c, const efa_
         uint8_t* at = static_cast<uint8_t*>(workspace);
         a.parts.cut = reinterpret_cast<PagedCut*>(at);
         a.parts.ml = reinterpret_cast<float2*>(at + plan.cut_bytes);
-        a.parts.o = reinterpret_cast<float*>(at + plan.cut_bytes + plan.ml_bytes);
+        a.parts.o = reinterpret_cast<float4*>(at + plan.cut_bytes + plan.ml_bytes);
     }
     const bool f8 = c.dtype == EFA_E4M3;
     if (int rc = plan.chunk ? paged_chunk_launch(args, a, c.d_h, f8, plan.blocks, stream) : paged_rows_launch(args, a, c.d_h, f8, plan.blocks, stream)) return rc;

@@ -6,13 +6,18 @@
 //     none, or keys that are not there, are boxes outside the tensor, which read as zeros.
 //   * Where some row of the item does not see some key of a stage (the last stages), values there that are not finite must not meet the weight 0
 //     of such a row: warps 10 and 11 put zeros in their place before the MMA may have the stage, and the rows that do see them add them at the end.
-//   * e4m3: the codes (and exponent bytes) arrive in a small ring of their own, and warps 10 and 11 convert every stage to fp16, exactly.
+//   * e4m3: the codes (and exponent bytes) arrive in a small ring of their own, and four more warps convert every stage to fp16, exactly.
 //   * Work is an equal share of all 128-key units of all items (paged_part), an item at a time; the barriers are rebuilt for each. What a share
 //     has of an item that is cut goes to the workspace, as fp32 O relative to the row's maximum, and is merged afterwards.
 #pragma once
 
 template <int D, bool F8>
 struct ChunkCfg {
+    // Threads: the softmax's 256, a warpgroup of producer, issuer and warps 10 and 11, and for e4m3 another that converts. Registers of each:
+    // together no more than the block is launched with.
+    static constexpr int THREADS    = F8 ? 512 : 384;
+    static constexpr int REG_SOFTMAX = F8 ? 208 : 224, REG_ISSUE = F8 ? 40 : 56, REG_CONVERT = 56;
+    static constexpr int REGS       = 256 * REG_SOFTMAX + 128 * REG_ISSUE + (F8 ? 128 * REG_CONVERT : 0);
     static constexpr int SWB        = D >= 64 ? 128 : D * 2;
     static constexpr int BOXC       = SWB / 2;
     static constexpr int NBOX       = D / BOXC;
@@ -35,6 +40,8 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                  :: "r"(dst), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
 }
+template <int N> __device__ __forceinline__ void setmaxnreg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(N)); }
+template <int N> __device__ __forceinline__ void setmaxnreg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(N)); }
 __device__ __forceinline__ uint4 lds128(uint32_t at)
 {
     uint4 v;
@@ -47,7 +54,7 @@ __device__ __forceinline__ void sts128(uint32_t at, const uint4& v)
 }
 
 template <int D, bool F8>
-__global__ void __launch_bounds__(WS_THREADS, 1)
+__global__ void __launch_bounds__((ChunkCfg<D, F8>::THREADS), 1)
 paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const PagedArgs c, const PagedAttnArgs a)
 {
     using C = ChunkCfg<D, F8>;
@@ -71,9 +78,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     __shared__ uint32_t tmem_base_smem;
     __shared__ int abort_word, poison;
     __shared__ PagedScratch scratch;
-    struct Piece { int h, b, rt, u_lo, u_hi, units, place; PagedSeq q; };
-    __shared__ Piece s_piece;
-    __shared__ int s_more;
+    __shared__ PagedPiece s_piece[2];                   // of this round and the next
+    __shared__ int s_place[2];                          // where it goes if it is not the whole item; -1: no piece, the share is done
 
     const int tid  = threadIdx.x;
     const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
@@ -92,21 +98,31 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     pdl_wait();
     pdl_trigger();
 
-    // ---- this block's share (thread 32 goes through it, an item at a time)
-    int begin = 0, end = 0;
-    PagedAt at{};
-    {
-        const bool any = paged_part<WS_THREADS>(c, a.w, blockIdx.x, gridDim.x, scratch, begin, end, at);
-        if (tid == 32) {
-            PagedCut here{};
-            if (any) here = PagedCut{begin - at.off, paged_units(a.w, paged_seq<true>(c, at.b, 53), at.rt), begin, at.h, at.b, at.rt, 0, 0};
-            a.parts.cut[blockIdx.x] = here;
+    // ---- this block's share: thread FINDER goes through it, a piece ahead of the others
+    constexpr int FINDER = 352;
+    PagedAt at{}, first;
+    int left = paged_part<C::THREADS>(c, a.w, blockIdx.x, gridDim.x, scratch, at);
+    first = at;
+    auto find_piece = [&](int slot) {
+        s_place[slot] = -1;
+        while (left > 0) {
+            const PagedPiece p = paged_piece(c, a.w, at, left);
+            const int other = at.h == first.h && at.b == first.b && at.rt == first.rt ? 0 : 1;
+            if (left > 0) paged_next(c, a.w, at);
+            if (p.u_hi == p.u_lo) continue;
+            s_piece[slot] = p;
+            s_place[slot] = (int)blockIdx.x * 2 + other;
+            return;
         }
-        if (!any) begin = end;
+    };
+    if (tid == FINDER) {
+        PagedCut here{};
+        if (left > 0) here = PagedCut{at.h, at.b, at.rt, max(0, at.off - a.w.extra), paged_units(a.w, paged_seq<true>(c, at.b, 53), at.rt), 0, 0, 0};
+        a.parts.cut[blockIdx.x] = here;
+        find_piece(0);
     }
-    int left = end - begin;
 
-    struct Item { Piece p; int r0, rows_q[2], nblk[2], nblk_max, jm; };
+    struct Item { PagedPiece p; int r0, rows_q[2], nblk[2], nblk_max, jm; };
     auto fetch_item = [&](int round, Item& it) -> bool {
         if (tid == 0) {
             poison = 0;
@@ -123,25 +139,14 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                 mbar_init(&p_full[q][1], WS_BM / 32);
                 mbar_init(&o_done[q], 1);
             }
-            for (int s = 0; s < NSK; s++) { mbar_init(&k_full[s], F8 ? 2 : 1); mbar_init(&k_empty[s], 1); }
-            for (int s = 0; s < NSV; s++) { mbar_init(&v_full[s], F8 ? 2 : 1); mbar_init(&v_empty[s], 1); mbar_init(&v_raw[s], 1); }
-            for (int s = 0; s < NRAW; s++) { mbar_init(&raw_full[s], 1); mbar_init(&raw_empty[s], 2); }
+            for (int s = 0; s < NSK; s++) { mbar_init(&k_full[s], F8 ? 4 : 1); mbar_init(&k_empty[s], 1); }
+            for (int s = 0; s < NSV; s++) { mbar_init(&v_full[s], F8 ? 4 : 2); mbar_init(&v_empty[s], 1); mbar_init(&v_raw[s], 1); }
+            for (int s = 0; s < NRAW; s++) { mbar_init(&raw_full[s], 1); mbar_init(&raw_empty[s], 4); }
             mbar_fence_init();
         }
-        if (tid == 32) {
-            if (round > 0 && left > 0) paged_next(c, a.w, at);
-            s_more = left > 0;
-            if (left > 0) {
-                Piece p{at.h, at.b, at.rt, at.off, 0, 0, (int)blockIdx.x * 2 + (round > 0 ? 1 : 0), paged_seq(c, at.b)};
-                p.units = paged_units(a.w, p.q, at.rt);
-                p.u_hi = min(p.units, at.off + left);
-                left -= p.u_hi - p.u_lo;
-                s_piece = p;
-            }
-        }
         __syncthreads();
-        if (__shfl_sync(0xffffffffu, s_more, 0) == 0 || abort_word != 0) return false;
-        it.p = s_piece;
+        if (__shfl_sync(0xffffffffu, s_place[round & 1], 0) < 0 || abort_word != 0) return false;
+        it.p = s_piece[round & 1];
         it.r0 = it.p.rt * 2 * WS_BM;
         const int rows = it.p.q.n * a.w.G - it.r0;
         #pragma unroll
@@ -164,7 +169,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     };
 
     if (warp >= 8) {
-        setmaxnreg_dec_56();
+        if (warp >= 12) setmaxnreg_dec<C::REG_CONVERT>(); else setmaxnreg_dec<C::REG_ISSUE>();
         for (int round = 0; ; round++) {
             Item it;
             if (!fetch_item(round, it)) break;
@@ -209,8 +214,9 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                         if (colb < C::NBOX) tma_load_3d(sK + sk * C::TILE_BYTES + colb * C::BOX_BYTES + box * box_rows * C::SWB, &tmK, &k_full[sk], colb * C::BOXC, row, page);
                         if (uv > 0) ok = __all_sync(0xffffffffu, mbar_wait(&v_empty[sv], (uint32_t)((uv - 1) & 1), &abort_word, 22));
                         if (!ok) break;
-                        uint64_t* bar = j >= jm ? &v_raw[sv] : &v_full[sv];
+                        uint64_t* bar = j >= jm ? &v_raw[sv] : &v_full[sv];       // v_full: two arrivals, those of warps 10 and 11, or both here
                         if (lane == 0) mbar_expect_tx(bar, C::TILE_BYTES);
+                        if (lane == 0 && j < jm) mbar_arrive(bar);
                         __syncwarp();
                         if (colb < C::NBOX) tma_load_3d(sV + sv * C::TILE_BYTES + colb * C::BOX_BYTES + box * box_rows * C::SWB, &tmV, bar, colb * C::BOXC, row, page);
                     }
@@ -279,8 +285,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                     }
                 }
             } else {
-                // ---- warps 10 and 11: values that are not finite (fp16, where the mask needs it), or all codes to fp16 (e4m3)
-                const int t64 = tid - 320;
+                if (tid == FINDER) find_piece((round + 1) & 1);
+                __syncwarp();
                 bool bad_seen = false;
                 auto clean = [&](uint4& x) {
                     uint32_t* w = &x.x;
@@ -293,30 +299,33 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                 };
                 bool ok = true;
                 if constexpr (F8) {
-                    constexpr int CH = D / 16;                                // 16-byte chunks of a row of codes
-                    for (int n = 0; n < 2 * nblk_max && ok; n++) {
+                    // ---- warps 12 to 15: all codes to fp16. A thread has one 16-byte chunk of RPT rows behind one another, 
+                    constexpr int CH = D / 16, RPT = CH;
+                    const int ch = tid % CH, row0 = (tid & 127) / CH * RPT;
+                    for (int n = 0; n < 2 * nblk_max && ok && warp >= 12; n++) {
                         const int j = n >> 1, isv = n & 1, s = n % NRAW;
                         const int NS = isv ? NSV : NSK, slot = j % NS, use = j / NS;
                         ok = __all_sync(0xffffffffu, mbar_wait(&raw_full[s], (uint32_t)((n / NRAW) & 1), &abort_word, 62));
                         if (use > 0) ok = ok && __all_sync(0xffffffffu, mbar_wait(isv ? &v_empty[slot] : &k_empty[slot], (uint32_t)((use - 1) & 1), &abort_word, 63));
                         if (!ok) break;
                         const uint32_t raw = smem_u32(sRaw + s * C::RAW_BYTES), dst = smem_u32((isv ? sV : sK) + slot * C::TILE_BYTES);
+                        const uint32_t col = dst + (uint32_t)(ch * 16 / C::BOXC) * C::BOX_BYTES, byte = (uint32_t)(ch * 16 % C::BOXC) * 2u;
                         const bool care = isv && j >= jm;
                         #pragma unroll 4
-                        for (int i = 0; i < 128 * CH / 64; i++) {
-                            const int idx = i * 64 + t64, r = idx / CH, ch = idx % CH;
-                            const uint4 x = lds128(raw + idx * 16);
+                        for (int i = 0; i < RPT; i++) {
+                            const uint4 x = lds128(raw + ((row0 + i) * CH + ch) * 16);
                             uint32_t e;
-                            asm volatile("ld.shared.u8 %0, [%1];" : "=r"(e) : "r"(raw + 128 * D + r) : "memory");
+                            asm volatile("ld.shared.u8 %0, [%1];" : "=r"(e) : "r"(raw + 128 * D + row0 + i) : "memory");
                             e = exp_byte_f16x2(e);
-                            uint4 lo = make_uint4(mul_f16x2(e4m3x2_to_f16x2(x.x & 0xffffu), e), mul_f16x2(e4m3x2_to_f16x2(x.x >> 16), e),
-                                                  mul_f16x2(e4m3x2_to_f16x2(x.y & 0xffffu), e), mul_f16x2(e4m3x2_to_f16x2(x.y >> 16), e));
-                            uint4 hi = make_uint4(mul_f16x2(e4m3x2_to_f16x2(x.z & 0xffffu), e), mul_f16x2(e4m3x2_to_f16x2(x.z >> 16), e),
-                                                  mul_f16x2(e4m3x2_to_f16x2(x.w & 0xffffu), e), mul_f16x2(e4m3x2_to_f16x2(x.w >> 16), e));
+                            uint4 lo, hi;
+                            e4m3x4_to_f16x4(x.x, lo.x, lo.y); e4m3x4_to_f16x4(x.y, lo.z, lo.w);
+                            e4m3x4_to_f16x4(x.z, hi.x, hi.y); e4m3x4_to_f16x4(x.w, hi.z, hi.w);
+                            lo = make_uint4(mul_f16x2(lo.x, e), mul_f16x2(lo.y, e), mul_f16x2(lo.z, e), mul_f16x2(lo.w, e));
+                            hi = make_uint4(mul_f16x2(hi.x, e), mul_f16x2(hi.y, e), mul_f16x2(hi.z, e), mul_f16x2(hi.w, e));
                             if (care) { clean(lo); clean(hi); }
-                            const uint32_t col = (uint32_t)(ch * 16 / C::BOXC) * C::BOX_BYTES, byte = (uint32_t)(ch * 16 % C::BOXC) * 2u;
-                            sts128(dst + col + swizzled<C::SWB>((uint32_t)r * C::SWB + byte), lo);
-                            sts128(dst + col + swizzled<C::SWB>((uint32_t)r * C::SWB + byte + 16), hi);
+                            const uint32_t at_row = (uint32_t)(row0 + i) * C::SWB + byte;
+                            sts128(col + swizzled<C::SWB>(at_row), lo);
+                            sts128(col + swizzled<C::SWB>(at_row + 16), hi);
                         }
                         if (care && bad_seen) *(volatile int*)&poison = 1;
                         fence_proxy_async_smem();
@@ -327,6 +336,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                         }
                     }
                 } else {
+                    // ---- warps 10 and 11: values that are not finite, where the mask needs it
+                    const int t64 = tid - 320;
                     for (int j = jm; j < nblk_max && ok; j++) {
                         const int slot = j % NSV;
                         ok = __all_sync(0xffffffffu, mbar_wait(&v_raw[slot], (uint32_t)(((j - jm) / NSV) & 1), &abort_word, 64));
@@ -340,15 +351,15 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                         }
                         if (bad_seen) *(volatile int*)&poison = 1;
                         fence_proxy_async_smem();
-                        asm volatile("bar.sync 2, 64;" ::: "memory");
-                        if (t64 == 0) mbar_arrive(&v_full[slot]);
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&v_full[slot]);
                     }
                 }
             }
             end_item();
         }
     } else {
-        setmaxnreg_inc_224();
+        setmaxnreg_inc<C::REG_SOFTMAX>();
         for (int round = 0; ; round++) {
             Item it;
             if (!fetch_item(round, it)) break;
@@ -357,21 +368,29 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
             const uint32_t tmem_S = tmem_base + q * 128 + lane_base;
             const uint32_t tmem_O = tmem_base + 256 + q * 128 + lane_base;
-            const int my_nblk = it.nblk[q], u_lo = it.p.u_lo, jm = it.jm;
+            const int my_nblk = q ? it.nblk[1] : it.nblk[0], u_lo = it.p.u_lo, jm = it.jm;
             const bool gives_back = (warp & 3) == 0 && lane == 0 && q == (it.nblk[1] > 0 ? 1 : 0);
-            const bool valid = row < it.rows_q[q];
+            const bool valid = row < (q ? it.rows_q[1] : it.rows_q[0]);
             const int r = it.r0 + q * WS_BM + row, token = valid ? r / a.w.G : 0;
             const int sees = valid ? min(a.w.causal ? it.p.q.kv - it.p.q.n + token + 1 : it.p.q.kv, it.p.q.kv) : it.p.q.kv;
             const int head = it.p.h * a.w.G + (valid ? r - token * a.w.G : 0);
 
-            // ---- this thread's row of Q into the tile
+            // ---- the warp's 32 rows of Q into the tile, as many lanes to a row as it has chunks of 16 bytes
             if (my_nblk > 0) {
-                const __half* src = a.Q + (long long)head * a.q_head + (long long)(it.p.q.row0 + token) * a.q_token;
+                const long long off = (long long)head * a.q_head + (long long)(it.p.q.row0 + token) * a.q_token;
                 const uint32_t dst = smem_u32(sQ + q * C::TILE_BYTES);
+                constexpr int CH = D / 8;
+                uint4 x[CH];
                 #pragma unroll
-                for (int ch = 0; ch < D / 8; ch++) {
-                    const uint4 x = valid ? *reinterpret_cast<const uint4*>(src + ch * 8) : make_uint4(0u, 0u, 0u, 0u);
-                    sts128(dst + (uint32_t)(ch * 8 / C::BOXC) * C::BOX_BYTES + swizzled<C::SWB>((uint32_t)row * C::SWB + (uint32_t)(ch * 8 % C::BOXC) * 2u), x);
+                for (int i = 0; i < CH; i++) {
+                    const int rr = (i * 32 + lane) / CH, ch = (i * 32 + lane) % CH;
+                    const long long from = __shfl_sync(0xffffffffu, off, rr);
+                    x[i] = (row & ~31) + rr < (q ? it.rows_q[1] : it.rows_q[0]) ? *reinterpret_cast<const uint4*>(a.Q + from + ch * 8) : make_uint4(0u, 0u, 0u, 0u);
+                }
+                #pragma unroll
+                for (int i = 0; i < CH; i++) {
+                    const int rr = (row & ~31) + (i * 32 + lane) / CH, ch = (i * 32 + lane) % CH;
+                    sts128(dst + (uint32_t)(ch * 8 / C::BOXC) * C::BOX_BYTES + swizzled<C::SWB>((uint32_t)rr * C::SWB + (uint32_t)(ch * 8 % C::BOXC) * 2u), x[i]);
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
@@ -482,13 +501,13 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             }
 
             // ---- epilogue (warps take it as a whole: the loads from tensor memory are collective)
-            if (ok && (warp & 3) * 32 < it.rows_q[q]) {
+            if (ok && (warp & 3) * 32 < (q ? it.rows_q[1] : it.rows_q[0])) {
                 const bool whole = it.p.u_lo == 0 && it.p.u_hi == it.p.units;
                 const bool none = sees <= 0;
                 float mult = none ? 0.f : 1.f / l_run;
                 if (!whole) mult = m_true == kNegInfW ? 1.f : ex2(m_ref - m_true);       // relative to the row's own maximum
-                const long long slot = (long long)it.p.place * (2 * WS_BM) + q * WS_BM + row;
-                if (!whole && valid) a.parts.ml[slot] = make_float2(m_true, l_run * mult);
+                const long long place = s_place[round & 1];
+                if (!whole && valid) a.parts.ml[place * (2 * WS_BM) + q * WS_BM + row] = make_float2(m_true, l_run * mult);
                 const bool patch = *(volatile int*)&poison != 0;
                 const int k0 = (u_lo + jm) * WS_BN, k1 = min(sees, it.p.u_hi * WS_BN);
                 #pragma unroll 1
@@ -527,10 +546,10 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                         dst[0] = w[0];
                         dst[1] = w[1];
                     } else {
-                        float4* dst = reinterpret_cast<float4*>(a.parts.o + slot * D + x * 16);
+                        float4* dst = a.parts.o + (place * (D / 4) + x * 4) * (2 * WS_BM) + q * WS_BM + row;
                         #pragma unroll
                         for (int i = 0; i < 4; i++)
-                            dst[i] = make_float4(__uint_as_float(o[4 * i]) * mult, __uint_as_float(o[4 * i + 1]) * mult,
+                            dst[i * 2 * WS_BM] = make_float4(__uint_as_float(o[4 * i]) * mult, __uint_as_float(o[4 * i + 1]) * mult,
                                                  __uint_as_float(o[4 * i + 2]) * mult, __uint_as_float(o[4 * i + 3]) * mult);
                     }
                 }
@@ -563,7 +582,7 @@ int launch_paged_chunk(const PagedArgs& c, const PagedAttnArgs& a, int blocks, c
         // The registers that the softmax warps take come out of what the block is launched with: with fewer they would wait for ever.
         cudaFuncAttributes attr;
         EFA_CUDA(cudaFuncGetAttributes(&attr, paged_chunk_kernel<D, F8>));
-        if ((attr.numRegs + 7) / 8 * 8 * WS_THREADS < 256 * 224 + 128 * 56) { set_error("attention kernel compiled to %d registers", attr.numRegs); return 1; }
+        if ((attr.numRegs + 7) / 8 * 8 * C::THREADS < C::REGS) { set_error("attention kernel compiled to %d registers", attr.numRegs); return 1; }
         EFA_CUDA(cudaFuncSetAttribute(paged_chunk_kernel<D, F8>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES));
         if (dev >= 0 && dev < 64) configured[dev] = true;
     }
@@ -573,6 +592,6 @@ int launch_paged_chunk(const PagedArgs& c, const PagedAttnArgs& a, int blocks, c
         if (make_tmap_pages(&tm[i], i ? c.v : c.k, F8 ? 1 : 2, D, (unsigned long long)page * c.H_kv, (unsigned long long)c.num_pages,
                             (unsigned long long)c.page_stride, F8 ? D : C::BOXC, (unsigned)box_rows, F8))
             return 1;
-    EFA_CUDA(paged_launch(paged_chunk_kernel<D, F8>, dim3(blocks), WS_THREADS, C::SMEM_BYTES, stream, tm[0], tm[1], c, a));
+    EFA_CUDA(paged_launch(paged_chunk_kernel<D, F8>, dim3(blocks), C::THREADS, C::SMEM_BYTES, stream, tm[0], tm[1], c, a));
     return 0;
 }

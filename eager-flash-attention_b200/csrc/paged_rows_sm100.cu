@@ -16,6 +16,8 @@
 #include "paged_kernels.cuh"
 #include "fa_args.cuh"
 
+#include <climits>
+
 namespace efa {
 
 namespace {
@@ -105,35 +107,33 @@ paged_rows_kernel(const PagedArgs c, const PagedAttnArgs a)
     pdl_wait();
     pdl_trigger();
 
-    int begin = 0, end = 1;
-    PagedAt at;
+    PagedAt at, first;
+    int left;
     const bool cut = a.parts.cut != nullptr;
     if (cut) {
-        const bool any = paged_part<PR_THREADS>(c, a.w, blockIdx.x, gridDim.x, scratch, begin, end, at);
+        left = paged_part<PR_THREADS>(c, a.w, blockIdx.x, gridDim.x, scratch, at);
+        first = at;
         if (tid == 0) {
             PagedCut here{};
-            if (any) here = PagedCut{begin - at.off, paged_units(a.w, paged_seq<true>(c, at.b, 51), at.rt), begin, at.h, at.b, at.rt, 0, 0};
+            if (left > 0) here = PagedCut{at.h, at.b, at.rt, max(0, at.off - a.w.extra), paged_units(a.w, paged_seq<true>(c, at.b, 51), at.rt), 0, 0, 0};
             a.parts.cut[blockIdx.x] = here;
         }
-        if (!any) return;
     } else {
         const int per = c.H_kv * a.w.max_tiles, b = blockIdx.x / per, rest = blockIdx.x - b * per;
-        at = PagedAt{rest % c.H_kv, b, rest / c.H_kv, 0};
-        const PagedSeq q = paged_seq(c, b);
+        at = first = PagedAt{rest % c.H_kv, b, rest / c.H_kv, 0};
         if (tid == 0 && rest == 0) paged_seq<true>(c, b, 51);
-        if (at.rt >= paged_tiles(a.w, q)) return;
-        end = paged_units(a.w, q, at.rt);
+        left = at.rt < paged_tiles(a.w, paged_seq(c, b)) ? INT_MAX : 0;
     }
 
     const uint32_t ring = smem_u32(smem_rows) + team * C::STAGE;       // stage s of this team: + s * UNIT_BYTES
 
-    bool first = true;
-    for (int left = end - begin; left > 0; paged_next(c, a.w, at), first = false) {
-        const PagedSeq q = paged_seq(c, at.b);
-        const int units = paged_units(a.w, q, at.rt);
-        const int u_lo = at.off, u_hi = min(units, at.off + left);
-        left -= u_hi - u_lo;
-        const bool whole = u_hi - u_lo == units;
+    for (; left > 0; paged_next(c, a.w, at)) {
+        const PagedPiece piece = paged_piece(c, a.w, at, left);
+        const PagedSeq& q = piece.q;
+        const int u_lo = piece.u_lo, u_hi = piece.u_hi;
+        const bool whole = u_lo == 0 && u_hi == piece.units;
+        if (!cut) left = 0;
+        if (u_hi == u_lo) continue;
         const int rows = min(C::TILE, q.n * a.w.G - at.rt * C::TILE), r0 = at.rt * C::TILE;      // of the item
 
         // ---- the asynchronous copies of a unit: this warp's 16 keys of the team's
@@ -362,9 +362,9 @@ paged_rows_kernel(const PagedArgs c, const PagedAttnArgs a)
             for (int j = 0; j < NT; j++) { dst[column(j, 0)] = o[j][half * 2]; dst[column(j, 1)] = o[j][half * 2 + 1]; }
         }
         __syncthreads();
-        const int place = (int)blockIdx.x * 2 + (first ? 0 : 1);
+        const int place = (int)blockIdx.x * 2 + (at.h == first.h && at.b == first.b && at.rt == first.rt ? 0 : 1);
         for (int e = tid; e < rows * (D / 8); e += PR_THREADS) {
-            const int rr = e / (D / 8), col = (e % (D / 8)) * 8;
+            const int rr = whole ? e / (D / 8) : e % rows, col = (whole ? e % (D / 8) : e / rows) * 8;
             float top = -INFINITY, sum = 0.f, acc[8] = {};
             #pragma unroll
             for (int i = 0; i < C::TEAMS; i++) top = fmaxf(top, sml[i * C::TILE + rr].x);
@@ -387,76 +387,106 @@ paged_rows_kernel(const PagedArgs c, const PagedAttnArgs a)
                 for (int x = 0; x < 4; x++) w[x] = none ? 0u : pack_f16x2(acc[2 * x] * inv, acc[2 * x + 1] * inv);
                 *reinterpret_cast<uint4*>(a.O + (long long)(q.row0 + token) * a.o_token + (long long)(at.h * a.w.G + r - token * a.w.G) * D + col) = out;
             } else {
-                const long long slot = (long long)place * C::TILE + rr;
-                float4* dst = reinterpret_cast<float4*>(a.parts.o + slot * D + col);
+                float4* dst = a.parts.o + ((long long)place * (D / 4) + col / 4) * C::TILE + rr;
                 dst[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
-                dst[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
-                if (col == 0) a.parts.ml[slot] = make_float2(top, sum);
+                dst[C::TILE] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+                if (col == 0) a.parts.ml[(long long)place * C::TILE + rr] = make_float2(top, sum);
             }
         }
         __syncthreads();
-        if (left <= 0) break;
+        if (left <= 0) break;          // not on to an item that is not there
     }
 }
 
 // Merge of what the blocks left of the items that a cut goes through (PagedCut), over the pieces i of an item:
 //     O = sum_i 2^(m_i - max m) O_i / sum_i 2^(m_i - max m) l_i.
-// Block (x, y) looks at the cut ahead of part x + 1: if it is the first in its item it merges the item's rows 4y .. 4y + 3, a warp each.
-template <int D>
-__global__ void __launch_bounds__(128)
+// Blocks (x, .) look at the beginning of share x + 1: where that is the first cut through its item they merge the item, a thread eight columns of
+// a row at a time. Bound by the latency of the pieces' loads: BATCH pieces are asked for at once, and PG threads share a row's pieces where an item may
+// be cut into many.
+constexpr int PM_THREADS = 256;
+template <int D, int PG>
+__global__ void __launch_bounds__(PM_THREADS)
 paged_merge_kernel(const PagedArgs c, const PagedAttnArgs a, int parts)
 {
+    constexpr int BATCH = PG > 1 ? 4 : 2;
+    __shared__ float sm_acc[PG > 1 ? (PG - 1) * (PM_THREADS / PG) : 1][11];
     pdl_wait();
     pdl_trigger();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int part = blockIdx.x + 1;
-    const PagedCut here = a.parts.cut[part];
-    const int ahead = a.parts.cut[part - 1].begin;         // where the part before it begins
-    if (here.begin <= here.item_begin || ahead > here.item_begin) return;     // not inside an item, or not the first in it
+    const PagedCut here = a.parts.cut[part], ahead = a.parts.cut[part - 1];
+    auto same = [&](const PagedCut& x) { return x.units > 0 && x.h == here.h && x.b == here.b && x.rt == here.rt; };
+    if (here.off == 0 || (same(ahead) && ahead.off > 0)) return;     // no cut, or not the item's first
     const PagedSeq q = paged_seq(c, here.b);
-    const int rr = blockIdx.y * 4 + warp, r = here.rt * a.w.tile + rr;
-    if (rr >= a.w.tile || r >= q.n * a.w.G) return;
-    const int stop = here.item_begin + here.units;         // unit behind the item
-    const int sees = min(paged_visible(a.w, q, r), q.kv);
+    const int tile = a.w.tile, rows = min(tile, q.n * a.w.G - here.rt * tile);
+    // Piece 0 is the one of share part - 1, piece i that of share part - 1 + i, which begins inside the item.
+    int pieces = 2, more;
+    do {
+        const int next = part - 1 + pieces + (int)threadIdx.x;
+        more = __syncthreads_count(next < parts && same(a.parts.cut[next]));
+        pieces += more;
+    } while (more == PM_THREADS);
+    const int place0 = (part - 1) * 2 + (same(ahead) ? 0 : 1);
+    const int group = threadIdx.x / (PM_THREADS / PG), local = threadIdx.x % (PM_THREADS / PG);
 
-    // Pieces: part - 1 (its last item, unless it begins with it), then the first item of part, part + 1, ...
-    const int first_place = (part - 1) * 2 + (ahead < here.item_begin ? 1 : 0);
-    auto place_of = [&](int i) { return i == 0 ? first_place : (part - 1 + i) * 2; };
-    auto exists = [&](int i) -> bool { return i == 0 || (part - 1 + i < parts && a.parts.cut[part - 1 + i].begin < stop && a.parts.cut[part - 1 + i].units > 0); };
-    float top = -INFINITY;
-    int n = 0;
-    for (int i0 = 0; ; i0 += 32) {
-        const bool is = exists(i0 + lane);
-        const float m = is ? a.parts.ml[(long long)place_of(i0 + lane) * a.w.tile + rr].x : -INFINITY;
-        float mx = m;
-        #pragma unroll
-        for (int d = 16; d > 0; d /= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-        top = fmaxf(top, mx);
-        const int here_n = __popc(__ballot_sync(0xffffffffu, is));
-        n += here_n;
-        if (here_n < 32) break;
-    }
-    constexpr int COLS = D >= 128 ? 4 : D >= 64 ? 2 : 1;   // columns of a lane
-    const int col = lane * COLS;
-    float acc[COLS] = {}, sum = 0.f;
-    if (col < D || D >= 32) {
-        for (int i = 0; i < n; i++) {
-            const long long slot = (long long)place_of(i) * a.w.tile + rr;
-            const float2 ml = a.parts.ml[slot];
-            const float w = ml.x == top ? 1.f : ex2(ml.x - top);
-            sum += w * ml.y;
-            const float* src = a.parts.o + slot * D + col;
-            if (col < D) {
+    for (int x = blockIdx.y * (PM_THREADS / PG) + local; x - local < rows * (D / 8); x += gridDim.y * (PM_THREADS / PG)) {
+        const bool mine = x < rows * (D / 8);
+        const int rr = mine ? x % rows : 0, col = mine ? x / rows * 8 : 0;
+        float top = -INFINITY, sum = 0.f, acc[8] = {};
+        for (int i0 = group; i0 < pieces && mine; i0 += PG * BATCH) {
+            float2 ml[BATCH];
+            float4 o[BATCH][2];
+            #pragma unroll
+            for (int k = 0; k < BATCH; k++) {
+                const int i = min(i0 + k * PG, pieces - 1);
+                const long long place = i == 0 ? place0 : (part - 1 + i) * 2;
+                ml[k] = __ldcg(a.parts.ml + place * tile + rr);
+                const float4* src = a.parts.o + (place * (D / 4) + col / 4) * tile + rr;
+                o[k][0] = __ldcg(src);
+                o[k][1] = __ldcg(src + tile);
+            }
+            #pragma unroll
+            for (int k = 0; k < BATCH; k++) {
+                if (i0 + k * PG >= pieces) break;
+                const float m = fmaxf(top, ml[k].x), old = top == m ? 1.f : ex2(top - m), w = ml[k].x == m ? 1.f : ex2(ml[k].x - m);
+                const float* v = &o[k][0].x;
+                top = m;
+                sum = sum * old + w * ml[k].y;
                 #pragma unroll
-                for (int x = 0; x < COLS; x++) acc[x] += w * src[x];
+                for (int y = 0; y < 8; y++) acc[y] = acc[y] * old + w * v[y];
             }
         }
+        if constexpr (PG > 1) {
+            float* to = sm_acc[group > 0 ? (group - 1) * (PM_THREADS / PG) + local : 0];
+            if (group > 0) {
+                to[0] = top; to[1] = sum;
+                #pragma unroll
+                for (int y = 0; y < 8; y++) to[2 + y] = acc[y];
+            }
+            __syncthreads();
+            if (group == 0) {
+                #pragma unroll
+                for (int k = 0; k < PG - 1; k++) {
+                    if (k + 1 >= pieces) break;
+                    const float* v = sm_acc[k * (PM_THREADS / PG) + local];
+                    const float m = fmaxf(top, v[0]), old = top == m ? 1.f : ex2(top - m), w = v[0] == m ? 1.f : ex2(v[0] - m);
+                    top = m;
+                    sum = sum * old + w * v[1];
+                    #pragma unroll
+                    for (int y = 0; y < 8; y++) acc[y] = acc[y] * old + w * v[2 + y];
+                }
+            }
+            __syncthreads();
+        }
+        if (!mine || group > 0) continue;
+        const int r = here.rt * tile + rr, token = r / a.w.G;
+        const bool none = paged_visible(a.w, q, r) <= 0;
+        const float inv = 1.f / sum;
+        uint4 out;
+        uint32_t* w = &out.x;
+        #pragma unroll
+        for (int y = 0; y < 4; y++) w[y] = none ? 0u : pack_f16x2(acc[2 * y] * inv, acc[2 * y + 1] * inv);
+        *reinterpret_cast<uint4*>(a.O + (long long)(q.row0 + token) * a.o_token + (long long)(here.h * a.w.G + r - token * a.w.G) * D + col) = out;
     }
-    if (col >= D) return;
-    const int token = r / a.w.G;
-    __half* dst = a.O + (long long)(q.row0 + token) * a.o_token + (long long)(here.h * a.w.G + r - token * a.w.G) * D + col;
-    #pragma unroll
-    for (int x = 0; x < COLS; x++) dst[x] = __float2half_rn(sees <= 0 ? 0.f : acc[x] / sum);
 }
 
 template <int D, bool F8, int WM>
@@ -500,16 +530,24 @@ int paged_rows_launch(const PagedArgs& c, const PagedAttnArgs& a, int d_h, bool 
     }
 }
 
+template <int D>
+static int launch_merge(const PagedArgs& c, const PagedAttnArgs& a, int blocks, int most_rows, cudaStream_t stream)
+{
+    // Tiles of few rows may be in hundreds of pieces, tiles of 256 rows mostly are in two or three.
+    const int units = most_rows * (D / 8);
+    if (a.w.tile <= 64) EFA_CUDA(paged_launch(paged_merge_kernel<D, 4>, dim3(blocks - 1, (units + 63) / 64), PM_THREADS, 0, stream, c, a, blocks));
+    else EFA_CUDA(paged_launch(paged_merge_kernel<D, 1>, dim3(blocks - 1, (units + 511) / 512), PM_THREADS, 0, stream, c, a, blocks));
+    return 0;
+}
+
 int paged_merge_launch(const PagedArgs& c, const PagedAttnArgs& a, int d_h, int blocks, int most_rows, cudaStream_t stream)
 {
-    const dim3 grid(blocks - 1, (most_rows + 3) / 4);
     switch (d_h) {
-        case 16:  EFA_CUDA(paged_launch(paged_merge_kernel<16>, grid, 128, 0, stream, c, a, blocks)); break;
-        case 32:  EFA_CUDA(paged_launch(paged_merge_kernel<32>, grid, 128, 0, stream, c, a, blocks)); break;
-        case 64:  EFA_CUDA(paged_launch(paged_merge_kernel<64>, grid, 128, 0, stream, c, a, blocks)); break;
-        default:  EFA_CUDA(paged_launch(paged_merge_kernel<128>, grid, 128, 0, stream, c, a, blocks)); break;
+        case 16:  return launch_merge<16>(c, a, blocks, most_rows, stream);
+        case 32:  return launch_merge<32>(c, a, blocks, most_rows, stream);
+        case 64:  return launch_merge<64>(c, a, blocks, most_rows, stream);
+        default:  return launch_merge<128>(c, a, blocks, most_rows, stream);
     }
-    return 0;
 }
 
 }  // namespace efa

@@ -57,7 +57,7 @@ def test_batches_that_are_refused(pkg, change, why):
 
 
 @pytest.mark.parametrize("change,why", [
-    (dict(H_q=0), "H_q"), (dict(H_q=12), "H_q"), (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"),
+    (dict(H_q=0), "H_q"), (dict(H_q=12), "H_q"), (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"), (dict(scale=0.0), "scale"), (dict(scale=-0.1), "scale"),
     (dict(q_head_stride=640), "strides"), (dict(q_head_stride=640, q_token_stride=132), "strides"), (dict(q_head_stride=64, q_token_stride=128), "strides"),
     (dict(o_token_stride=1016), "o_token_stride"), (dict(o_token_stride=1028), "o_token_stride")])
 def test_attention_parameters_that_are_refused(pkg, change, why):
