@@ -231,11 +231,11 @@ PagedPlan plan_attention(const efa_paged_cache& c, const efa_paged_batch& b, con
     const long long rows = (long long)b.max_q * G, kv_cap = std::min<long long>(b.max_kv, (long long)b.max_pages * c.page_size);
     // Rows for which the keys' way to the SM is the time go to the kernel of small tiles, more to the tensor cores' tiles of 256.
     plan.chunk = rows > 64;
-    const int tile = plan.chunk ? PAGED_CHUNK_TILE : paged_rows_tile((int)rows), unit = plan.chunk ? PAGED_CHUNK_UNIT : PAGED_ROWS_UNIT;
+    const int tile = plan.chunk ? PAGED_CHUNK_TILE : paged_rows_tile((int)rows), unit = plan.chunk ? PAGED_CHUNK_UNIT : paged_rows_unit(c.dtype == EFA_E4M3);
     plan.w = PagedShape{G, p.causal ? 1 : 0, tile, unit, plan.chunk ? PAGED_CHUNK_EXTRA : PAGED_ROWS_EXTRA, (int)((rows + tile - 1) / tile)};
     const long long items = (long long)b.num_seqs * c.H_kv * plan.w.max_tiles, units = std::max<long long>(1, (kv_cap + unit - 1) / unit);
     const int parts = device_sms() * (plan.chunk ? 1 : paged_rows_blocks_per_sm(c.d_h, c.dtype == EFA_E4M3));
-    plan.cut = plan.chunk || units > 8;
+    plan.cut = plan.chunk || units * unit > 512;
     plan.blocks = (int)std::min<long long>(plan.cut ? std::min<long long>(parts, items * units) : items, INT_MAX);
     if (plan.cut) {
         plan.cut_bytes = ((size_t)plan.blocks * sizeof(PagedCut) + 255) / 256 * 256;

@@ -17,7 +17,8 @@ struct PagedAttnArgs {
 
 // mma.sync over tiles of up to 64 rows (paged_rows_sm100.cu).
 int paged_rows_tile(int rows);              // rows of a tile for chunks of up to `rows` rows (tokens x heads of a group)
-constexpr int PAGED_ROWS_UNIT = 64, PAGED_ROWS_EXTRA = 1;
+constexpr int PAGED_ROWS_EXTRA = 1;
+int paged_rows_unit(bool f8);               // keys of a unit
 int paged_rows_blocks_per_sm(int d_h, bool f8);
 int paged_rows_launch(const PagedArgs& c, const PagedAttnArgs& a, int d_h, bool f8, int blocks, cudaStream_t stream);
 

@@ -12,7 +12,7 @@
 //
 // fp16 keys reach the registers by ldmatrix. Codes of e4m3 are read as 16 bytes of a key per thread and converted there (exactly): the order of
 // the head's elements in Q K^T, and that of O's columns, is then each thread's own, and Q's fragments and the stores follow it. The exponents of keys
-// multiply the scores; those of values multiply the converted values, which is exact too.
+// multiply the scores, those of values the weights.
 #include "paged_kernels.cuh"
 #include "fa_args.cuh"
 
@@ -26,7 +26,9 @@ constexpr int PR_THREADS = 128;
 
 template <int D, bool F8, int WM>
 struct RowsCfg {
-    static constexpr int TEAMS = 4 / WM, TILE = 16 * WM, KS = 16 * WM;       // a team's keys of a unit
+    static constexpr int WK = F8 ? 32 : 16;                                   // keys that a warp copies of a unit
+    static constexpr int TEAMS = 4 / WM, TILE = 16 * WM, KS = WK * WM, UNIT = KS * TEAMS;       // rows; a team's keys of a unit; keys of a unit
+    static constexpr int STEP = KS >= 32 ? 2 : 1;                             // 16-key blocks to a step of the softmax
     static constexpr int RB = D * (F8 ? 1 : 2);                               // bytes of a key
     static constexpr int STAGE = 2 * KS * RB + (F8 ? 2 * KS : 0);             // of a team
     static constexpr int UNIT_BYTES = TEAMS * STAGE;
@@ -81,11 +83,18 @@ __device__ __forceinline__ void load_words(uint32_t addr, uint32_t (&w)[4])
     if constexpr (BYTES == 2) asm volatile("{\n.reg .b16 x;\nld.shared.b16 x, [%1];\ncvt.u32.u16 %0, x;\n}\n" : "=r"(w[0]) : "r"(addr) : "memory");
 }
 
-__device__ __forceinline__ unsigned load_byte(uint32_t addr)
+__device__ __forceinline__ uint32_t load_half(uint32_t addr)
 {
-    uint32_t x;
-    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(x) : "r"(addr) : "memory");
-    return x;
+    uint32_t w[4];
+    load_words<2>(addr, w);
+    return w[0];
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c)
+{
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
 }
 
 template <int D, bool F8, int WM>
@@ -136,32 +145,43 @@ paged_rows_kernel(const PagedArgs c, const PagedAttnArgs a)
         if (u_hi == u_lo) continue;
         const int rows = min(C::TILE, q.n * a.w.G - at.rt * C::TILE), r0 = at.rt * C::TILE;      // of the item
 
-        // ---- the asynchronous copies of a unit: this warp's 16 keys of the team's
-        int page_of = 0, page_from = u_lo - 32;            // lane l: page of this warp's keys in unit page_from + l
+        // ---- the asynchronous copies of a unit: this warp's WK keys of the team's, 16 at a time (they are in one page)
+        int page_of = 0, page_from = u_lo - 32;            // lane l: page of 16 keys, WK / 16 lanes to a unit from unit page_from on
+        const int first_key = team * KS + mrow * C::WK;
+        constexpr int PER = C::WK / 16, AHEAD = 32 / PER;
+        uint32_t to[PER][(RB + 31) / 32];                  // where this lane's chunks go in a stage
+        #pragma unroll
+        for (int x = 0; x < PER; x++)
+            #pragma unroll
+            for (int i = 0; i < (RB + 31) / 32; i++) to[x][i] = ring + rows_swizzled<RB>(mrow * C::WK + x * 16 + (i * 32 + lane) / (RB / 16), (i * 32 + lane) % (RB / 16));
         auto load = [&](int u) {
             if (u < u_hi) {
-                if (u - page_from >= 32) {
+                if (u - page_from >= AHEAD) {
                     page_from = u;
-                    const int key = (u + lane) * PAGED_ROWS_UNIT + team * KS + mrow * 16;
-                    page_of = key < q.kv && u + lane < u_hi ? paged_page(c, at.b, key, 52) : -1;
+                    const int un = u + lane / PER, key = un * C::UNIT + first_key + lane % PER * 16;
+                    page_of = key < q.kv && un < u_hi ? paged_page(c, at.b, key, 52) : -1;
                 }
-                const int page = __shfl_sync(0xffffffffu, page_of, u - page_from);
-                const int key = u * PAGED_ROWS_UNIT + team * KS + mrow * 16;
-                const int there = page >= 0 ? q.kv - key : 0;                     // keys that exist
-                const uint32_t dst = ring + ((u - u_lo) % C::STAGES) * C::UNIT_BYTES;
-                const int row = (at.h << c.page_shift) + (key & ((1 << c.page_shift) - 1));
-                const long long src = (long long)max(page, 0) * c.page_stride + (long long)row * RB;
+                const uint32_t stage = ((u - u_lo) % C::STAGES) * C::UNIT_BYTES;
                 #pragma unroll
-                for (int i = 0; i < (RB + 31) / 32; i++) {
-                    const int idx = i * 32 + lane, r = idx / (RB / 16), ch = idx % (RB / 16);
-                    if (RB < 32 && idx >= RB) break;
-                    const uint32_t to = dst + rows_swizzled<RB>(mrow * 16 + r, ch);
-                    copy16(to, c.k + src + idx * 16, r < there);
-                    copy16(to + KS * RB, c.v + src + idx * 16, r < there);
-                }
-                if (F8 && lane < 2) {
-                    const long long e = ((long long)max(page, 0) * c.H_kv << c.page_shift) + row;
-                    copy16(dst + 2 * KS * RB + lane * KS + mrow * 16, (lane ? c.v_exp : c.k_exp) + e, there > 0);
+                for (int x = 0; x < PER; x++) {
+                    const int page = __shfl_sync(0xffffffffu, page_of, (u - page_from) * PER + x);
+                    const int key = u * C::UNIT + first_key + x * 16;
+                    const int there = page >= 0 ? q.kv - key : 0;                 // keys that exist
+                    const int row = (at.h << c.page_shift) + (key & ((1 << c.page_shift) - 1));
+                    const long long src = (long long)max(page, 0) * c.page_stride + (long long)row * RB + lane * 16;
+                    const uint8_t* ks = c.k + src;
+                    const uint8_t* vs = c.v + src;
+                    #pragma unroll
+                    for (int i = 0; i < (RB + 31) / 32; i++) {
+                        const bool is = (i * 32 + lane) / (RB / 16) < there;
+                        if (RB < 32 && lane >= RB) break;
+                        copy16(to[x][i] + stage, ks + i * 512, is);
+                        copy16(to[x][i] + stage + KS * RB, vs + i * 512, is);
+                    }
+                    if (F8 && lane < 2) {
+                        const long long e = ((long long)max(page, 0) * c.H_kv << c.page_shift) + row;
+                        copy16(ring + stage + 2 * KS * RB + lane * KS + mrow * C::WK + x * 16, (lane ? c.v_exp : c.k_exp) + e, there > 0);
+                    }
                 }
             }
             copy_commit();
@@ -206,60 +226,80 @@ paged_rows_kernel(const PagedArgs c, const PagedAttnArgs a)
             else asm volatile("bar.sync %0, %1;" :: "r"(1 + team), "n"(32 * WM) : "memory");
             load(u + C::STAGES - 1);
             const uint32_t sk = ring + ((u - u_lo) % C::STAGES) * C::UNIT_BYTES, sv = sk + KS * RB, se = sv + KS * RB;
+            constexpr int STEP = C::STEP, KT = 2 * STEP;   // key tiles of 8 in a step
             #pragma unroll 1
-            for (int blk = 0; blk < WM; blk++) {
-                const int key0 = u * PAGED_ROWS_UNIT + team * KS + blk * 16;
+            for (int blk = 0; blk < KS / 16; blk += STEP) {
+                const int key0 = u * C::UNIT + team * KS + blk * 16;
                 if (key0 >= q.kv) break;
-                // ---- S = Q K^T, 16 rows x 16 keys
-                float s[2][4] = {};
+                // ---- S = Q K^T, 16 rows x KT * 8 keys
+                float s[KT][4] = {};
                 if constexpr (F8) {
                     #pragma unroll
-                    for (int nt = 0; nt < 2; nt++)
+                    for (int nt = 0; nt < KT; nt++)
                         #pragma unroll
                         for (int i = 0; i < D / (4 * EB); i++) {
                             uint32_t w[4];
                             const int byte = (t + 4 * i) * EB;
                             load_words<EB>(sk + rows_swizzled<RB>(blk * 16 + nt * 8 + g, byte >> 4) + (byte & 15), w);
                             #pragma unroll
-                            for (int x = 0; x < EB / 4; x++)
-                                mma16816(s[nt], qf[i * (EB / 4) + x], e4m3x2_to_f16x2(w[x] & 0xffffu), e4m3x2_to_f16x2(w[x] >> 16));
+                            for (int x = 0; x < EB / 4; x++) {
+                                uint32_t b0, b1;
+                                e4m3x4_to_f16x4(w[x], b0, b1);
+                                mma16816(s[nt], qf[i * (EB / 4) + x], b0, b1);
+                            }
                         }
                 } else {
                     #pragma unroll
-                    for (int st = 0; st < KSTEPS; st++) {
-                        uint32_t w[4];
-                        ldsm4(sk + rows_swizzled<RB>(blk * 16 + (lane & 7) + ((lane >> 4) << 3), st * 2 + ((lane >> 3) & 1)), w);
-                        mma16816(s[0], qf[st], w[0], w[1]);
-                        mma16816(s[1], qf[st], w[2], w[3]);
-                    }
+                    for (int st = 0; st < KSTEPS; st++)
+                        #pragma unroll
+                        for (int y = 0; y < STEP; y++) {
+                            uint32_t w[4];
+                            ldsm4(sk + rows_swizzled<RB>((blk + y) * 16 + (lane & 7) + ((lane >> 4) << 3), st * 2 + ((lane >> 3) & 1)), w);
+                            mma16816(s[2 * y], qf[st], w[0], w[1]);
+                            mma16816(s[2 * y + 1], qf[st], w[2], w[3]);
+                        }
                 }
                 // ---- softmax; this thread has keys key0 + nt * 8 + t * 2 + {0, 1} of rows g (s[.][0..1]) and g + 8
-                const bool masked = key0 + 16 > all_see;
-                uint32_t vexp[2][2];
+                float vscale[KT][2], vlog[KT][2];          // e4m3: 2^exponent of the values, and the exponent
                 #pragma unroll
-                for (int nt = 0; nt < 2; nt++)
-                    #pragma unroll
-                    for (int x = 0; x < 2; x++) {
-                        float f = a.scale_log2e;
-                        if constexpr (F8) {
-                            const int kk = blk * 16 + nt * 8 + t * 2 + x;
-                            f *= exp_byte_f32(load_byte(se + kk));
-                            vexp[nt][x] = exp_byte_f16x2(load_byte(se + KS + kk));
-                        }
-                        #pragma unroll
-                        for (int half = 0; half < 2; half++) {
-                            float& e = s[nt][half * 2 + x];
-                            e *= f;
-                            if (masked && key0 + nt * 8 + t * 2 + x >= min(sees[half], q.kv)) e = -INFINITY;
-                        }
+                for (int nt = 0; nt < KT; nt++) {
+                    float f0 = a.scale_log2e, f1 = f0;
+                    if constexpr (F8) {
+                        const uint32_t ke = load_half(se + blk * 16 + nt * 8 + t * 2), ve = load_half(se + KS + blk * 16 + nt * 8 + t * 2);
+                        f0 *= exp_byte_f32(ke & 0xffu);
+                        f1 *= exp_byte_f32(ke >> 8);
+                        vscale[nt][0] = exp_byte_f32(ve & 0xffu);
+                        vscale[nt][1] = exp_byte_f32(ve >> 8);
+                        vlog[nt][0] = (float)(int)(ve & 0xffu) - 127.f;
+                        vlog[nt][1] = (float)(int)(ve >> 8) - 127.f;
                     }
+                    s[nt][0] *= f0; s[nt][1] *= f1; s[nt][2] *= f0; s[nt][3] *= f1;
+                }
+                const bool masked = key0 + STEP * 16 > all_see;
+                if (masked) {
+                    #pragma unroll
+                    for (int nt = 0; nt < KT; nt++)
+                        #pragma unroll
+                        for (int x = 0; x < 4; x++)
+                        {
+                            const int key = key0 + nt * 8 + t * 2 + (x & 1);
+                            if (key >= min(sees[x >> 1], q.kv)) s[nt][x] = -INFINITY;
+                            if (F8 && key >= q.kv) vscale[nt][x & 1] = 0.f;      // no key: its bytes may be anything
+                        }
+                }
+                // The offset is the largest weight's so far: of e4m3 with the exponent of its value, which stays out of the converted values (exact) and
+                // goes into the weights, so that what is rounded to fp16 is largest where it counts.
                 float off[2], alpha[2];
                 #pragma unroll
                 for (int half = 0; half < 2; half++) {
-                    float mx = fmaxf(fmaxf(s[0][half * 2], s[0][half * 2 + 1]), fmaxf(s[1][half * 2], s[1][half * 2 + 1]));
+                    float mx = m[half];
+                    #pragma unroll
+                    for (int nt = 0; nt < KT; nt++) {
+                        if constexpr (F8) mx = max3(mx, s[nt][half * 2] + vlog[nt][0], s[nt][half * 2 + 1] + vlog[nt][1]);
+                        else mx = max3(mx, s[nt][half * 2], s[nt][half * 2 + 1]);
+                    }
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                    mx = fmaxf(mx, m[half]);
                     off[half] = mx == -INFINITY ? 0.f : mx;
                     alpha[half] = m[half] == mx ? 1.f : ex2(m[half] - off[half]);
                     m[half] = mx;
@@ -270,47 +310,49 @@ paged_rows_kernel(const PagedArgs c, const PagedAttnArgs a)
                     l[0] *= alpha[0];
                     l[1] *= alpha[1];
                 }
-                uint32_t p[4];
+                uint32_t p[STEP][4];
                 #pragma unroll
-                for (int nt = 0; nt < 2; nt++)
+                for (int nt = 0; nt < KT; nt++)
                     #pragma unroll
                     for (int half = 0; half < 2; half++) {
-                        const float p0 = ex2(s[nt][half * 2] - off[half]), p1 = ex2(s[nt][half * 2 + 1] - off[half]);
+                        float p0 = ex2(s[nt][half * 2] - off[half]), p1 = ex2(s[nt][half * 2 + 1] - off[half]);
                         l[half] += p0 + p1;
-                        p[nt * 2 + half] = pack_f16x2(p0, p1);
+                        if constexpr (F8) { p0 *= vscale[nt][0]; p1 *= vscale[nt][1]; }
+                        p[nt >> 1][(nt & 1) * 2 + half] = pack_f16x2(p0, p1);
                     }
                 // ---- O += P V. A masked weight is 0, and 0 times what is not finite is not 0: such values are left out here and, for the rows that
                 // do see them, put in at the end.
-                auto clean = [&](uint32_t (&w)[4]) {
-                    #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const uint32_t bad = nonfinite_f16x2(w[i]);
-                        poison |= bad != 0;
-                        w[i] &= ~bad;
-                    }
+                auto clean = [&](uint32_t& w) {
+                    const uint32_t bad = nonfinite_f16x2(w);
+                    poison |= bad != 0;
+                    w &= ~bad;
                 };
-                if constexpr (F8) {
-                    uint32_t w[4][4];                      // keys t * 2, t * 2 + 1, t * 2 + 8, t * 2 + 9
-                    #pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        load_words<VB>(sv + rows_swizzled<RB>(blk * 16 + (i >> 1) * 8 + t * 2 + (i & 1), (g * VB) >> 4) + ((g * VB) & 15), w[i]);
-                    #pragma unroll
-                    for (int j = 0; j < NT; j += 2) {
-                        uint32_t h[4];
+                #pragma unroll
+                for (int y = 0; y < STEP; y++) {
+                    if constexpr (F8) {
+                        uint32_t w[4][4];                  // keys t * 2, t * 2 + 1, t * 2 + 8, t * 2 + 9
                         #pragma unroll
-                        for (int i = 0; i < 4; i++) h[i] = mul_f16x2(e4m3x2_to_f16x2((w[i][j >> 2] >> ((j & 2) * 8)) & 0xffffu), vexp[i >> 1][i & 1]);
-                        if (masked) clean(h);
-                        mma16816(o[j], p, __byte_perm(h[0], h[1], 0x5410), __byte_perm(h[2], h[3], 0x5410));
-                        mma16816(o[j + 1], p, __byte_perm(h[0], h[1], 0x7632), __byte_perm(h[2], h[3], 0x7632));
-                    }
-                } else {
-                    #pragma unroll
-                    for (int j = 0; j < NT; j += 2) {
-                        uint32_t w[4];
-                        ldsm4_t(sv + rows_swizzled<RB>(blk * 16 + (lane & 7) + (((lane >> 3) & 1) << 3), j + (lane >> 4)), w);
-                        if (masked) clean(w);
-                        mma16816(o[j], p, w[0], w[1]);
-                        mma16816(o[j + 1], p, w[2], w[3]);
+                        for (int i = 0; i < 4; i++)
+                            load_words<VB>(sv + rows_swizzled<RB>((blk + y) * 16 + (i >> 1) * 8 + t * 2 + (i & 1), (g * VB) >> 4) + ((g * VB) & 15), w[i]);
+                        #pragma unroll
+                        for (int j = 0; j < NT; j += 2) {  // columns j and j + 1: of each the codes of two keys side by side, then converted
+                            const uint32_t sel = j & 2 ? 0x7362 : 0x5140;
+                            uint32_t b0, b1, b2, b3;
+                            e4m3x4_to_f16x4(__byte_perm(w[0][j >> 2], w[1][j >> 2], sel), b0, b2);
+                            e4m3x4_to_f16x4(__byte_perm(w[2][j >> 2], w[3][j >> 2], sel), b1, b3);
+                            if (masked) { clean(b0); clean(b1); clean(b2); clean(b3); }
+                            mma16816(o[j], p[y], b0, b1);
+                            mma16816(o[j + 1], p[y], b2, b3);
+                        }
+                    } else {
+                        #pragma unroll
+                        for (int j = 0; j < NT; j += 2) {
+                            uint32_t w[4];
+                            ldsm4_t(sv + rows_swizzled<RB>((blk + y) * 16 + (lane & 7) + (((lane >> 3) & 1) << 3), j + (lane >> 4)), w);
+                            if (masked) { clean(w[0]); clean(w[1]); clean(w[2]); clean(w[3]); }
+                            mma16816(o[j], p[y], w[0], w[1]);
+                            mma16816(o[j + 1], p[y], w[2], w[3]);
+                        }
                     }
                 }
             }
@@ -321,10 +363,10 @@ paged_rows_kernel(const PagedArgs c, const PagedAttnArgs a)
         auto column = [&](int j, int x) { return F8 ? (t * 2 + x) * VB + j : j * 8 + t * 2 + x; };
         if (__any_sync(0xffffffffu, poison)) {
             // Rare: the values that are not finite, of keys that some row of the warp does not see, for the rows that see them.
-            for (int u = max(u_lo, max(all_see, 0) / PAGED_ROWS_UNIT); u < u_hi; u++)
+            for (int u = max(u_lo, max(all_see, 0) / C::UNIT); u < u_hi; u++)
                 for (int x = 0; x < KS; x++) {
-                    const int key = u * PAGED_ROWS_UNIT + team * KS + x;
-                    if (key >= q.kv || (key | 15) < all_see) continue;
+                    const int key = u * C::UNIT + team * KS + x;
+                    if (key >= q.kv || (key | (16 * C::STEP - 1)) < all_see) continue;
                     const int page = paged_page(c, at.b, key, 52);
                     if (page < 0) continue;
                     const int row = (at.h << c.page_shift) + (key & ((1 << c.page_shift) - 1));
@@ -519,6 +561,7 @@ int launch_rows(const PagedArgs& c, const PagedAttnArgs& a, int blocks, cudaStre
 int paged_rows_tile(int rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
 
 int paged_rows_blocks_per_sm(int d_h, bool f8) { (void)d_h; (void)f8; return 2; }
+int paged_rows_unit(bool f8) { return f8 ? 128 : 64; }
 
 int paged_rows_launch(const PagedArgs& c, const PagedAttnArgs& a, int d_h, bool f8, int blocks, cudaStream_t stream)
 {
