@@ -69,7 +69,7 @@ __device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4])
 
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
 {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
@@ -235,19 +235,20 @@ paged_rows_kernel(const PagedArgs c, const PagedAttnArgs a)
                 float s[KT][4] = {};
                 if constexpr (F8) {
                     #pragma unroll
-                    for (int nt = 0; nt < KT; nt++)
+                    for (int i = 0; i < D / (4 * EB); i++) {
+                        uint32_t w[KT][4];
+                        const int byte = (t + 4 * i) * EB;
                         #pragma unroll
-                        for (int i = 0; i < D / (4 * EB); i++) {
-                            uint32_t w[4];
-                            const int byte = (t + 4 * i) * EB;
-                            load_words<EB>(sk + rows_swizzled<RB>(blk * 16 + nt * 8 + g, byte >> 4) + (byte & 15), w);
+                        for (int nt = 0; nt < KT; nt++) load_words<EB>(sk + rows_swizzled<RB>(blk * 16 + nt * 8 + g, byte >> 4) + (byte & 15), w[nt]);
+                        #pragma unroll
+                        for (int x = 0; x < EB / 4; x++)
                             #pragma unroll
-                            for (int x = 0; x < EB / 4; x++) {
+                            for (int nt = 0; nt < KT; nt++) {
                                 uint32_t b0, b1;
-                                e4m3x4_to_f16x4(w[x], b0, b1);
+                                e4m3x4_to_f16x4(w[nt][x], b0, b1);
                                 mma16816(s[nt], qf[i * (EB / 4) + x], b0, b1);
                             }
-                        }
+                    }
                 } else {
                     #pragma unroll
                     for (int st = 0; st < KSTEPS; st++)
