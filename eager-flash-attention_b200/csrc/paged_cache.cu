@@ -222,7 +222,7 @@ int move_rows(const char* what, bool read, const void* K, const void* V, long lo
     }
 }
 
-struct PagedPlan { PagedShape w; int blocks; bool cut, chunk; size_t cut_bytes, ml_bytes, o_bytes; };
+struct PagedPlan { PagedShape w; int blocks, cluster; bool cut, chunk; size_t cut_bytes, ml_bytes, o_bytes; };
 
 PagedPlan plan_attention(const efa_paged_cache& c, const efa_paged_batch& b, const efa_paged_attention_params& p)
 {
@@ -235,7 +235,14 @@ PagedPlan plan_attention(const efa_paged_cache& c, const efa_paged_batch& b, con
     plan.w = PagedShape{G, p.causal ? 1 : 0, tile, unit, plan.chunk ? PAGED_CHUNK_EXTRA : PAGED_ROWS_EXTRA, (int)((rows + tile - 1) / tile)};
     const long long items = (long long)b.num_seqs * c.H_kv * plan.w.max_tiles, units = std::max<long long>(1, (kv_cap + unit - 1) / unit);
     const int parts = device_sms() * (plan.chunk ? 1 : paged_rows_blocks_per_sm(c.d_h, c.dtype == EFA_E4M3));
-    plan.cut = plan.chunk || units * unit > 512;
+    // Few rows: a block per item, or where there are few items a cluster of up to eight that shares one, merged in shared memory, as long as a block's part of
+    // the longest item stays short; else equal shares of everything, which cost a merge in a launch of its own but leave no SM idle, whatever the
+    // lengths. us, clusters / shares, one token: 16 heads of 64 1000 keys 5.6 / 10.2, 8000 12.4 / 14.4, 16000 20.3 / 18.9; 32 heads of 128 on 8,
+    // 1000 keys 6.8 / 10.6, 8000 15.8 / 17.2, 16000 26.4 / 19.9; 8 bits 7.2 / 10.9, 16.0 / 17.0, 25.5 / 20.2; 64 such sequences (no clusters) 1000 keys 45 / 50.
+    plan.cluster = 1;
+    if (!plan.chunk) while (plan.cluster < 8 && plan.cluster * 2 <= units && items * plan.cluster * 2 <= parts) plan.cluster *= 2;
+    plan.cut = plan.chunk || units * unit > (c.d_h == 128 ? 1024 : 1536) * plan.cluster;
+    if (plan.cut) plan.cluster = 1;
     plan.blocks = (int)std::min<long long>(plan.cut ? std::min<long long>(parts, items * units) : items, INT_MAX);
     if (plan.cut) {
         plan.cut_bytes = ((size_t)plan.blocks * sizeof(PagedCut) + 255) / 256 * 256;
@@ -327,7 +334,7 @@ int paged_attention(const void* Q, void* O, const efa_paged_cache& c, const efa_
         a.parts.o = reinterpret_cast<float4*>(at + plan.cut_bytes + plan.ml_bytes);
     }
     const bool f8 = c.dtype == EFA_E4M3;
-    if (int rc = plan.chunk ? paged_chunk_launch(args, a, c.d_h, f8, plan.blocks, stream) : paged_rows_launch(args, a, c.d_h, f8, plan.blocks, stream)) return rc;
+    if (int rc = plan.chunk ? paged_chunk_launch(args, a, c.d_h, f8, plan.blocks, stream) : paged_rows_launch(args, a, c.d_h, f8, plan.blocks, plan.cluster, stream)) return rc;
     if (!plan.cut || plan.blocks < 2) return 0;
     return paged_merge_launch(args, a, c.d_h, plan.blocks, (int)std::min<long long>(plan.w.tile, (long long)b.max_q * plan.w.G), stream);
 }

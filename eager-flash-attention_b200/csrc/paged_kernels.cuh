@@ -20,7 +20,8 @@ int paged_rows_tile(int rows);              // rows of a tile for chunks of up t
 constexpr int PAGED_ROWS_EXTRA = 1;
 int paged_rows_unit(bool f8);               // keys of a unit
 int paged_rows_blocks_per_sm(int d_h, bool f8);
-int paged_rows_launch(const PagedArgs& c, const PagedAttnArgs& a, int d_h, bool f8, int blocks, cudaStream_t stream);
+// blocks: items, or shares; cluster: blocks that share an item (items only).
+int paged_rows_launch(const PagedArgs& c, const PagedAttnArgs& a, int d_h, bool f8, int blocks, int cluster, cudaStream_t stream);
 
 // tcgen05 over tiles of 256 rows (paged_chunk.cuh). Always cuts.
 constexpr int PAGED_CHUNK_TILE = 256, PAGED_CHUNK_UNIT = 128, PAGED_CHUNK_EXTRA = 3;
@@ -29,11 +30,11 @@ int paged_chunk_launch(const PagedArgs& c, const PagedAttnArgs& a, int d_h, bool
 // Merge of the items that the cuts of `blocks` parts go through.
 int paged_merge_launch(const PagedArgs& c, const PagedAttnArgs& a, int d_h, int blocks, int most_rows, cudaStream_t stream);
 
-// A launch like launch_early's (host_util.h) of a kernel whose name the caller has as a value.
+// A launch like launch_early's (host_util.h) of a kernel whose name the caller has as a value. grid.z: a cluster's blocks.
 template <class... P, class... A>
 cudaError_t paged_launch(void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem, cudaStream_t stream, const A&... args)
 {
-    return launch_kernel(true, 1, kernel, grid, threads, smem, stream, args...);
+    return launch_kernel(true, (int)grid.z, kernel, grid, threads, smem, stream, args...);
 }
 
 }  // namespace efa

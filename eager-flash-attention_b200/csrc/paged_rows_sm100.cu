@@ -35,7 +35,7 @@ struct RowsCfg {
     static constexpr int STAGES = UNIT_BYTES >= 32768 ? 3 : UNIT_BYTES >= 16384 ? 6 : 8;
     static constexpr int RING = STAGES * UNIT_BYTES;
     static constexpr int OPITCH = D + 4;
-    static constexpr int MERGE = 4 * 16 * OPITCH * 4 + 4 * 16 * 8;            // four warps' O, and (m, l)
+    static constexpr int MERGE = 4 * 16 * OPITCH * 4 + 8 * 16 * 8;            // four warps' O, their (m, l), and that of the block
     static constexpr int SMEM = RING > MERGE ? RING : MERGE;
 };
 
@@ -97,6 +97,29 @@ __device__ __forceinline__ float max3(float a, float b, float c)
     return r;
 }
 
+template <int N>
+__device__ __forceinline__ void load_cluster(uint32_t addr, float (&v)[N])
+{
+    if constexpr (N == 2) {
+        asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v[0]), "=f"(v[1]) : "r"(addr) : "memory");
+    } else {
+        #pragma unroll
+        for (int i = 0; i < N; i += 4)
+            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[i]), "=f"(v[i + 1]), "=f"(v[i + 2]), "=f"(v[i + 3]) : "r"(addr + i * 4) : "memory");
+    }
+}
+
+// Eight columns of a row of O; none: the row sees nothing.
+__device__ __forceinline__ void store_row8(__half* dst, const float (&acc)[8], float sum, bool none)
+{
+    const float inv = 1.f / sum;
+    uint4 out;
+    uint32_t* w = &out.x;
+    #pragma unroll
+    for (int x = 0; x < 4; x++) w[x] = none ? 0u : pack_f16x2(acc[2 * x] * inv, acc[2 * x + 1] * inv);
+    *reinterpret_cast<uint4*>(dst) = out;
+}
+
 template <int D, bool F8, int WM>
 __global__ void __launch_bounds__(PR_THREADS, 2)
 paged_rows_kernel(const PagedArgs c, const PagedAttnArgs a)
@@ -130,7 +153,7 @@ paged_rows_kernel(const PagedArgs c, const PagedAttnArgs a)
     } else {
         const int per = c.H_kv * a.w.max_tiles, b = blockIdx.x / per, rest = blockIdx.x - b * per;
         at = first = PagedAt{rest % c.H_kv, b, rest / c.H_kv, 0};
-        if (tid == 0 && rest == 0) paged_seq<true>(c, b, 51);
+        if (tid == 0 && rest == 0 && blockIdx.z == 0) paged_seq<true>(c, b, 51);
         left = at.rt < paged_tiles(a.w, paged_seq(c, b)) ? INT_MAX : 0;
     }
 
@@ -139,10 +162,17 @@ paged_rows_kernel(const PagedArgs c, const PagedAttnArgs a)
     for (; left > 0; paged_next(c, a.w, at)) {
         const PagedPiece piece = paged_piece(c, a.w, at, left);
         const PagedSeq& q = piece.q;
-        const int u_lo = piece.u_lo, u_hi = piece.u_hi;
+        int u_lo = piece.u_lo, u_hi = piece.u_hi;
         const bool whole = u_lo == 0 && u_hi == piece.units;
-        if (!cut) left = 0;
-        if (u_hi == u_lo) continue;
+        if (cut) {
+            if (u_hi == u_lo) continue;
+        } else {
+            left = 0;
+            if (gridDim.z > 1) {                           // a cluster's blocks share the item
+                u_lo = (int)((unsigned)(piece.units * blockIdx.z) / gridDim.z);
+                u_hi = (int)((unsigned)(piece.units * (blockIdx.z + 1)) / gridDim.z);
+            }
+        }
         const int rows = min(C::TILE, q.n * a.w.G - at.rt * C::TILE), r0 = at.rt * C::TILE;      // of the item
 
         // ---- the asynchronous copies of a unit: this warp's WK keys of the team's, 16 at a time (they are in one page)
@@ -420,21 +450,41 @@ paged_rows_kernel(const PagedArgs c, const PagedAttnArgs a)
                 #pragma unroll
                 for (int x = 0; x < 8; x++) acc[x] += w * src[x];
             }
-            if (whole) {
-                const int r = r0 + rr, token = r / a.w.G;
-                const bool none = paged_visible(a.w, q, r) <= 0;                       // nothing to see: zeros
-                const float inv = none ? 0.f : 1.f / sum;
-                uint4 out;
-                uint32_t* w = &out.x;
+            if (gridDim.z > 1) {
+                float* dst = so + rr * C::OPITCH + col;                                // the first team's place, which only this thread reads
                 #pragma unroll
-                for (int x = 0; x < 4; x++) w[x] = none ? 0u : pack_f16x2(acc[2 * x] * inv, acc[2 * x + 1] * inv);
-                *reinterpret_cast<uint4*>(a.O + (long long)(q.row0 + token) * a.o_token + (long long)(at.h * a.w.G + r - token * a.w.G) * D + col) = out;
+                for (int x = 0; x < 8; x++) dst[x] = acc[x];
+                if (col == 0) sml[4 * 16 + rr] = make_float2(top, sum);
+            } else if (whole) {
+                const int r = r0 + rr, token = r / a.w.G;
+                store_row8(a.O + (long long)(q.row0 + token) * a.o_token + (long long)(at.h * a.w.G + r - token * a.w.G) * D + col, acc, sum, paged_visible(a.w, q, r) <= 0);
             } else {
                 float4* dst = a.parts.o + ((long long)place * (D / 4) + col / 4) * C::TILE + rr;
                 dst[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
                 dst[C::TILE] = make_float4(acc[4], acc[5], acc[6], acc[7]);
                 if (col == 0) a.parts.ml[(long long)place * C::TILE + rr] = make_float2(top, sum);
             }
+        }
+        if (gridDim.z > 1) {
+            // The cluster's blocks, each for its part of the elements, out of one another's shared memory.
+            cluster_sync();
+            for (int e = blockIdx.z * PR_THREADS + tid; e < rows * (D / 8); e += gridDim.z * PR_THREADS) {
+                const int rr = e / (D / 8), col = (e % (D / 8)) * 8, r = r0 + rr, token = r / a.w.G;
+                float top = -INFINITY, sum = 0.f, acc[8] = {};
+                #pragma unroll 4
+                for (unsigned i = 0; i < gridDim.z; i++) {
+                    float ml[2], v[8];
+                    load_cluster(cluster_addr(&sml[4 * 16 + rr], i), ml);
+                    load_cluster(cluster_addr(so + rr * C::OPITCH + col, i), v);
+                    const float m = fmaxf(top, ml[0]), old = top == m ? 1.f : ex2(top - m), w = ml[0] == m ? 1.f : ex2(ml[0] - m);
+                    top = m;
+                    sum = sum * old + w * ml[1];
+                    #pragma unroll
+                    for (int x = 0; x < 8; x++) acc[x] = acc[x] * old + w * v[x];
+                }
+                store_row8(a.O + (long long)(q.row0 + token) * a.o_token + (long long)(at.h * a.w.G + r - token * a.w.G) * D + col, acc, sum, paged_visible(a.w, q, r) <= 0);
+            }
+            cluster_sync();
         }
         __syncthreads();
         if (left <= 0) break;          // not on to an item that is not there
@@ -522,18 +572,12 @@ paged_merge_kernel(const PagedArgs c, const PagedAttnArgs a, int parts)
         }
         if (!mine || group > 0) continue;
         const int r = here.rt * tile + rr, token = r / a.w.G;
-        const bool none = paged_visible(a.w, q, r) <= 0;
-        const float inv = 1.f / sum;
-        uint4 out;
-        uint32_t* w = &out.x;
-        #pragma unroll
-        for (int y = 0; y < 4; y++) w[y] = none ? 0u : pack_f16x2(acc[2 * y] * inv, acc[2 * y + 1] * inv);
-        *reinterpret_cast<uint4*>(a.O + (long long)(q.row0 + token) * a.o_token + (long long)(here.h * a.w.G + r - token * a.w.G) * D + col) = out;
+        store_row8(a.O + (long long)(q.row0 + token) * a.o_token + (long long)(here.h * a.w.G + r - token * a.w.G) * D + col, acc, sum, paged_visible(a.w, q, r) <= 0);
     }
 }
 
 template <int D, bool F8, int WM>
-int launch_rows(const PagedArgs& c, const PagedAttnArgs& a, int blocks, cudaStream_t stream)
+int launch_rows(const PagedArgs& c, const PagedAttnArgs& a, int blocks, int cluster, cudaStream_t stream)
 {
     using C = RowsCfg<D, F8, WM>;
     static bool configured[64] = {};
@@ -543,17 +587,17 @@ int launch_rows(const PagedArgs& c, const PagedAttnArgs& a, int blocks, cudaStre
         EFA_CUDA(cudaFuncSetAttribute(paged_rows_kernel<D, F8, WM>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
         if (dev >= 0 && dev < 64) configured[dev] = true;
     }
-    EFA_CUDA(paged_launch(paged_rows_kernel<D, F8, WM>, dim3(blocks), PR_THREADS, C::SMEM, stream, c, a));
+    EFA_CUDA(paged_launch(paged_rows_kernel<D, F8, WM>, dim3(blocks, 1, cluster), PR_THREADS, C::SMEM, stream, c, a));
     return 0;
 }
 
 template <int D, bool F8>
-int launch_rows(const PagedArgs& c, const PagedAttnArgs& a, int blocks, cudaStream_t stream)
+int launch_rows(const PagedArgs& c, const PagedAttnArgs& a, int blocks, int cluster, cudaStream_t stream)
 {
     switch (a.w.tile) {
-        case 16: return launch_rows<D, F8, 1>(c, a, blocks, stream);
-        case 32: return launch_rows<D, F8, 2>(c, a, blocks, stream);
-        default: return launch_rows<D, F8, 4>(c, a, blocks, stream);
+        case 16: return launch_rows<D, F8, 1>(c, a, blocks, cluster, stream);
+        case 32: return launch_rows<D, F8, 2>(c, a, blocks, cluster, stream);
+        default: return launch_rows<D, F8, 4>(c, a, blocks, cluster, stream);
     }
 }
 
@@ -564,13 +608,13 @@ int paged_rows_tile(int rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
 int paged_rows_blocks_per_sm(int d_h, bool f8) { (void)d_h; (void)f8; return 2; }
 int paged_rows_unit(bool f8) { return f8 ? 128 : 64; }
 
-int paged_rows_launch(const PagedArgs& c, const PagedAttnArgs& a, int d_h, bool f8, int blocks, cudaStream_t stream)
+int paged_rows_launch(const PagedArgs& c, const PagedAttnArgs& a, int d_h, bool f8, int blocks, int cluster, cudaStream_t stream)
 {
     switch (d_h) {
-        case 16:  return f8 ? launch_rows<16, true>(c, a, blocks, stream) : launch_rows<16, false>(c, a, blocks, stream);
-        case 32:  return f8 ? launch_rows<32, true>(c, a, blocks, stream) : launch_rows<32, false>(c, a, blocks, stream);
-        case 64:  return f8 ? launch_rows<64, true>(c, a, blocks, stream) : launch_rows<64, false>(c, a, blocks, stream);
-        default:  return f8 ? launch_rows<128, true>(c, a, blocks, stream) : launch_rows<128, false>(c, a, blocks, stream);
+        case 16:  return f8 ? launch_rows<16, true>(c, a, blocks, cluster, stream) : launch_rows<16, false>(c, a, blocks, cluster, stream);
+        case 32:  return f8 ? launch_rows<32, true>(c, a, blocks, cluster, stream) : launch_rows<32, false>(c, a, blocks, cluster, stream);
+        case 64:  return f8 ? launch_rows<64, true>(c, a, blocks, cluster, stream) : launch_rows<64, false>(c, a, blocks, cluster, stream);
+        default:  return f8 ? launch_rows<128, true>(c, a, blocks, cluster, stream) : launch_rows<128, false>(c, a, blocks, cluster, stream);
     }
 }
 
