@@ -61,12 +61,11 @@ __device__ __forceinline__ int paged_page(const PagedArgs& c, int b, int key, in
 // ---------------------------------------------------------------------------------------------
 __device__ __forceinline__ float exp_byte_f32(unsigned byte) { return __uint_as_float(byte << 23); }     // byte 0, which nothing is stored with, as 0
 
-// 2^(byte - 127) twice as fp16; beyond fp16's range 0 or 2^15.
+// 2^(byte - 127) twice as fp16. Of bytes that the writer does not store (below 103, above 142) something finite.
 __device__ __forceinline__ uint32_t exp_byte_f16x2(unsigned byte)
 {
-    const int e = (int)byte - 127;
-    const uint32_t h = e >= -14 ? (uint32_t)(min(e, 15) + 15) << 10 : e >= -24 ? 1u << (e + 24) : 0u;
-    return h | h << 16;
+    const uint32_t normal = (min(byte, 142u) - 112u) << 10, h = byte > 112u ? normal : 1u << ((byte - 103u) & 15u);
+    return __byte_perm(h, h, 0x1010);
 }
 
 __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two)

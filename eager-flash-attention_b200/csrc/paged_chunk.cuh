@@ -299,35 +299,56 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                 };
                 bool ok = true;
                 if constexpr (F8) {
-                    // ---- warps 12 to 15: all codes to fp16. A thread has one 16-byte chunk of RPT rows behind one another, 
-                    constexpr int CH = D / 16, RPT = CH;
+                    // ---- warps 12 to 15: all codes to fp16. A thread has one 16-byte chunk of RPT rows behind one another. Every second thread (hi) takes its rows
+                    // in the order 1, 0, 3, 2, ..., so that eight lanes' stores lie in eight different bank groups: shared memory is what the
+                    // warps here, and the MMAs, contend for (Q K^T alone takes all of it for 512 cycles a tile).
+                    constexpr int CH = D / 16, RPT = CH, HALF = RPT > 4 ? 4 : RPT;
                     const int ch = tid % CH, row0 = (tid & 127) / CH * RPT;
+                    const int hi = CH == 8 ? ch >> 2 : CH == 4 ? (lane >> 2) & 1 : 0;
+                    const uint32_t col = (uint32_t)(ch * 16 / C::BOXC) * C::BOX_BYTES, byte = (uint32_t)(ch * 16 % C::BOXC) * 2u;
+                    // Rows of 128 bytes: row0 + (i ^ hi), chunk byte / 16 of it under the swizzle, as an exclusive or of what is known for i with the thread's own.
+                    const uint32_t own = (uint32_t)row0 * 128u + (byte ^ (uint32_t)(hi * 0x90) ^ (uint32_t)(row0 & 4 ? 0x40 : 0));
+                    auto place_of = [&](int i) { return RPT >= 4 ? own ^ (uint32_t)(i * 0x90) : swizzled<C::SWB>((uint32_t)(row0 + i) * C::SWB + byte); };
                     for (int n = 0; n < 2 * nblk_max && ok && warp >= 12; n++) {
                         const int j = n >> 1, isv = n & 1, s = n % NRAW;
                         const int NS = isv ? NSV : NSK, slot = j % NS, use = j / NS;
-                        ok = __all_sync(0xffffffffu, mbar_wait(&raw_full[s], (uint32_t)((n / NRAW) & 1), &abort_word, 62));
-                        if (use > 0) ok = ok && __all_sync(0xffffffffu, mbar_wait(isv ? &v_empty[slot] : &k_empty[slot], (uint32_t)((use - 1) & 1), &abort_word, 63));
+                        ok = __all_sync(0xffffffffu, (use == 0 || mbar_wait(isv ? &v_empty[slot] : &k_empty[slot], (uint32_t)((use - 1) & 1), &abort_word, 63)) &&
+                                                     mbar_wait(&raw_full[s], (uint32_t)((n / NRAW) & 1), &abort_word, 62));
                         if (!ok) break;
-                        const uint32_t raw = smem_u32(sRaw + s * C::RAW_BYTES), dst = smem_u32((isv ? sV : sK) + slot * C::TILE_BYTES);
-                        const uint32_t col = dst + (uint32_t)(ch * 16 / C::BOXC) * C::BOX_BYTES, byte = (uint32_t)(ch * 16 % C::BOXC) * 2u;
-                        const bool care = isv && j >= jm;
-                        #pragma unroll 4
-                        for (int i = 0; i < RPT; i++) {
-                            const uint4 x = lds128(raw + ((row0 + i) * CH + ch) * 16);
-                            uint32_t e;
-                            asm volatile("ld.shared.u8 %0, [%1];" : "=r"(e) : "r"(raw + 128 * D + row0 + i) : "memory");
-                            e = exp_byte_f16x2(e);
-                            uint4 lo, hi;
-                            e4m3x4_to_f16x4(x.x, lo.x, lo.y); e4m3x4_to_f16x4(x.y, lo.z, lo.w);
-                            e4m3x4_to_f16x4(x.z, hi.x, hi.y); e4m3x4_to_f16x4(x.w, hi.z, hi.w);
-                            lo = make_uint4(mul_f16x2(lo.x, e), mul_f16x2(lo.y, e), mul_f16x2(lo.z, e), mul_f16x2(lo.w, e));
-                            hi = make_uint4(mul_f16x2(hi.x, e), mul_f16x2(hi.y, e), mul_f16x2(hi.z, e), mul_f16x2(hi.w, e));
-                            if (care) { clean(lo); clean(hi); }
-                            const uint32_t at_row = (uint32_t)(row0 + i) * C::SWB + byte;
-                            sts128(col + swizzled<C::SWB>(at_row), lo);
-                            sts128(col + swizzled<C::SWB>(at_row + 16), hi);
+                        const uint32_t raw = smem_u32(sRaw + s * C::RAW_BYTES);
+                        const uint32_t dst = smem_u32((isv ? sV : sK) + slot * C::TILE_BYTES) + col;
+                        #pragma unroll 1       // small: the softmax's code and this are more than the instruction caches hold (unrolled 115 us, so 86: 512 tokens x 32 heads, 8192 keys)
+                        for (int i0 = 0; i0 < RPT; i0 += HALF) {
+                            uint4 x[HALF];
+                            uint32_t exps;
+                            if constexpr (HALF == 4) asm volatile("ld.shared.b32 %0, [%1];" : "=r"(exps) : "r"(raw + 128 * D + row0 + i0) : "memory");
+                            if constexpr (HALF == 2) asm volatile("{\n.reg .b16 x;\nld.shared.b16 x, [%1];\ncvt.u32.u16 %0, x;\n}\n" : "=r"(exps) : "r"(raw + 128 * D + row0) : "memory");
+                            if constexpr (HALF == 1) asm volatile("ld.shared.u8 %0, [%1];" : "=r"(exps) : "r"(raw + 128 * D + row0) : "memory");
+                            #pragma unroll
+                            for (int i = 0; i < HALF; i++) x[i] = lds128(raw + ((row0 + (i0 + i ^ hi)) * CH + ch) * 16);
+                            if (HALF == 4 && hi) exps = __byte_perm(exps, 0, 0x2301);
+                            #pragma unroll
+                            for (int i = 0; i < HALF; i++) {
+                                const uint32_t e = exp_byte_f16x2((exps >> (8 * i)) & 0xffu);
+                                uint4 lo, up;
+                                e4m3x4_to_f16x4(x[i].x, lo.x, lo.y); e4m3x4_to_f16x4(x[i].y, lo.z, lo.w);
+                                e4m3x4_to_f16x4(x[i].z, up.x, up.y); e4m3x4_to_f16x4(x[i].w, up.z, up.w);
+                                lo = make_uint4(mul_f16x2(lo.x, e), mul_f16x2(lo.y, e), mul_f16x2(lo.z, e), mul_f16x2(lo.w, e));
+                                up = make_uint4(mul_f16x2(up.x, e), mul_f16x2(up.y, e), mul_f16x2(up.z, e), mul_f16x2(up.w, e));
+                                sts128(dst + place_of(i0 + i), lo);
+                                sts128(dst + (place_of(i0 + i) ^ 16u), up);
+                            }
                         }
-                        if (care && bad_seen) *(volatile int*)&poison = 1;
+                        if (isv && j >= jm) {
+                            #pragma unroll 1
+                            for (int i = 0; i < 2 * RPT; i++) {
+                                const uint32_t at = dst + (place_of(i >> 1) ^ (i & 1 ? 16u : 0u));
+                                uint4 x = lds128(at);
+                                clean(x);
+                                sts128(at, x);
+                            }
+                            if (bad_seen) *(volatile int*)&poison = 1;
+                        }
                         fence_proxy_async_smem();
                         __syncwarp();
                         if (lane == 0) {
