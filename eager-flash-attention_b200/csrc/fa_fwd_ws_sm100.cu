@@ -51,6 +51,7 @@
 #include "sm100_ptx.cuh"
 
 #include <algorithm>
+#include <climits>
 #include <cmath>
 
 namespace efa {

@@ -234,15 +234,36 @@ PagedPlan plan_attention(const efa_paged_cache& c, const efa_paged_batch& b, con
     const int tile = plan.chunk ? PAGED_CHUNK_TILE : paged_rows_tile((int)rows), unit = plan.chunk ? PAGED_CHUNK_UNIT : paged_rows_unit(c.dtype == EFA_E4M3);
     plan.w = PagedShape{G, p.causal ? 1 : 0, tile, unit, plan.chunk ? PAGED_CHUNK_EXTRA : PAGED_ROWS_EXTRA, (int)((rows + tile - 1) / tile)};
     const long long items = (long long)b.num_seqs * c.H_kv * plan.w.max_tiles, units = std::max<long long>(1, (kv_cap + unit - 1) / unit);
-    const int parts = device_sms() * (plan.chunk ? 1 : paged_rows_blocks_per_sm(c.d_h, c.dtype == EFA_E4M3));
-    // Few rows: a block per item, or where there are few items a cluster of up to eight that shares one, merged in shared memory, as long as a block's part of
-    // the longest item stays short; else equal shares of everything, which cost a merge in a launch of its own but leave no SM idle, whatever the
-    // lengths. us, clusters / shares, one token: 16 heads of 64 1000 keys 5.6 / 10.2, 8000 12.4 / 14.4, 16000 20.3 / 18.9; 32 heads of 128 on 8,
-    // 1000 keys 6.8 / 10.6, 8000 15.8 / 17.2, 16000 26.4 / 19.9; 8 bits 7.2 / 10.9, 16.0 / 17.0, 25.5 / 20.2; 64 such sequences (no clusters) 1000 keys 45 / 50.
+    const bool f8 = c.dtype == EFA_E4M3;
     plan.cluster = 1;
-    if (!plan.chunk) while (plan.cluster < 8 && plan.cluster * 2 <= units && items * plan.cluster * 2 <= parts) plan.cluster *= 2;
-    plan.cut = plan.chunk || units * unit > (c.d_h == 128 ? 1024 : 1536) * plan.cluster;
-    if (plan.cut) plan.cluster = 1;
+    int parts = device_sms();
+    if (plan.chunk) {
+        // A block per item, those of the last rows first, or equal shares of everything with a merge behind: in units of 128 keys (about 2 us), for chunks and
+        // sequences as long as the bounds allow. Items of about one length go in waves; else, longest first, they come out even. Shares pay for the
+        // merge, for pieces half of which begin and end within an item, and for reading keys at different places at a time: blocks in step on many tiles of one
+        // sequence find them in the L2. Below MIN_SHARE a block spends its time on anything but keys. us, items / shares: prompts, 16 heads of 64, 1024 tokens
+        // 19 / 21, 4096 59 / 68; 32 heads of 128 on 8, 2048 45 / 61, 8192 516 / 559; 2048 tokens over 32768 keys 1004 / 1070, of 8 bits 1099 / 1039; eight
+        // sequences, 512 tokens over 4096 keys 310 / 279; one, 64 tokens over 2000 keys 34 / 30.
+        constexpr double MIN_SHARE = 6, MERGE = 6;
+        const double tiles = std::min<double>((double)b.num_seqs * plan.w.max_tiles, (double)b.tokens * G / tile + b.num_seqs) * c.H_kv;
+        const double longest = (double)units + PAGED_CHUNK_EXTRA;
+        const double first = p.causal ? std::max<double>(1, ((double)kv_cap - b.max_q + (double)tile / G) / unit) + PAGED_CHUNK_EXTRA : longest;
+        const bool even = first * 2 >= longest;
+        const double each = tiles * (first + longest) / 2 / parts;
+        const double by_item = even ? std::ceil(tiles / parts) * longest : std::max(longest, each * 1.05);
+        const double by_share = std::max(MIN_SHARE, each) * 1.05 + MERGE;
+        plan.cut = by_item > by_share * (!f8 && plan.w.max_tiles >= 16 ? 1.1 : 1.0);
+        parts = (int)std::min<double>(parts, std::max(1.0, each * parts / MIN_SHARE));
+    } else {
+        // Few rows: a block per item, or where there are few items a cluster of up to eight that shares one, merged in shared memory, as long as a block's part of
+        // the longest item stays short; else equal shares of everything, which cost a merge in a launch of its own but leave no SM idle, whatever the
+        // lengths. us, clusters / shares, one token: 16 heads of 64 1000 keys 5.6 / 10.2, 8000 12.4 / 14.4, 16000 20.3 / 18.9; 32 heads of 128 on 8,
+        // 1000 keys 6.8 / 10.6, 8000 15.8 / 17.2, 16000 26.4 / 19.9; 8 bits 7.2 / 10.9, 16.0 / 17.0, 25.5 / 20.2; 64 such sequences (no clusters) 1000 keys 45 / 50.
+        parts *= paged_rows_blocks_per_sm(c.d_h, f8);
+        while (plan.cluster < 8 && plan.cluster * 2 <= units && items * plan.cluster * 2 <= parts) plan.cluster *= 2;
+        plan.cut = units * unit > (c.d_h == 128 ? 1024 : 1536) * plan.cluster;
+        if (plan.cut) plan.cluster = 1;
+    }
     plan.blocks = (int)std::min<long long>(plan.cut ? std::min<long long>(parts, items * units) : items, INT_MAX);
     if (plan.cut) {
         plan.cut_bytes = ((size_t)plan.blocks * sizeof(PagedCut) + 255) / 256 * 256;

@@ -101,13 +101,22 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     // ---- this block's share: thread FINDER goes through it, a piece ahead of the others
     constexpr int FINDER = 352;
     PagedAt at{}, first;
-    int left = paged_part<C::THREADS>(c, a.w, blockIdx.x, gridDim.x, scratch, at);
+    int left;
+    const bool cut = a.parts.cut != nullptr;
+    if (cut) {
+        left = paged_part<C::THREADS>(c, a.w, blockIdx.x, gridDim.x, scratch, at);
+    } else {                                            // an item per block, of all sequences those of the last rows first: they are the longest
+        const int group = c.H_kv * c.num_seqs, level = blockIdx.x / group, rest = blockIdx.x - level * group;
+        at = PagedAt{rest % c.H_kv, rest / c.H_kv, a.w.max_tiles - 1 - level, 0};
+        left = at.rt < paged_tiles(a.w, paged_seq(c, at.b)) ? INT_MAX : 0;
+    }
     first = at;
     auto find_piece = [&](int slot) {
         s_place[slot] = -1;
         while (left > 0) {
             const PagedPiece p = paged_piece(c, a.w, at, left);
             const int other = at.h == first.h && at.b == first.b && at.rt == first.rt ? 0 : 1;
+            if (!cut) left = 0;
             if (left > 0) paged_next(c, a.w, at);
             if (p.u_hi == p.u_lo) continue;
             s_piece[slot] = p;
@@ -116,9 +125,13 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         }
     };
     if (tid == FINDER) {
-        PagedCut here{};
-        if (left > 0) here = PagedCut{at.h, at.b, at.rt, max(0, at.off - a.w.extra), paged_units(a.w, paged_seq<true>(c, at.b, 53), at.rt), 0, 0, 0};
-        a.parts.cut[blockIdx.x] = here;
+        if (cut) {
+            PagedCut here{};
+            if (left > 0) here = PagedCut{at.h, at.b, at.rt, max(0, at.off - a.w.extra), paged_units(a.w, paged_seq<true>(c, at.b, 53), at.rt), 0, 0, 0};
+            a.parts.cut[blockIdx.x] = here;
+        } else if (at.rt == 0 && at.h == 0) {
+            paged_seq<true>(c, at.b, 53);
+        }
         find_piece(0);
     }
 

@@ -23,7 +23,7 @@ int paged_rows_blocks_per_sm(int d_h, bool f8);
 // blocks: items, or shares; cluster: blocks that share an item (items only).
 int paged_rows_launch(const PagedArgs& c, const PagedAttnArgs& a, int d_h, bool f8, int blocks, int cluster, cudaStream_t stream);
 
-// tcgen05 over tiles of 256 rows (paged_chunk.cuh). Always cuts.
+// tcgen05 over tiles of 256 rows (paged_chunk.cuh); blocks: items, or shares.
 constexpr int PAGED_CHUNK_TILE = 256, PAGED_CHUNK_UNIT = 128, PAGED_CHUNK_EXTRA = 3;
 int paged_chunk_launch(const PagedArgs& c, const PagedAttnArgs& a, int d_h, bool f8, int blocks, cudaStream_t stream);
 
