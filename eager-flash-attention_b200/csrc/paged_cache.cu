@@ -17,7 +17,7 @@ namespace efa {
 namespace {
 
 constexpr int PC_THREADS = 256;
-constexpr int PC_HEADS = 4;          // heads that a thread moves at a time: what it has in flight
+template <bool F8> constexpr int PC_HEADS = F8 ? 4 : 2;      // heads that a thread moves at a time: what it has in flight
 
 struct PagedRows {
     __half* k;
@@ -73,7 +73,7 @@ __device__ __forceinline__ uint4 from_e4m3(const uint2& x, unsigned byte)
 }
 
 // Rows into pages (READ: out of them). A row of a head is D / 8 lanes of 16 bytes fp16; a warp takes the 256 / D rows that it holds of one token range and up to
-// PC_HEADS heads of K and V at a time. HBM-bound for prompts, a chain of three loads (lengths, page, row) for single tokens.
+// PC_HEADS<F8> heads of K and V at a time. HBM-bound for prompts, a chain of three loads (lengths, page, row) for single tokens.
 template <int D, bool F8, bool READ>
 __global__ void __launch_bounds__(PC_THREADS)
 paged_move_kernel(const PagedArgs c, const PagedRows rows)
@@ -84,14 +84,14 @@ paged_move_kernel(const PagedArgs c, const PagedRows rows)
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int sub = lane % LANES;
     const int row = (blockIdx.x * (PC_THREADS / 32) + warp) * PER_WARP + lane / LANES;
-    const int h0 = blockIdx.y * PC_HEADS;
+    const int h0 = blockIdx.y * PC_HEADS<F8>;
     const bool there = row < c.tokens;
     const long long at = (long long)row * rows.token + sub * 8;
 
-    uint4 k[PC_HEADS], v[PC_HEADS];
+    uint4 k[PC_HEADS<F8>], v[PC_HEADS<F8>];
     if constexpr (!READ) {                                 // asked for ahead of the search for their place
         #pragma unroll
-        for (int i = 0; i < PC_HEADS; i++)
+        for (int i = 0; i < PC_HEADS<F8>; i++)
             if (there && h0 + i < c.H_kv) {
                 k[i] = *reinterpret_cast<const uint4*>(rows.k + (h0 + i) * rows.head + at);
                 v[i] = *reinterpret_cast<const uint4*>(rows.v + (h0 + i) * rows.head + at);
@@ -112,7 +112,7 @@ paged_move_kernel(const PagedArgs c, const PagedRows rows)
         }
     }
     #pragma unroll
-    for (int i = 0; i < PC_HEADS; i++) {
+    for (int i = 0; i < PC_HEADS<F8>; i++) {
         const int h = h0 + i;
         if (h >= c.H_kv) break;
         const int in_page = (h << c.page_shift) + slot;
@@ -195,7 +195,7 @@ template <int D, bool F8>
 int launch_move(bool read, const PagedArgs& a, const PagedRows& rows, cudaStream_t stream)
 {
     const int per_block = PC_THREADS / 32 * (256 / D);
-    const dim3 grid((a.tokens + per_block - 1) / per_block, (a.H_kv + PC_HEADS - 1) / PC_HEADS);
+    const dim3 grid((a.tokens + per_block - 1) / per_block, (a.H_kv + PC_HEADS<F8> - 1) / PC_HEADS<F8>);
     EFA_CUDA(read ? paged_launch(paged_move_kernel<D, F8, true>, grid, PC_THREADS, 0, stream, a, rows)
                   : paged_launch(paged_move_kernel<D, F8, false>, grid, PC_THREADS, 0, stream, a, rows));
     return 0;
@@ -229,8 +229,10 @@ PagedPlan plan_attention(const efa_paged_cache& c, const efa_paged_batch& b, con
     PagedPlan plan{};
     const int G = p.H_q / c.H_kv;
     const long long rows = (long long)b.max_q * G, kv_cap = std::min<long long>(b.max_kv, (long long)b.max_pages * c.page_size);
-    // Rows for which the keys' way to the SM is the time go to the kernel of small tiles, more to the tensor cores' tiles of 256.
-    plan.chunk = rows > 64;
+    // Rows for which the keys' way to the SM is the time go to the kernel of small tiles, more to the tensor cores' tiles of 256; in between the small tiles are
+    // faster while there are few keys. us, small tiles / tiles of 256: 64 rows, 8 heads of 128, 1000 keys 14 / 19, 2 x 16000 keys 57 / 47, 16 x 16000
+    // 296 / 190, of 8 bits 310 / 228; 64 rows, 8 x 16 heads of 64, 1000 keys 21 / 17; 32 rows, 16 x 16000 keys 171 / 186.
+    plan.chunk = rows > 64 || (rows > 32 && (double)b.num_seqs * c.H_kv * (double)kv_cap > 65536);
     const int tile = plan.chunk ? PAGED_CHUNK_TILE : paged_rows_tile((int)rows), unit = plan.chunk ? PAGED_CHUNK_UNIT : paged_rows_unit(c.dtype == EFA_E4M3);
     plan.w = PagedShape{G, p.causal ? 1 : 0, tile, unit, plan.chunk ? PAGED_CHUNK_EXTRA : PAGED_ROWS_EXTRA, (int)((rows + tile - 1) / tile)};
     const long long items = (long long)b.num_seqs * c.H_kv * plan.w.max_tiles, units = std::max<long long>(1, (kv_cap + unit - 1) / unit);
@@ -252,7 +254,7 @@ PagedPlan plan_attention(const efa_paged_cache& c, const efa_paged_batch& b, con
         const double each = tiles * (first + longest) / 2 / parts;
         const double by_item = even ? std::ceil(tiles / parts) * longest : std::max(longest, each * 1.05);
         const double by_share = std::max(MIN_SHARE, each) * 1.05 + MERGE;
-        plan.cut = by_item > by_share * (!f8 && plan.w.max_tiles >= 16 ? 1.1 : 1.0);
+        plan.cut = by_item > by_share * (!f8 && plan.w.max_tiles >= 16 ? 1.15 : 1.0);
         parts = (int)std::min<double>(parts, std::max(1.0, each * parts / MIN_SHARE));
     } else {
         // Few rows: a block per item, or where there are few items a cluster of up to eight that shares one, merged in shared memory, as long as a block's part of

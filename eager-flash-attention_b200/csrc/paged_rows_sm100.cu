@@ -24,6 +24,12 @@ namespace {
 
 constexpr int PR_THREADS = 128;
 
+// Blocks of an SM and stages of each: where loading is the time (fp16 heads of 64 and 128) few blocks with deep rings, else more warps. us, 64 sequences of 4096
+// keys, one token, as here / as two blocks of 96 KB: 16 heads of 64 fp16 172 / 172 (three blocks of 64 KB: 210), 8 bits 124 / 138; 32 heads of
+// 32 179 / 206, 183 / 254; 64 heads of 16 269 / 484, 312 / 563; 16 sequences of 16000 keys, 8 heads of 128 165 / 165, 97 / 101.
+constexpr int rows_blocks(int d, bool f8) { return d >= 64 ? (f8 ? 3 : 2) : d == 16 && f8 ? 6 : 4; }
+constexpr int rows_stages(int d, bool f8) { return d == 128 ? (f8 ? 2 : 3) : d == 64 ? (f8 ? 4 : 6) : d == 16 && f8 ? 4 : 6; }
+
 template <int D, bool F8, int WM>
 struct RowsCfg {
     static constexpr int WK = F8 ? 32 : 16;                                   // keys that a warp copies of a unit
@@ -32,7 +38,8 @@ struct RowsCfg {
     static constexpr int RB = D * (F8 ? 1 : 2);                               // bytes of a key
     static constexpr int STAGE = 2 * KS * RB + (F8 ? 2 * KS : 0);             // of a team
     static constexpr int UNIT_BYTES = TEAMS * STAGE;
-    static constexpr int STAGES = UNIT_BYTES >= 32768 ? 3 : UNIT_BYTES >= 16384 ? 6 : 8;
+    static constexpr int BLOCKS = rows_blocks(D, F8);
+    static constexpr int STAGES = rows_stages(D, F8);
     static constexpr int RING = STAGES * UNIT_BYTES;
     static constexpr int OPITCH = D + 4;
     static constexpr int MERGE = 4 * 16 * OPITCH * 4 + 8 * 16 * 8;            // four warps' O, their (m, l), and that of the block
@@ -121,7 +128,7 @@ __device__ __forceinline__ void store_row8(__half* dst, const float (&acc)[8], f
 }
 
 template <int D, bool F8, int WM>
-__global__ void __launch_bounds__(PR_THREADS, 2)
+__global__ void __launch_bounds__(PR_THREADS, (RowsCfg<D, F8, WM>::BLOCKS))
 paged_rows_kernel(const PagedArgs c, const PagedAttnArgs a)
 {
     using C = RowsCfg<D, F8, WM>;
@@ -605,7 +612,7 @@ int launch_rows(const PagedArgs& c, const PagedAttnArgs& a, int blocks, int clus
 
 int paged_rows_tile(int rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
 
-int paged_rows_blocks_per_sm(int d_h, bool f8) { (void)d_h; (void)f8; return 2; }
+int paged_rows_blocks_per_sm(int d_h, bool f8) { return rows_blocks(d_h, f8); }
 int paged_rows_unit(bool f8) { return f8 ? 128 : 64; }
 
 int paged_rows_launch(const PagedArgs& c, const PagedAttnArgs& a, int d_h, bool f8, int blocks, int cluster, cudaStream_t stream)
