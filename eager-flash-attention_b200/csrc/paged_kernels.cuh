@@ -10,7 +10,7 @@ struct PagedAttnArgs {
     const __half* Q;
     __half* O;
     long long q_head, q_token, o_token;     // strides in elements
-    float scale_log2e, rescale_above;       // log2 units by which a maximum may outgrow the exponent offset in use (paged_chunk_kernel)
+    float scale_log2e, rescale_above;       // log2 units by which a maximum may outgrow the exponent offset in use
     PagedShape w;
     PagedParts parts;                       // all null: nothing is cut, one block per item
 };

@@ -325,29 +325,35 @@ paged_rows_kernel(const PagedArgs c, const PagedAttnArgs a)
                             if (F8 && key >= q.kv) vscale[nt][x & 1] = 0.f;      // no key: its bytes may be anything
                         }
                 }
-                // The offset is the largest weight's so far: of e4m3 with the exponent of its value, which stays out of the converted values (exact) and
-                // goes into the weights, so that what is rounded to fp16 is largest where it counts.
-                float off[2], alpha[2];
+                // The offset m is a row's largest weight so far, or up to rescale_above less: O is rescaled when it moves, and of 16 rows one would nearly always have a
+                // new maximum. Of e4m3 with the exponent of the value, which stays out of the converted values (exact) and goes into the weights, so
+                // that what is rounded to fp16 is largest where it counts.
+                float off[2], mx[2];
                 #pragma unroll
                 for (int half = 0; half < 2; half++) {
-                    float mx = m[half];
+                    mx[half] = -INFINITY;
                     #pragma unroll
                     for (int nt = 0; nt < KT; nt++) {
-                        if constexpr (F8) mx = max3(mx, s[nt][half * 2] + vlog[nt][0], s[nt][half * 2 + 1] + vlog[nt][1]);
-                        else mx = max3(mx, s[nt][half * 2], s[nt][half * 2 + 1]);
+                        if constexpr (F8) mx[half] = max3(mx[half], s[nt][half * 2] + vlog[nt][0], s[nt][half * 2 + 1] + vlog[nt][1]);
+                        else mx[half] = max3(mx[half], s[nt][half * 2], s[nt][half * 2 + 1]);
                     }
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                    off[half] = mx == -INFINITY ? 0.f : mx;
-                    alpha[half] = m[half] == mx ? 1.f : ex2(m[half] - off[half]);
-                    m[half] = mx;
+                    mx[half] = fmaxf(mx[half], __shfl_xor_sync(0xffffffffu, mx[half], 1));
+                    mx[half] = fmaxf(mx[half], __shfl_xor_sync(0xffffffffu, mx[half], 2));
                 }
-                if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
+                if (__any_sync(0xffffffffu, mx[0] > m[0] + a.rescale_above || mx[1] > m[1] + a.rescale_above)) {
+                    float alpha[2];
+                    #pragma unroll
+                    for (int half = 0; half < 2; half++) {
+                        const float top = fmaxf(m[half], mx[half]);
+                        alpha[half] = m[half] == top ? 1.f : ex2(m[half] - (top == -INFINITY ? 0.f : top));
+                        m[half] = top;
+                        l[half] *= alpha[half];
+                    }
                     #pragma unroll
                     for (int j = 0; j < NT; j++) { o[j][0] *= alpha[0]; o[j][1] *= alpha[0]; o[j][2] *= alpha[1]; o[j][3] *= alpha[1]; }
-                    l[0] *= alpha[0];
-                    l[1] *= alpha[1];
                 }
+                #pragma unroll
+                for (int half = 0; half < 2; half++) off[half] = m[half] == -INFINITY ? 0.f : m[half];
                 uint32_t p[STEP][4];
                 #pragma unroll
                 for (int nt = 0; nt < KT; nt++)
