@@ -346,6 +346,8 @@ def paged_cache(k, v, k_exp=None, v_exp=None) -> PagedCache:
         raise EfaError(f"paged_cache: {k.dtype} is neither fp16 nor 8-bit codes")
     if tuple(k.stride()[1:]) != (size * d_h, d_h, 1):
         raise EfaError("paged_cache: a page must be dense")
+    if any(x is not None and x.device != k.device for x in (v, k_exp, v_exp)):
+        raise EfaError("paged_cache: the tensors must be on one device")
     for e in (k_exp, v_exp):
         if (dtype == E4M3) != (e is not None):
             raise EfaError("paged_cache: 8-bit codes come with k_exp and v_exp, fp16 without")
@@ -362,6 +364,8 @@ def paged_batch(q_start, kv_len, pages, tokens: int, max_q: int, max_kv: int) ->
     n = kv_len.numel()
     if any(str(x.dtype) != "torch.int32" or not x.is_contiguous() for x in (q_start, kv_len, pages)):
         raise EfaError("paged_batch: q_start, kv_len and pages must be dense int32 tensors")
+    if kv_len.device != q_start.device or pages.device != q_start.device:
+        raise EfaError("paged_batch: the tensors must be on one device")
     if q_start.numel() != n + 1 or pages.dim() != 2 or pages.shape[0] != n:
         raise EfaError("paged_batch: q_start must be [num_seqs + 1], kv_len [num_seqs], pages [num_seqs][max_pages]")
     b = PagedBatch(_ptr(q_start), _ptr(kv_len), _ptr(pages), n, pages.shape[1], tokens, max_q, max_kv)

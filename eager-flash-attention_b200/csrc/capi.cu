@@ -107,21 +107,21 @@ extern "C" size_t efa_paged_attention_workspace(const efa_paged_cache* cache, co
 extern "C" int efa_cache_write(const void* K, const void* V, int64_t head_stride, int64_t token_stride,
                                const efa_paged_cache* cache, const efa_paged_batch* batch, void* stream)
 {
-    if (!K || !V || !cache || !batch) { set_error("efa_cache_write: null argument"); return 2; }
+    if (!cache || !batch) { set_error("efa_cache_write: null argument"); return 2; }
     return cache_write(K, V, head_stride, token_stride, *cache, *batch, (cudaStream_t)stream);
 }
 
 extern "C" int efa_cache_read(void* K, void* V, int64_t head_stride, int64_t token_stride,
                               const efa_paged_cache* cache, const efa_paged_batch* batch, void* stream)
 {
-    if (!K || !V || !cache || !batch) { set_error("efa_cache_read: null argument"); return 2; }
+    if (!cache || !batch) { set_error("efa_cache_read: null argument"); return 2; }
     return cache_read(K, V, head_stride, token_stride, *cache, *batch, (cudaStream_t)stream);
 }
 
 extern "C" int efa_paged_attention(const void* Q, void* O, const efa_paged_cache* cache, const efa_paged_batch* batch,
                                    const efa_paged_attention_params* p, void* workspace, size_t workspace_bytes, void* stream)
 {
-    if (!Q || !O || !cache || !batch || !p) { set_error("efa_paged_attention: null argument"); return 2; }
+    if (!cache || !batch || !p) { set_error("efa_paged_attention: null argument"); return 2; }
     return paged_attention(Q, O, *cache, *batch, *p, workspace, workspace_bytes, (cudaStream_t)stream);
 }
 

@@ -100,11 +100,12 @@ def test_a_workspace_that_is_missing_or_short_is_refused(pkg):
 def test_empty_batches_launch_nothing(pkg):
     """Without a GPU a launch would fail."""
     ap = pkg.paged_attention_params(8, 128)
-    for b in (_batch(pkg, num_seqs=0), _batch(pkg, tokens=0)):
-        pkg.cache_write(AT, AT, _cache(pkg), b)
-        pkg.cache_read(AT, AT, _cache(pkg), b)
-        pkg.paged_attention(AT, AT, _cache(pkg), b, ap)
-    pkg.paged_attention(AT, AT, _cache(pkg), _batch(pkg, max_q=0), ap)
+    i = lambda *shape: torch.zeros(shape, dtype=torch.int32)  # noqa: E731
+    for b in (_batch(pkg, num_seqs=0), _batch(pkg, tokens=0), _batch(pkg, max_q=0), pkg.paged_batch(i(1), i(0), i(0, 4), 0, 0, 0)):
+        for rows in (AT, torch.zeros(8, 0, 128, dtype=torch.float16)):       # an empty tensor has no address
+            pkg.cache_write(rows, rows, _cache(pkg), b)
+            pkg.cache_read(rows, rows, _cache(pkg), b)
+            pkg.paged_attention(rows, rows, _cache(pkg), b, ap)
 
 
 def test_tensors_that_do_not_fit_together_are_refused(pkg):
