@@ -152,9 +152,9 @@ __device__ __forceinline__ PagedPiece paged_piece(const PagedArgs& c, const Page
 struct PagedScratch { int warp_sum[32]; PagedAt at; };
 
 // The weight of share `part` of `parts` and where it begins, found by all THREADS threads of a block together; 0: there is less weight
-// than shares, and none for this one.
+// than shares, and none for this one. Block 0, which like all others looks at every sequence, reports lengths that are wrong.
 template <int THREADS>
-__device__ int paged_part(const PagedArgs& c, const PagedShape& w, int part, int parts, PagedScratch& s, PagedAt& at)
+__device__ int paged_part(const PagedArgs& c, const PagedShape& w, int part, int parts, PagedScratch& s, PagedAt& at, int site)
 {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int entries = c.num_seqs * w.max_tiles, per = (int)((unsigned)(entries + THREADS - 1) / THREADS);
@@ -162,7 +162,7 @@ __device__ int paged_part(const PagedArgs& c, const PagedShape& w, int part, int
     int sum = 0;
     for (int e = e0; e < e1; ) {
         const int b = (int)((unsigned)e / (unsigned)w.max_tiles), rt0 = e - b * w.max_tiles;
-        const PagedSeq q = paged_seq(c, b);
+        const PagedSeq q = part == 0 ? paged_seq<true>(c, b, site) : paged_seq(c, b);
         const int stop = min(paged_tiles(w, q), rt0 + e1 - e);
         for (int rt = rt0; rt < stop; rt++) sum += paged_units(w, q, rt) + w.extra;
         e = (b + 1) * w.max_tiles;

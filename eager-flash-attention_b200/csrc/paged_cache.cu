@@ -292,7 +292,7 @@ const char* paged_check(const efa_paged_cache& c, const efa_paged_batch& b)
     if (b.num_seqs < 0 || b.tokens < 0 || b.max_q < 0 || b.max_kv < 0) return "paged: negative size";
     if (b.max_pages < 1) return "paged: max_pages must be positive";
     if (b.num_seqs > 0 && (!b.q_start || !b.kv_len || !b.pages)) return "paged: q_start, kv_len and pages must not be null";
-    if ((long long)b.num_seqs * b.max_pages > INT_MAX || (long long)c.H_kv * c.page_size * c.d_h > INT_MAX) return "paged: sizes too large";
+    if (b.tokens > 1 << 30 || b.max_q > 1 << 30 || b.max_kv > 1 << 30 || (long long)b.num_seqs * b.max_pages > INT_MAX || (long long)c.H_kv * c.page_size * c.d_h > INT_MAX) return "paged: sizes too large";
     return nullptr;
 }
 

@@ -104,7 +104,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     int left;
     const bool cut = a.parts.cut != nullptr;
     if (cut) {
-        left = paged_part<C::THREADS>(c, a.w, blockIdx.x, gridDim.x, scratch, at);
+        left = paged_part<C::THREADS>(c, a.w, blockIdx.x, gridDim.x, scratch, at, 53);
     } else {                                            // an item per block, of all sequences those of the last rows first: they are the longest
         const int group = c.H_kv * c.num_seqs, level = blockIdx.x / group, rest = blockIdx.x - level * group;
         at = PagedAt{rest % c.H_kv, rest / c.H_kv, a.w.max_tiles - 1 - level, 0};
@@ -127,7 +127,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     if (tid == FINDER) {
         if (cut) {
             PagedCut here{};
-            if (left > 0) here = PagedCut{at.h, at.b, at.rt, max(0, at.off - a.w.extra), paged_units(a.w, paged_seq<true>(c, at.b, 53), at.rt), 0, 0, 0};
+            if (left > 0) here = PagedCut{at.h, at.b, at.rt, max(0, at.off - a.w.extra), paged_units(a.w, paged_seq(c, at.b), at.rt), 0, 0, 0};
             a.parts.cut[blockIdx.x] = here;
         } else if (at.rt == 0 && at.h == 0) {
             paged_seq<true>(c, at.b, 53);

@@ -150,11 +150,11 @@ paged_rows_kernel(const PagedArgs c, const PagedAttnArgs a)
     int left;
     const bool cut = a.parts.cut != nullptr;
     if (cut) {
-        left = paged_part<PR_THREADS>(c, a.w, blockIdx.x, gridDim.x, scratch, at);
+        left = paged_part<PR_THREADS>(c, a.w, blockIdx.x, gridDim.x, scratch, at, 51);
         first = at;
         if (tid == 0) {
             PagedCut here{};
-            if (left > 0) here = PagedCut{at.h, at.b, at.rt, max(0, at.off - a.w.extra), paged_units(a.w, paged_seq<true>(c, at.b, 51), at.rt), 0, 0, 0};
+            if (left > 0) here = PagedCut{at.h, at.b, at.rt, max(0, at.off - a.w.extra), paged_units(a.w, paged_seq(c, at.b), at.rt), 0, 0, 0};
             a.parts.cut[blockIdx.x] = here;
         }
     } else {

@@ -205,7 +205,8 @@ typedef struct efa_paged_attention_params {
 
 const char* efa_paged_attention_check(const efa_paged_cache* cache, const efa_paged_batch* batch, const efa_paged_attention_params* p);
 
-/* Bytes of workspace that efa_paged_attention needs for these sizes on the current device (may be 0). Host arithmetic only. */
+/* Bytes of workspace that efa_paged_attention needs for these sizes on the current device; may be 0, and is 0 for what efa_paged_attention_check
+ * refuses. Host arithmetic only. */
 size_t efa_paged_attention_workspace(const efa_paged_cache* cache, const efa_paged_batch* batch, const efa_paged_attention_params* p);
 
 /* Attention of the chunks over the cache, the chunk's own keys included (efa_cache_write first): O[row][h * d_h + x], fp16, what
@@ -219,7 +220,7 @@ int efa_paged_attention(const void* Q, void* O, const efa_paged_cache* cache, co
 
 /* Status word written by kernels whose bounded waits ran out, or that found lengths or pages of a paged batch wrong: out4 = {code, block, site, 0};
  * code 0 = no kernel reported a problem since the last efa_kernel_status_reset(), 1 = a wait ran out, 2 = a page outside the pool, 3 = a
- * length outside its bounds (2, 3: the sequence in place of the block; site 50 = write or read, 51, 52 = attention). */
+ * length outside its bounds (2, 3: the sequence in place of the block; site 50 = write or read, 51 to 54 = attention). */
 int efa_kernel_status(int* out4);
 int efa_kernel_status_reset(void);
 

@@ -49,7 +49,8 @@ def test_caches_that_are_refused(pkg, change, why):
 
 @pytest.mark.parametrize("change,why", [
     (dict(num_seqs=-1), "negative"), (dict(tokens=-1), "negative"), (dict(max_q=-1), "negative"), (dict(max_kv=-1), "negative"), (dict(max_pages=0), "max_pages"),
-    (dict(q_start=None), "null"), (dict(kv_len=None), "null"), (dict(pages=None), "null"), (dict(num_seqs=1 << 20, max_pages=1 << 20), "too large")])
+    (dict(q_start=None), "null"), (dict(kv_len=None), "null"), (dict(pages=None), "null"), (dict(num_seqs=1 << 20, max_pages=1 << 20), "too large"),
+    (dict(max_kv=(1 << 30) + 1), "too large"), (dict(max_q=(1 << 30) + 1), "too large"), (dict(tokens=(1 << 30) + 1), "too large")])
 def test_batches_that_are_refused(pkg, change, why):
     assert why in pkg.paged_check(_cache(pkg), _batch(pkg, **change))
     with pytest.raises(pkg.EfaError, match=why):

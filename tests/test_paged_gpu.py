@@ -1,5 +1,6 @@
 """The paged key/value cache on a GPU: writing, reading back and attention against the definitions in 64 bits."""
 import math
+import random
 
 import pytest
 import torch
@@ -147,6 +148,28 @@ def test_strides_of_rows_and_pages(pkg, bits):
     assert torch.equal(O[:, :6 * d], want) and torch.all(O[:, 6 * d:] == 9)
 
 
+def test_rows_may_begin_anywhere_and_sequences_be_empty(pkg):
+    """Rows ahead of the first sequence's belong to nobody; a batch padded with empty sequences; more of them than a block has threads."""
+    d, H = 64, 2
+    kv, q = [0, 5, 0] + [3] * 300 + [0, 77, 0], [0, 5, 0] + [1] * 300 + [0, 9, 0]
+    batch = Batch(pkg, kv, q, 16, first_row=7, extra_rows=4)
+    for bits in (16, 8):
+        pool = Pool(pkg, batch.num_pages, H, 16, d, bits)
+        fill_random(pool, batch, 1)
+        K, V, Q = _rows(1, H, batch.tokens, d), _rows(2, H, batch.tokens, d), _rows(3, 6, batch.tokens, d)
+        pkg.cache_write(K, V, pool.cache, batch.batch)
+        Ko, Vo = torch.full_like(K, 5), torch.full_like(V, 5)
+        pkg.cache_read(Ko, Vo, pool.cache, batch.batch)
+        torch.cuda.synchronize()
+        last = batch.starts[-1]
+        assert torch.equal(Ko[:, 7:last], (K if bits == 16 else decode(*encode(K)).half())[:, 7:last])
+        assert torch.all(Ko[:, :7] == 5) and torch.all(Ko[:, last:] == 5) and torch.all(Vo[:, :7] == 5) and torch.all(Vo[:, last:] == 5)
+        O = _attend(pkg, Q, pool, batch)
+        check_attention(O, Q, pool, batch, d ** -0.5, 1)
+        assert torch.all(O[:7] == 777) and torch.all(O[last:] == 777)
+    assert pkg.kernel_status()[0] == 0
+
+
 # ---- attention ---------------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("bits", [16, 8])
 @pytest.mark.parametrize("d", [16, 32, 64, 128])
@@ -180,6 +203,56 @@ def test_attention_over_long_sequences(pkg, bits, d, H, G, kv, q):
     fill_random(pool, batch, 3)
     Q = _rows(9, H * G, batch.tokens, d, spread=3)
     check_attention(_attend(pkg, Q, pool, batch), Q, pool, batch, d ** -0.5, 1)
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("H,G,d,q", [(1, 33, 64, 1), (1, 48, 128, 2), (1, 100, 32, 1), (2, 128, 128, 1), (1, 300, 16, 3)])
+def test_groups_of_many_heads(pkg, bits, H, G, d, q):
+    for kv in ([40, 130], [9000, 77]):
+        batch = Batch(pkg, kv, [q] * len(kv), 32)
+        pool = Pool(pkg, batch.num_pages, H, 32, d, bits)
+        fill_random(pool, batch, 3)
+        Q = _rows(9, H * G, batch.tokens, d, spread=3)
+        check_attention(_attend(pkg, Q, pool, batch), Q, pool, batch, d ** -0.5, 1)
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_batches_at_random(pkg, seed):
+    """Every kind of launch: blocks or clusters that have an item, equal shares with a merge, small tiles and tiles of 256 rows; loose and tight bounds."""
+    rng = random.Random(seed)
+    size = lambda lo, hi: int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))  # noqa: E731
+    d, bits, page = rng.choice([16, 32, 64, 128]), rng.choice([16, 8]), rng.choice([16, 32, 64, 128, 256])
+    H, G, causal = rng.choice([1, 2, 3, 8]), rng.choice([1, 2, 4, 5, 8]), rng.random() < 0.8
+    seqs, most, rows = size(1, 40), size(1, 12000), size(1, 700)
+    while seqs * most * H * d > 1 << 26 or seqs * most * rows * H * G > 1 << 27:
+        seqs, most, rows = max(1, seqs // 2), max(1, most * 2 // 3), max(1, rows * 2 // 3)
+    kv = [rng.choice([0, 1, most, rng.randint(0, most)]) if rng.random() < 0.5 else rng.randint(most // 2, most) for _ in range(seqs)]
+    q = [min(rng.choice([0, 1, rows, rng.randint(0, rows)]), n + 3) for n in kv]
+    loose = rng.random() < 0.4
+    batch = Batch(pkg, kv, q, page, seed=seed, extra_rows=rng.randint(0, 3), first_row=rng.randint(0, 2), max_q=rows + 3 if loose else None,
+                  max_kv=most + rng.randint(0, 5000) if loose else None, width=-(-max(kv + [1]) // page) + (40 if loose else 0))
+    pool = Pool(pkg, batch.num_pages, H, page, d, bits, gap=rng.choice([0, 0, 64]))
+    fill_random(pool, batch, seed)
+    Q = _rows(seed, H * G, batch.tokens, d, spread=rng.choice([0.5, 2, 6]))
+    O = _attend(pkg, Q, pool, batch, int(causal))
+    check_attention(O, Q, pool, batch, d ** -0.5, causal)
+    assert torch.all(O[:batch.starts[0]] == 777) and torch.all(O[batch.starts[-1]:] == 777)
+    assert pkg.kernel_status()[0] == 0
+
+
+def test_wrong_lengths_anywhere_in_a_large_batch_are_reported(pkg):
+    for max_kv in (64, 4000):                                                # a block per item; equal shares
+        batch = Batch(pkg, [50] * 200, [1] * 200, 16, max_kv=max_kv, width=max_kv // 16)
+        pool = Pool(pkg, batch.num_pages, 1, 16, 64, 16)
+        fill_random(pool, batch, 1)
+        Q = _rows(4, 2, batch.tokens, 64)
+        for b in (0, 1, 77, 199):
+            batch.dev[1][b] = max_kv + 1
+            O = _attend(pkg, Q, pool, batch)
+            assert pkg.kernel_status()[:2] == (3, b)
+            pkg.kernel_status_reset()
+            batch.dev[1][b] = 50
+            check_attention(O, Q, pool, batch, 0.125, 1, skip=(b,))
 
 
 @pytest.mark.parametrize("bits", [16, 8])
