@@ -11,11 +11,13 @@
 //     has of an item that is cut goes to the workspace, as fp32 O relative to the row's maximum, and is merged afterwards.
 #pragma once
 
+template <bool F8> constexpr int chunk_threads = F8 ? 512 : 384;
+
 template <int D, bool F8>
 struct ChunkCfg {
     // Threads: the softmax's 256, a warpgroup of producer, issuer and warps 10 and 11, and for e4m3 another that converts. Registers of each:
     // together no more than the block is launched with.
-    static constexpr int THREADS    = F8 ? 512 : 384;
+    static constexpr int THREADS    = chunk_threads<F8>;
     static constexpr int REG_SOFTMAX = F8 ? 208 : 224, REG_ISSUE = F8 ? 40 : 56, REG_CONVERT = 56;
     static constexpr int REGS       = 256 * REG_SOFTMAX + 128 * REG_ISSUE + (F8 ? 128 * REG_CONVERT : 0);
     static constexpr int SWB        = D >= 64 ? 128 : D * 2;
@@ -54,7 +56,7 @@ __device__ __forceinline__ void sts128(uint32_t at, const uint4& v)
 }
 
 template <int D, bool F8>
-__global__ void __launch_bounds__((ChunkCfg<D, F8>::THREADS), 1)
+__global__ void __launch_bounds__(chunk_threads<F8>, 1)
 paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const PagedArgs c, const PagedAttnArgs a)
 {
     using C = ChunkCfg<D, F8>;

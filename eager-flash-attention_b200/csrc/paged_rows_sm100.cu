@@ -28,6 +28,7 @@ constexpr int PR_THREADS = 128;
 // keys, one token, as here / as two blocks of 96 KB: 16 heads of 64 fp16 172 / 172 (three blocks of 64 KB: 210), 8 bits 124 / 138; 32 heads of
 // 32 179 / 206, 183 / 254; 64 heads of 16 269 / 484, 312 / 563; 16 sequences of 16000 keys, 8 heads of 128 165 / 165, 97 / 101.
 constexpr int rows_blocks(int d, bool f8) { return d >= 64 ? (f8 ? 3 : 2) : d == 16 && f8 ? 6 : 4; }
+template <int D, bool F8> constexpr int blocks_of = rows_blocks(D, F8);
 constexpr int rows_stages(int d, bool f8) { return d == 128 ? (f8 ? 2 : 3) : d == 64 ? (f8 ? 4 : 6) : d == 16 && f8 ? 4 : 6; }
 
 template <int D, bool F8, int WM>
@@ -38,7 +39,6 @@ struct RowsCfg {
     static constexpr int RB = D * (F8 ? 1 : 2);                               // bytes of a key
     static constexpr int STAGE = 2 * KS * RB + (F8 ? 2 * KS : 0);             // of a team
     static constexpr int UNIT_BYTES = TEAMS * STAGE;
-    static constexpr int BLOCKS = rows_blocks(D, F8);
     static constexpr int STAGES = rows_stages(D, F8);
     static constexpr int RING = STAGES * UNIT_BYTES;
     static constexpr int OPITCH = D + 4;
@@ -128,7 +128,7 @@ __device__ __forceinline__ void store_row8(__half* dst, const float (&acc)[8], f
 }
 
 template <int D, bool F8, int WM>
-__global__ void __launch_bounds__(PR_THREADS, (RowsCfg<D, F8, WM>::BLOCKS))
+__global__ void __launch_bounds__(PR_THREADS, blocks_of<D, F8>)
 paged_rows_kernel(const PagedArgs c, const PagedAttnArgs a)
 {
     using C = RowsCfg<D, F8, WM>;
