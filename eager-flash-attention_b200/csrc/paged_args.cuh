@@ -101,9 +101,14 @@ __device__ __forceinline__ uint32_t nonfinite_f16x2(uint32_t x)
 // `unit` keys, as many as its last row sees, and its weight is its units plus `extra` for what an item costs besides them. All items
 // in a row (heads outermost) are cut into as many shares of equal weight as there are blocks: no length of any sequence leaves an SM idle.
 // An item that a cut goes through is merged afterwards (paged_merge_kernel).
+// Equal shares of what memory has to deliver do not end together: some SMs get a tenth less of it than others (64 sequences of 8000 keys, 8 heads of 128:
+// blocks end between 252 and 309 us). So the last `late` blocks, which start as others end, have a tenth of a share each, if that is still
+// LATE_UNITS: the faster SMs take them.
 struct PagedShape {
     int G, causal, tile, unit, extra, max_tiles;   // query heads per kv head; rows of a tile; keys of a unit; ...; tiles of the longest chunk
+    int late;
 };
+constexpr unsigned LATE_UNITS = 4, LATE_RATIO = 10;
 
 __device__ __forceinline__ int paged_tiles(const PagedShape& w, const PagedSeq& s) { return (int)((unsigned)(s.n * w.G + w.tile - 1) / (unsigned)w.tile); }
 
@@ -183,10 +188,19 @@ __device__ int paged_part(const PagedArgs& c, const PagedShape& w, int part, int
     }
     before -= sum;
     const unsigned all = (unsigned)total * (unsigned)c.H_kv;        // below 2^31 (paged_attention_check)
-    parts = (int)min(all, (unsigned)parts);
-    if (part >= parts) return 0;
-    const unsigned each = all / (unsigned)parts, more = all - each * (unsigned)parts;        // the first `more` shares have one more
-    const unsigned begin = (unsigned)part * each + min((unsigned)part, more);
+    const unsigned big = (unsigned)(parts - w.late), weights = big * LATE_RATIO + (unsigned)w.late;
+    unsigned begin, end;
+    if (w.late > 0 && all / LATE_UNITS >= weights) {
+        auto at_part = [&](unsigned p) { return (unsigned)((unsigned long long)all * (min(p, big) * LATE_RATIO + (p > big ? p - big : 0)) / weights); };
+        begin = at_part((unsigned)part);
+        end = at_part((unsigned)part + 1);
+    } else {
+        const unsigned n = min(all, big);
+        if ((unsigned)part >= n) return 0;
+        const unsigned each = all / n, more = all - each * n;               // the first `more` shares have one more
+        begin = (unsigned)part * each + min((unsigned)part, more);
+        end = begin + each + ((unsigned)part < more ? 1 : 0);
+    }
     const int h = (int)(begin / (unsigned)total), rest = (int)begin - h * total;
     if (rest >= before && rest < before + sum) {
         int left = rest - before;
@@ -204,7 +218,7 @@ __device__ int paged_part(const PagedArgs& c, const PagedShape& w, int part, int
     }
     __syncthreads();
     at = s.at;
-    return (int)each + ((unsigned)part < more ? 1 : 0);
+    return (int)(end - begin);
 }
 
 // Where blocks leave their pieces of items that a cut goes through: two places a block, one for the item that its share begins with and one

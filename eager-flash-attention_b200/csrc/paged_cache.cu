@@ -278,7 +278,7 @@ PagedPlan plan_attention(const efa_paged_cache& c, const efa_paged_batch& b, con
     // 296 / 190, of 8 bits 310 / 228; 64 rows, 8 x 16 heads of 64, 1000 keys 21 / 17; 32 rows, 16 x 16000 keys 171 / 186.
     plan.chunk = rows > 64 || (rows > 32 && (double)b.num_seqs * c.H_kv * (double)kv_cap > 65536);
     const int tile = plan.chunk ? PAGED_CHUNK_TILE : paged_rows_tile((int)rows), unit = plan.chunk ? PAGED_CHUNK_UNIT : paged_rows_unit(c.dtype == EFA_E4M3);
-    plan.w = PagedShape{G, p.causal ? 1 : 0, tile, unit, plan.chunk ? PAGED_CHUNK_EXTRA : PAGED_ROWS_EXTRA, (int)((rows + tile - 1) / tile)};
+    plan.w = PagedShape{G, p.causal ? 1 : 0, tile, unit, plan.chunk ? PAGED_CHUNK_EXTRA : PAGED_ROWS_EXTRA, (int)((rows + tile - 1) / tile), 0};
     const long long items = (long long)b.num_seqs * c.H_kv * plan.w.max_tiles, units = std::max<long long>(1, (kv_cap + unit - 1) / unit);
     const bool f8 = c.dtype == EFA_E4M3;
     plan.cluster = 1;
@@ -308,7 +308,13 @@ PagedPlan plan_attention(const efa_paged_cache& c, const efa_paged_batch& b, con
         parts *= paged_rows_blocks_per_sm(c.d_h, f8);
         while (plan.cluster < 8 && plan.cluster * 2 <= units && items * plan.cluster * 2 <= parts) plan.cluster *= 2;
         plan.cut = units * unit > (c.d_h == 128 ? 1024 : 1536) * plan.cluster;
-        if (plan.cut) plan.cluster = 1;
+        if (plan.cut) {
+            plan.cluster = 1;
+            // Where memory is the time (8 bits are not: 177 us without, 185 with): 64 sequences of 4096 keys, 16 heads of 64 173 -> 164 us, of up to 8192, 8 heads of 128
+            // 175 -> 169.5.
+            if (!f8 && c.d_h >= 64 && items * units >= (long long)parts * LATE_RATIO * LATE_UNITS) plan.w.late = parts * 3 / 4;
+            parts += plan.w.late;
+        }
     }
     plan.blocks = (int)std::min<long long>(plan.cut ? std::min<long long>(parts, items * units) : items, INT_MAX);
     if (plan.cut) {
