@@ -53,6 +53,7 @@
 #include <algorithm>
 #include <climits>
 #include <cmath>
+#include <type_traits>
 
 namespace efa {
 
@@ -783,6 +784,36 @@ int launch_form(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap&
 }
 
 #include "paged_chunk.cuh"
+#include "paged_chains.cuh"
+
+// The kernel for a head size and type, its threads, registers and shared memory.
+template <int D, bool F8>
+int launch_paged_chunk(const PagedArgs& c, const PagedAttnArgs& a, int blocks, cudaStream_t stream)
+{
+    constexpr bool CHAINS = !F8 && D <= 64;
+    using C = std::conditional_t<CHAINS, PagedChainCfg<CHAINS ? D : 64>, ChunkCfg<D, F8>>;
+    void (*kernel)(CUtensorMap, CUtensorMap, PagedArgs, PagedAttnArgs);
+    if constexpr (CHAINS) kernel = paged_chains_kernel<D>; else kernel = paged_chunk_kernel<D, F8>;
+    static bool configured[64] = {};
+    int dev = 0;
+    EFA_CUDA(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64 || !configured[dev]) {
+        // The registers that the softmax warps take come out of what the block is launched with: with fewer they would wait for ever.
+        cudaFuncAttributes attr;
+        EFA_CUDA(cudaFuncGetAttributes(&attr, kernel));
+        if ((attr.numRegs + 7) / 8 * 8 * C::THREADS < C::REGS) { set_error("attention kernel compiled to %d registers", attr.numRegs); return 1; }
+        EFA_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES));
+        if (dev >= 0 && dev < 64) configured[dev] = true;
+    }
+    const int page = 1 << c.page_shift, box_rows = page < WS_BN ? page : WS_BN;
+    CUtensorMap tm[2];
+    for (int i = 0; i < 2; i++)
+        if (make_tmap_pages(&tm[i], i ? c.v : c.k, F8 ? 1 : 2, D, (unsigned long long)page * c.H_kv, (unsigned long long)c.num_pages,
+                            (unsigned long long)c.page_stride, F8 ? D : C::SWB / 2, (unsigned)box_rows, F8))
+            return 1;
+    EFA_CUDA(paged_launch(kernel, dim3(blocks), C::THREADS, C::SMEM_BYTES, stream, tm[0], tm[1], c, a));
+    return 0;
+}
 
 template <int D>
 void ring_of(FaPlan& plan, bool halves)

@@ -1,5 +1,5 @@
 // Attention of long chunks over the paged cache (tensor-bound): tiles of 256 rows (token, query head of a group) of one sequence and kv head against its keys,
-// 128 at a time. Included by fa_fwd_ws_sm100.cu, whose kernel's roles, chains and softmax it has: two 128-row tiles, each a chain
+// 128 at a time; heads of 128, and smaller ones of 8 bits (of fp16 they have a kernel of their own, paged_chains.cuh). Included by fa_fwd_ws_sm100.cu, whose kernel's roles, chains and softmax it has: two 128-row tiles, each a chain
 // S -> softmax -> P -> P*V -> Q*K^T -> S in tensor memory, half a period apart. What differs:
 //   * Q's rows come from anywhere (a row's token and head are r / G and r % G): the softmax threads load a row each and swizzle it by hand.
 //   * A stage's keys are pages: one TMA box per page and 64 columns, issued by the lanes of the producer warp side by side. A page that is
@@ -605,29 +605,4 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         __syncthreads();
     }
     if (warp == 9) tmem_dealloc(tmem_base, 512);
-}
-
-template <int D, bool F8>
-int launch_paged_chunk(const PagedArgs& c, const PagedAttnArgs& a, int blocks, cudaStream_t stream)
-{
-    using C = ChunkCfg<D, F8>;
-    static bool configured[64] = {};
-    int dev = 0;
-    EFA_CUDA(cudaGetDevice(&dev));
-    if (dev < 0 || dev >= 64 || !configured[dev]) {
-        // The registers that the softmax warps take come out of what the block is launched with: with fewer they would wait for ever.
-        cudaFuncAttributes attr;
-        EFA_CUDA(cudaFuncGetAttributes(&attr, paged_chunk_kernel<D, F8>));
-        if ((attr.numRegs + 7) / 8 * 8 * C::THREADS < C::REGS) { set_error("attention kernel compiled to %d registers", attr.numRegs); return 1; }
-        EFA_CUDA(cudaFuncSetAttribute(paged_chunk_kernel<D, F8>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES));
-        if (dev >= 0 && dev < 64) configured[dev] = true;
-    }
-    const int page = 1 << c.page_shift, box_rows = page < WS_BN ? page : WS_BN;
-    CUtensorMap tm[2];
-    for (int i = 0; i < 2; i++)
-        if (make_tmap_pages(&tm[i], i ? c.v : c.k, F8 ? 1 : 2, D, (unsigned long long)page * c.H_kv, (unsigned long long)c.num_pages,
-                            (unsigned long long)c.page_stride, F8 ? D : C::BOXC, (unsigned)box_rows, F8))
-            return 1;
-    EFA_CUDA(paged_launch(paged_chunk_kernel<D, F8>, dim3(blocks), C::THREADS, C::SMEM_BYTES, stream, tm[0], tm[1], c, a));
-    return 0;
 }
