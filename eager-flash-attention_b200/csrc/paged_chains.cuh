@@ -265,13 +265,17 @@ paged_chains_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
             const uint32_t tmem_S = tmem_base + ch * 64 + lane_base;
             const uint32_t tmem_O = tmem_base + 256 + ch * 64 + lane_base;
             const int blocks = blocks_of(s_piece[round & 1], tile), n = (blocks - way + 1) >> 1;
-            const int rows = rows_of(s_piece[round & 1], tile), jm = masked_from(s_piece[round & 1]), u_lo = s_piece[round & 1].u_lo;
-            int sees;                                              // keys below this
+            const int jm = masked_from(s_piece[round & 1]);
+            // Little is kept in registers through the loop: what the end needs is found again.
+            auto sees_below = [&](const PagedPiece& p) {           // keys that this thread's row sees; with no such row all that there are
+                return row < rows_of(p, tile) ? min(paged_visible(a.w, p.q, p.rt * 2 * WS_BM + tile * WS_BM + row), p.q.kv) : p.q.kv;
+            };
+            const int lim0 = sees_below(s_piece[round & 1]) - (s_piece[round & 1].u_lo * 2 + way) * 64;
             {
                 const PagedPiece& p = s_piece[round & 1];
+                const int rows = rows_of(p, tile);
                 const bool valid = row < rows;
                 const int r = p.rt * 2 * WS_BM + tile * WS_BM + row;
-                sees = valid ? min(paged_visible(a.w, p.q, r), p.q.kv) : p.q.kv;
                 // ---- half of the warp's 32 rows of Q into the tile (the other chain's warp takes the rest), as many lanes to a row as it has chunks of 16 bytes
                 if (blocks > 0) {
                     const int token = valid ? r / a.w.G : 0;
@@ -309,7 +313,7 @@ paged_chains_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
                 tmem_wait_ld();
 
                 if (i >= jm) {
-                    const int lim = sees - ((u_lo + i) * 2 + way) * 64;
+                    const int lim = lim0 - i * WS_BN;
                     #pragma unroll
                     for (int x = 0; x < 2; x++)
                         #pragma unroll
@@ -402,9 +406,10 @@ paged_chains_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
             constexpr int PER = D / 2 < 16 ? 16 : D / 2;              // columns; of 16 one chain has all
             const int c_lo = way * PER;
 
-            if (ok && (warp & 3) * 32 < rows) {
+            if (ok && (warp & 3) * 32 < rows_of(s_piece[round & 1], tile)) {
                 const PagedPiece& p = s_piece[round & 1];
-                const bool whole = p.u_lo == 0 && p.u_hi == p.units, valid = row < rows, none = sees <= 0;
+                const int sees = sees_below(p), u_lo = p.u_lo;
+                const bool whole = u_lo == 0 && p.u_hi == p.units, valid = row < rows_of(p, tile), none = sees <= 0;
                 const int r = p.rt * 2 * WS_BM + tile * WS_BM + row, token = valid ? r / a.w.G : 0;
                 const float mult = !whole ? 1.f : none ? 0.f : 1.f / l_run;
                 const long long place = s_place[round & 1];
