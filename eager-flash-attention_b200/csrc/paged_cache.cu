@@ -273,14 +273,17 @@ PagedPlan plan_attention(const efa_paged_cache& c, const efa_paged_batch& b, con
     PagedPlan plan{};
     const int G = p.H_q / c.H_kv;
     const long long rows = (long long)b.max_q * G, kv_cap = std::min<long long>(b.max_kv, (long long)b.max_pages * c.page_size);
-    // Rows for which the keys' way to the SM is the time go to the kernel of small tiles, more to the tensor cores' tiles of 256; in between the small tiles are
-    // faster while there are few keys. us, small tiles / tiles of 256: 64 rows, 8 heads of 128, 1000 keys 14 / 19, 2 x 16000 keys 57 / 47, 16 x 16000
-    // 296 / 190, of 8 bits 310 / 228; 64 rows, 8 x 16 heads of 64, 1000 keys 21 / 17; 32 rows, 16 x 16000 keys 171 / 186.
-    plan.chunk = rows > 64 || (rows > 32 && (double)b.num_seqs * c.H_kv * (double)kv_cap > 65536);
-    const int tile = plan.chunk ? PAGED_CHUNK_TILE : paged_rows_tile((int)rows), unit = plan.chunk ? PAGED_CHUNK_UNIT : paged_rows_unit(c.dtype == EFA_E4M3);
+    // Up to 32 rows the keys' way to the SM is the time: small tiles. More go to the tensor cores' tiles of 256 unless there is little work, counted as 64 rows x 64 keys:
+    // small tiles start and end faster, and clusters share theirs. us, small tiles / tiles of 256: 64 rows, 8 heads of 128, 1000 keys 14 / 19, 2 x 16000 keys
+    // 57 / 47, 16 x 16000 296 / 190, of 8 bits 310 / 228; 32 rows, 16 x 16000 keys 171 / 186; prompts, 16 heads of 64, 128 tokens 7.8 / 8.6, 512 12.9 / 14.0,
+    // of 8 bits 256 10.0 / 11.0, 512 18.8 / 14.2; 8 heads of 16, 200 tokens over 400 keys 6.9 / 11.9; 32 heads of 128 on 8, 4 x 64 tokens 9.5 / 11.4, 128 11.2 / 11.3,
+    // 256 16.1 / 12.8.
+    const bool f8 = c.dtype == EFA_E4M3;
+    const double work = (double)b.num_seqs * c.H_kv * (double)((rows + 63) / 64) * (double)((kv_cap + 63) / 64);
+    plan.chunk = rows > 32 && work > (rows <= 64 ? 1024 : c.d_h == 128 ? 128 : c.d_h == 64 ? (f8 ? 256 : 1024) : 2048);
+    const int tile = plan.chunk ? PAGED_CHUNK_TILE : paged_rows_tile((int)rows), unit = plan.chunk ? PAGED_CHUNK_UNIT : paged_rows_unit(f8);
     plan.w = PagedShape{G, p.causal ? 1 : 0, tile, unit, plan.chunk ? PAGED_CHUNK_EXTRA : PAGED_ROWS_EXTRA, (int)((rows + tile - 1) / tile), 0};
     const long long items = (long long)b.num_seqs * c.H_kv * plan.w.max_tiles, units = std::max<long long>(1, (kv_cap + unit - 1) / unit);
-    const bool f8 = c.dtype == EFA_E4M3;
     plan.cluster = 1;
     int parts = device_sms();
     if (plan.chunk) {

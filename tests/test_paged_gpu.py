@@ -181,6 +181,9 @@ def test_rows_may_begin_anywhere_and_sequences_be_empty(pkg):
     (3, 4, 16, [700, 90, 333], [4, 7, 1]),                                   # several tokens: 28 rows
     (2, 3, 128, [400, 77], [17, 20]),                                        # 60 rows
     (2, 2, 32, [300, 700, 33], [130, 33, 33]),                               # more than one tile, chunks from the first token on
+    (8, 3, 16, [2100, 700], [300, 250]),                                     # tiles of 256 rows
+    (8, 4, 64, [6000, 100], [64, 60]),                                       # the same in equal shares
+    (5, 5, 128, [129, 1500, 1025], [129, 205, 1]),
     (1, 1, 256, [900], [700])])
 def test_attention_of_a_chunk(pkg, bits, d, H, G, page, kv, q):
     batch = Batch(pkg, kv, q, page, seed=G, extra_rows=2)
@@ -216,15 +219,15 @@ def test_groups_of_many_heads(pkg, bits, H, G, d, q):
         check_attention(_attend(pkg, Q, pool, batch), Q, pool, batch, d ** -0.5, 1)
 
 
-@pytest.mark.parametrize("seed", range(40))
+@pytest.mark.parametrize("seed", range(60))
 def test_batches_at_random(pkg, seed):
     """Every kind of launch: blocks or clusters that have an item, equal shares with a merge, small tiles and tiles of 256 rows; loose and tight bounds."""
     rng = random.Random(seed)
     size = lambda lo, hi: int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))  # noqa: E731
     d, bits, page = rng.choice([16, 32, 64, 128]), rng.choice([16, 8]), rng.choice([16, 32, 64, 128, 256])
-    H, G, causal = rng.choice([1, 2, 3, 8]), rng.choice([1, 2, 4, 5, 8]), rng.random() < 0.8
+    H, G, causal = rng.choice([1, 2, 3, 8, 16]), rng.choice([1, 2, 4, 5, 8]), rng.random() < 0.8
     seqs, most, rows = size(1, 40), size(1, 12000), size(1, 700)
-    while seqs * most * H * d > 1 << 26 or seqs * most * rows * H * G > 1 << 27:
+    while seqs * most * H * d > 1 << 26 or seqs * most * rows * H * G > 1 << 28:
         seqs, most, rows = max(1, seqs // 2), max(1, most * 2 // 3), max(1, rows * 2 // 3)
     kv = [rng.choice([0, 1, most, rng.randint(0, most)]) if rng.random() < 0.5 else rng.randint(most // 2, most) for _ in range(seqs)]
     q = [min(rng.choice([0, 1, rows, rng.randint(0, rows)]), n + 3) for n in kv]
@@ -307,10 +310,10 @@ def test_rows_that_see_nothing_are_zeros(pkg, bits, long):
 
 @pytest.mark.parametrize("bits", [16, 8])
 @pytest.mark.parametrize("d", [16, 64, 128])
-@pytest.mark.parametrize("kv,q,G", [([40, 700], [9, 6], 2), ([333, 64], [140, 64], 1), ([1500], [300], 4)])
-def test_values_that_are_not_finite_reach_only_the_rows_that_see_them(pkg, bits, d, kv, q, G):
+@pytest.mark.parametrize("H,kv,q,G", [(2, [40, 700], [9, 6], 2), (2, [333, 64], [140, 64], 1), (2, [1500], [300], 4), (8, [1500, 300], [400, 300], 4), (8, [5000], [60], 5)])
+def test_values_that_are_not_finite_reach_only_the_rows_that_see_them(pkg, bits, d, H, kv, q, G):
     batch = Batch(pkg, kv, q, 32)
-    pool = Pool(pkg, batch.num_pages, 2, 32, d, bits)
+    pool = Pool(pkg, batch.num_pages, H, 32, d, bits)
     fill_random(pool, batch, 2)
     for b, (n, m) in enumerate(zip(kv, q)):
         V = pool.values(batch, b, "v").clone()
@@ -320,18 +323,18 @@ def test_values_that_are_not_finite_reach_only_the_rows_that_see_them(pkg, bits,
             V = torch.where(torch.isfinite(V), V, torch.full_like(V, math.nan))
         pool.put(batch, b, "v", V)
         K = pool.values(batch, b, "k").clone()
-        K[1, n - 1, 3] = math.nan                                             # the last token's key: its own row alone
+        K[H - 1, n - 1, 3] = math.nan                                         # the last token's key: its own row alone
         pool.put(batch, b, "k", K)
-    Q = _rows(4, 2 * G, batch.tokens, d)
+    Q = _rows(4, H * G, batch.tokens, d)
     O = _attend(pkg, Q, pool, batch)
     for b, (n, m) in enumerate(zip(kv, q)):
         lo = batch.starts[b]
-        got = O[lo:lo + m].reshape(m, 2 * G, d).transpose(0, 1).double()
+        got = O[lo:lo + m].reshape(m, H * G, d).transpose(0, 1).double()
         K, V = pool.values(batch, b, "k"), pool.values(batch, b, "v")
         ref, tol = attention_ref(Q[:, lo:lo + m - 1].double(), K[:, :-1], V[:, :-1], m - 1, n - 1, d ** -0.5, 1)
         assert torch.equal(torch.isfinite(got[:, :-1]), torch.isfinite(ref))
         assert bool(((got[:, :-1] - ref).abs().nan_to_num() <= tol).all())
-        assert bool(torch.isnan(got[G:, -1]).all())                          # a score that is NaN
+        assert bool(torch.isnan(got[(H - 1) * G:, -1]).all())                # a score that is NaN
 
 
 def test_keys_without_finite_scores(pkg):
@@ -353,15 +356,15 @@ def test_keys_without_finite_scores(pkg):
 
 
 @pytest.mark.parametrize("bits", [16, 8])
-@pytest.mark.parametrize("q", [[1, 1, 1], [40, 100, 3]])
-def test_wrong_pages_and_lengths_are_reported(pkg, bits, q):
+@pytest.mark.parametrize("H,q", [(2, [1, 1, 1]), (2, [40, 100, 3]), (16, [200, 300, 64])])
+def test_wrong_pages_and_lengths_are_reported(pkg, bits, H, q):
     """... and the call stays inside its buffers, with the other sequences as they should be."""
     kv = [600, 700, 64]
     batch = Batch(pkg, kv, q, 32)
-    pool = Pool(pkg, batch.num_pages, 2, 32, 64, bits)
+    pool = Pool(pkg, batch.num_pages, H, 32, 64, bits)
     fill_random(pool, batch, 1)
-    Q = _rows(4, 4, batch.tokens, 64)
-    K, V = _rows(5, 2, batch.tokens, 64), _rows(6, 2, batch.tokens, 64)
+    Q = _rows(4, 2 * H, batch.tokens, 64)
+    K, V = _rows(5, H, batch.tokens, 64), _rows(6, H, batch.tokens, 64)
     for wrong in (-1, batch.num_pages, 1 << 30, -(1 << 31)):
         was = [x.clone() for x in (pool.k, pool.v)]
         good = batch.dev[2][1, 21].item()
