@@ -7,8 +7,15 @@
 //   * Where some row of the item does not see some key of a stage (the last stages), values there that are not finite must not meet the weight 0
 //     of such a row: warps 10 and 11 put zeros in their place before the MMA may have the stage, and the rows that do see them add them at the end.
 //   * e4m3: the codes (and exponent bytes) arrive in a small ring of their own, and four more warps convert every stage to fp16, exactly.
-//   * Work is an equal share of all 128-key units of all items (paged_part), an item at a time; the barriers are rebuilt for each. What a share
+//   * Work is an item, or an equal share of all 128-key units of all items (paged_part), an item at a time; the barriers are rebuilt for each. What a share
 //     has of an item that is cut goes to the workspace, as fp32 O relative to the row's maximum, and is merged afterwards.
+//
+// Measured: 2048 tokens x 32 heads of 128 on 8, 32768 keys: 1020 us (1.04 PFLOP/s, 0.63 of the burst peak, 0.77 of the sustained one; at the power limit), as shares 1080. A
+// unit (256 rows x 128 keys) is 2.0 to 2.3 us, of 8 bits 2.6; what an item costs besides is 4 us to its first scores (lengths, Q, first keys), 1.5 behind the last (its
+// softmax and P*V) and 2 to store. ncu (512 tokens, 8192 keys): tensor pipe 51 % of active cycles, 38 MB from DRAM. The conversion of 8 bits is in a loop
+// that is not unrolled: with the softmax's code it is then about what the instruction caches hold (512 tokens, 8192 keys: 84 us, unrolled 115, fp16 75). Slower
+// still: codes from memory straight into the converting warps' registers (167, they spill), two warps on keys and two on values (164). O through shared memory
+// for stores of whole lines: +3 %.
 #pragma once
 
 template <bool F8> constexpr int chunk_threads = F8 ? 512 : 384;
