@@ -216,7 +216,7 @@ int check_memory(const char* what, const void* const* p, int n)
         if (!p[i]) continue;
         cudaPointerAttributes attr;
         EFA_CUDA(cudaPointerGetAttributes(&attr, p[i]));
-        if (attr.type == cudaMemoryTypeUnregistered) { set_error("%s: argument %d is not memory that a GPU can use", what, i); return 2; }
+        if (attr.type == cudaMemoryTypeUnregistered || attr.type == cudaMemoryTypeHost) { set_error("%s: argument %d is memory of the host", what, i); return 2; }
         if (attr.type == cudaMemoryTypeDevice && attr.device != dev) {
             set_error("%s: argument %d is memory of device %d, the current device is %d", what, i, attr.device, dev);
             return 2;

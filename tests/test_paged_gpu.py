@@ -450,6 +450,46 @@ def test_a_captured_call_follows_lengths_and_pages(pkg):
     assert pkg.kernel_status()[0] == 0
 
 
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("H,d,q,max_kv", [(2, 128, 1, 60000), (8, 128, 300, 4000), (8, 64, 300, 4000), (8, 64, 64, 30000)])
+def test_captured_steps_of_every_kind(pkg, bits, H, d, q, max_kv):
+    """Write, attention (a block per item; equal shares with their merge; small and large tiles) and read in one graph, replayed on other rows and lengths."""
+    kv, n = [1700, 900], [q, max(1, q // 2)]
+    batch = Batch(pkg, kv, n, 64, max_kv=max_kv, width=-(-max_kv // 64))
+    pool = Pool(pkg, batch.num_pages, H, 64, d, bits)
+    fill_random(pool, batch, 1)
+    K, V, Q = _rows(2, H, batch.tokens, d), _rows(3, H, batch.tokens, d), _rows(4, 4 * H, batch.tokens, d)
+    ap = pkg.paged_attention_params(4 * H, d)
+    ws = torch.empty(max(16, pkg.paged_attention_workspace(pool.cache, batch.batch, ap)), dtype=torch.uint8, device="cuda")
+    O, Ko, Vo = torch.empty(batch.tokens, 4 * H * d, dtype=torch.float16, device="cuda"), torch.empty_like(K), torch.empty_like(V)
+    stream = torch.cuda.Stream()
+
+    def step():
+        pkg.cache_write(K, V, pool.cache, batch.batch, stream=stream)
+        pkg.paged_attention(Q, O, pool.cache, batch.batch, ap, ws, stream=stream)
+        pkg.cache_read(Ko, Vo, pool.cache, batch.batch, stream=stream)
+
+    torch.cuda.synchronize()
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        step()
+    for again in range(3):
+        for x, seed in ((K, 10), (V, 20), (Q, 30)):
+            x.copy_(_rows(seed + again, *x.shape))
+        if again == 2:
+            batch.kv = [1650, 64 + n[1]]
+            batch.dev[1].copy_(torch.tensor(batch.kv, dtype=torch.int32))
+        ws.fill_(0xFF), O.fill_(777)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        check_attention(O, Q, pool, batch, d ** -0.5, 1)
+        assert torch.equal(Ko, K if bits == 16 else decode(*encode(K)).half()) and torch.equal(Vo, V if bits == 16 else decode(*encode(V)).half())
+    assert pkg.kernel_status()[0] == 0
+
+
 def test_streams_of_the_caller(pkg):
     """Write, attention and read on a stream of their own, behind one another without a wait of the host."""
     stream = torch.cuda.Stream()
@@ -467,8 +507,9 @@ def test_memory_of_the_host_is_refused(pkg):
     batch = Batch(pkg, [20], [2], 16)
     pool = Pool(pkg, batch.num_pages, 1, 16, 64, 16)
     host = torch.zeros(1, 2, 64, dtype=torch.float16)
-    with pytest.raises(pkg.EfaError, match="memory"):
-        pkg.cache_write(host, host, pool.cache, batch.batch)
+    for rows in (host, host.pin_memory()):
+        with pytest.raises(pkg.EfaError, match="memory of the host"):
+            pkg.cache_write(rows, rows, pool.cache, batch.batch)
     lens = pkg.paged_batch(*(x.cpu() for x in batch.dev), batch.tokens, 2, 20)
     with pytest.raises(pkg.EfaError, match="memory"):
         pkg.paged_attention(host.cuda(), torch.zeros(2, 64, dtype=torch.float16, device="cuda"), pool.cache, lens, pkg.paged_attention_params(1, 64))
