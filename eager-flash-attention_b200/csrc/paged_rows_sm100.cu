@@ -5,7 +5,7 @@
 //
 // Few rows do little with each key that they load, so it is the loading that takes the time: every key and value comes from memory once per
 // group of heads, and the blocks' work is a contiguous share of all keys of all sequences (paged_part), whatever their lengths.
-// A block is four warps in teams: WM warps of 16 rows each share a team's keys, 4 / WM teams take 16 * WM keys each of a unit of 64 keys. A team has a
+// A block is four warps in teams: WM warps of 16 rows each share a team's keys, 4 / WM teams take 16 * WM keys each of a unit of 64 (8 bits: twice as many). A team has a
 // ring of stages in shared memory that its warps fill with asynchronous 16-byte copies and wait for by themselves, so no barrier of
 // the block is in the loop. The products are mma.sync m16n8k16: a tile of 16 rows is what there is, and tcgen05's least 64 rows would need the
 // softmax to cross tensor memory for nothing.

@@ -151,7 +151,7 @@ def _kernels():
 def test_kernels_that_start_early_presume_no_read_only_memory():
     """They are on the GPU while what they read may still be written (launch_early): a wait ahead of the first access, and ordinary loads."""
     kernels = _kernels()
-    assert {"paged_move_kernel", "paged_rows_kernel", "paged_merge_kernel"} <= set(kernels)
+    assert set(kernels) == {"paged_move_kernel", "paged_rows_kernel", "paged_merge_kernel", "paged_chunk_kernel", "paged_chains_kernel"}
     for name, body in kernels.items():
         assert "pdl_wait()" in body and "pdl_trigger()" in body, name
         assert not re.search(r"__restrict__|__ldg\b|\.nc\b|__constant__", body), name
