@@ -15,7 +15,8 @@
 // softmax and P*V) and 2 to store. ncu (512 tokens, 8192 keys): tensor pipe 51 % of active cycles, 38 MB from DRAM. The conversion of 8 bits is in a loop
 // that is not unrolled: with the softmax's code it is then about what the instruction caches hold (512 tokens, 8192 keys: 84 us, unrolled 115, fp16 75). Slower
 // still: codes from memory straight into the converting warps' registers (167, they spill), two warps on keys and two on values (164). O through shared memory
-// for stores of whole lines: +3 %.
+// for stores of whole lines: +3 %. An item of one tile by both warpgroups, every second stage each: fp16, 64 rows x 16000 keys, 198 -> 188, but items of two tiles +3 %
+// and 8 bits +30 %, where the conversion is then the chain; the softmax's registers go to it.
 #pragma once
 
 template <bool F8> constexpr int chunk_threads = F8 ? 512 : 384;
