@@ -346,6 +346,8 @@ def paged_cache(k, v, k_exp=None, v_exp=None) -> PagedCache:
         raise EfaError(f"paged_cache: {k.dtype} is neither fp16 nor 8-bit codes")
     if tuple(k.stride()[1:]) != (size * d_h, d_h, 1):
         raise EfaError("paged_cache: a page must be dense")
+    if pages > 1 and k.stride(0) < heads * size * d_h:         # expanded tensors too: a stride of 0 means dense below
+        raise EfaError("paged_cache: the pages overlap")
     if any(x is not None and x.device != k.device for x in (v, k_exp, v_exp)):
         raise EfaError("paged_cache: the tensors must be on one device")
     for e in (k_exp, v_exp):

@@ -130,6 +130,14 @@ def test_tensors_that_do_not_fit_together_are_refused(pkg):
             pkg.paged_batch(*args, 9, 4, 50)
 
 
+def test_pages_that_overlap_are_refused(pkg):
+    one = torch.zeros(1, 2, 16, 64, dtype=torch.float16)
+    for pool in (one.expand(5, 2, 16, 64), torch.zeros(2 * 2 * 16 * 64, dtype=torch.float16).as_strided((3, 2, 16, 64), (16 * 64, 16 * 64, 64, 1))):
+        with pytest.raises(pkg.EfaError, match="overlap"):
+            pkg.paged_cache(pool, pool)
+    assert pkg.paged_cache(one, one).page_stride == 0
+
+
 def _kernels():
     """Name and body of every kernel that paged_launch starts."""
     found = {}
