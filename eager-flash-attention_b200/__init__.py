@@ -370,6 +370,8 @@ def paged_batch(q_start, kv_len, pages, tokens: int, max_q: int, max_kv: int) ->
         raise EfaError("paged_batch: the tensors must be on one device")
     if q_start.numel() != n + 1 or pages.dim() != 2 or pages.shape[0] != n:
         raise EfaError("paged_batch: q_start must be [num_seqs + 1], kv_len [num_seqs], pages [num_seqs][max_pages]")
+    if not all(0 <= x < 2 ** 31 for x in (tokens, max_q, max_kv)):
+        raise EfaError("paged_batch: tokens, max_q and max_kv must be from 0 to 2^31 - 1")
     b = PagedBatch(_ptr(q_start), _ptr(kv_len), _ptr(pages), n, pages.shape[1], tokens, max_q, max_kv)
     b.tensors = (q_start, kv_len, pages)
     return b

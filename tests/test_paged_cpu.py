@@ -138,6 +138,16 @@ def test_pages_that_overlap_are_refused(pkg):
     assert pkg.paged_cache(one, one).page_stride == 0
 
 
+@pytest.mark.parametrize("at", [0, 1, 2])
+@pytest.mark.parametrize("size", [2 ** 31, 2 ** 32, 2 ** 32 + 1, -1])
+def test_sizes_of_more_than_31_bits_are_refused(pkg, at, size):
+    i = lambda *shape: torch.zeros(shape, dtype=torch.int32)  # noqa: E731
+    sizes = [9, 4, 50]
+    sizes[at] = size
+    with pytest.raises(pkg.EfaError, match="tokens, max_q and max_kv"):
+        pkg.paged_batch(i(4), i(3), i(3, 7), *sizes)
+
+
 def _kernels():
     """Name and body of every kernel that paged_launch starts."""
     found = {}
