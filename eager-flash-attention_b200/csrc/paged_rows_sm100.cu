@@ -314,8 +314,9 @@ paged_rows_kernel(const PagedArgs c, const PagedAttnArgs a)
                         f1 *= exp_byte_f32(ke >> 8);
                         vscale[nt][0] = exp_byte_f32(ve & 0xffu);
                         vscale[nt][1] = exp_byte_f32(ve >> 8);
-                        vlog[nt][0] = (float)(int)(ve & 0xffu) - 127.f;
-                        vlog[nt][1] = (float)(int)(ve >> 8) - 127.f;
+                        // Of the byte 0, which a key of a missing page has, as of the smallest that is written: weights stay below 2^32, and their sum finite.
+                        vlog[nt][0] = (float)(int)max(ve & 0xffu, 103u) - 127.f;
+                        vlog[nt][1] = (float)(int)max(ve >> 8, 103u) - 127.f;
                     }
                     s[nt][0] *= f0; s[nt][1] *= f1; s[nt][2] *= f0; s[nt][3] *= f1;
                 }
