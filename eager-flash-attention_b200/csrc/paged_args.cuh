@@ -68,6 +68,14 @@ __device__ __forceinline__ uint32_t exp_byte_f16x2(unsigned byte)
     return __byte_perm(h, h, 0x1010);
 }
 
+// The same of two bytes, one to a half.
+__device__ __forceinline__ uint32_t exp_bytes_f16x2(uint32_t two)
+{
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(exp_byte_f32(min(two >> 8, 142u))), "f"(exp_byte_f32(min(two & 0xffu, 142u))));
+    return r;
+}
+
 __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two)
 {
     uint32_t r;

@@ -18,7 +18,9 @@
 //
 // fp16 keys reach the registers by ldmatrix. Codes of e4m3 are read as 16 bytes of a key per thread and converted there (exactly): the order of
 // the head's elements in Q K^T, and that of O's columns, is then each thread's own, and Q's fragments and the stores follow it. The exponents of keys
-// multiply the scores, those of values the weights.
+// multiply the scores; those of values the converted values, which stay exact. In the weights, which are rounded to fp16, they would leave the others' a few bits beside
+// a value row 2^16 times as large, in columns where they are all there is; and be slower for the softmax's part in it (us, 64 sequences of 4096 keys, one token, exponents
+// in the weights / here: 32 heads of 128 on 8 102.2 / 100.6, 16 of 64 128.4 / 121.2, 32 of 32 185.5 / 170.2, 64 of 16 322.6 / 277.6).
 #include "paged_kernels.cuh"
 #include "fa_args.cuh"
 
@@ -32,7 +34,7 @@ constexpr int PR_THREADS = 128;
 
 // Blocks of an SM and stages of each: where loading is the time (fp16 heads of 64 and 128) few blocks with deep rings, else more warps. us, 64 sequences of 4096
 // keys, one token, as here / as two blocks of 96 KB: 16 heads of 64 fp16 172 / 172 (three blocks of 64 KB: 210), 8 bits 124 / 138; 32 heads of
-// 32 179 / 206, 183 / 254; 64 heads of 16 269 / 484, 312 / 563; 16 sequences of 16000 keys, 8 heads of 128 165 / 165, 97 / 101.
+// 32 179 / 206, 183 / 254; 64 heads of 16 269 / 484, 312 / 563 (8 bits before the exponents went to the values); 16 sequences of 16000 keys, 8 heads of 128 165 / 165, 97 / 101.
 constexpr int rows_blocks(int d, bool f8) { return d >= 64 ? (f8 ? 3 : 2) : d == 16 && f8 ? 6 : 4; }
 template <int D, bool F8> constexpr int blocks_of = rows_blocks(D, F8);
 constexpr int rows_stages(int d, bool f8) { return d == 128 ? (f8 ? 2 : 3) : d == 64 ? (f8 ? 4 : 6) : d == 16 && f8 ? 4 : 6; }
@@ -304,7 +306,7 @@ paged_rows_kernel(const PagedArgs c, const PagedAttnArgs a)
                         }
                 }
                 // ---- softmax; this thread has keys key0 + nt * 8 + t * 2 + {0, 1} of rows g (s[.][0..1]) and g + 8
-                float vscale[KT][2], vlog[KT][2];          // e4m3: 2^exponent of the values, and the exponent
+                uint32_t vexp[KT];                         // e4m3: 2^exponent of the two keys' values
                 #pragma unroll
                 for (int nt = 0; nt < KT; nt++) {
                     float f0 = a.scale_log2e, f1 = f0;
@@ -312,11 +314,7 @@ paged_rows_kernel(const PagedArgs c, const PagedAttnArgs a)
                         const uint32_t ke = load_half(se + blk * 16 + nt * 8 + t * 2), ve = load_half(se + KS + blk * 16 + nt * 8 + t * 2);
                         f0 *= exp_byte_f32(ke & 0xffu);
                         f1 *= exp_byte_f32(ke >> 8);
-                        vscale[nt][0] = exp_byte_f32(ve & 0xffu);
-                        vscale[nt][1] = exp_byte_f32(ve >> 8);
-                        // Of the byte 0, which a key of a missing page has, as of the smallest that is written: weights stay below 2^32, and their sum finite.
-                        vlog[nt][0] = (float)(int)max(ve & 0xffu, 103u) - 127.f;
-                        vlog[nt][1] = (float)(int)max(ve >> 8, 103u) - 127.f;
+                        vexp[nt] = exp_bytes_f16x2(ve);
                     }
                     s[nt][0] *= f0; s[nt][1] *= f1; s[nt][2] *= f0; s[nt][3] *= f1;
                 }
@@ -326,24 +324,16 @@ paged_rows_kernel(const PagedArgs c, const PagedAttnArgs a)
                     for (int nt = 0; nt < KT; nt++)
                         #pragma unroll
                         for (int x = 0; x < 4; x++)
-                        {
-                            const int key = key0 + nt * 8 + t * 2 + (x & 1);
-                            if (key >= min(sees[x >> 1], q.kv)) s[nt][x] = -INFINITY;
-                            if (F8 && key >= q.kv) vscale[nt][x & 1] = 0.f;      // no key: its bytes may be anything
-                        }
+                            if (key0 + nt * 8 + t * 2 + (x & 1) >= min(sees[x >> 1], q.kv)) s[nt][x] = -INFINITY;
                 }
                 // The offset m is a row's largest weight so far, or up to rescale_above less: O is rescaled when it moves, and of 16 rows one would nearly always have a
-                // new maximum. Of e4m3 with the exponent of the value, which stays out of the converted values (exact) and goes into the weights, so
-                // that what is rounded to fp16 is largest where it counts.
+                // new maximum.
                 float off[2], mx[2];
                 #pragma unroll
                 for (int half = 0; half < 2; half++) {
                     mx[half] = -INFINITY;
                     #pragma unroll
-                    for (int nt = 0; nt < KT; nt++) {
-                        if constexpr (F8) mx[half] = max3(mx[half], s[nt][half * 2] + vlog[nt][0], s[nt][half * 2 + 1] + vlog[nt][1]);
-                        else mx[half] = max3(mx[half], s[nt][half * 2], s[nt][half * 2 + 1]);
-                    }
+                    for (int nt = 0; nt < KT; nt++) mx[half] = max3(mx[half], s[nt][half * 2], s[nt][half * 2 + 1]);
                     mx[half] = fmaxf(mx[half], __shfl_xor_sync(0xffffffffu, mx[half], 1));
                     mx[half] = fmaxf(mx[half], __shfl_xor_sync(0xffffffffu, mx[half], 2));
                 }
@@ -366,9 +356,8 @@ paged_rows_kernel(const PagedArgs c, const PagedAttnArgs a)
                 for (int nt = 0; nt < KT; nt++)
                     #pragma unroll
                     for (int half = 0; half < 2; half++) {
-                        float p0 = ex2(s[nt][half * 2] - off[half]), p1 = ex2(s[nt][half * 2 + 1] - off[half]);
+                        const float p0 = ex2(s[nt][half * 2] - off[half]), p1 = ex2(s[nt][half * 2 + 1] - off[half]);
                         l[half] += p0 + p1;
-                        if constexpr (F8) { p0 *= vscale[nt][0]; p1 *= vscale[nt][1]; }
                         p[nt >> 1][(nt & 1) * 2 + half] = pack_f16x2(p0, p1);
                     }
                 // ---- O += P V. A masked weight is 0, and 0 times what is not finite is not 0: such values are left out here and, for the rows that
@@ -391,6 +380,8 @@ paged_rows_kernel(const PagedArgs c, const PagedAttnArgs a)
                             uint32_t b0, b1, b2, b3;
                             e4m3x4_to_f16x4(__byte_perm(w[0][j >> 2], w[1][j >> 2], sel), b0, b2);
                             e4m3x4_to_f16x4(__byte_perm(w[2][j >> 2], w[3][j >> 2], sel), b1, b3);
+                            b0 = mul_f16x2(b0, vexp[2 * y]); b1 = mul_f16x2(b1, vexp[2 * y + 1]);
+                            b2 = mul_f16x2(b2, vexp[2 * y]); b3 = mul_f16x2(b3, vexp[2 * y + 1]);
                             if (masked) { clean(b0); clean(b1); clean(b2); clean(b3); }
                             mma16816(o[j], p[y], b0, b1);
                             mma16816(o[j + 1], p[y], b2, b3);
