@@ -142,7 +142,7 @@ paged_move_kernel(const PagedArgs c, const PagedRows rows)
     if (there) {
         const int b = sequence_of(c, row);
         if (b >= 0) {
-            const PagedSeq q = sub == 0 && h0 == 0 ? paged_seq<true>(c, b, 50) : paged_seq(c, b);
+            const PagedSeq q = paged_seq(c, b);
             const int i = row - q.row0, position = q.kv - q.n + i;
             owned = i >= 0 && i < q.n;
             if (owned && position >= 0) {
@@ -189,6 +189,9 @@ paged_move_kernel(const PagedArgs c, const PagedRows rows)
             *reinterpret_cast<uint4*>(pv + o) = v[i];
         }
     }
+    // Wrong lengths, of sequences without rows as well.
+    if (blockIdx.x == 0 && blockIdx.y == 0)
+        for (int b = threadIdx.x; b < c.num_seqs; b += PC_THREADS) paged_seq<true>(c, b, 50);
 }
 
 PagedArgs device_args(const efa_paged_cache& c, const efa_paged_batch& b)
