@@ -223,7 +223,6 @@ class _Call:
         c, self.pkg = s["case"], importlib.import_module("eager-flash-attention_b200")
         self.cache = self.pkg.paged_cache(s["k"], s["v"], s.get("k_exp"), s.get("v_exp"))
         self.batch = self.pkg.paged_batch(s["q_start"], s["kv_len"], s["pages"], s["tokens"], c["q"], c["kv"])
-        self.stream = torch.cuda.current_stream().cuda_stream
         if c["op"] == "attend":
             self.how = self.pkg.paged_attention_params(c["heads"], c["d_h"], causal=1)
             size = self.pkg.paged_attention_workspace(self.cache, self.batch, self.how)
@@ -234,15 +233,15 @@ def _through_package(s):
     call = s.get("call")
     if call is None:
         call = s["call"] = _Call(s)
-    pkg, op = call.pkg, s["case"]["op"]
+    pkg, op, stream = call.pkg, s["case"]["op"], torch.cuda.current_stream().cuda_stream
     if op == "attend":
-        pkg.paged_attention(s["Q"], s["O"], call.cache, call.batch, call.how, call.workspace, stream=call.stream)
+        pkg.paged_attention(s["Q"], s["O"], call.cache, call.batch, call.how, call.workspace, stream=stream)
         return s["O"]
     if op != "read":
-        pkg.cache_write(s["K"], s["V"], call.cache, call.batch, stream=call.stream)
+        pkg.cache_write(s["K"], s["V"], call.cache, call.batch, stream=stream)
         if op == "write":
             return {"k": s["k"], "v": s["v"]}
-    pkg.cache_read(s["K_out"], s["V_out"], call.cache, call.batch, stream=call.stream)
+    pkg.cache_read(s["K_out"], s["V_out"], call.cache, call.batch, stream=stream)
     return {"K": s["K_out"], "V": s["V_out"]}
 
 
