@@ -221,6 +221,7 @@ class _Call:
 
     def __init__(self, s):
         c, self.pkg = s["case"], importlib.import_module("eager-flash-attention_b200")
+        self.device = s["k"].device.index
         self.cache = self.pkg.paged_cache(s["k"], s["v"], s.get("k_exp"), s.get("v_exp"))
         self.batch = self.pkg.paged_batch(s["q_start"], s["kv_len"], s["pages"], s["tokens"], c["q"], c["kv"])
         if c["op"] == "attend":
@@ -233,7 +234,7 @@ def _through_package(s):
     call = s.get("call")
     if call is None:
         call = s["call"] = _Call(s)
-    pkg, op, stream = call.pkg, s["case"]["op"], torch.cuda.current_stream().cuda_stream
+    pkg, op, stream = call.pkg, s["case"]["op"], torch._C._cuda_getCurrentRawStream(call.device)    # the current stream, without 3 us for an object of it
     if op == "attend":
         pkg.paged_attention(s["Q"], s["O"], call.cache, call.batch, call.how, call.workspace, stream=stream)
         return s["O"]
