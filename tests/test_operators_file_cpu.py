@@ -13,9 +13,10 @@ def test_calls_go_to_the_stream_that_is_current(pkg, monkeypatch):
                                  paged_attention_workspace=lambda *a: 0)
     monkeypatch.setattr(operators, "importlib", types.SimpleNamespace(import_module=lambda name: fake))
     for op in ("attend", "write", "keep", "read"):
-        state = dict(case=dict(op=op, q=1, kv=1, heads=1, d_h=16), tokens=1, **{x: None for x in ("k", "v", "q_start", "kv_len", "pages", "K", "V", "Q", "O", "K_out", "V_out")})
+        state = dict(case=dict(op=op, q=1, kv=1, heads=1, d_h=16), tokens=1, k=types.SimpleNamespace(device=torch.device("cuda", 0)),
+                     **{x: None for x in ("v", "q_start", "kv_len", "pages", "K", "V", "Q", "O", "K_out", "V_out")})
         for stream in (11, 12):
-            monkeypatch.setattr(torch.cuda, "current_stream", lambda: types.SimpleNamespace(cuda_stream=stream))
+            monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda device: stream)
             made.clear()
             operators._through_package(state)
             sent = [s for s in made if s is not None]
