@@ -115,6 +115,7 @@ __device__ __forceinline__ uint32_t nonfinite_f16x2(uint32_t x)
 struct PagedShape {
     int G, causal, tile, unit, extra, max_tiles;   // query heads per kv head; rows of a tile; keys of a unit; ...; tiles of the longest chunk
     int late;
+    int limit;              // weight of all items that a batch of these sizes may have
 };
 constexpr unsigned LATE_UNITS = 4, LATE_RATIO = 10;
 
@@ -165,37 +166,40 @@ __device__ __forceinline__ PagedPiece paged_piece(const PagedArgs& c, const Page
 struct PagedScratch { int warp_sum[32]; PagedAt at; };
 
 // The weight of share `part` of `parts` and where it begins, found by all THREADS threads of a block together; 0: there is less weight
-// than shares, and none for this one. Block 0, which like all others looks at every sequence, reports lengths that are wrong.
+// than shares, and none for this one. Block 0, which like all others looks at every sequence, reports lengths that are wrong. Sequences that overlap
+// (q_start falls) may add up to more than any legal batch of these sizes; sums stop at 2^31 - 1, and nobody has a share then.
 template <int THREADS>
 __device__ int paged_part(const PagedArgs& c, const PagedShape& w, int part, int parts, PagedScratch& s, PagedAt& at, int site)
 {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int entries = c.num_seqs * w.max_tiles, per = (int)((unsigned)(entries + THREADS - 1) / THREADS);
     const int e0 = min(tid * per, entries), e1 = min(e0 + per, entries);
+    auto add = [](int x, int y) { return (int)min((unsigned)x + (unsigned)y, 0x7fffffffu); };
     int sum = 0;
     for (int e = e0; e < e1; ) {
         const int b = (int)((unsigned)e / (unsigned)w.max_tiles), rt0 = e - b * w.max_tiles;
         const PagedSeq q = part == 0 ? paged_seq<true>(c, b, site) : paged_seq(c, b);
         const int stop = min(paged_tiles(w, q), rt0 + e1 - e);
-        for (int rt = rt0; rt < stop; rt++) sum += paged_units(w, q, rt) + w.extra;
+        for (int rt = rt0; rt < stop; rt++) sum = add(sum, paged_units(w, q, rt) + w.extra);
         e = (b + 1) * w.max_tiles;
     }
     int before = sum;
     #pragma unroll
     for (int d = 1; d < 32; d *= 2) {
         const int o = __shfl_up_sync(0xffffffffu, before, d);
-        if (lane >= d) before += o;
+        if (lane >= d) before = add(before, o);
     }
     if (lane == 31) s.warp_sum[warp] = before;
     __syncthreads();
     int total = 0;
     #pragma unroll
     for (int i = 0; i < THREADS / 32; i++) {
-        if (i < warp) before += s.warp_sum[i];
-        total += s.warp_sum[i];
+        if (i < warp) before = add(before, s.warp_sum[i]);
+        total = add(total, s.warp_sum[i]);
     }
+    if ((long long)total * c.H_kv > w.limit) return 0;
     before -= sum;
-    const unsigned all = (unsigned)total * (unsigned)c.H_kv;        // below 2^31 (paged_attention_check)
+    const unsigned all = (unsigned)total * (unsigned)c.H_kv;
     const unsigned big = (unsigned)(parts - w.late), weights = big * LATE_RATIO + (unsigned)w.late;
     unsigned begin, end;
     if (w.late > 0 && all / LATE_UNITS >= weights) {

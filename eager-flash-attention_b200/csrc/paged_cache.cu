@@ -270,24 +270,46 @@ int move_rows(const char* what, bool read, const void* K, const void* V, long lo
     }
 }
 
-struct PagedPlan { PagedShape w; int blocks, cluster; bool cut, chunk; size_t cut_bytes, ml_bytes, o_bytes; };
+// Which of the two kinds of kernel, its tiles and units, and bounds: keys of a sequence, tiles of a chunk, items of a launch with one block to each, the weight of all items.
+// Rows of different sequences are different rows of Q, so that however long single chunks may be their tiles are no more than `tokens` has, and one
+// more for each sequence.
+struct PagedKind { bool chunk; int tile, unit, extra; long long kv_cap, units; double max_tiles, items, weight; };
 
-PagedPlan plan_attention(const efa_paged_cache& c, const efa_paged_batch& b, const efa_paged_attention_params& p)
+PagedKind kind_of(const efa_paged_cache& c, const efa_paged_batch& b, const efa_paged_attention_params& p)
 {
-    PagedPlan plan{};
+    PagedKind k{};
     const int G = p.H_q / c.H_kv;
-    const long long rows = (long long)b.max_q * G, kv_cap = std::min<long long>(b.max_kv, (long long)b.max_pages * c.page_size);
+    const long long rows = (long long)b.max_q * G;
+    k.kv_cap = std::min<long long>(b.max_kv, (long long)b.max_pages * c.page_size);
     // Up to 32 rows the keys' way to the SM is the time: small tiles. More go to the tensor cores' tiles of 256 unless there is little work, counted as 64 rows x 64 keys:
     // small tiles start and end faster, and clusters share theirs. us, small tiles / tiles of 256: 64 rows, 8 heads of 128, 1000 keys 14 / 19, 2 x 16000 keys
     // 57 / 47, 16 x 16000 296 / 190, of 8 bits 310 / 228; 32 rows, 16 x 16000 keys 171 / 186; prompts, 16 heads of 64, 128 tokens 7.8 / 8.6, 512 12.9 / 14.0,
     // of 8 bits 256 10.0 / 11.0, 512 18.8 / 14.2; 8 heads of 16, 200 tokens over 400 keys 6.9 / 11.9; 32 heads of 128 on 8, 4 x 64 tokens 9.5 / 11.4, 128 11.2 / 11.3,
     // 256 16.1 / 12.8.
     const bool f8 = c.dtype == EFA_E4M3;
-    const double work = (double)b.num_seqs * c.H_kv * (double)((rows + 63) / 64) * (double)((kv_cap + 63) / 64);
-    plan.chunk = rows > 32 && work > (rows <= 64 ? 1024 : c.d_h == 128 ? 128 : c.d_h == 64 ? (f8 ? 256 : 1024) : 2048);
-    const int tile = plan.chunk ? PAGED_CHUNK_TILE : paged_rows_tile((int)rows), unit = plan.chunk ? PAGED_CHUNK_UNIT : paged_rows_unit(f8);
-    plan.w = PagedShape{G, p.causal ? 1 : 0, tile, unit, plan.chunk ? PAGED_CHUNK_EXTRA : PAGED_ROWS_EXTRA, (int)((rows + tile - 1) / tile), 0};
-    const long long items = (long long)b.num_seqs * c.H_kv * plan.w.max_tiles, units = std::max<long long>(1, (kv_cap + unit - 1) / unit);
+    const double work = (double)b.num_seqs * c.H_kv * (double)((rows + 63) / 64) * (double)((k.kv_cap + 63) / 64);
+    k.chunk = rows > 32 && work > (rows <= 64 ? 1024 : c.d_h == 128 ? 128 : c.d_h == 64 ? (f8 ? 256 : 1024) : 2048);
+    k.tile = k.chunk ? PAGED_CHUNK_TILE : paged_rows_tile((int)std::min<long long>(rows, INT_MAX));
+    k.unit = k.chunk ? PAGED_CHUNK_UNIT : paged_rows_unit(f8);
+    k.extra = k.chunk ? PAGED_CHUNK_EXTRA : PAGED_ROWS_EXTRA;
+    k.units = std::max<long long>(1, (k.kv_cap + k.unit - 1) / k.unit);
+    k.max_tiles = (double)((rows + k.tile - 1) / k.tile);
+    k.items = (double)b.num_seqs * c.H_kv * k.max_tiles;
+    k.weight = std::min((double)b.num_seqs * k.max_tiles, std::floor((double)b.tokens * G / k.tile) + b.num_seqs) * c.H_kv * (double)(k.units + k.extra);
+    return k;
+}
+
+struct PagedPlan { PagedShape w; int blocks, cluster; bool cut, chunk; size_t cut_bytes, ml_bytes, o_bytes; };
+
+PagedPlan plan_attention(const efa_paged_cache& c, const efa_paged_batch& b, const efa_paged_attention_params& p)
+{
+    PagedPlan plan{};
+    const PagedKind k = kind_of(c, b, p);
+    const int G = p.H_q / c.H_kv, tile = k.tile, unit = k.unit;
+    const bool f8 = c.dtype == EFA_E4M3;
+    plan.chunk = k.chunk;
+    plan.w = PagedShape{G, p.causal ? 1 : 0, tile, unit, k.extra, (int)k.max_tiles, 0, (int)k.weight};
+    const long long items = (long long)k.items, units = k.units;
     plan.cluster = 1;
     int parts = device_sms();
     if (plan.chunk) {
@@ -300,7 +322,7 @@ PagedPlan plan_attention(const efa_paged_cache& c, const efa_paged_batch& b, con
         constexpr double MIN_SHARE = 6, MERGE = 6;
         const double tiles = std::min<double>((double)b.num_seqs * plan.w.max_tiles, (double)b.tokens * G / tile + b.num_seqs) * c.H_kv;
         const double longest = (double)units + PAGED_CHUNK_EXTRA;
-        const double first = p.causal ? std::max<double>(1, ((double)kv_cap - b.max_q + (double)tile / G) / unit) + PAGED_CHUNK_EXTRA : longest;
+        const double first = p.causal ? std::max<double>(1, ((double)k.kv_cap - b.max_q + (double)tile / G) / unit) + PAGED_CHUNK_EXTRA : longest;
         const bool even = first * 2 >= longest;
         const double each = tiles * (first + longest) / 2 / parts;
         const double by_item = even ? std::ceil(tiles / parts) * longest : std::max(longest, each * 1.05);
@@ -323,7 +345,7 @@ PagedPlan plan_attention(const efa_paged_cache& c, const efa_paged_batch& b, con
             parts += plan.w.late;
         }
     }
-    plan.blocks = (int)std::min<long long>(plan.cut ? std::min<long long>(parts, items * units) : items, INT_MAX);
+    plan.blocks = (int)(plan.cut ? std::min<long long>(parts, items * units) : items);
     if (plan.cut) {
         plan.cut_bytes = ((size_t)plan.blocks * sizeof(PagedCut) + 255) / 256 * 256;
         plan.ml_bytes = (size_t)plan.blocks * 2 * tile * sizeof(float2);
@@ -360,8 +382,8 @@ const char* paged_attention_check(const efa_paged_cache& c, const efa_paged_batc
         if (p.q_head_stride < c.d_h || p.q_token_stride < c.d_h || p.q_head_stride % 8 || p.q_token_stride % 8) return "paged: row strides must be multiples of 8 and at least d_h";
     }
     if (p.o_token_stride != 0 && (p.o_token_stride < (long long)p.H_q * c.d_h || p.o_token_stride % 8)) return "paged: o_token_stride must be 0 or a multiple of 8 that holds H_q * d_h";
-    const long long rows = (long long)b.max_q * (p.H_q / c.H_kv), units = ((long long)b.max_kv + 63) / 64 + 8;
-    if (rows > INT_MAX / 2 || (double)b.num_seqs * c.H_kv * ((double)rows / 16 + 1) * (double)units > (double)INT_MAX) return "paged: sizes too large";
+    const PagedKind k = kind_of(c, b, p);                  // counted in 31 bits; of items and rows the kernels add a block's to the number
+    if ((long long)b.max_q * (p.H_q / c.H_kv) > INT_MAX / 2 || k.items > (double)(INT_MAX / 2) || k.weight > (double)INT_MAX) return "paged: sizes too large";
     return nullptr;
 }
 

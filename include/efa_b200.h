@@ -169,7 +169,8 @@ typedef struct efa_paged_cache {
  * The three arrays are device memory, read when the kernels run: a captured graph follows their contents. The host gives
  * bounds: max_q >= every n_b, max_kv >= every kv_len[b]; tight ones choose faster kernels. Lengths outside the bounds or the
  * buffers, and page numbers outside the pool where a key lies, are reported by efa_kernel_status (code 3 and 2, sequence, site); the call then stays
- * inside its buffers: lengths are cut to the bounds, keys of a missing page read as zeros and are not written.
+ * inside its buffers: lengths are cut to the bounds, keys of a missing page read as zeros and are not written. Where q_start falls, so that sequences
+ * have rows in common, attention may leave O as it was.
  * Sequences may share pages; a page that efa_cache_write writes to in one call should belong to one sequence. */
 typedef struct efa_paged_batch {
     const int* q_start;     /* [num_seqs + 1] */
