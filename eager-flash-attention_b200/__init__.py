@@ -392,15 +392,47 @@ def paged_check(cache: PagedCache, batch: PagedBatch, ap: Optional[PagedAttentio
     return None if why is None else why.decode()
 
 
+_half = None     # torch.float16, once a tensor of it has been seen
+
+
+def _rows(what: str, x, batch: PagedBatch, need: int, dense: bool) -> Optional[int]:
+    """Address of fp16 rows of which the last ends ``need`` elements behind the beginning of the first. A tensor is refused if its type is another, if it is not dense
+    and no strides say how it lies, or if the rows of the batch go beyond it: the kernels know its address only."""
+    global _half
+    dtype = getattr(x, "dtype", None)
+    if dtype is not None and dtype is _half and x.numel() >= need and x.is_contiguous():
+        return x.data_ptr()
+    if not hasattr(x, "data_ptr"):
+        return _ptr(x)
+    if str(dtype) != "torch.float16":
+        raise EfaError(f"{what}: rows must be torch.float16, not {dtype}")
+    _half = dtype
+    if batch.num_seqs == 0 or batch.tokens == 0 or batch.max_q == 0:        # nothing is read
+        return x.data_ptr()
+    if dense and not (x.numel() >= need and x.is_contiguous()):
+        raise EfaError(f"{what}: rows must be a dense tensor of {need} elements, or their strides be given")
+    if x.untyped_storage().nbytes() // 2 - x.storage_offset() < need:
+        raise EfaError(f"{what}: rows of these strides end {need} elements behind the tensor's first, beyond its memory")
+    return x.data_ptr()
+
+
 def cache_write(K, V, cache: PagedCache, batch: PagedBatch, stream=None, head_stride: int = 0, token_stride: int = 0) -> None:
-    """Rows of the batch's chunks (fp16 ``[H_kv][tokens][d_h]``, or with strides in elements) into their pages, rounded to
+    """Rows of the batch's chunks (fp16 ``[H_kv][tokens][d_h]``, or with strides in elements, then K and V tell where they begin) into their pages, rounded to
     8 bits with an exponent per row where the cache is e4m3. Asynchronous on ``stream``."""
-    _check(lib().efa_cache_write(_ptr(K), _ptr(V), head_stride, token_stride, cache, batch, _stream(stream)), "cache_write")
+    need, dense = cache.H_kv * batch.tokens * cache.d_h, True
+    if head_stride or token_stride:
+        need, dense = (cache.H_kv - 1) * head_stride + (batch.tokens - 1) * token_stride + cache.d_h, False
+    K, V = _rows("cache_write", K, batch, need, dense), _rows("cache_write", V, batch, need, dense)
+    _check(lib().efa_cache_write(K, V, head_stride, token_stride, cache, batch, _stream(stream)), "cache_write")
 
 
 def cache_read(K, V, cache: PagedCache, batch: PagedBatch, stream=None, head_stride: int = 0, token_stride: int = 0) -> None:
     """The inverse of cache_write: the last keys and values of each sequence into fp16 rows."""
-    _check(lib().efa_cache_read(_ptr(K), _ptr(V), head_stride, token_stride, cache, batch, _stream(stream)), "cache_read")
+    need, dense = cache.H_kv * batch.tokens * cache.d_h, True
+    if head_stride or token_stride:
+        need, dense = (cache.H_kv - 1) * head_stride + (batch.tokens - 1) * token_stride + cache.d_h, False
+    K, V = _rows("cache_read", K, batch, need, dense), _rows("cache_read", V, batch, need, dense)
+    _check(lib().efa_cache_read(K, V, head_stride, token_stride, cache, batch, _stream(stream)), "cache_read")
 
 
 def paged_attention_workspace(cache: PagedCache, batch: PagedBatch, ap: PagedAttentionParams) -> int:
@@ -418,7 +450,12 @@ def paged_attention(Q, O, cache: PagedCache, batch: PagedBatch, ap: PagedAttenti
     other call until this one is done. Asynchronous on ``stream``."""
     if workspace_bytes is None:
         workspace_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
-    _check(lib().efa_paged_attention(_ptr(Q), _ptr(O), cache, batch, ap, _ptr(workspace), workspace_bytes, _stream(stream)), "paged_attention")
+    tokens, d_h, by_head, by_token, o_token = batch.tokens, cache.d_h, ap.q_head_stride, ap.q_token_stride, ap.o_token_stride
+    width = ap.H_q * d_h
+    need = (ap.H_q - 1) * by_head + (tokens - 1) * by_token + d_h if by_head or by_token else width * tokens
+    Q = _rows("paged_attention", Q, batch, need, not (by_head or by_token))
+    O = _rows("paged_attention", O, batch, (tokens - 1) * o_token + width if o_token else width * tokens, not o_token)
+    _check(lib().efa_paged_attention(Q, O, cache, batch, ap, _ptr(workspace), workspace_bytes, _stream(stream)), "paged_attention")
 
 
 def kernel_status() -> Sequence[int]:
