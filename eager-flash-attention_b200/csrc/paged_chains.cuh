@@ -184,16 +184,19 @@ paged_chains_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
                     const int s = j % NS;
                     if (!__all_sync(0xffffffffu, mbar_wait(&v_raw[s], (uint32_t)(((j - jm) / NS) & 1), &abort_word, 64))) break;
                     const uint32_t v = smem_u32(sV + s * C::TILE_BYTES) + (tid & 63) * 16;
+                    const int there = p.q.kv - (p.u_lo + j) * WS_BN;
                     #pragma unroll 2
                     for (int i = 0; i < C::TILE_BYTES / 16 / 64; i++) {
                         uint4 x = lds128(v + i * 1024);
                         uint32_t* w = &x.x;
+                        uint32_t any = 0u;
                         #pragma unroll
                         for (int k = 0; k < 4; k++) {
                             const uint32_t bad = nonfinite_f16x2(w[k]);
-                            bad_seen |= bad != 0;
+                            any |= bad;
                             w[k] &= ~bad;
                         }
+                        bad_seen |= any != 0u && (i * 64 + (tid & 63)) / (C::SWB / 16) < there;      // what lies behind the last key is nobody's to see
                         sts128(v + i * 1024, x);
                     }
                     if (bad_seen) *(volatile int*)&poison = 1;

@@ -5,7 +5,8 @@
 //   * A stage's keys are pages: one TMA box per page and 64 columns, issued by the lanes of the producer warp side by side. A page that is
 //     none, or keys that are not there, are boxes outside the tensor, which read as zeros.
 //   * Where some row of the item does not see some key of a stage (the last stages), values there that are not finite must not meet the weight 0
-//     of such a row: warps 10 and 11 put zeros in their place before the MMA may have the stage, and the rows that do see them add them at the end.
+//     of such a row: warps 10 and 11 put zeros in their place before the MMA may have the stage, and the rows that do see them add them at the end. What a page holds
+//     behind the last key is left out of that: it may be anything, and the search for it cost prompts four to six times their time.
 //   * e4m3: the codes (and exponent bytes) arrive in a small ring of their own, and four more warps convert every stage to fp16, exactly.
 //   * Work is an item, or an equal share of all 128-key units of all items (paged_part), an item at a time; the barriers are rebuilt for each. What a share
 //     has of an item that is cut goes to the workspace, as fp32 O relative to the row's maximum, and is merged afterwards.
@@ -311,14 +312,16 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                 if (tid == FINDER) find_piece((round + 1) & 1);
                 __syncwarp();
                 bool bad_seen = false;
-                auto clean = [&](uint4& x) {
+                auto clean = [&](uint4& x, int key) {            // what lies behind the last key is nobody's to see
                     uint32_t* w = &x.x;
+                    uint32_t any = 0u;
                     #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         const uint32_t bad = nonfinite_f16x2(w[i]);
-                        bad_seen |= bad != 0;
+                        any |= bad;
                         w[i] &= ~bad;
                     }
+                    bad_seen |= any != 0u && key < kv;
                 };
                 bool ok = true;
                 if constexpr (F8) {
@@ -367,7 +370,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                             for (int i = 0; i < 2 * RPT; i++) {
                                 const uint32_t at = dst + (place_of(i >> 1) ^ (i & 1 ? 16u : 0u));
                                 uint4 x = lds128(at);
-                                clean(x);
+                                clean(x, (u_lo + j) * WS_BN + row0 + ((i >> 1) ^ hi));
                                 sts128(at, x);
                             }
                             if (bad_seen) *(volatile int*)&poison = 1;
@@ -390,7 +393,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                         #pragma unroll 4
                         for (int i = 0; i < C::TILE_BYTES / 16 / 64; i++) {
                             uint4 x = lds128(v + (i * 64 + t64) * 16);
-                            clean(x);
+                            clean(x, (u_lo + j) * WS_BN + (i * 64 + t64) % (C::BOX_BYTES / 16) / (C::SWB / 16));
                             sts128(v + (i * 64 + t64) * 16, x);
                         }
                         if (bad_seen) *(volatile int*)&poison = 1;
