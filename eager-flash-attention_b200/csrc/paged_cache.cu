@@ -318,14 +318,16 @@ PagedPlan plan_attention(const efa_paged_cache& c, const efa_paged_batch& b, con
         // merge, for pieces half of which begin and end within an item, and for reading keys at different places at a time: blocks in step on many tiles of one
         // sequence find them in the L2. Below MIN_SHARE a block spends its time on anything but keys. us, items / shares: prompts, 16 heads of 64, 1024 tokens
         // 19 / 21, 4096 59 / 68; 32 heads of 128 on 8, 2048 45 / 61, 8192 516 / 559; 2048 tokens over 32768 keys 1004 / 1070, of 8 bits 1099 / 1039; eight
-        // sequences, 512 tokens over 4096 keys 310 / 279; one, 64 tokens over 2000 keys 34 / 30.
-        constexpr double MIN_SHARE = 6, MERGE = 6;
+        // sequences, 512 tokens over 4096 keys 310 / 279; one, 64 tokens over 2000 keys 34 / 30. Tiles of max_q that a sequence does not have are blocks as well,
+        // of 1.7 us each (tensor memory, lengths): one chunk with single tokens beside it, 32 heads of 128 on 8, 4096 keys, 512 tokens and 63 sequences 276 / 247,
+        // 4096 and 127 1286 / 610, 4096 and 255 of 300 keys 1819 / 322.
+        constexpr double MIN_SHARE = 6, MERGE = 6, EMPTY = 0.85;
         const double tiles = std::min<double>((double)b.num_seqs * plan.w.max_tiles, (double)b.tokens * G / tile + b.num_seqs) * c.H_kv;
         const double longest = (double)units + PAGED_CHUNK_EXTRA;
         const double first = p.causal ? std::max<double>(1, ((double)k.kv_cap - b.max_q + (double)tile / G) / unit) + PAGED_CHUNK_EXTRA : longest;
         const bool even = first * 2 >= longest;
         const double each = tiles * (first + longest) / 2 / parts;
-        const double by_item = even ? std::ceil(tiles / parts) * longest : std::max(longest, each * 1.05);
+        const double by_item = (even ? std::ceil(tiles / parts) * longest : std::max(longest, each * 1.05)) + std::max(0.0, k.items - tiles) / parts * EMPTY;
         const double by_share = std::max(MIN_SHARE, each) * 1.05 + MERGE;
         plan.cut = by_item > by_share * (!f8 && plan.w.max_tiles >= 16 ? 1.15 : 1.0);
         parts = (int)std::min<double>(parts, std::max(1.0, each * parts / MIN_SHARE));
