@@ -165,12 +165,13 @@ typedef struct efa_paged_cache {
 /* A ragged batch. Sequence b has kv_len[b] keys in the cache; key j is row j % page_size of page pages[b * max_pages + j / page_size]. The last
  * n_b = q_start[b + 1] - q_start[b] of them are its chunk (the new tokens), and belong to rows q_start[b] ... of the row tensors, which
  * have `tokens` rows to a head. Row i of a chunk stands at position kv_len[b] - n_b + i; one at a negative position (n_b > kv_len[b]) has no place in
- * the cache and no key to see. Rows of no sequence (before q_start[0], from q_start[num_seqs] on) are neither read nor written.
+ * the cache, and under a causal mask no key to see (without one it sees all kv_len[b]). Rows of no sequence (before q_start[0], from q_start[num_seqs] on)
+ * have no part in anything and are not written; their memory is there, and may be read.
  * The three arrays are device memory, read when the kernels run: a captured graph follows their contents. The host gives
  * bounds: max_q >= every n_b, max_kv >= every kv_len[b]; tight ones choose faster kernels. Lengths outside the bounds or the
  * buffers, and page numbers outside the pool where a key lies, are reported by efa_kernel_status (code 3 and 2, sequence, site); the call then stays
  * inside its buffers: lengths are cut to the bounds, keys of a missing page read as zeros and are not written. Where q_start falls, so that sequences
- * have rows in common, attention may leave O as it was.
+ * have rows in common, attention may leave O as it was. With num_seqs, tokens or max_q 0 a call does nothing and looks at no array.
  * Sequences may share pages; a page that efa_cache_write writes to in one call should belong to one sequence. */
 typedef struct efa_paged_batch {
     const int* q_start;     /* [num_seqs + 1] */
