@@ -17,8 +17,9 @@ namespace efa {
 namespace {
 
 constexpr int PC_THREADS = 256;
-// Heads that a thread moves at a time: what it has in flight, against the blocks that there are. us with 1 / 2 / 4 (8): fp16 chunks of 8192 keys in 30.2 / 30.4 / 30.8, whole
-// sequences out 91.7 / 92.8 / 94.6; 8 bits, 12225 tokens in and out 35 / 28.8 / 29.6 (38.6), whole sequences out 110 / 102 / 99.8 (101.9).
+// Heads that a thread moves at a time: what it has in flight, against the blocks that there are. us with 1 / 2 / 4 (8): fp16, 5822 tokens x 32 heads of
+// 128 in 31.9 / 32.2 / 32.2 (33.3), 73472 keys x 16 heads of 64 out 93.8 / 94.3 / 96.0 (98.4); 8 bits, 12225 tokens x 8 heads of 128 in and out 34.1 / 30.3 / 31.0 (39.4),
+// 100451 keys x 8 of 128 out 113.9 / 104.3 / 101.8 (103.7).
 template <bool F8, bool READ> constexpr int PC_HEADS = !F8 ? 1 : READ ? 4 : 2;
 
 struct PagedRows {
@@ -75,7 +76,7 @@ __device__ __noinline__ uint2 to_e4m3_any(uint4 x, unsigned& byte)
 }
 
 // The same. Rows that are finite and below 57344 without leaving fp16: x * 2^-e is exact there, or so small that its code is 0 whatever the rounding.
-// 45 instructions a chunk against 150 (12225 tokens x 8 heads of 128: 27 -> 21 us cold, with the reading back 35.3 -> 29.6).
+// The kernel executes 112 instructions for 16 bytes, 83 without a conversion (ncu). 12225 tokens x 8 heads of 128: 27 us the way above, so 21 (cold).
 template <int LANES>
 __device__ __forceinline__ uint2 to_e4m3(const uint4& x, unsigned& byte)
 {
@@ -110,8 +111,8 @@ __device__ __forceinline__ uint4 from_e4m3(const uint2& x, unsigned byte)
 }
 
 // Rows into pages (READ: out of them). A row of a head is D / 8 lanes of 16 bytes fp16; a warp takes the 256 / D rows that it holds of one token range and up to
-// PC_HEADS heads of K and V at a time. HBM-bound for prompts (5822 tokens x 32 heads of 128 in: 30.3 us, 6.3 TB/s; 73472 x 16 of 64 out 91.7 us, 6.6 TB/s; of 8 bits
-// 100451 x 8 of 128 out 99.8 us, 6.2 TB/s), a chain of three loads (lengths, page, row) for single tokens, less than the 4.4 us that the host takes for the call.
+// PC_HEADS heads of K and V at a time. HBM-bound for prompts (5822 tokens x 32 heads of 128 in: 31.5 us, 6.1 TB/s; 73472 x 16 of 64 out 94 us, 6.4 TB/s; of 8 bits
+// 100451 x 8 of 128 out 101 us, 6.1 TB/s), a chain of three loads (lengths, page, row) for single tokens, less than the 4.7 us that the host takes for the call.
 template <int D, bool F8, bool READ>
 __global__ void __launch_bounds__(PC_THREADS)
 paged_move_kernel(const PagedArgs c, const PagedRows rows)
@@ -283,8 +284,8 @@ PagedKind kind_of(const efa_paged_cache& c, const efa_paged_batch& b, const efa_
     k.kv_cap = std::min<long long>(b.max_kv, (long long)b.max_pages * c.page_size);
     // Up to 32 rows the keys' way to the SM is the time: small tiles. More go to the tensor cores' tiles of 256 unless there is little work, counted as 64 rows x 64 keys:
     // small tiles start and end faster, and clusters share theirs. us, small tiles / tiles of 256: 64 rows, 8 heads of 128, 1000 keys 14 / 19, 2 x 16000 keys
-    // 57 / 47, 16 x 16000 296 / 190, of 8 bits 310 / 228; 32 rows, 16 x 16000 keys 171 / 186; prompts, 16 heads of 64, 128 tokens 7.8 / 8.6, 512 12.9 / 14.0,
-    // of 8 bits 256 10.0 / 11.0, 512 18.8 / 14.2; 8 heads of 16, 200 tokens over 400 keys 6.9 / 11.9; 32 heads of 128 on 8, 4 x 64 tokens 9.5 / 11.4, 128 11.2 / 11.3,
+    // 57 / 47, 16 x 16000 304 / 190, of 8 bits 307 / 230; 32 rows, 16 x 16000 keys 171 / 186; prompts, 16 heads of 64, 128 tokens 7.8 / 8.6, 512 12.9 / 14.0,
+    // of 8 bits 256 11.2 / 12.0, 512 19.3 / 14.9; 8 heads of 16, 200 tokens over 400 keys 6.9 / 11.9; 32 heads of 128 on 8, 4 x 64 tokens 9.5 / 11.4, 128 11.2 / 11.3,
     // 256 16.1 / 12.8.
     const bool f8 = c.dtype == EFA_E4M3;
     const double work = (double)b.num_seqs * c.H_kv * (double)((rows + 63) / 64) * (double)((k.kv_cap + 63) / 64);
@@ -335,14 +336,14 @@ PagedPlan plan_attention(const efa_paged_cache& c, const efa_paged_batch& b, con
         // Few rows: a block per item, or where there are few items a cluster of up to eight that shares one, merged in shared memory, as long as a block's part of
         // the longest item stays short; else equal shares of everything, which cost a merge in a launch of its own but leave no SM idle, whatever the
         // lengths. us, clusters / shares, one token: 16 heads of 64 1000 keys 5.6 / 10.2, 8000 12.4 / 14.4, 16000 20.3 / 18.9; 32 heads of 128 on 8,
-        // 1000 keys 6.8 / 10.6, 8000 15.8 / 17.2, 16000 26.4 / 19.9; 8 bits 7.2 / 10.9, 16.0 / 17.0, 25.5 / 20.2; 64 such sequences (no clusters) 1000 keys 45 / 50.
+        // 1000 keys 6.8 / 10.6, 8000 15.8 / 17.2, 16000 26.4 / 19.9; 8 bits (with the host's part) 8.8 / 13.1, 18.1 / 21.6, 29.0 / 27.3; 64 such sequences (no clusters) 1000 keys 45 / 50.
         parts *= paged_rows_blocks_per_sm(c.d_h, f8);
         while (plan.cluster < 8 && plan.cluster * 2 <= units && items * plan.cluster * 2 <= parts) plan.cluster *= 2;
         plan.cut = units * unit > (c.d_h == 128 ? 1024 : 1536) * plan.cluster;
         if (plan.cut) {
             plan.cluster = 1;
-            // Where memory is the time (8 bits are not: 177 us without, 185 with): 64 sequences of 4096 keys, 16 heads of 64 173 -> 164 us, of up to 8192, 8 heads of 128
-            // 175 -> 169.5.
+            // Where memory is the time: us without / with, 64 sequences of 4096 keys, 16 heads of 64 176.6 / 167.0, of up to 8192, 8 heads of 128 176.5 / 172.0; but
+            // of 8 bits 121.7 / 126.8, 105.7 / 110.
             if (!f8 && c.d_h >= 64 && items * units >= (long long)parts * LATE_RATIO * LATE_UNITS) plan.w.late = parts * 3 / 4;
             parts += plan.w.late;
         }

@@ -12,7 +12,7 @@
 //
 // Measured (64 sequences of 129 to 8192 keys, one token, 32 heads of 128 on 8, fp16): 1.11 GB in 170 us, 6.5 TB/s; call after call on inputs in turn 177 us (6.27 TB/s,
 // 0.96 of a copy). ncu (32 x 4096 keys): 537 MB from DRAM for 537 MB of keys and values, three of four stalls are waits for them.
-// Of 8 bits: 16 sequences of 2051 to 32768 keys, up to four tokens: 0.60 GB in 110 us, 125 in turn (4.8 TB/s): half the bytes for the same arithmetic and the conversion, issue
+// Of 8 bits: 16 sequences of 2051 to 32768 keys, up to four tokens: 0.60 GB in 110 us, 118 in turn (5.1 TB/s): half the bytes for the same arithmetic and the conversion, issue
 // slots half busy with twelve warps that wait for their own results. Tried and slower: all keys' heads in another order of shares (0), two to six times as many
 // shares (+0 to +20 %), values that are not finite made 0 in shared memory instead of in registers (small calls +15 %).
 //
@@ -33,8 +33,8 @@ namespace {
 constexpr int PR_THREADS = 128;
 
 // Blocks of an SM and stages of each: where loading is the time (fp16 heads of 64 and 128) few blocks with deep rings, else more warps. us, 64 sequences of 4096
-// keys, one token, as here / as two blocks of 96 KB: 16 heads of 64 fp16 172 / 172 (three blocks of 64 KB: 210), 8 bits 124 / 138; 32 heads of
-// 32 179 / 206, 183 / 254; 64 heads of 16 269 / 484, 312 / 563 (8 bits before the exponents went to the values); 16 sequences of 16000 keys, 8 heads of 128 165 / 165, 97 / 101.
+// keys, one token, as here / as two blocks of 96 KB: 16 heads of 64 fp16 168 / 168 (three blocks of 64 KB: 210), 8 bits 122 / 133; 32 heads of
+// 32 181 / 207, 171 / 196; 64 heads of 16 256 / 352, 276 / 394; 16 sequences of 16000 keys, 8 heads of 128 165 / 166, 95 / 101.
 constexpr int rows_blocks(int d, bool f8) { return d >= 64 ? (f8 ? 3 : 2) : d == 16 && f8 ? 6 : 4; }
 template <int D, bool F8> constexpr int blocks_of = rows_blocks(D, F8);
 constexpr int rows_stages(int d, bool f8) { return d == 128 ? (f8 ? 2 : 3) : d == 64 ? (f8 ? 4 : 6) : d == 16 && f8 ? 4 : 6; }

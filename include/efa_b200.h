@@ -184,7 +184,7 @@ typedef struct efa_paged_batch {
 const char* efa_paged_check(const efa_paged_cache* cache, const efa_paged_batch* batch);
 
 /* Rows K, V (fp16) of the batch's chunks into their pages. Element (head, row, x) at head * head_stride + row * token_stride + x; both strides 0:
- * [H_kv][tokens][d_h], as efa_compute_qkv_f16 writes them. Strides are multiples of 8, K and V 16-byte aligned.
+ * [H_kv][tokens][d_h], as efa_compute_qkv_f16 writes them. Strides are multiples of 8 and at least d_h, rows do not overlap, K and V are 16-byte aligned.
  * e4m3: per row the smallest exponent e >= -24 with max |x| <= 448 * 2^e, codes x * 2^-e rounded to nearest, ties to even (with e = 8 cut at
  * 240, as 256 * 2^8 is no fp16); infinities and NaN are stored as NaN and do not count for the maximum. Asynchronous on `stream`. The first call of
  * these entry points on a device must come before any stream capture (the status word is allocated then). */
@@ -213,7 +213,8 @@ size_t efa_paged_attention_workspace(const efa_paged_cache* cache, const efa_pag
 
 /* Attention of the chunks over the cache, the chunk's own keys included (efa_cache_write first): O[row][h * d_h + x], fp16, what
  * efa_project_f16 takes. Scores, maxima, sums and O are accumulated in fp32; the softmax weights are rounded to fp16 for their product with V.
- * A row that sees no key becomes zeros. Values that are not finite reach only the rows that see them.
+ * A row that sees no key becomes zeros. Values that are not finite reach only the rows that see them; of finite ones up to 65472 O is finite (the weights'
+ * rounding may lift a mean of 65504, fp16's largest, above it).
  * workspace: 16-byte aligned device memory that no other call uses until this one is done (two captured graphs that may run
  * side by side need one each); its contents do not matter before and after. Equal calls give equal bits; the bits of a sequence
  * may depend on the lengths of the others, by the fp32 order in which parts of long sequences are added. Asynchronous on `stream`. */
