@@ -44,7 +44,7 @@ paged_chains_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     __shared__ __align__(8) uint64_t s_full[4], p_full[4], o_done[4];
     __shared__ float ends[4][2][WS_BM];                           // offset and sum of every chain's rows
     __shared__ uint32_t tmem_base_smem;
-    __shared__ int abort_word, poison;
+    __shared__ int abort_word, poison, far_word;
     __shared__ PagedScratch scratch;
     __shared__ PagedPiece s_piece[2];
     __shared__ int s_place[2];
@@ -106,6 +106,7 @@ paged_chains_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     auto fetch_item = [&](int round) -> bool {
         if (tid == 0) {
             poison = 0;
+            far_word = 0;
             if (round > 0) {
                 for (int t = 0; t < 2; t++) mbar_inval(&q_full[t]);
                 for (int s = 0; s < NS; s++) { mbar_inval(&k_full[s]); mbar_inval(&k_empty[s]); mbar_inval(&v_full[s]); mbar_inval(&v_empty[s]); mbar_inval(&v_raw[s]); }
@@ -290,6 +291,7 @@ paged_chains_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
                     const uint32_t dst = smem_u32(sQ + tile * C::TILE_BYTES);
                     constexpr int CH = D / 8, STEPS = CH / 2 > 0 ? CH / 2 : 1;
                     uint4 x[STEPS];
+                    uint32_t top = 0u;
                     #pragma unroll
                     for (int i = 0; i < STEPS; i++) {
                         const int rr = way * 16 + (i * 32 + lane) / CH, k = (i * 32 + lane) % CH;
@@ -300,17 +302,22 @@ paged_chains_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
                     for (int i = 0; i < STEPS; i++) {
                         const int rr = (row & ~31) + way * 16 + (i * 32 + lane) / CH, k = (i * 32 + lane) % CH;
                         sts128(dst + swizzled<C::SWB>((uint32_t)rr * C::SWB + (uint32_t)k * 16u), x[i]);
+                        top = max_abs_f16x2(max_abs_f16x2(max_abs_f16x2(max_abs_f16x2(top, x[i].x), x[i].y), x[i].z), x[i].w);
                     }
+                    if (scores_far<D>(top, a.scale_log2e)) *(volatile int*)&far_word = 1;      // for the other chain's warps too
                     fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&q_full[tile]);
                 }
             }
 
+            bool ok = n == 0 || __all_sync(0xffffffffu, mbar_wait(&q_full[tile], 0u, &abort_word, 33));
+            const bool far = __shfl_sync(0xffffffffu, *(volatile int*)&far_word, 0) != 0;
+            const float scale = far ? 1.f : a.scale_log2e;            // of the scores as the loop has them
+            const int slow_from = far ? 0 : jm;                       // stages that are masked or scaled
             float m_ref = kNegInfW;     // exponent offset in use (a past row maximum), scaled by scale*log2(e)
             float l_run = 0.f;          // running denominator relative to m_ref
-            bool ok = true;
-            for (int i = 0; i < n; i++) {
+            for (int i = 0; i < n && ok; i++) {
                 ok = __all_sync(0xffffffffu, mbar_wait(&s_full[ch], (uint32_t)(i & 1), &abort_word, 31));
                 if (!ok) break;
                 tc_fence_after_sync();
@@ -319,7 +326,13 @@ paged_chains_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
                 tmem_ld32(tmem_S + 32, su[1]);
                 tmem_wait_ld();
 
-                if (i >= jm) {
+                if (i >= slow_from) {
+                    if (far) {
+                        #pragma unroll
+                        for (int x = 0; x < 2; x++)
+                            #pragma unroll
+                            for (int k = 0; k < 32; k++) su[x][k] = __float_as_uint(__uint_as_float(su[x][k]) * a.scale_log2e);
+                    }
                     const int lim = lim0 - i * WS_BN;
                     #pragma unroll
                     for (int x = 0; x < 2; x++)
@@ -336,7 +349,7 @@ paged_chains_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
                     mx2 = max3(mx2, __uint_as_float(su[1][k]), __uint_as_float(su[1][k + 1]));
                     mx3 = max3(mx3, __uint_as_float(su[1][16 + k]), __uint_as_float(su[1][17 + k]));
                 }
-                const float mx = fmaxf(max3(mx0, mx1, mx2), mx3) * a.scale_log2e;
+                const float mx = fmaxf(max3(mx0, mx1, mx2), mx3) * scale;
 
                 // Move the exponent offset only when the maximum grew by more than the threshold.
                 float alpha = 1.f;
@@ -345,7 +358,7 @@ paged_chains_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
                     m_ref = mx;
                 }
                 const float m_off = (m_ref == kNegInfW) ? 0.f : m_ref;
-                const uint64_t scale2 = pack2(a.scale_log2e, a.scale_log2e), off2 = pack2(-m_off, -m_off);
+                const uint64_t scale2 = pack2(scale, scale), off2 = pack2(-m_off, -m_off);
                 uint64_t psum2[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
                 // Complete with S(i): PV(i-1), so O may be rescaled and P take the place of S.
                 auto rescale = [&]() {

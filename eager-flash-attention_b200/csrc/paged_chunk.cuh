@@ -46,6 +46,22 @@ struct ChunkCfg {
 template <int SWB>
 __device__ __forceinline__ uint32_t swizzled(uint32_t at) { return at ^ ((at >> 3) & (SWB == 128 ? 0x70u : SWB == 64 ? 0x30u : 0x10u)); }
 
+// Weights are 2^(scale * s - offset) in one instruction, the offset a rounded scale * max: off by half its last bit, for all keys of a row alike, which cancels as long as fp16
+// holds the weights: up to offsets of 2^27 (a factor of 2^4, beside 2^8 by which a maximum may outgrow the offset). Rows of Q that might go beyond that, with keys of
+// 65504, have their scores scaled first; a difference to the maximum is exact then.
+__device__ __forceinline__ uint32_t max_abs_f16x2(uint32_t a, uint32_t b)
+{
+    uint32_t r;
+    asm("max.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+template <int D>
+__device__ __forceinline__ bool scores_far(uint32_t top /* largest |q|, of either half */, float scale_log2e)
+{
+    const float2 q = __half22float2(*reinterpret_cast<const __half2*>(&top));
+    return fmaxf(fabsf(q.x), fabsf(q.y)) * (65504.f * D) * scale_log2e > 134217728.f;
+}
+
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar)
 {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
@@ -423,11 +439,13 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             const int head = it.p.h * a.w.G + (valid ? r - token * a.w.G : 0);
 
             // ---- the warp's 32 rows of Q into the tile, as many lanes to a row as it has chunks of 16 bytes
+            bool far = false;
             if (my_nblk > 0) {
                 const long long off = (long long)head * a.q_head + (long long)(it.p.q.row0 + token) * a.q_token;
                 const uint32_t dst = smem_u32(sQ + q * C::TILE_BYTES);
                 constexpr int CH = D / 8;
                 uint4 x[CH];
+                uint32_t top = 0u;
                 #pragma unroll
                 for (int i = 0; i < CH; i++) {
                     const int rr = (i * 32 + lane) / CH, ch = (i * 32 + lane) % CH;
@@ -438,12 +456,16 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                 for (int i = 0; i < CH; i++) {
                     const int rr = (row & ~31) + (i * 32 + lane) / CH, ch = (i * 32 + lane) % CH;
                     sts128(dst + (uint32_t)(ch * 8 / C::BOXC) * C::BOX_BYTES + swizzled<C::SWB>((uint32_t)rr * C::SWB + (uint32_t)(ch * 8 % C::BOXC) * 2u), x[i]);
+                    top = max_abs_f16x2(max_abs_f16x2(max_abs_f16x2(max_abs_f16x2(top, x[i].x), x[i].y), x[i].z), x[i].w);
                 }
+                far = __any_sync(0xffffffffu, scores_far<D>(top, a.scale_log2e));
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&q_full[q]);
             }
 
+            const float scale = far ? 1.f : a.scale_log2e;              // of the scores as the loop has them
+            const int slow_from = far ? 0 : jm;                         // stages that are masked or scaled
             float m_ref = kNegInfW, m_true = kNegInfW, l_run = 0.f;     // as in fa_fwd_ws_kernel
             bool ok = true;
             for (int j = 0; j < my_nblk; j++) {
@@ -460,7 +482,13 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                 for (int x = 0; x < 4; x++) tmem_ld32(tmem_S + x * 32, su[x]);
                 tmem_wait_ld();
 
-                if (j >= jm) {
+                if (j >= slow_from) {
+                    if (far) {
+                        #pragma unroll
+                        for (int x = 0; x < 4; x++)
+                            #pragma unroll
+                            for (int i = 0; i < 32; i++) su[x][i] = __float_as_uint(__uint_as_float(su[x][i]) * a.scale_log2e);
+                    }
                     const int lim = sees - (u_lo + j) * WS_BN;           // keys of the stage that the row sees
                     #pragma unroll
                     for (int x = 0; x < 4; x++)
@@ -478,7 +506,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                     mx3 = max3(mx3, __uint_as_float(su[3][i]), __uint_as_float(su[3][i + 1]));
                 }
                 const float mx = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3));
-                m_true = fmaxf(m_true, mx * a.scale_log2e);
+                m_true = fmaxf(m_true, mx * scale);
 
                 float alpha = 1.f;
                 if (m_true - m_ref > a.rescale_above || m_ref == kNegInfW) {
@@ -489,7 +517,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                 }
                 const float m_off = (m_ref == kNegInfW) ? 0.f : m_ref;
 
-                const uint64_t scale2 = pack2(a.scale_log2e, a.scale_log2e), off2 = pack2(-m_off, -m_off);
+                const uint64_t scale2 = pack2(scale, scale), off2 = pack2(-m_off, -m_off);
                 uint64_t psum2[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
                 auto weights = [&](int x, uint32_t (&pk)[16]) {
                     #pragma unroll
