@@ -12,7 +12,7 @@
 //
 // Measured (64 sequences of 129 to 8192 keys, one token, 32 heads of 128 on 8, fp16): 1.11 GB in 170 us, 6.5 TB/s; call after call on inputs in turn 177 us (6.27 TB/s,
 // 0.96 of a copy). ncu (32 x 4096 keys): 537 MB from DRAM for 537 MB of keys and values, three of four stalls are waits for them.
-// Of 8 bits: 16 sequences of 2051 to 32768 keys, up to four tokens: 0.60 GB in 110 us, 118 in turn (5.1 TB/s): half the bytes for the same arithmetic and the conversion, issue
+// Of 8 bits: 16 sequences of 2051 to 32768 keys, up to four tokens: 0.60 GB in 110 us, 118 to 125 in turn, by the box (5.1 to 4.8 TB/s): half the bytes for the same arithmetic and the conversion, issue
 // slots half busy with twelve warps that wait for their own results. Tried and slower: all keys' heads in another order of shares (0), two to six times as many
 // shares (+0 to +20 %), values that are not finite made 0 in shared memory instead of in registers (small calls +15 %).
 //
