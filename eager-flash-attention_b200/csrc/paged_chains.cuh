@@ -7,7 +7,7 @@
 //
 // What bounds it: the special-function unit (63 % busy in ncu at 2048 tokens x 16 heads over 8192 keys, tensor pipe 35 %), and per item about 7 us besides its units of
 // 1.45 us (256 rows x 128 keys; two chains of 128 keys 1.63): us, two chains / this: 16 heads of 64, 4096 tokens 59.0 / 56.7, 8192 196 / 181; 64 rows, 16 x 16000 keys
-// 159 / 129. Prompts of 1024 tokens and less are the same or 5 % slower, and mostly go to the small tiles.
+// 159 / 129 (since then 1 to 2 % for scores far from zero and slots behind the last key). Prompts of 1024 tokens and less are the same or 5 % slower, and mostly go to the small tiles.
 #pragma once
 
 template <int D>
