@@ -327,7 +327,7 @@ class _Call:
             self.pool = pkg.page_pool(s["refs"], s["pages"], s["kv_len"], c["page"])
             if "k" in s:
                 self.cache = pkg.paged_cache(s["k"], s["v"], s.get("k_exp"), s.get("v_exp"))
-            size = pkg.pages_workspace(self.pool) if op in ("fork", "take") else 0
+            size = pkg.pages_workspace(self.pool) if op != "copy" else 0
             self.workspace = torch.empty(size, dtype=torch.uint8, device="cuda") if size else None
 
 
@@ -347,7 +347,7 @@ def _through_package(s):
         pkg.pages_fork(call.pool, call.cache, s["parents"], s["children"], call.workspace, stream=stream)
         pkg.pages_free(call.pool, s["children"], stream=stream)
     elif op == "compact":
-        pkg.pages_compact(call.pool, call.cache, s["pages_out"], s["refs_out"], s["moved"], stream=stream)
+        pkg.pages_compact(call.pool, call.cache, s["pages_out"], s["refs_out"], s["moved"], call.workspace, stream=stream)
     else:
         pkg.pages_copy(call.cache, s["src"], s["dst"], stream=stream)
 
