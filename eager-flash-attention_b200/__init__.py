@@ -30,6 +30,8 @@ REDUCE_NCCL, REDUCE_P2P, REDUCE_NVLS, REDUCE_PULL = 0, 1, 2, 3
 ROWS_AUTO, ROWS_ASCENDING, ROWS_DESCENDING, ROWS_MIXED = 0, 1, 2, 3
 WIRE_AUTO, WIRE_F16, WIRE_F32 = 0, 1, 2
 RECIPE_REF, RECIPE_NORMAL = 0, 1
+NORM_RMS, NORM_LAYER = 0, 1
+GATE_NONE, GATE_PLAIN, GATE_SIGMOID = 0, 1, 2
 
 
 class EfaError(RuntimeError):
@@ -100,6 +102,25 @@ class PagedAttentionParams(C.Structure):
                 ("q_head_stride", C.c_int64), ("q_token_stride", C.c_int64), ("o_token_stride", C.c_int64)]
 
 
+class PagePool(C.Structure):
+    """efa_page_pool: which pages of a cache are whose. ``page_pool`` makes one of tensors and keeps them alive."""
+    _fields_ = [("refs", C.c_void_p), ("pages", C.c_void_p), ("kv_len", C.c_void_p),
+                ("num_pages", C.c_int), ("page_size", C.c_int), ("num_seqs", C.c_int), ("max_pages", C.c_int)]
+
+
+class BlockNormParams(C.Structure):
+    """efa_block_norm_params; strides in elements, 0 = dense."""
+    _fields_ = [("d", C.c_int), ("kind", C.c_int), ("post", C.c_int), ("pre", C.c_int), ("gate", C.c_int), ("gate_rows", C.c_int),
+                ("eps", C.c_float), ("residual_scale", C.c_float), ("block_scale", C.c_float), ("x_dtype", C.c_int), ("y_dtype", C.c_int),
+                ("x_stride", C.c_int64), ("y_stride", C.c_int64), ("out_stride", C.c_int64), ("h_stride", C.c_int64), ("gate_stride", C.c_int64)]
+
+
+class W4(C.Structure):
+    """efa_w4: a projection's weights in 4 bits. ``w4_weight`` makes one of tensors and keeps them alive."""
+    _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p), ("zeros", C.c_void_p), ("d_in", C.c_int), ("d_out", C.c_int), ("group", C.c_int),
+                ("code_stride", C.c_int64), ("scale_stride", C.c_int64), ("zero_stride", C.c_int64)]
+
+
 class StreamGroup(C.Structure):
     """efa_stream_group: tiles [first_tile, first_tile + ntiles) share one projection and one AllReduce."""
     _fields_ = [("first_tile", C.c_int), ("ntiles", C.c_int)]
@@ -134,6 +155,17 @@ _SIGNATURES = {
     "efa_cache_read": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.POINTER(PagedCache), C.POINTER(PagedBatch), C.c_void_p]),
     "efa_paged_attention": (C.c_int, [C.c_void_p, C.c_void_p, C.POINTER(PagedCache), C.POINTER(PagedBatch),
                                       C.POINTER(PagedAttentionParams), C.c_void_p, C.c_size_t, C.c_void_p]),
+    "efa_page_pool_check": (C.c_char_p, [C.POINTER(PagePool)]),
+    "efa_pages_workspace": (C.c_size_t, [C.POINTER(PagePool)]),
+    "efa_pages_take": (C.c_int, [C.POINTER(PagePool), C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "efa_pages_fork": (C.c_int, [C.POINTER(PagePool), C.POINTER(PagedCache), C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "efa_pages_free": (C.c_int, [C.POINTER(PagePool), C.c_void_p, C.c_int, C.c_void_p]),
+    "efa_pages_compact": (C.c_int, [C.POINTER(PagePool), C.POINTER(PagedCache), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "efa_pages_copy": (C.c_int, [C.POINTER(PagedCache), C.c_void_p, C.c_void_p, C.c_int, C.c_void_p]),
+    "efa_block_norm_check": (C.c_char_p, [C.POINTER(BlockNormParams), C.c_int]),
+    "efa_block_norm": (C.c_int, [C.c_void_p] * 9 + [C.c_int, C.POINTER(BlockNormParams), C.c_void_p]),
+    "efa_w4_check": (C.c_char_p, [C.POINTER(W4)]),
+    "efa_project_w4": (C.c_int, [C.c_void_p, C.c_int64, C.POINTER(W4), C.c_void_p, C.c_int, C.c_int64, C.c_int, C.c_void_p]),
     "efa_kernel_status": (C.c_int, [C.POINTER(C.c_int)]),
     "efa_kernel_status_reset": (C.c_int, []),
     "efa_mode_name": (C.c_char_p, [C.c_int]),
@@ -456,6 +488,192 @@ def paged_attention(Q, O, cache: PagedCache, batch: PagedBatch, ap: PagedAttenti
     Q = _rows("paged_attention", Q, batch, need, not (by_head or by_token))
     O = _rows("paged_attention", O, batch, (tokens - 1) * o_token + width if o_token else width * tokens, not o_token)
     _check(lib().efa_paged_attention(Q, O, cache, batch, ap, _ptr(workspace), workspace_bytes, _stream(stream)), "paged_attention")
+
+
+# ------------------------------------------------------------------------------------------------
+# Pages of a cache
+# ------------------------------------------------------------------------------------------------
+_int32 = None    # torch.int32, once a tensor of it has been seen
+
+
+def _ints(what: str, x, need: int) -> Optional[int]:
+    """Address of ``need`` int32 numbers, one after another."""
+    global _int32
+    dtype = getattr(x, "dtype", None)
+    if dtype is not None and dtype is _int32 and x.numel() >= need and x.is_contiguous():
+        return x.data_ptr()
+    if not hasattr(x, "data_ptr"):
+        return _ptr(x)
+    if str(dtype) != "torch.int32" or x.numel() < need or not x.is_contiguous():
+        raise EfaError(f"{what} must be a dense int32 tensor of {need} numbers")
+    _int32 = dtype
+    return x.data_ptr()
+
+
+def page_pool(refs, pages, kv_len, page_size: int) -> PagePool:
+    """A pool of int32 tensors: ``refs [num_pages]`` (uses of each page, 0 = free; zeros to begin with), and a server's slots, ``pages [num_seqs][max_pages]``
+    and ``kv_len [num_seqs]``: the tensors that ``paged_batch`` takes. The calls below change them."""
+    if any(str(x.dtype) != "torch.int32" or not x.is_contiguous() for x in (refs, pages, kv_len)):
+        raise EfaError("page_pool: refs, pages and kv_len must be dense int32 tensors")
+    if pages.device != refs.device or kv_len.device != refs.device:
+        raise EfaError("page_pool: the tensors must be on one device")
+    if refs.dim() != 1 or kv_len.dim() != 1 or pages.dim() != 2 or pages.shape[0] != kv_len.numel():
+        raise EfaError("page_pool: refs must be [num_pages], pages [num_seqs][max_pages], kv_len [num_seqs]")
+    p = PagePool(_ptr(refs), _ptr(pages), _ptr(kv_len), refs.numel(), page_size, kv_len.numel(), pages.shape[1])
+    p.tensors = (refs, pages, kv_len)
+    why = lib().efa_page_pool_check(p)
+    if why is not None:
+        raise EfaError(f"page_pool: {why.decode()}")
+    return p
+
+
+def pages_workspace(pool: PagePool) -> int:
+    """Bytes of workspace that pages_take, pages_fork and pages_compact need."""
+    return lib().efa_pages_workspace(pool)
+
+
+def _pairs(what: str, a, b) -> int:
+    if a.numel() != b.numel():
+        raise EfaError(f"{what} must be as many")
+    return a.numel()
+
+
+def _space(workspace, workspace_bytes: Optional[int]):
+    if workspace_bytes is None:
+        workspace_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    return _ptr(workspace), workspace_bytes
+
+
+def pages_take(pool: PagePool, q_start, workspace, stream=None, workspace_bytes: Optional[int] = None) -> None:
+    """Every slot grows by its new tokens, ``q_start[b + 1] - q_start[b]``, and gets the lowest free pages for them. What the pool cannot give becomes -1 in
+    the table and is reported (kernel_status code 4)."""
+    _check(lib().efa_pages_take(pool, _ints("pages_take: q_start", q_start, pool.num_seqs + 1), *_space(workspace, workspace_bytes), _stream(stream)), "pages_take")
+
+
+def pages_fork(pool: PagePool, cache: PagedCache, parents, children, workspace, stream=None, n: Optional[int] = None, workspace_bytes: Optional[int] = None) -> None:
+    """Slots ``children`` (empty ones) become copies of slots ``parents``: full pages are shared, a partly filled last page is copied."""
+    n = _pairs("pages_fork: parents and children", parents, children) if n is None else n
+    _check(lib().efa_pages_fork(pool, cache, _ints("pages_fork: parents", parents, n), _ints("pages_fork: children", children, n), n,
+                                *_space(workspace, workspace_bytes), _stream(stream)), "pages_fork")
+
+
+def pages_free(pool: PagePool, seqs, stream=None, n: Optional[int] = None) -> None:
+    """Slots ``seqs`` become empty; their pages are free when no other slot has them."""
+    n = seqs.numel() if n is None else n
+    _check(lib().efa_pages_free(pool, _ints("pages_free: seqs", seqs, n), n, _stream(stream)), "pages_free")
+
+
+def pages_compact(pool: PagePool, cache: PagedCache, pages_out, refs_out, moved, workspace, stream=None, workspace_bytes: Optional[int] = None) -> None:
+    """The pages in use become the pool's first ones: keys move, ``pages_out`` and ``refs_out`` (the pool's own tensors, or others) are table and counts after that,
+    ``moved [num_pages]`` the new place of each page (-1: a free one)."""
+    _check(lib().efa_pages_compact(pool, cache, _ints("pages_compact: pages_out", pages_out, pool.num_seqs * pool.max_pages),
+                                   _ints("pages_compact: refs_out", refs_out, pool.num_pages), _ints("pages_compact: moved", moved, pool.num_pages),
+                                   *_space(workspace, workspace_bytes), _stream(stream)), "pages_compact")
+
+
+def pages_copy(cache: PagedCache, src, dst, stream=None, n: Optional[int] = None) -> None:
+    """Pages ``src[i]`` to pages ``dst[i]``, keys, values and exponents."""
+    n = _pairs("pages_copy: src and dst", src, dst) if n is None else n
+    _check(lib().efa_pages_copy(cache, _ints("pages_copy: src", src, n), _ints("pages_copy: dst", dst, n), n, _stream(stream)), "pages_copy")
+
+
+# ------------------------------------------------------------------------------------------------
+# Around the block: norms, projections with 4-bit weights
+# ------------------------------------------------------------------------------------------------
+_REAL = {"torch.float16": F16, "torch.float32": F32}
+_real = {}       # torch's types themselves, as they are seen
+
+
+def _dtype(what: str, x, want: Optional[int] = None) -> int:
+    kind = _real.get(x.dtype)
+    if kind is None:
+        kind = _REAL.get(str(x.dtype))
+        if kind is None:
+            raise EfaError(f"{what} must be torch.float16 or torch.float32, not {x.dtype}")
+        _real[x.dtype] = kind
+    if want is not None and kind != want:
+        raise EfaError(f"{what} must be torch.{'float16' if want == F16 else 'float32'}, not {x.dtype}")
+    return kind
+
+
+def _matrix(what: str, x, rows: int, width: int, stride: int, kind: int) -> Optional[int]:
+    """Address of ``rows`` rows of ``width`` elements, ``stride`` apart (0: dense). A tensor of another type or that ends before them is refused."""
+    if x is None or not hasattr(x, "data_ptr"):
+        return _ptr(x)
+    _dtype(what, x, kind)
+    if rows <= 0:
+        return x.data_ptr()
+    need = (rows - 1) * (stride or width) + width
+    if x.numel() >= need and x.is_contiguous():
+        return x.data_ptr()
+    if not stride:
+        raise EfaError(f"{what} must be a dense tensor of {need} elements, or its stride be given")
+    if x.stride(-1) != 1 and x.shape[-1] > 1:
+        raise EfaError(f"{what}: the elements of a row must be neighbours")
+    if x.untyped_storage().nbytes() // x.element_size() - x.storage_offset() < need:
+        raise EfaError(f"{what}: rows of this stride end {need} elements behind the tensor's first, beyond its memory")
+    return x.data_ptr()
+
+
+def block_norm_params(d: int, kind: int = NORM_RMS, eps: float = 1e-6, post: bool = False, pre: bool = True, gate: int = GATE_NONE, gate_rows: bool = False,
+                      residual_scale: float = 1.0, block_scale: float = 1.0, x_dtype: int = F16, y_dtype: int = F16, x_stride: int = 0, y_stride: int = 0,
+                      out_stride: int = 0, h_stride: int = 0, gate_stride: int = 0) -> BlockNormParams:
+    """``post``: the block's output is normalised; ``pre``: the sum is, into h. Strides in elements from a row to the next, 0 = dense."""
+    return BlockNormParams(d, kind, int(bool(post)), int(bool(pre)), gate, int(bool(gate_rows)), eps, residual_scale, block_scale, x_dtype, y_dtype,
+                           x_stride, y_stride, out_stride, h_stride, gate_stride)
+
+
+def block_norm_check(bp: BlockNormParams, rows: int) -> Optional[str]:
+    """None if block_norm is legal for these sizes, else the reason. Host arithmetic."""
+    why = lib().efa_block_norm_check(C.byref(bp), rows)
+    return None if why is None else why.decode()
+
+
+def block_norm(x, y, x_out, h, rows: int, bp: BlockNormParams, gate=None, post_w=None, post_b=None, pre_w=None, pre_b=None, stream=None) -> None:
+    """Norms after and before a block with its gate and residual addition, per row: ``n = post ? norm(y) * post_w + post_b : y``,
+    ``x_out = residual_scale * x + block_scale * act(gate) * n``, ``h = norm(x_out before its rounding) * pre_w + pre_b``. None: no such input or output
+    (weights: ones, biases: zeros). x_out and h may be x or y. Asynchronous on ``stream``."""
+    d = bp.d
+    _check(lib().efa_block_norm(
+        _matrix("block_norm: x", x, rows, d, bp.x_stride, bp.x_dtype), _matrix("block_norm: y", y, rows, d, bp.y_stride, bp.y_dtype),
+        _matrix("block_norm: gate", gate, rows if bp.gate_rows else 1, d, bp.gate_stride, F16),
+        _matrix("block_norm: post_w", post_w, 1, d, 0, F16), _matrix("block_norm: post_b", post_b, 1, d, 0, F16),
+        _matrix("block_norm: pre_w", pre_w, 1, d, 0, F16), _matrix("block_norm: pre_b", pre_b, 1, d, 0, F16),
+        _matrix("block_norm: x_out", x_out, rows, d, bp.out_stride, bp.x_dtype), _matrix("block_norm: h", h, rows, d, bp.h_stride, F16),
+        rows, bp, _stream(stream)), "block_norm")
+
+
+def w4_weight(codes, scales, zeros=None) -> W4:
+    """Weights of tensors: ``codes`` uint8 ``[d_out][d_in / 2]`` (the even k in the low half), ``scales`` fp16 and ``zeros`` uint8 (None: 8) ``[d_in / group][d_out]``.
+    Slices of larger tensors (a rank's rows or columns) as they are: a row's elements must be neighbours."""
+    if codes.dim() != 2 or scales.dim() != 2 or str(codes.dtype) != "torch.uint8" or str(scales.dtype) != "torch.float16":
+        raise EfaError("w4_weight: codes must be uint8 [d_out][d_in / 2], scales fp16 [d_in / group][d_out]")
+    d_out, d_in, groups = codes.shape[0], 2 * codes.shape[1], scales.shape[0]
+    if scales.shape[1] != d_out or groups < 1 or d_in % groups:
+        raise EfaError("w4_weight: codes must be uint8 [d_out][d_in / 2], scales fp16 [d_in / group][d_out]")
+    if zeros is not None and (str(zeros.dtype) != "torch.uint8" or zeros.shape != scales.shape):
+        raise EfaError("w4_weight: zeros must be uint8, of the scales' shape")
+    if any(x is not None and x.device != codes.device for x in (scales, zeros)):
+        raise EfaError("w4_weight: the tensors must be on one device")
+    for x in (codes, scales, zeros):
+        if x is not None and ((x.stride(1) != 1 and x.shape[1] > 1) or (x.shape[0] > 1 and x.stride(0) < x.shape[1])):
+            raise EfaError("w4_weight: the elements of a row must be neighbours, and rows not overlap")
+    strides = [x.stride(0) if x is not None and x.shape[0] > 1 else 0 for x in (codes, scales, zeros)]
+    w = W4(_ptr(codes), _ptr(scales), _ptr(zeros), d_in, d_out, d_in // groups, *strides)
+    w.tensors = (codes, scales, zeros)
+    why = lib().efa_w4_check(w)
+    if why is not None:
+        raise EfaError(f"w4_weight: {why.decode()}")
+    return w
+
+
+def project_w4(X, w: W4, out, rows: int, stream=None, x_stride: int = 0, out_stride: int = 0, out_dtype: Optional[int] = None) -> None:
+    """``out[rows][d_out] = X[rows][d_in] @ w``, out fp16 or fp32 (``out_dtype`` where out is an address; strides in elements, 0 = dense). Made for few rows; prompts
+    go through ``project`` with fp16 weights. Asynchronous on ``stream``."""
+    if out_dtype is None:
+        out_dtype = _dtype("project_w4: out", out) if hasattr(out, "dtype") else F16
+    _check(lib().efa_project_w4(_matrix("project_w4: X", X, rows, w.d_in, x_stride, F16), x_stride, w,
+                                _matrix("project_w4: out", out, rows, w.d_out, out_stride, out_dtype), out_dtype, out_stride, rows, _stream(stream)), "project_w4")
 
 
 def kernel_status() -> Sequence[int]:

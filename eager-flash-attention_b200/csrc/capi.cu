@@ -4,6 +4,7 @@
 #include "nvls_reduce.h"
 #include "paged_attention.h"
 #include "runtime.h"
+#include "serving.h"
 
 #include <cuda_fp16.h>
 
@@ -123,6 +124,75 @@ extern "C" int efa_paged_attention(const void* Q, void* O, const efa_paged_cache
 {
     if (!cache || !batch || !p) { set_error("efa_paged_attention: null argument"); return 2; }
     return paged_attention(Q, O, *cache, *batch, *p, workspace, workspace_bytes, (cudaStream_t)stream);
+}
+
+extern "C" const char* efa_page_pool_check(const efa_page_pool* pool)
+{
+    if (!pool) return "null argument";
+    return page_pool_check(*pool);
+}
+
+extern "C" size_t efa_pages_workspace(const efa_page_pool* pool)
+{
+    if (!pool || page_pool_check(*pool)) return 0;
+    return pages_bytes(*pool);
+}
+
+extern "C" int efa_pages_take(const efa_page_pool* pool, const int* q_start, void* workspace, size_t workspace_bytes, void* stream)
+{
+    if (!pool) { set_error("efa_pages_take: null argument"); return 2; }
+    return pages_take(*pool, q_start, workspace, workspace_bytes, (cudaStream_t)stream);
+}
+
+extern "C" int efa_pages_fork(const efa_page_pool* pool, const efa_paged_cache* cache, const int* parents, const int* children, int n,
+                              void* workspace, size_t workspace_bytes, void* stream)
+{
+    if (!pool || !cache) { set_error("efa_pages_fork: null argument"); return 2; }
+    return pages_fork(*pool, *cache, parents, children, n, workspace, workspace_bytes, (cudaStream_t)stream);
+}
+
+extern "C" int efa_pages_free(const efa_page_pool* pool, const int* seqs, int n, void* stream)
+{
+    if (!pool) { set_error("efa_pages_free: null argument"); return 2; }
+    return pages_free(*pool, seqs, n, (cudaStream_t)stream);
+}
+
+extern "C" int efa_pages_compact(const efa_page_pool* pool, const efa_paged_cache* cache, int* pages_out, int* refs_out, int* moved,
+                                 void* workspace, size_t workspace_bytes, void* stream)
+{
+    if (!pool || !cache) { set_error("efa_pages_compact: null argument"); return 2; }
+    return pages_compact(*pool, *cache, pages_out, refs_out, moved, workspace, workspace_bytes, (cudaStream_t)stream);
+}
+
+extern "C" int efa_pages_copy(const efa_paged_cache* cache, const int* src, const int* dst, int n, void* stream)
+{
+    if (!cache) { set_error("efa_pages_copy: null argument"); return 2; }
+    return pages_copy(*cache, src, dst, n, (cudaStream_t)stream);
+}
+
+extern "C" const char* efa_block_norm_check(const efa_block_norm_params* p, int rows)
+{
+    if (!p) return "null argument";
+    return block_norm_check(*p, rows);
+}
+
+extern "C" int efa_block_norm(const void* x, const void* y, const void* gate, const void* post_w, const void* post_b, const void* pre_w, const void* pre_b,
+                              void* x_out, void* h, int rows, const efa_block_norm_params* p, void* stream)
+{
+    if (!p) { set_error("efa_block_norm: null argument"); return 2; }
+    return block_norm(x, y, gate, post_w, post_b, pre_w, pre_b, x_out, h, rows, *p, (cudaStream_t)stream);
+}
+
+extern "C" const char* efa_w4_check(const efa_w4* w)
+{
+    if (!w) return "null argument";
+    return w4_check(*w);
+}
+
+extern "C" int efa_project_w4(const void* X, int64_t x_stride, const efa_w4* w, void* out, int out_dtype, int64_t out_stride, int rows, void* stream)
+{
+    if (!w) { set_error("efa_project_w4: null argument"); return 2; }
+    return project_w4(X, x_stride, *w, out, out_dtype, out_stride, rows, (cudaStream_t)stream);
 }
 
 extern "C" int efa_kernel_status(int* out4)

@@ -167,6 +167,23 @@ bool own_device_memory(const void* p)
     return attr.type == cudaMemoryTypeDevice && attr.device == dev;
 }
 
+int check_memory(const char* what, const void* const* p, int n)
+{
+    int dev = -1;
+    EFA_CUDA(cudaGetDevice(&dev));
+    for (int i = 0; i < n; i++) {
+        if (!p[i]) continue;
+        cudaPointerAttributes attr;
+        EFA_CUDA(cudaPointerGetAttributes(&attr, p[i]));
+        if (attr.type == cudaMemoryTypeUnregistered || attr.type == cudaMemoryTypeHost) { set_error("%s: argument %d is memory of the host", what, i); return 2; }
+        if (attr.type == cudaMemoryTypeDevice && attr.device != dev) {
+            set_error("%s: argument %d is memory of device %d, the current device is %d", what, i, attr.device, dev);
+            return 2;
+        }
+    }
+    return 0;
+}
+
 static int make_tmap(CUtensorMap* out, CUtensorMapDataType type, unsigned elem_bytes, const void* base, int rank,
                      const unsigned long long* dims, const unsigned long long* strides_bytes, const unsigned* box)
 {

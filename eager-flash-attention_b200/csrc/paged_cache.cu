@@ -210,27 +210,6 @@ PagedArgs device_args(const efa_paged_cache& c, const efa_paged_batch& b)
     return a;
 }
 
-// Memory that the kernels may use: a call on another device's tensors, or the host's, is refused here and not found out by the GPU. One pointer
-// of each group that belongs together: 0.08 us each, of 4 us that a call takes on the host.
-int check_memory(const char* what, const void* const* p, int n)
-{
-    int dev = -1;
-    EFA_CUDA(cudaGetDevice(&dev));
-    for (int i = 0; i < n; i++) {
-        if (!p[i]) continue;
-        cudaPointerAttributes attr;
-        EFA_CUDA(cudaPointerGetAttributes(&attr, p[i]));
-        if (attr.type == cudaMemoryTypeUnregistered || attr.type == cudaMemoryTypeHost) { set_error("%s: argument %d is memory of the host", what, i); return 2; }
-        if (attr.type == cudaMemoryTypeDevice && attr.device != dev) {
-            set_error("%s: argument %d is memory of device %d, the current device is %d", what, i, attr.device, dev);
-            return 2;
-        }
-    }
-    return 0;
-}
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-
 const char* check_rows(const efa_paged_cache& c, const efa_paged_batch& b, long long& head, long long& token)
 {
     if (head == 0 && token == 0) { token = c.d_h; head = (long long)b.tokens * c.d_h; return nullptr; }

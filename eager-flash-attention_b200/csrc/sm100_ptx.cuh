@@ -21,6 +21,8 @@ enum KernelStatus : int {
     KS_WAIT_TIMEOUT = 1,
     KS_BAD_PAGE = 2,          // a page table entry outside the pool; spare words: sequence, site
     KS_BAD_LENGTH = 3,        // lengths of a batch outside its buffers or bounds
+    KS_NO_PAGE = 4,           // a pool without a free page
+    KS_BAD_SLOT = 5,          // a sequence that a call may not name
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p)

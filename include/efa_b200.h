@@ -221,9 +221,105 @@ size_t efa_paged_attention_workspace(const efa_paged_cache* cache, const efa_pag
 int efa_paged_attention(const void* Q, void* O, const efa_paged_cache* cache, const efa_paged_batch* batch,
                         const efa_paged_attention_params* p, void* workspace, size_t workspace_bytes, void* stream);
 
+/* Pages of a cache handed out, shared and taken back on the device, without the host knowing the lengths (no counterpart in the reference, which has no
+ * cache). pages and kv_len are the arrays that an efa_paged_batch points to, over all num_seqs slots a server has; a slot without keys is an empty sequence.
+ * refs[p]: how many entries of sequences name page p; 0 = free. All zeros is an empty pool; refs may be raised by the caller to keep pages (a shared
+ * prefix), and lowered again. Entries behind a sequence's last page are neither read nor written.
+ * A page that is not full belongs to one sequence: efa_pages_fork copies it, full pages are shared. So efa_cache_write always writes into pages of one sequence.
+ * Calls change the arrays in stream order; a captured graph follows their contents. What is found wrong is reported by efa_kernel_status (site 60
+ * take, 61 fork, 62 free, 63 compact, 64 copy; sequence or page in place of the block) and the call stays inside its buffers: code 2 a page outside the
+ * pool (the entry counts as no page), 3 a length outside the table, 4 no free page (the entry becomes -1, whose keys efa_cache_write does not
+ * write and attention reads as zeros), 5 a sequence that may not be named (outside the pool of slots, or a child that is not empty or named twice). */
+typedef struct efa_page_pool {
+    int* refs;              /* [num_pages] */
+    int* pages;             /* [num_seqs][max_pages] */
+    int* kv_len;            /* [num_seqs] */
+    int  num_pages, page_size, num_seqs, max_pages;
+} efa_page_pool;
+
+/* NULL when calls on this pool are legal, else a static description. */
+const char* efa_page_pool_check(const efa_page_pool* pool);
+
+/* Bytes of workspace that efa_pages_take, efa_pages_fork and efa_pages_compact need (16-byte aligned device memory that no other call uses until this one is done). */
+size_t efa_pages_workspace(const efa_page_pool* pool);
+
+/* kv_len[b] += q_start[b + 1] - q_start[b] for every slot, with pages for the new keys: the lowest free ones, slots in order. The arrays are then those of
+ * the step's efa_paged_batch. Where there are no free pages left the entries become -1; lengths end where the table does. */
+int efa_pages_take(const efa_page_pool* pool, const int* q_start, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Slots children[i] (empty, each named once) become copies of slots parents[i] as they were before the call, for i in [0, n): full pages are shared, the keys of a
+ * partly filled last page are copied into the lowest free pages, children in order (the rest of such a page stays as it was). Slots that are
+ * named wrongly are left as they were. */
+int efa_pages_fork(const efa_page_pool* pool, const efa_paged_cache* cache, const int* parents, const int* children, int n,
+                   void* workspace, size_t workspace_bytes, void* stream);
+
+/* Slots seqs[i] become empty, for i in [0, n); their pages are free when no other sequence has them. A slot may be named more than once. */
+int efa_pages_free(const efa_page_pool* pool, const int* seqs, int n, void* stream);
+
+/* The pool's L pages in use become pages 0 to L - 1: the k-th page in use at or behind L moves to the k-th free page before L, with its keys. pages_out
+ * and refs_out (the pool's own arrays, or others that do not overlap them) become the table and counts of the pool after that; entries behind a sequence's last page
+ * are not written. moved [num_pages]: the new place of each page, -1 of free ones; for tables that the caller keeps. Pages at or behind L keep their contents, so that
+ * with other arrays for the output the old table stays good until a page is taken. */
+int efa_pages_compact(const efa_page_pool* pool, const efa_paged_cache* cache, int* pages_out, int* refs_out, int* moved,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
+/* Pages src[i] of the cache to pages dst[i], keys, values and exponents, for i in [0, n). No page of dst is named twice or by src. */
+int efa_pages_copy(const efa_paged_cache* cache, const int* src, const int* dst, int n, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Around the block: norms, projections with 4-bit weights
+ * ------------------------------------------------------------------------------------------ */
+
+/* The norms after and before a block with its gate and residual addition, in one pass (the reference stops at the AllReduce output buffer; efa_run_mode_residual
+ * is the addition alone). Per row, in fp32:
+ *     n = post ? norm(y) * post_w + post_b : y
+ *     r = residual_scale * x + block_scale * act(gate) * n
+ *     x_out = r,    h = pre ? norm(r) * pre_w + pre_b : not written
+ * norm(v) = v / sqrt(mean(v^2) + eps) (EFA_NORM_RMS) or (v - mean(v)) / sqrt(mean((v - mean(v))^2) + eps) (EFA_NORM_LAYER); act: the identity or the sigmoid. The
+ * second norm takes r before it is rounded. */
+enum { EFA_NORM_RMS = 0, EFA_NORM_LAYER = 1 };
+enum { EFA_GATE_NONE = 0, EFA_GATE_PLAIN = 1, EFA_GATE_SIGMOID = 2 };
+typedef struct efa_block_norm_params {
+    int     d;                  /* elements of a row, 1 to 32768 */
+    int     kind, post, pre, gate;
+    int     gate_rows;          /* 0: one gate [d] for all rows; 1: [rows][d] */
+    float   eps, residual_scale, block_scale;
+    int     x_dtype, y_dtype;   /* EFA_F16 or EFA_F32: x and x_out; y. gate, weights and h are fp16 */
+    int64_t x_stride, y_stride, out_stride, h_stride, gate_stride;   /* elements from a row to the next, 0 = dense */
+} efa_block_norm_params;
+
+const char* efa_block_norm_check(const efa_block_norm_params* p, int rows);
+
+/* y NULL: no block output (r = residual_scale * x: the norm before the first block; then neither post nor gate). x NULL: no residual. x_out or h NULL: not
+ * wanted (not both). post_w, post_b, pre_w, pre_b: fp16 [d], NULL: ones and zeros. x_out and h may be x or y themselves where type and stride are the same.
+ * Any alignment; rows, strides and d that are multiples of 8 with 16-byte aligned tensors go faster. Asynchronous on `stream`. */
+int efa_block_norm(const void* x, const void* y, const void* gate, const void* post_w, const void* post_b, const void* pre_w, const void* pre_b,
+                   void* x_out, void* h, int rows, const efa_block_norm_params* p, void* stream);
+
+/* A projection's weights in 4 bits: w[k][n] = scales[k / group][n] * (code(n, k) - zeros[k / group][n]); zeros NULL: 8. codes [d_out][d_in / 2], two to a byte, the
+ * even k in the low half; scales fp16, zeros bytes [d_in / group][d_out]. group 32, 64 or 128, d_in a multiple of it. Strides: bytes from a row of codes to the
+ * next (a multiple of 16), elements of scales and of zeros; 0 = dense. A shard of rows (d_in) or columns (d_out) of a larger matrix is that matrix with other
+ * pointers and its strides. codes is 16-byte aligned. */
+typedef struct efa_w4 {
+    const uint8_t* codes;
+    const void*    scales;
+    const uint8_t* zeros;
+    int            d_in, d_out, group;
+    int64_t        code_stride, scale_stride, zero_stride;
+} efa_w4;
+
+const char* efa_w4_check(const efa_w4* w);
+
+/* out[rows][d_out] = X[rows][d_in] * w: efa_project_f16 for few rows, where reading the weights is all the time (the reference's project, attn_main.cu:262-273, is
+ * fp32 throughout). X fp16, 16-byte aligned, x_stride (elements, 0 = dense) a multiple of 8; out fp16 (EFA_F16) or fp32 (EFA_F32), out_stride elements. Codes
+ * minus zeros are fp16 numbers exactly; products and sums are fp32, the scales are applied to the sums of their groups: nothing is rounded but the result. Made
+ * for up to 64 rows; more go in tiles of 64 that read the weights again. The order of the sum depends on the sizes only. Asynchronous on `stream`. */
+int efa_project_w4(const void* X, int64_t x_stride, const efa_w4* w, void* out, int out_dtype, int64_t out_stride, int rows, void* stream);
+
 /* Status word written by kernels whose bounded waits ran out, or that found lengths or pages of a paged batch wrong: out4 = {code, block, site, 0};
  * code 0 = no kernel reported a problem since the last efa_kernel_status_reset(), 1 = a wait ran out, 2 = a page outside the pool, 3 = a
- * length outside its bounds (2, 3: the sequence in place of the block; site 50 = write or read, 51 to 54 = attention). */
+ * length outside its bounds, 4 = no free page, 5 = a slot that may not be named (2 to 5: the sequence in place of the block; site 50 = write or read,
+ * 51 to 54 = attention, 60 to 64 = pages). */
 int efa_kernel_status(int* out4);
 int efa_kernel_status_reset(void);
 

@@ -1,0 +1,133 @@
+"""Projections with weights of 4 bits against the definition in 64 bits.
+
+Tolerance, with S = sum over the groups of scale * sum |x (code - zero)|: a product is exact (11 bits times at most 9); a group's sum of G products in fp32, where the
+tensor cores may cut instead of rounding, is off by (G + 4) 2^-23 of its magnitudes, adding the scaled groups, warps and blocks by 2^-24 each: groups + 70 of
+them at most; then the result is rounded, 2^-11 (2^-25 at the bottom) of fp16, 2^-24 of fp32."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def make(rows, d_in, d_out, group, zeros, seed, top_zero=16):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    codes = torch.randint(0, 256, (d_out, d_in // 2), generator=gen, device="cuda", dtype=torch.uint8)
+    scales = ((0.5 + torch.rand(d_in // group, d_out, generator=gen, device="cuda")) * d_in ** -0.5 / 4).half()
+    z = torch.randint(0, top_zero, (d_in // group, d_out), generator=gen, device="cuda", dtype=torch.uint8) if zeros else None
+    return torch.randn(rows, d_in, generator=gen, device="cuda").half(), codes, scales, z
+
+
+def reference(X, codes, scales, zeros, out_dtype):
+    group = 2 * codes.shape[1] // scales.shape[0]
+    q = torch.stack([codes & 15, codes >> 4], -1).reshape(codes.shape[0], -1, group).double()
+    w = q - (8 if zeros is None else zeros.t().double().unsqueeze(-1))
+    s = scales.t().double().unsqueeze(-1)
+    W = (w * s).reshape(codes.shape[0], -1)
+    ref, size = X.double() @ W.t(), X.double().abs() @ W.abs().t()
+    tol = ((group + 4) * 2.0 ** -23 + (scales.shape[0] + 70) * 2.0 ** -24) * size
+    return ref, tol + (2.0 ** -11 * ref.abs() + 2.0 ** -25 if out_dtype == torch.float16 else 2.0 ** -24 * ref.abs())
+
+
+def check(got, ref, tol):
+    assert torch.isfinite(got).all()
+    worst = ((got.double() - ref).abs() / tol).max().item()
+    assert worst <= 1, f"{worst:.2f} times the tolerance"
+
+
+def project(pkg, X, codes, scales, zeros, out_dtype=torch.float16):
+    out = torch.full((X.shape[0], codes.shape[0]), 777.0, dtype=out_dtype, device="cuda")
+    pkg.project_w4(X, pkg.w4_weight(codes, scales, zeros), out, X.shape[0])
+    torch.cuda.synchronize()
+    return out
+
+
+@pytest.mark.parametrize("rows", [1, 2, 5, 8, 9, 16, 17, 24, 31, 32, 33, 48, 63, 64, 65, 130])
+@pytest.mark.parametrize("group,zeros", [(32, True), (64, False), (128, True)])
+def test_rows(pkg, torch_cuda, rows, group, zeros):
+    a = make(rows, 1152, 200, group, zeros, rows)
+    check(project(pkg, *a), *reference(*a, torch.float16))
+
+
+# Lengths of the sum: one group, not a multiple of 128, fewer units than warps, many; widths: one channel, odd ones, below and above a tile.
+@pytest.mark.parametrize("d_in,d_out,group", [(32, 1, 32), (32, 8, 32), (64, 33, 64), (96, 7, 32), (128, 64, 128), (160, 31, 32), (192, 65, 64), (224, 129, 32), (384, 16, 128), (1056, 100, 32),
+                                              (1088, 257, 64), (4096, 1003, 128), (4096, 4096, 64), (16384, 40, 128), (16384, 1, 64), (8192, 2500, 32)])
+@pytest.mark.parametrize("rows", [1, 7, 13, 64])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_sizes(pkg, torch_cuda, d_in, d_out, group, rows, zeros):
+    for dtype in (torch.float16, torch.float32):
+        a = make(rows, d_in, d_out, group, zeros, d_in + d_out)
+        check(project(pkg, *a, dtype), *reference(*a, dtype))
+
+
+def test_every_code_and_zero(pkg, torch_cuda):
+    """X picks one k at a time: the values of all codes under all zero points, exactly."""
+    for group in (32, 64, 128):
+        d_in, d_out = 2 * group, 256
+        codes = torch.randint(0, 256, (d_out, d_in // 2), device="cuda", dtype=torch.uint8)
+        zeros = torch.arange(256, device="cuda", dtype=torch.uint8).repeat(2, 1)             # more than four bits are taken as they are
+        scales = torch.ones(2, d_out, dtype=torch.float16, device="cuda")
+        q = torch.stack([codes & 15, codes >> 4], -1).reshape(d_out, d_in).float()
+        for k in range(0, d_in, 64):
+            X = torch.eye(d_in, dtype=torch.float16, device="cuda")[k:k + 64].contiguous()
+            assert torch.equal(project(pkg, X, codes, scales, zeros, torch.float32), (q - zeros[0, :, None].float()).t()[k:k + 64])
+            assert torch.equal(project(pkg, X, codes, scales, None, torch.float32), (q - 8).t()[k:k + 64])
+
+
+def test_shards_of_a_larger_matrix(pkg, torch_cuda):
+    """Rows and columns of a matrix as they lie in it; strides of X and out; what lies around out stays."""
+    X, codes, scales, zeros = make(11, 512, 96, 64, True, 5)
+    for k0, k1, n0, n1 in ((0, 256, 0, 96), (128, 512, 16, 80), (64, 128, 3, 4), (384, 512, 95, 96)):
+        part = (codes[n0:n1, k0 // 2:k1 // 2], scales[k0 // 64:k1 // 64, n0:n1], zeros[k0 // 64:k1 // 64, n0:n1])
+        store = torch.full((13, 100), 777.0, dtype=torch.float32, device="cuda")
+        pkg.project_w4(X[:, k0:k1], pkg.w4_weight(*part), store[1:12, 2:], 11, x_stride=512, out_stride=100)
+        check(store[1:12, 2:2 + n1 - n0].clone(), *reference(X[:, k0:k1], *(p.contiguous() for p in part), torch.float32))
+        store[1:12, 2:2 + n1 - n0] = 777
+        assert torch.all(store == 777)
+
+
+@pytest.mark.parametrize("rows", [1, 16, 64])
+def test_a_row_has_no_part_in_others(pkg, torch_cuda, rows):
+    X, codes, scales, zeros = make(rows, 1024, 300, 128, True, 6)
+    clean = project(pkg, X, codes, scales, zeros)
+    X[rows - 1, 5] = float("nan")
+    got = project(pkg, X, codes, scales, zeros)
+    assert torch.isnan(got[-1]).all() and torch.equal(got[:-1], clean[:-1])
+    X[rows - 1, 5] = float("inf")
+    got = project(pkg, X, codes, scales, None)
+    assert not torch.isfinite(got[-1]).any() and torch.isfinite(got[:-1]).all()
+
+
+def test_large_results_become_infinite_and_small_ones_are_kept(pkg, torch_cuda):
+    X = torch.full((2, 128), 60000.0, dtype=torch.float16, device="cuda")
+    codes = torch.full((8, 64), 0xFF, dtype=torch.uint8, device="cuda")
+    scales = torch.ones(1, 8, dtype=torch.float16, device="cuda")
+    assert torch.all(project(pkg, X, codes, scales, None) == float("inf"))
+    assert torch.all(project(pkg, X, codes, scales, None, torch.float32) == 60000 * 7 * 128)
+    X.fill_(2.0 ** -24), scales.fill_(2.0 ** -24)
+    assert torch.all(project(pkg, X, codes, scales, None, torch.float32) == 7 * 128 * 2.0 ** -48)
+
+
+def test_equal_calls_give_equal_bits_and_go_where_they_are_sent(pkg, torch_cuda):
+    a = make(16, 4096, 1000, 64, True, 7)
+    want = project(pkg, *a)
+    w, out = pkg.w4_weight(*a[1:]), torch.zeros_like(want)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            pkg.project_w4(a[0], w, out, 16, stream=side)
+    for _ in range(5):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+    with pytest.raises(pkg.EfaError, match="memory of the host"):
+        pkg.project_w4(a[0].cpu(), w, out, 16)
+
+
+def test_no_rows(pkg, torch_cuda):
+    X, codes, scales, zeros = make(1, 128, 8, 128, False, 8)
+    out = torch.full((1, 8), 777.0, dtype=torch.float16, device="cuda")
+    pkg.project_w4(X, pkg.w4_weight(codes, scales), out, 0)
+    torch.cuda.synchronize()
+    assert torch.all(out == 777)
