@@ -219,6 +219,12 @@ int make_tmap_f16(CUtensorMap* out, const void* base, int rank, const unsigned l
     return make_tmap(out, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2u, base, rank, dims, strides_bytes, box);
 }
 
+int make_tmap_u8(CUtensorMap* out, const void* base, int rank, const unsigned long long* dims,
+                 const unsigned long long* strides_bytes, const unsigned* box)
+{
+    return make_tmap(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1u, base, rank, dims, strides_bytes, box);
+}
+
 int make_tmap_f32(CUtensorMap* out, const void* base, int rank, const unsigned long long* dims,
                   const unsigned long long* strides_bytes, const unsigned* box)
 {

@@ -127,6 +127,9 @@ cudaError_t launch_value(void (*kernel)(P...), dim3 grid, unsigned threads, size
 int make_tmap_f16(CUtensorMap* out, const void* base, int rank,
                   const unsigned long long* dims, const unsigned long long* strides_bytes /* rank-1 */,
                   const unsigned* box);
+// The same over bytes.
+int make_tmap_u8(CUtensorMap* out, const void* base, int rank, const unsigned long long* dims,
+                 const unsigned long long* strides_bytes, const unsigned* box);
 // The same over fp32 data.
 int make_tmap_f32(CUtensorMap* out, const void* base, int rank, const unsigned long long* dims,
                   const unsigned long long* strides_bytes, const unsigned* box);

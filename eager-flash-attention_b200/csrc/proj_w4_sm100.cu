@@ -6,35 +6,24 @@
 // lie: a lane's four bytes are eight neighbouring k of one channel, `(word >> 4 i) & 0x000f000f` is the pair (k + i, k + i + 4) of two products' fragments, and x is
 // paired alike. A code c becomes the fp16 number 1024 + c (or 1024 + 16 c, times 1/16) by one logical operation, and c - zero exactly by one more. All
 // four lanes that share a channel must be in one group: 16, 8 or 4 bytes to a lane and load for groups of 128, 64 or 32.
-#include "host_util.h"
+#include "proj_w4.cuh"
 #include "serving.h"
-#include "sm100_ptx.cuh"
 
 #include <algorithm>
-#include <climits>
 
 namespace efa {
 
 namespace {
 
-constexpr int W4_UNIT = 128;            // k that a warp takes at a time
-constexpr int W4_ROWS = 64;             // rows of a tile
+// Eight warps, and two blocks to an SM: four warps to a scheduler hide one another's waits. Of up to three stages as many as leave room for the second block.
+constexpr int W4_WARPS = 8, W4_BLOCKS = 2, W4_STAGES = 3, W4_SMEM = 113 * 1024;
+constexpr int W4_MT = 2;                // tiles of 16 channels to a warp
 
-struct W4Args {
-    const uint8_t* codes;
-    const __half* scales;
-    const uint8_t* zeros;
-    const __half* X;
-    void* out;
-    int rows, d_in, d_out;
-    long long code_stride, scale_stride, zero_stride, x_stride, out_stride;
-    bool out_f32;
-};
-
-__device__ __forceinline__ uint32_t lop_and_or(uint32_t a, uint32_t mask, uint32_t with)
+// (a & mask) | with
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t mask, uint32_t with)
 {
     uint32_t r;
-    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(a), "r"(mask), "r"(with));     // (a & mask) | with
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(a), "r"(mask), "r"(with));
     return r;
 }
 __device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b)
@@ -50,100 +39,190 @@ __device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c)
     return r;
 }
 
-// Eight codes to four pairs (i, i + 4) of numbers code - zero. low: 1024 + zero twice; high: -(64 + zero) twice.
+// Eight codes to four pairs (i, i + 4) of numbers code - zero, exactly. low: 1024 + zero twice; high: -(64 + zero) twice.
 __device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t low, uint32_t high, uint32_t (&f)[4])
 {
-    constexpr uint32_t MAGIC = 0x64006400u, SIXTEENTH = 0x2c002c00u;
+    constexpr uint32_t MAGIC = 0x64006400u, SIXTEENTH = 0x2c002c00u;            // 1024, 1/16
     const uint32_t v = w >> 8;
-    f[0] = sub2(lop_and_or(w, 0x000f000fu, MAGIC), low);
-    f[1] = fma2(lop_and_or(w, 0x00f000f0u, MAGIC), SIXTEENTH, high);
-    f[2] = sub2(lop_and_or(v, 0x000f000fu, MAGIC), low);
-    f[3] = fma2(lop_and_or(v, 0x00f000f0u, MAGIC), SIXTEENTH, high);
+    f[0] = sub2(and_or(w, 0x000f000fu, MAGIC), low);
+    f[1] = fma2(and_or(w, 0x00f000f0u, MAGIC), SIXTEENTH, high);
+    f[2] = sub2(and_or(v, 0x000f000fu, MAGIC), low);
+    f[3] = fma2(and_or(v, 0x00f000f0u, MAGIC), SIXTEENTH, high);
 }
 
-__device__ __forceinline__ void mma_w4(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
+// c += A B, or (first) c = A B.
+__device__ __forceinline__ void mma_w4(float (&c)[4], bool first, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
 {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    if (first)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// A block: 16 MT channels, 8 NT rows, all k, its warps (and the blocks of its cluster, along z) taking units of 128 k in turn, added at the end in shared memory in the
-// order of the warps and blocks.
+template <int N> __device__ __forceinline__ void load_shared(uint32_t addr, uint32_t (&w)[N])
+{
+    if constexpr (N == 4) asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr) : "memory");
+    else if constexpr (N == 2) asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr) : "memory");
+    else asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[0]) : "r"(addr) : "memory");
+}
+
+// What a warp keeps in shared memory: stages of codes (128 bytes of each of 16 MT channels), of X (512 bytes of each row), and two units of scales.
+constexpr int W4_K = 256;               // k of a unit
 template <int G, int MT, int NT>
-__global__ void __launch_bounds__(256)
-proj_w4_kernel(const W4Args a)
+struct W4Cfg {
+    static constexpr int CHANNELS = 16 * MT, SUBS = W4_K / G;
+    static constexpr int CODE_BYTES = CHANNELS * 128, TABLE = SUBS * CHANNELS * (int)sizeof(float2), TILE = CHANNELS * 8 * NT;
+    static int smem(int rows, int stages) { return 1024 + W4_WARPS * std::max(stages * (CODE_BYTES + rows * 512) + 2 * TABLE, TILE * (int)sizeof(float)); }
+    static_assert(CODE_BYTES % 1024 == 0, "");
+};
+
+// Which channel of eight a lane's fragments hold, so that the lanes that read codes together find different banks: 16-byte chunk c of a row's eight lies at
+// c ^ (row % 8) (the 128-byte swizzle of the copy). Of X, chunk c of a row's sixteen to 128 k at x_place.
+template <int G> __device__ __forceinline__ int channel_of(int g) { return G == 128 ? g >> 1 | (g & 1) << 2 : G == 64 ? (g & 3) * 2 + (g >> 2) : g; }
+template <int G> __device__ __forceinline__ int x_place(int row, int c)
 {
-    constexpr int SUBS = W4_UNIT / G, WORDS = G / 32;          // groups of a unit, words of codes of a lane and group
-    extern __shared__ float sum[];                             // [warp][8 NT][16 MT]
+    return G == 128 ? c ^ (c >> 3 & 1) ^ (row & 1) << 1 : G == 64 ? c ^ (row & 1) : c ^ (row & 1) << 2;
+}
+
+// A block: 16 MT channels, 8 NT rows, all k, its warps (and the blocks of its cluster, along z) taking the units of 256 k in turn, added at the end in shared
+// memory in the order of the warps and blocks. A warp has its own units copied ahead, codes by TMA, X by its lanes: nobody waits for anybody before the sums.
+template <int G, int MT, int NT>
+__global__ void __launch_bounds__(32 * W4_WARPS, W4_BLOCKS)
+proj_w4_kernel(const W4Args a, int stages, const __grid_constant__ CUtensorMap codes_map)
+{
+    using C = W4Cfg<G, MT, NT>;
+    constexpr int SUBS = C::SUBS, WORDS = G / 32;              // groups of a unit, words of codes of a lane and group
+    constexpr int CHANNELS = C::CHANNELS, PER_LANE = (CHANNELS + 31) / 32;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint64_t bars[W4_WARPS][W4_STAGES];
+    __shared__ int abort_word;
+    constexpr int warps = W4_WARPS;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int n0 = blockIdx.x * CHANNELS, m0 = blockIdx.y * 8 * NT, rows = min(a.rows - m0, 8 * NT);
+    const int parts = gridDim.z, part = parts > 1 ? (int)cluster_rank() : 0;
+    const int units = (a.d_in + W4_K - 1) / W4_K;
+    // Warps take the units of a block in turn, so that what they read at a time is neighbours in the rows of codes.
+    const int step = warps, u0 = (int)((long long)units * part / parts) + warp, u1 = (int)((long long)units * (part + 1) / parts);
+
+    uint8_t* const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    // Codes of all warps first, then X, then the tables.
+    uint8_t* const slots = smem + warp * (stages * C::CODE_BYTES);
+    const uint32_t x_slots = smem_u32(smem) + warps * (stages * C::CODE_BYTES) + warp * (stages * rows * 512);
+    uint2* const table = reinterpret_cast<uint2*>(smem + warps * stages * (C::CODE_BYTES + rows * 512) + warp * 2 * C::TABLE);
+    uint64_t* const bar = bars[warp];
+    if (lane == 0) {
+        for (int i = 0; i < stages; i++) mbar_init(&bar[i], 33);               // the copy of codes, and what each lane copies of X
+        mbar_fence_init();
+        tma_prefetch_desc(&codes_map);
+    }
+    if (threadIdx.x == 0) abort_word = 0;
+    __syncthreads();
     pdl_wait();
     pdl_trigger();
-    const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int n0 = blockIdx.x * 16 * MT, m0 = blockIdx.y * W4_ROWS;
-    const int parts = gridDim.z, part = parts > 1 ? (int)cluster_rank() : 0;
-    const int units = (a.d_in + W4_UNIT - 1) / W4_UNIT;
-    const long long shares = (long long)warps * parts, share = (long long)part * warps + warp;
-    const int u0 = (int)(units * share / shares), u1 = (int)(units * (share + 1) / shares);
 
-    const uint8_t* row[MT][2];
-    int channel[MT][2];
-    #pragma unroll
-    for (int m = 0; m < MT; m++)
-        #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            channel[m][h] = min(n0 + 16 * m + 8 * h + g, a.d_out - 1);
-            row[m][h] = a.codes + channel[m][h] * a.code_stride + t * (G / 8);
+    auto fetch = [&](int u, int slot) {
+        if (lane == 0) {
+            mbar_expect_tx(&bar[slot], C::CODE_BYTES);
+            tma_load_2d(slots + slot * C::CODE_BYTES, &codes_map, &bar[slot], u * (W4_K / 2), n0);
         }
-    const __half* x[NT];
+        if (u * W4_K + 8 * lane < a.d_in)
+            for (int r = 0; r < rows; r++)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
+                             :: "r"(x_slots + (slot * rows + r) * 512 + ((lane & 16) | x_place<G>(r, lane & 15)) * 16), "l"(a.X + (m0 + r) * a.x_stride + u * W4_K + 8 * lane) : "memory");
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" :: "r"(smem_u32(&bar[slot])) : "memory");
+    };
+    for (int i = 0; i < stages && u0 + i * step < u1; i++) fetch(u0 + i * step, i);
+    // Scales and zeros of a unit's channels: to registers a unit ahead, and from there as scale and 1024 + zero (twice, fp16) to the table.
+    const __half* s_at[PER_LANE];
+    const uint8_t* z_at[PER_LANE];
     #pragma unroll
-    for (int n = 0; n < NT; n++) x[n] = m0 + 8 * n + g < a.rows ? a.X + (long long)(m0 + 8 * n + g) * a.x_stride + t * (G / 4) : nullptr;
-
+    for (int i = 0; i < PER_LANE; i++) {
+        const int n = min(n0 + lane + 32 * i, a.d_out - 1);
+        s_at[i] = a.scales + (long long)u0 * SUBS * a.scale_stride + n;
+        z_at[i] = a.zeros + (long long)u0 * SUBS * a.zero_stride + n;
+    }
+    const int groups = a.d_in / G;
+    __half s_next[SUBS][PER_LANE];
+    uint8_t z_next[SUBS][PER_LANE];
+    auto ask = [&](int u) {
+        #pragma unroll
+        for (int s = 0; s < SUBS; s++)
+            if (u * SUBS + s < groups) {
+                #pragma unroll
+                for (int i = 0; i < PER_LANE; i++) {
+                    s_next[s][i] = s_at[i][s * a.scale_stride];
+                    if (a.zeros) z_next[s][i] = z_at[i][s * a.zero_stride];
+                }
+            }
+        #pragma unroll
+        for (int i = 0; i < PER_LANE; i++) {
+            s_at[i] += (long long)step * SUBS * a.scale_stride;
+            z_at[i] += (long long)step * SUBS * a.zero_stride;
+        }
+    };
+    auto tabulate = [&](uint2* to) {
+        #pragma unroll
+        for (int s = 0; s < SUBS; s++)
+            #pragma unroll
+            for (int i = 0; i < PER_LANE; i++)
+                if (CHANNELS >= 32 || lane < CHANNELS)
+                    to[s * CHANNELS + lane + 32 * i] = make_uint2(__float_as_uint(__half2float(s_next[s][i])), 0x64006400u + 0x00010001u * (a.zeros ? (uint32_t)z_next[s][i] : 8u));
+    };
+    if (u0 < u1) ask(u0);
+    const int row = channel_of<G>(g);
+    const uint32_t code_base = smem_u32(slots) + row * 128, x_base = x_slots + g * 512;
     float acc[MT][NT][4] = {};
-    for (int u = u0; u < u1; u++) {
+    int slot = 0;
+    uint32_t phase = 0;
+    for (int u = u0, odd = 0; u < u1; u += step, odd ^= 1) {
+        uint2* const scales = table + odd * (SUBS * CHANNELS);
+        tabulate(scales);
+        if (u + step < u1) ask(u + step);
+        if (!mbar_wait(&bar[slot], phase, &abort_word, 70)) break;
+        __syncwarp();
+        const uint32_t codes = code_base + slot * C::CODE_BYTES, x = x_base + slot * (rows * 512);
         #pragma unroll
         for (int s = 0; s < SUBS; s++) {
-            const int k = u * W4_UNIT + s * G;
-            if (k >= a.d_in) break;
-            const long long group = k / G;
+            if (u * W4_K + s * G >= a.d_in) break;
             uint32_t w[MT][2][WORDS];
-            float scale[MT][2];
-            uint32_t low[MT][2], high[MT][2];
+            const int at = s * (G / 2) + t * (G / 8);          // byte of the row's 128
+            const uint32_t code_at = ((at >> 4) ^ row) * 16 + (at & 15);
+            #pragma unroll
+            for (int m = 0; m < MT; m++)
+                #pragma unroll
+                for (int h = 0; h < 2; h++) load_shared(codes + code_at + (16 * m + 8 * h) * 128, w[m][h]);
+            uint2 scale[MT][2];
+            uint32_t high[MT][2];
             #pragma unroll
             for (int m = 0; m < MT; m++)
                 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    const uint8_t* p = row[m][h] + (k >> 1);
-                    if constexpr (WORDS == 4) {
-                        const uint4 q = *reinterpret_cast<const uint4*>(p);
-                        w[m][h][0] = q.x; w[m][h][1] = q.y; w[m][h][2] = q.z; w[m][h][3] = q.w;
-                    } else if constexpr (WORDS == 2) {
-                        const uint2 q = *reinterpret_cast<const uint2*>(p);
-                        w[m][h][0] = q.x; w[m][h][1] = q.y;
-                    } else w[m][h][0] = *reinterpret_cast<const uint32_t*>(p);
-                    scale[m][h] = __half2float(a.scales[group * a.scale_stride + channel[m][h]]);
-                    const uint32_t z = a.zeros ? a.zeros[group * a.zero_stride + channel[m][h]] : 8u;
-                    const uint32_t hl = __half_as_ushort(__uint2half_rn(1024u + z)), hh = __half_as_ushort(__int2half_rn(-(int)(64u + z)));
-                    low[m][h] = hl | hl << 16;
-                    high[m][h] = hh | hh << 16;
+                    scale[m][h] = scales[s * CHANNELS + 16 * m + 8 * h + row];
+                    high[m][h] = sub2(0x63806380u, scale[m][h].y);              // 960 - (1024 + zero)
                 }
-            float part_sum[MT][NT][4] = {};
+            float sum[MT][NT][4];
             #pragma unroll
             for (int i = 0; i < WORDS; i++) {
-                uint32_t f[MT][2][4];
-                #pragma unroll
-                for (int m = 0; m < MT; m++) {
-                    codes_to_f16(w[m][0][i], low[m][0], high[m][0], f[m][0]);
-                    codes_to_f16(w[m][1][i], low[m][1], high[m][1], f[m][1]);
-                }
+                uint32_t b[NT][4];
                 #pragma unroll
                 for (int n = 0; n < NT; n++) {
-                    uint4 q = make_uint4(0u, 0u, 0u, 0u);
-                    if (x[n]) q = *reinterpret_cast<const uint4*>(x[n] + k + 8 * i);
-                    const uint32_t b0 = __byte_perm(q.x, q.z, 0x5410), b1 = __byte_perm(q.x, q.z, 0x7632);
-                    const uint32_t b2 = __byte_perm(q.y, q.w, 0x5410), b3 = __byte_perm(q.y, q.w, 0x7632);
+                    uint32_t q[4] = {0u, 0u, 0u, 0u};
+                    const int c = s * (G / 8) + t * WORDS + i;     // 16-byte chunk of the row's 512
+                    if (8 * n + g < rows) load_shared(x + n * 4096 + ((c & 16) | x_place<G>(g, c & 15)) * 16, q);
+                    b[n][0] = __byte_perm(q[0], q[2], 0x5410); b[n][1] = __byte_perm(q[0], q[2], 0x7632);
+                    b[n][2] = __byte_perm(q[1], q[3], 0x5410); b[n][3] = __byte_perm(q[1], q[3], 0x7632);
+                }
+                #pragma unroll
+                for (int m = 0; m < MT; m++) {
+                    uint32_t p[4], q[4];
+                    codes_to_f16(w[m][0][i], scale[m][0].y, high[m][0], p);
+                    codes_to_f16(w[m][1][i], scale[m][1].y, high[m][1], q);
                     #pragma unroll
-                    for (int m = 0; m < MT; m++) {
-                        mma_w4(part_sum[m][n], f[m][0][0], f[m][1][0], f[m][0][1], f[m][1][1], b0, b1);
-                        mma_w4(part_sum[m][n], f[m][0][2], f[m][1][2], f[m][0][3], f[m][1][3], b2, b3);
+                    for (int n = 0; n < NT; n++) {
+                        mma_w4(sum[m][n], i == 0, p[0], q[0], p[1], q[1], b[n][0], b[n][1]);
+                        mma_w4(sum[m][n], false, p[2], q[2], p[3], q[3], b[n][2], b[n][3]);
                     }
                 }
             }
@@ -152,25 +231,41 @@ proj_w4_kernel(const W4Args a)
                 #pragma unroll
                 for (int n = 0; n < NT; n++)
                     #pragma unroll
-                    for (int i = 0; i < 4; i++) acc[m][n][i] = fmaf(scale[m][i >> 1], part_sum[m][n][i], acc[m][n][i]);
+                    for (int j = 0; j < 4; j++) acc[m][n][j] = fmaf(__uint_as_float(scale[m][j >> 1].x), sum[m][n][j], acc[m][n][j]);
         }
+        __syncwarp();
+        if (u + stages * step < u1) fetch(u + stages * step, slot);
+        if (++slot == stages) { slot = 0; phase ^= 1; }
     }
-    constexpr int TILE = 16 * MT * 8 * NT;
-    float* const mine = sum + warp * TILE;
+    // Sums of the warps, in the shared memory that they had for their copies: [warp][8 NT][16 MT].
+    constexpr int TILE = C::TILE;
+    float* const sum = reinterpret_cast<float*>(smem);
+    __syncthreads();
+    if (abort_word != 0) {                                     // copies in flight land first, then what the block has is written
+        for (int i = 0; i < 64; i++) __nanosleep(100000);
+        if (threadIdx.x == 0 && a.status != nullptr && atomicCAS(a.status, 0, (int)KS_WAIT_TIMEOUT) == 0) {
+            a.status[1] = blockIdx.x;
+            a.status[2] = abort_word;
+        }
+        __syncthreads();
+    }
     #pragma unroll
     for (int m = 0; m < MT; m++)
         #pragma unroll
         for (int n = 0; n < NT; n++)
             #pragma unroll
-            for (int i = 0; i < 4; i++) mine[(8 * n + 2 * t + (i & 1)) * (16 * MT) + 16 * m + 8 * (i >> 1) + g] = acc[m][n][i];
+            for (int i = 0; i < 4; i++) sum[warp * TILE + (8 * n + 2 * t + (i & 1)) * CHANNELS + 16 * m + 8 * (i >> 1) + row] = acc[m][n][i];
     __syncthreads();
-    for (int e = threadIdx.x; e < TILE; e += blockDim.x) {
-        float v = sum[e];
-        for (int w = 1; w < warps; w++) v += sum[w * TILE + e];
-        sum[e] = v;
+    const int wanted = rows * CHANNELS;
+    if (parts > 1) {
+        for (int e = threadIdx.x; e < wanted; e += blockDim.x) {
+            float v = sum[e];
+            for (int w = 1; w < warps; w++) v += sum[w * TILE + e];
+            sum[e] = v;
+        }
+        cluster_sync();
     }
-    if (parts > 1) cluster_sync(); else __syncthreads();
-    for (int e = part * (int)blockDim.x + threadIdx.x; e < TILE; e += parts * blockDim.x) {
+    for (int e = part * (int)blockDim.x + threadIdx.x; e < wanted; e += parts * blockDim.x) {
         float v = 0.f;
         if (parts > 1) {
             for (int q = 0; q < parts; q++) {
@@ -178,9 +273,11 @@ proj_w4_kernel(const W4Args a)
                 asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(y) : "r"(cluster_addr(sum + e, q)));
                 v += y;
             }
-        } else v = sum[e];
-        const int m = m0 + e / (16 * MT), n = n0 + e % (16 * MT);
-        if (m < a.rows && n < a.d_out) {
+        } else {
+            for (int w = 0; w < warps; w++) v += sum[w * TILE + e];
+        }
+        const int m = m0 + e / CHANNELS, n = n0 + e % CHANNELS;
+        if (n < a.d_out) {
             if (a.out_f32) static_cast<float*>(a.out)[m * a.out_stride + n] = v;
             else static_cast<__half*>(a.out)[m * a.out_stride + n] = __float2half_rn(v);
         }
@@ -188,29 +285,38 @@ proj_w4_kernel(const W4Args a)
     if (parts > 1) cluster_sync();                             // the others may still read this block's sums
 }
 
-template <int G, int MT, int NT>
+template <int G, int NT>
 int launch_w4(const W4Args& a, cudaStream_t stream)
 {
-    const int tiles = (a.d_out + 16 * MT - 1) / (16 * MT), units = (a.d_in + W4_UNIT - 1) / W4_UNIT;
-    const int warps = 8;
-    int cluster = 1;
-    while (cluster < 8 && cluster * 2 * warps <= units && (long long)tiles * cluster < 2 * device_sms()) cluster *= 2;
-    const dim3 grid(tiles, (a.rows + W4_ROWS - 1) / W4_ROWS, cluster);
-    const size_t smem = (size_t)warps * 16 * MT * 8 * NT * sizeof(float);
-    static bool set = false;
-    if (smem > 48 * 1024 && !set) { EFA_CUDA(cudaFuncSetAttribute(proj_w4_kernel<G, MT, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)); set = true; }
-    EFA_CUDA(launch_value(proj_w4_kernel<G, MT, NT>, grid, warps * 32, smem, stream, a));
+    using C = W4Cfg<G, W4_MT, NT>;
+    constexpr auto kernel = proj_w4_kernel<G, W4_MT, NT>;
+    const int tiles = (a.d_out + C::CHANNELS - 1) / C::CHANNELS, row_tiles = (a.rows + 8 * NT - 1) / (8 * NT), units = (a.d_in + W4_K - 1) / W4_K;
+    // Few tiles: a cluster shares k, as long as every warp has a unit and every block an SM. us in 1 / 2 / 4 parts: 16 rows, 8192 x 1024 10.0 / 7.0 / 5.6,
+    // 4096 x 4096 (one part) 6.8 / 7.2.
+    int parts = 1;
+    while (parts < 8 && 2 * parts * W4_WARPS <= units && (long long)tiles * row_tiles * 2 * parts <= device_sms()) parts *= 2;
+    CUtensorMap codes;
+    const unsigned long long dims[2] = {(unsigned long long)a.d_in / 2, (unsigned long long)a.d_out}, strides[1] = {(unsigned long long)a.code_stride};
+    const unsigned box[2] = {W4_K / 2, C::CHANNELS};
+    if (make_tmap_u8(&codes, a.codes, 2, dims, strides, box)) return 1;
+    const int rows = std::min(a.rows, 8 * NT);
+    int stages = W4_STAGES;
+    while (stages > 1 && C::smem(rows, stages) > W4_SMEM) stages--;
+    static bool set[64] = {};
+    int dev = 0;
+    EFA_CUDA(cudaGetDevice(&dev));
+    if (dev >= 64 || !set[dev]) {
+        EFA_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, std::max(W4_SMEM, C::smem(8 * NT, 1))));
+        if (dev < 64) set[dev] = true;
+    }
+    EFA_CUDA(launch_value(kernel, dim3(tiles, row_tiles, parts), W4_WARPS * 32, C::smem(rows, stages), stream, a, stages, codes));
     return 0;
 }
 
 template <int G>
 int launch_group(const W4Args& a, cudaStream_t stream)
 {
-    const int rows = std::min(a.rows, W4_ROWS);
-    if (rows <= 8) return launch_w4<G, 2, 1>(a, stream);
-    if (rows <= 16) return launch_w4<G, 2, 2>(a, stream);
-    if (rows <= 32) return launch_w4<G, 2, 4>(a, stream);
-    return launch_w4<G, 2, 8>(a, stream);
+    return a.rows <= 8 ? launch_w4<G, 1>(a, stream) : launch_w4<G, 2>(a, stream);
 }
 
 }  // namespace
@@ -244,7 +350,11 @@ int project_w4(const void* X, long long x_stride, const efa_w4& w, void* out, in
     if (int rc = check_memory("project_w4", mem, 5)) return rc;
     const W4Args a{w.codes, static_cast<const __half*>(w.scales), w.zeros, static_cast<const __half*>(X), out, rows, w.d_in, w.d_out,
                    w.code_stride ? w.code_stride : w.d_in / 2, w.scale_stride ? w.scale_stride : w.d_out, w.zero_stride ? w.zero_stride : w.d_out,
-                   x_stride ? x_stride : w.d_in, out_stride ? out_stride : w.d_out, out_dtype == EFA_F32};
+                   x_stride ? x_stride : w.d_in, out_stride ? out_stride : w.d_out, out_dtype == EFA_F32, kernel_status_word()};
+    // Up to eight rows the products of mma.sync are not the time. Beyond, tiles of 16 rows that read the weights again, or tcgen05 with up to 64 rows to a tile, whose start and
+    // end cost more: by the work, in weights times tiles of 16. us, tiles of 16 / tcgen05: 16 rows, 4096 x 4096 6.8 / 8.8, 4096 x 6144 13.2 / 10.7, 8192 x 32768 55 / 39;
+    // 32 rows, 2048 x 4096 7.9 / 8.2, 8192 x 1024 6.9 / 9.8, 4096 x 4096 9.8 / 10.1; 64 rows, 1024 x 1024 3.4 / 7.3, 1056 x 4163 15 / 12.4, 4096 x 4096 18 / 12.
+    if (rows > 8 && (double)((rows + 15) / 16) * w.d_in * w.d_out > (double)(1 << 24)) return w4_tc_launch(a, w.group, stream);
     return w.group == 128 ? launch_group<128>(a, stream) : w.group == 64 ? launch_group<64>(a, stream) : launch_group<32>(a, stream);
 }
 

@@ -1,8 +1,8 @@
 """Projections with weights of 4 bits against the definition in 64 bits.
 
-Tolerance, with S = sum over the groups of scale * sum |x (code - zero)|: a product is exact (11 bits times at most 9); a group's sum of G products in fp32, where the
-tensor cores may cut instead of rounding, is off by (G + 4) 2^-23 of its magnitudes, adding the scaled groups, warps and blocks by 2^-24 each: groups + 70 of
-them at most; then the result is rounded, 2^-11 (2^-25 at the bottom) of fp16, 2^-24 of fp32."""
+Tolerance, with S = sum over the groups of scale * sum |x| (code + zero), as products with codes and with zeros are summed apart: a product is exact (11 bits times
+at most 8); a group's sum of G products in fp32, where the tensor cores may cut instead of rounding, is off by (G + 4) 2^-23 of its magnitudes, adding the scaled
+groups, warps and blocks by 2^-24 each: groups + 70 of them at most; then the result is rounded, 2^-11 (2^-25 at the bottom) of fp16, 2^-24 of fp32."""
 import pytest
 import torch
 
@@ -23,7 +23,7 @@ def reference(X, codes, scales, zeros, out_dtype):
     w = q - (8 if zeros is None else zeros.t().double().unsqueeze(-1))
     s = scales.t().double().unsqueeze(-1)
     W = (w * s).reshape(codes.shape[0], -1)
-    ref, size = X.double() @ W.t(), X.double().abs() @ W.abs().t()
+    ref, size = X.double() @ W.t(), X.double().abs() @ ((2 * q - w) * s).reshape(codes.shape[0], -1).t()
     tol = ((group + 4) * 2.0 ** -23 + (scales.shape[0] + 70) * 2.0 ** -24) * size
     return ref, tol + (2.0 ** -11 * ref.abs() + 2.0 ** -25 if out_dtype == torch.float16 else 2.0 ** -24 * ref.abs())
 
