@@ -27,179 +27,328 @@ struct NormArgs {
     __half* h;
     int rows, d;
     bool layer, post, pre, sigmoid, x_f32, y_f32;
-    float eps, residual_scale, block_scale;
+    float eps, residual_scale, block_scale, inv_d;
     long long x_stride, y_stride, out_stride, h_stride, gate_stride;
 };
 
-// Elements of a row that a thread has: VEC, chunks of eight next to one another; else every threads-th element.
-template <bool VEC>
-struct Place {
-    int lane, threads;
-    __device__ __forceinline__ int at(int chunk, int i) const { return VEC ? (chunk * threads + lane) * 8 + i : (chunk * 8 + i) * threads + lane; }
+// How a thread has its elements. ALIGNED: chunks of eight neighbours, each 16 bytes of fp16. SHIFTED: rows that begin anywhere, but at the same place within 16
+// bytes in all tensors (dense ones of an odd width): chunks from the row's first 16-byte boundary on, and what is left at both ends, 15 elements at most, one
+// to a thread. SINGLE: every T-th element.
+enum { ALIGNED, SHIFTED, SINGLE };
+
+// Eight elements as they lie in memory: fp16 in four words (SINGLE: one to a word), fp32 one to a word. They are turned into numbers where they are used, so that
+// nothing waits for a load before all of them are under way.
+template <int W> struct Raw { uint32_t w[W]; };
+
+// The part of a row that a thread has.
+template <int T, int MODE>
+struct Share {
+    static constexpr int ENDS = MODE != SHIFTED ? 0 : T >= 16 ? 1 : 2;          // elements of the ends
+    int lane, d, head, body;             // elements before the first boundary, chunks behind it
+
+    __device__ __forceinline__ Share(int lane_, int d_, unsigned past /* elements from a boundary to the row's first */) : lane(lane_), d(d_)
+    {
+        head = MODE == SHIFTED ? (int)(8u - past) & 7 : 0;
+        // Where there is a head the weights of a chunk are in two of theirs, of which the second has to be there whole.
+        body = MODE == SHIFTED && head ? max(0, (d - 8) / 8) : d / 8;
+    }
+    __device__ __forceinline__ bool has(int chunk) const { return MODE == SINGLE || chunk * T + lane < body; }
+    __device__ __forceinline__ int at(int chunk) const { return head + (chunk * T + lane) * 8; }                  // first element of a chunk
+    __device__ __forceinline__ int single(int chunk, int i) const { return (chunk * 8 + i) * T + lane; }
+    // Element k of the ends, d or more: there is none.
+    __device__ __forceinline__ int end(int k) const { const int j = k * T + lane; return j < head ? j : j + 8 * body; }
 };
 
-template <bool VEC>
-__device__ __forceinline__ void load8(const void* base, bool f32, long long row0, const Place<VEC>& p, int chunk, int d, float (&v)[8])
+// Two fp32 at a time (the same roundings as one by one): half of the arithmetic, of which rows that are normalised twice have as much as memory has bytes.
+__device__ __forceinline__ float2 two(float x) { return make_float2(x, x); }
+__device__ __forceinline__ float2 from_bits(unsigned long long x) { return *reinterpret_cast<float2*>(&x); }
+__device__ __forceinline__ unsigned long long bits(float2 x) { return *reinterpret_cast<unsigned long long*>(&x); }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) { unsigned long long r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits(a)), "l"(bits(b))); return from_bits(r); }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) { unsigned long long r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits(a)), "l"(bits(b))); return from_bits(r); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
 {
-    if constexpr (VEC) {
-        const int at = p.at(chunk, 0);
-        if (at >= d) {
-            #pragma unroll
-            for (int i = 0; i < 8; i++) v[i] = 0.f;
-            return;
-        }
-        if (f32) {
-            const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(base) + row0 + at);
-            const float4 a = q[0], b = q[1];
-            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-        } else {
-            const uint4 q = *reinterpret_cast<const uint4*>(static_cast<const __half*>(base) + row0 + at);
-            const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-            #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-                v[2 * i] = f.x; v[2 * i + 1] = f.y;
-            }
-        }
-    } else {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(bits(a)), "l"(bits(b)), "l"(bits(c)));
+    return from_bits(r);
+}
+
+__device__ __forceinline__ float element(const void* row, bool f32, int e) { return f32 ? static_cast<const float*>(row)[e] : __half2float(static_cast<const __half*>(row)[e]); }
+
+// Streamed rows do not stay in the L1: what all rows read (KEEP; fp16) does, and is read where it is used.
+template <bool KEEP = false, int T, int MODE, int W>
+__device__ __forceinline__ void load8(Raw<W>& r, const void* row, bool f32, const Share<T, MODE>& p, int chunk)
+{
+    if constexpr (MODE == SINGLE) {
         #pragma unroll
         for (int i = 0; i < 8; i++) {
-            const int at = p.at(chunk, i);
-            v[i] = at >= d ? 0.f : f32 ? static_cast<const float*>(base)[row0 + at] : __half2float(static_cast<const __half*>(base)[row0 + at]);
+            const int e = p.single(chunk, i);
+            r.w[i] = e >= p.d ? 0u : f32 ? static_cast<const uint32_t*>(row)[e] : (uint32_t)static_cast<const unsigned short*>(row)[e];
+        }
+    } else if (!p.has(chunk)) {
+        #pragma unroll
+        for (int i = 0; i < W; i++) r.w[i] = 0u;
+    } else if constexpr (KEEP) {
+        const uint4* const q = reinterpret_cast<const uint4*>(static_cast<const __half*>(row) + p.at(chunk) - p.head);
+        const uint4 lo = q[0];
+        if (MODE == ALIGNED || p.head == 0) { r.w[0] = lo.x; r.w[1] = lo.y; r.w[2] = lo.z; r.w[3] = lo.w; return; }
+        // The weights begin at a boundary: the two chunks that hold the eight elements, moved by the head's bits.
+        const uint4 hi = q[1];
+        const uint32_t s[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+        uint32_t t[6], u[5];
+        #pragma unroll
+        for (int i = 0; i < 6; i++) t[i] = p.head & 4 ? s[i + 2] : s[i];
+        #pragma unroll
+        for (int i = 0; i < 5; i++) u[i] = p.head & 2 ? t[i + 1] : t[i];
+        #pragma unroll
+        for (int i = 0; i < 4; i++) r.w[i] = __funnelshift_r(u[i], u[i + 1], (p.head & 1) * 16);
+    } else {
+        const char* q = static_cast<const char*>(row) + (long long)p.at(chunk) * (f32 ? 4 : 2);
+        asm volatile("ld.global.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3]) : "l"(q) : "memory");
+        if constexpr (W == 8)
+            if (f32) asm volatile("ld.global.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r.w[4]), "=r"(r.w[5]), "=r"(r.w[6]), "=r"(r.w[7]) : "l"(q + 16) : "memory");
+    }
+}
+
+template <int MODE, int W>
+__device__ __forceinline__ void numbers(const Raw<W>& r, bool f32, float2 (&v)[4])
+{
+    if (W == 8 && f32) {
+        #pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = make_float2(__uint_as_float(r.w[2 * i % W]), __uint_as_float(r.w[(2 * i + 1) % W]));
+    } else {
+        #pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if constexpr (MODE != SINGLE) v[i] = __half22float2(*reinterpret_cast<const __half2*>(&r.w[i]));
+            else v[i] = make_float2(__half2float(__ushort_as_half((unsigned short)r.w[2 * i % W])), __half2float(__ushort_as_half((unsigned short)r.w[(2 * i + 1) % W])));
         }
     }
 }
 
-template <bool VEC>
-__device__ __forceinline__ void store8(void* base, bool f32, long long row0, const Place<VEC>& p, int chunk, int d, const float (&v)[8])
+__device__ __forceinline__ void store1(void* row, bool f32, int e, float v)
 {
-    if constexpr (VEC) {
-        const int at = p.at(chunk, 0);
-        if (at >= d) return;
-        if (f32) {
-            float4* q = reinterpret_cast<float4*>(static_cast<float*>(base) + row0 + at);
-            q[0] = make_float4(v[0], v[1], v[2], v[3]);
-            q[1] = make_float4(v[4], v[5], v[6], v[7]);
-        } else {
-            *reinterpret_cast<uint4*>(static_cast<__half*>(base) + row0 + at) =
-                make_uint4(pack_f16x2(v[0], v[1]), pack_f16x2(v[2], v[3]), pack_f16x2(v[4], v[5]), pack_f16x2(v[6], v[7]));
-        }
-    } else {
+    if (f32) static_cast<float*>(row)[e] = v;
+    else static_cast<__half*>(row)[e] = __float2half_rn(v);
+}
+template <int T, int MODE>
+__device__ __forceinline__ void store8(void* row, bool f32, const Share<T, MODE>& p, int chunk, const float2 (&v)[4])
+{
+    if constexpr (MODE == SINGLE) {
         #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const int at = p.at(chunk, i);
-            if (at >= d) continue;
-            if (f32) static_cast<float*>(base)[row0 + at] = v[i];
-            else static_cast<__half*>(base)[row0 + at] = __float2half_rn(v[i]);
+        for (int i = 0; i < 8; i++)
+            if (p.single(chunk, i) < p.d) store1(row, f32, p.single(chunk, i), i & 1 ? v[i / 2].y : v[i / 2].x);
+    } else if (p.has(chunk)) {
+        if (f32) {
+            float4* q = reinterpret_cast<float4*>(static_cast<float*>(row) + p.at(chunk));
+            q[0] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+            q[1] = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
+        } else {
+            *reinterpret_cast<uint4*>(static_cast<__half*>(row) + p.at(chunk)) =
+                make_uint4(pack_f16x2(v[0].x, v[0].y), pack_f16x2(v[1].x, v[1].y), pack_f16x2(v[2].x, v[2].y), pack_f16x2(v[3].x, v[3].y));
         }
     }
 }
 
-// Sum over the threads of a row: a warp (WARP), or the block. `slot` is another one each time until all threads have passed the barrier after next.
-template <bool WARP>
+// Sum over the T threads of a row. `slot` alternates: when it comes round again all threads have passed the barrier in between.
+template <int T>
 __device__ __forceinline__ float row_sum(float v, float (*part)[32], int& slot)
 {
     #pragma unroll
-    for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
-    if constexpr (WARP) return v;
-    const int lane = threadIdx.x & 31;
-    if (lane == 0) part[slot][threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = lane < (int)(blockDim.x >> 5) ? part[slot][lane] : 0.f;
-    #pragma unroll
-    for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
-    slot ^= 1;
+    for (int d = (T < 32 ? T : 32) / 2; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+    if constexpr (T > 32) {
+        constexpr int WARPS = T / 32;
+        if ((threadIdx.x & 31) == 0) part[slot][threadIdx.x >> 5] = v;
+        __syncthreads();
+        v = part[slot][threadIdx.x & (WARPS - 1)];
+        #pragma unroll
+        for (int d = WARPS / 2; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+        slot ^= 1;
+    }
     return v;
 }
 
-template <int NC, bool VEC, bool WARP>
-__device__ __forceinline__ void normalise(float (&v)[NC][8], const NormArgs& a, const Place<VEC>& p, const __half* w, const __half* b, float (*part)[32], int& slot)
+template <int NC, int T, int MODE>
+__device__ __forceinline__ void normalise(float2 (&v)[NC][4], float (&ends)[2], const NormArgs& a, const Share<T, MODE>& p, const __half* weights, const __half* biases, float (*part)[32], int& slot)
 {
-    float s = 0.f;
+    constexpr int ENDS = Share<T, MODE>::ENDS;
+    float2 s = two(0.f);
     if (a.layer) {
         #pragma unroll
         for (int c = 0; c < NC; c++)
             #pragma unroll
-            for (int i = 0; i < 8; i++) s += v[c][i];
-        const float mean = row_sum<WARP>(s, part, slot) / (float)a.d;
-        s = 0.f;
+            for (int i = 0; i < 4; i++) s = add2(s, v[c][i]);
         #pragma unroll
-        for (int c = 0; c < NC; c++)
+        for (int k = 0; k < ENDS; k++) s.x += ends[k];
+        const float mean = row_sum<T>(s.x + s.y, part, slot) * a.inv_d;
+        s = two(0.f);
+        #pragma unroll
+        for (int c = 0; c < NC; c++) {
+            const float2 off = two(MODE == SINGLE || p.has(c) ? -mean : 0.f);   // what is behind the row stays 0
             #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                v[c][i] = p.at(c, i) < a.d ? v[c][i] - mean : 0.f;
-                s += v[c][i] * v[c][i];
+            for (int i = 0; i < 4; i++) {
+                v[c][i] = add2(v[c][i], off);
+                if constexpr (MODE == SINGLE) {
+                    if (p.single(c, 2 * i) >= a.d) v[c][i].x = 0.f;
+                    if (p.single(c, 2 * i + 1) >= a.d) v[c][i].y = 0.f;
+                }
+                s = fma2(v[c][i], v[c][i], s);
             }
+        }
+        #pragma unroll
+        for (int k = 0; k < ENDS; k++) {
+            ends[k] = p.end(k) < a.d ? ends[k] - mean : 0.f;
+            s.x = fmaf(ends[k], ends[k], s.x);
+        }
     } else {
         #pragma unroll
         for (int c = 0; c < NC; c++)
             #pragma unroll
-            for (int i = 0; i < 8; i++) s += v[c][i] * v[c][i];
+            for (int i = 0; i < 4; i++) s = fma2(v[c][i], v[c][i], s);
+        #pragma unroll
+        for (int k = 0; k < ENDS; k++) s.x = fmaf(ends[k], ends[k], s.x);
     }
-    const float scale = rsqrtf(row_sum<WARP>(s, part, slot) / (float)a.d + a.eps);
+    const float scale = rsqrtf(row_sum<T>(s.x + s.y, part, slot) * a.inv_d + a.eps);
     #pragma unroll
     for (int c = 0; c < NC; c++) {
-        float g[8];
-        if (w) load8<VEC>(w, false, 0, p, c, a.d, g);
+        float2 g[4];
+        Raw<MODE == SINGLE ? 8 : 4> w;
         #pragma unroll
-        for (int i = 0; i < 8; i++) v[c][i] = w ? v[c][i] * scale * g[i] : v[c][i] * scale;
-        if (b) {
-            load8<VEC>(b, false, 0, p, c, a.d, g);
+        for (int i = 0; i < 4; i++) v[c][i] = mul2(v[c][i], two(scale));
+        if (weights) {
+            load8<true>(w, weights, false, p, c);
+            numbers<MODE>(w, false, g);
             #pragma unroll
-            for (int i = 0; i < 8; i++) v[c][i] += g[i];
+            for (int i = 0; i < 4; i++) v[c][i] = mul2(v[c][i], g[i]);
         }
+        if (biases) {
+            load8<true>(w, biases, false, p, c);
+            numbers<MODE>(w, false, g);
+            #pragma unroll
+            for (int i = 0; i < 4; i++) v[c][i] = add2(v[c][i], g[i]);
+        }
+    }
+    #pragma unroll
+    for (int k = 0; k < ENDS; k++) {
+        const int e = p.end(k);
+        if (e >= a.d) continue;
+        ends[k] *= scale;
+        if (weights) ends[k] *= __half2float(weights[e]);
+        if (biases) ends[k] += __half2float(biases[e]);
     }
 }
 
-// A row to a block, or (WARP) to a warp, NC chunks of eight elements to a thread.
-template <int NC, bool VEC, bool WARP>
-__global__ void __launch_bounds__(WARP ? 128 : NC == 1 ? 512 : 1024)
+// Blocks that registers are kept free for: 64 to 128 of them to a thread.
+constexpr int blocks_per_sm(int threads, int chunks, bool lean, bool lazy)
+{
+    const int registers = chunks == 1 ? 64 : lazy ? 64 : chunks == 2 ? (lean ? 64 : 96) : chunks == 3 ? (lean ? 80 : 112) : 128;
+    return 65536 / (registers * threads) > 0 ? 65536 / (registers * threads) : 1;
+}
+
+// A row to T threads, NC chunks of eight elements to a thread; below 32 threads several rows to a warp. All that a row reads is asked for at once; LAZY: where a thread
+// has too much for that, x and the gate in their turn.
+template <int T, int NC, int MODE, bool WIDE, bool LAZY>
+__global__ void __launch_bounds__(T <= 32 ? 128 : T, blocks_per_sm(T <= 32 ? 128 : T, NC, MODE != SINGLE && !WIDE, LAZY))
 block_norm_kernel(const NormArgs a)
 {
     __shared__ float part[2][32];
+    constexpr int PER_BLOCK = T <= 32 ? 128 / T : 1;
     pdl_wait();
     pdl_trigger();
-    const int per_block = WARP ? blockDim.x >> 5 : 1;
-    const Place<VEC> p{WARP ? (int)(threadIdx.x & 31) : (int)threadIdx.x, WARP ? 32 : (int)blockDim.x};
+    const int lane = threadIdx.x % T, first = blockIdx.x * PER_BLOCK + (T <= 32 ? threadIdx.x / T : 0), step = gridDim.x * PER_BLOCK;
     int slot = 0;
-    for (int row = blockIdx.x * per_block + (WARP ? threadIdx.x >> 5 : 0); row < a.rows; row += gridDim.x * per_block) {
-        // v: the block's output, then the sum. x is asked for together with y, so that it is there when the first norm is done; not where a thread
-        // has 32 elements of each.
-        float v[NC][8], x[NC == 4 ? 1 : NC][8];
-        #pragma unroll
-        for (int c = 0; c < NC; c++) {
-            if (a.y) load8<VEC>(a.y, a.y_f32, row * a.y_stride, p, c, a.d, v[c]);
-            if (NC < 4 && a.x) load8<VEC>(a.x, a.x_f32, row * a.x_stride, p, c, a.d, x[NC == 4 ? 0 : c]);
-        }
-        if (a.y && a.post) normalise<NC, VEC, WARP>(v, a, p, a.post_w, a.post_b, part, slot);
-        #pragma unroll
-        for (int c = 0; c < NC; c++) {
-            float g[8], (&xc)[8] = x[NC == 4 ? 0 : c];
-            if (NC == 4 && a.x) load8<VEC>(a.x, a.x_f32, row * a.x_stride, p, c, a.d, xc);
-            if (a.gate) load8<VEC>(a.gate, false, row * a.gate_stride, p, c, a.d, g);
+    constexpr int H = MODE == SINGLE ? 8 : 4, W = MODE == SINGLE || WIDE ? 8 : 4;   // words of eight fp16, and of what may be fp32
+    const bool x_f32 = WIDE && a.x_f32, y_f32 = WIDE && a.y_f32;
+    // The lanes of a warp go round together: rows behind the last are the last, without a store.
+    const int rounds = (a.rows - blockIdx.x * PER_BLOCK + step - 1) / step;
+    for (int i = 0, at = first; i < rounds; i++, at += step) {
+        const bool there = T > 32 || at < a.rows;
+        const long long row = T > 32 ? at : min(at, a.rows - 1);
+        const char* const xr = static_cast<const char*>(a.x) + row * a.x_stride * (x_f32 ? 4 : 2);
+        const char* const yr = static_cast<const char*>(a.y) + row * a.y_stride * (y_f32 ? 4 : 2);
+        const __half* const gr = a.gate + row * a.gate_stride;
+        constexpr int ENDS = Share<T, MODE>::ENDS;
+        const Share<T, MODE> p(lane, a.d, (unsigned)row * (unsigned)a.x_stride & 7u);
+        float2 v[NC][4];
+        float ends[2] = {0.f, 0.f}, x_ends[2], g_ends[2];
+        Raw<W> x[LAZY ? 1 : NC];
+        Raw<H> g[LAZY ? 1 : NC];
+        {
+            Raw<W> y[NC];
             #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                float n = v[c][i] * a.block_scale;
-                if (a.gate) n = a.sigmoid ? n / (1.f + __expf(-g[i])) : n * g[i];
-                v[c][i] = !a.y ? a.residual_scale * xc[i] : a.x ? fmaf(a.residual_scale, xc[i], n) : n;
+            for (int c = 0; c < NC; c++) {
+                if (a.y) load8(y[c], yr, y_f32, p, c);
+                if constexpr (!LAZY) {
+                    if (a.x) load8(x[c], xr, x_f32, p, c);
+                    if (a.gate) a.gate_stride ? load8(g[c], gr, false, p, c) : load8<true>(g[c], gr, false, p, c);
+                }
             }
-            if (a.x_out) store8<VEC>(a.x_out, a.x_f32, row * a.out_stride, p, c, a.d, v[c]);
+            #pragma unroll
+            for (int k = 0; k < ENDS; k++)
+                if (p.end(k) < a.d) {
+                    if (a.y) ends[k] = element(yr, y_f32, p.end(k));
+                    if (a.x) x_ends[k] = element(xr, x_f32, p.end(k));
+                    if (a.gate) g_ends[k] = __half2float(gr[p.end(k)]);
+                }
+            #pragma unroll
+            for (int c = 0; c < NC; c++) numbers<MODE>(y[c], y_f32, v[c]);
+        }
+        if (a.post) normalise(v, ends, a, p, a.post_w, a.post_b, part, slot);
+        auto gated = [&](float n, float gate) { return a.sigmoid ? __fdividef(n, 1.f + __expf(-gate)) : n * gate; };
+        auto summed = [&](float n, float residual) { return a.y ? fmaf(a.residual_scale, residual, a.block_scale * n) : a.residual_scale * residual; };
+        char* const out = static_cast<char*>(a.x_out) + row * a.out_stride * (x_f32 ? 4 : 2);
+        #pragma unroll
+        for (int c = 0; c < NC; c++) {
+            float2 n[4];
+            if constexpr (LAZY) {
+                if (a.x) load8(x[0], xr, x_f32, p, c);
+                if (a.gate) a.gate_stride ? load8(g[0], gr, false, p, c) : load8<true>(g[0], gr, false, p, c);
+            }
+            if (a.gate) {
+                numbers<MODE>(g[LAZY ? 0 : c], false, n);
+                #pragma unroll
+                for (int i = 0; i < 4; i++) v[c][i] = a.sigmoid ? make_float2(gated(v[c][i].x, n[i].x), gated(v[c][i].y, n[i].y)) : mul2(v[c][i], n[i]);
+            }
+            if (a.x) {
+                numbers<MODE>(x[LAZY ? 0 : c], x_f32, n);
+                #pragma unroll
+                for (int i = 0; i < 4; i++) v[c][i] = a.y ? fma2(two(a.residual_scale), n[i], mul2(two(a.block_scale), v[c][i])) : mul2(two(a.residual_scale), n[i]);
+            } else {
+                #pragma unroll
+                for (int i = 0; i < 4; i++) v[c][i] = mul2(v[c][i], two(a.block_scale));
+            }
+            if (a.x_out && there) store8(out, x_f32, p, c, v[c]);
+        }
+        #pragma unroll
+        for (int k = 0; k < ENDS; k++) {
+            if (p.end(k) >= a.d) continue;
+            if (a.gate) ends[k] = gated(ends[k], g_ends[k]);
+            ends[k] = a.x ? summed(ends[k], x_ends[k]) : a.block_scale * ends[k];
+            if (a.x_out && there) store1(out, x_f32, p.end(k), ends[k]);
         }
         if (a.pre) {
-            normalise<NC, VEC, WARP>(v, a, p, a.pre_w, a.pre_b, part, slot);
+            normalise(v, ends, a, p, a.pre_w, a.pre_b, part, slot);
             #pragma unroll
-            for (int c = 0; c < NC; c++) store8<VEC>(a.h, false, row * a.h_stride, p, c, a.d, v[c]);
+            for (int c = 0; c < NC; c++)
+                if (there) store8(a.h + row * a.h_stride, false, p, c, v[c]);
+            #pragma unroll
+            for (int k = 0; k < ENDS; k++)
+                if (there && p.end(k) < a.d) store1(a.h + row * a.h_stride, false, p.end(k), ends[k]);
         }
     }
 }
 
-template <int NC, bool VEC>
-int launch_norm(const NormArgs& a, int threads, bool warp, cudaStream_t stream)
+template <int T, int NC, bool LAZY = false>
+int launch_norm(const NormArgs& a, int mode, cudaStream_t stream)
 {
-    const int per_block = warp ? threads / 32 : 1;
-    const unsigned blocks = (unsigned)std::min<long long>((a.rows + per_block - 1) / per_block, (long long)device_sms() * 32);
-    EFA_CUDA(warp ? launch_value(block_norm_kernel<NC, VEC, true>, dim3(blocks), threads, 0, stream, a)
-                  : launch_value(block_norm_kernel<NC, VEC, false>, dim3(blocks), threads, 0, stream, a));
+    constexpr int PER_BLOCK = T <= 32 ? 128 / T : 1, AT_ONCE = 1024 / (T <= 32 ? 128 : T);     // about as many blocks as an SM holds
+    const long long blocks = ((long long)a.rows + PER_BLOCK - 1) / PER_BLOCK, most = (long long)device_sms() * AT_ONCE;
+    // Many rows: as many blocks as there is room for, with equal numbers of rows. Few: a block to each, which the hardware spreads better.
+    const long long rounds = blocks >= 4 * most ? (blocks + most - 1) / most : 1;
+    const dim3 grid((unsigned)((blocks + rounds - 1) / rounds));
+    const bool wide = a.x_f32 || a.y_f32;
+    const auto kernel = mode == ALIGNED ? (wide ? block_norm_kernel<T, NC, ALIGNED, true, LAZY> : block_norm_kernel<T, NC, ALIGNED, false, LAZY>)
+                      : mode == SHIFTED ? (wide ? block_norm_kernel<T, NC, SHIFTED, true, LAZY> : block_norm_kernel<T, NC, SHIFTED, false, LAZY>)
+                                        : (wide ? block_norm_kernel<T, NC, SINGLE, true, LAZY> : block_norm_kernel<T, NC, SINGLE, false, LAZY>);
+    EFA_CUDA(launch_value(kernel, grid, T <= 32 ? 128 : T, 0, stream, a));
     return 0;
 }
 
@@ -234,17 +383,29 @@ int block_norm(const void* x, const void* y, const void* gate, const void* post_
     const auto stride = [&](int64_t s) { return s ? (long long)s : (long long)p.d; };
     NormArgs a{x, y, static_cast<const __half*>(gate), static_cast<const __half*>(post_w), static_cast<const __half*>(post_b), static_cast<const __half*>(pre_w),
                static_cast<const __half*>(pre_b), x_out, static_cast<__half*>(h), rows, p.d, p.kind == EFA_NORM_LAYER, p.post != 0, h != nullptr, p.gate == EFA_GATE_SIGMOID,
-               p.x_dtype == EFA_F32, p.y_dtype == EFA_F32, p.eps, p.residual_scale, p.block_scale,
+               p.x_dtype == EFA_F32, p.y_dtype == EFA_F32, p.eps, p.residual_scale, p.block_scale, (float)(1.0 / p.d),
                stride(p.x_stride), stride(p.y_stride), stride(p.out_stride), stride(p.h_stride), p.gate_rows ? stride(p.gate_stride) : 0};
-    bool vec = p.d % 8 == 0;
-    for (const void* q : mem) vec = vec && aligned16(q);
-    for (const long long s : {a.x_stride, a.y_stride, a.out_stride, a.h_stride, a.gate_stride}) vec = vec && s % 8 == 0;
-    const int chunks = (p.d + 7) / 8;
-    const bool warp = chunks <= 128;
-    const int nc = warp ? (chunks <= 32 ? 1 : chunks <= 64 ? 2 : 4) : chunks <= 512 ? 1 : chunks <= 2048 ? 2 : 4;
-    const int threads = warp ? 128 : ((chunks + nc - 1) / nc + 31) / 32 * 32;
-    if (vec) return nc == 1 ? launch_norm<1, true>(a, threads, warp, stream) : nc == 2 ? launch_norm<2, true>(a, threads, warp, stream) : launch_norm<4, true>(a, threads, warp, stream);
-    return nc == 1 ? launch_norm<1, false>(a, threads, warp, stream) : nc == 2 ? launch_norm<2, false>(a, threads, warp, stream) : launch_norm<4, false>(a, threads, warp, stream);
+    bool aligned = true, alike = true;
+    for (const void* q : mem) aligned = aligned && aligned16(q);
+    const long long strides[] = {x ? a.x_stride : a.y_stride, y ? a.y_stride : a.x_stride, x_out ? a.out_stride : a.x_stride, h ? a.h_stride : a.x_stride, gate && a.gate_stride ? a.gate_stride : a.x_stride};
+    for (const long long t : strides) alike = alike && (t - strides[0]) % 8 == 0;
+    a.x_stride = strides[0];
+    const int mode = !aligned || !alike ? SINGLE : strides[0] % 8 == 0 && p.d % 8 == 0 ? ALIGNED : SHIFTED;
+    // Threads to a row and chunks to a thread by d alone, not by the number of rows.
+    const int d = mode == SINGLE ? p.d : p.d / 8 * 8;          // in chunks; the ends of a row are extra
+    if (d <= 64) return launch_norm<8, 1>(a, mode, stream);
+    if (d <= 128) return launch_norm<16, 1>(a, mode, stream);
+    if (d <= 256) return launch_norm<32, 1>(a, mode, stream);
+    if (d <= 512) return launch_norm<32, 2>(a, mode, stream);
+    if (d <= 1024) return launch_norm<64, 2>(a, mode, stream);
+    if (d <= 2048) return launch_norm<128, 2>(a, mode, stream);
+    if (d <= 128 * 24) return launch_norm<128, 3>(a, mode, stream);
+    if (d <= 4096) return launch_norm<256, 2>(a, mode, stream);
+    if (d <= 256 * 24) return launch_norm<256, 3>(a, mode, stream);
+    if (d <= 8192) return launch_norm<512, 2>(a, mode, stream);
+    if (d <= 512 * 24) return launch_norm<512, 3>(a, mode, stream);
+    if (d <= 16384) return launch_norm<512, 4>(a, mode, stream);
+    return launch_norm<1024, 4, true>(a, mode, stream);
 }
 
 }  // namespace efa
