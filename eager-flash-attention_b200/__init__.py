@@ -17,6 +17,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 from typing import Optional, Sequence
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -598,7 +599,12 @@ def _dtype(what: str, x, want: Optional[int] = None) -> int:
 
 def _matrix(what: str, x, rows: int, width: int, stride: int, kind: int) -> Optional[int]:
     """Address of ``rows`` rows of ``width`` elements, ``stride`` apart (0: dense). A tensor of another type or that ends before them is refused."""
-    if x is None or not hasattr(x, "data_ptr"):
+    if x is None:
+        return None
+    try:
+        if _real.get(x.dtype) == kind and not stride and x.is_contiguous() and x.numel() >= rows * width:
+            return x.data_ptr()
+    except AttributeError:
         return _ptr(x)
     _dtype(what, x, kind)
     if rows <= 0:
@@ -629,17 +635,20 @@ def block_norm_check(bp: BlockNormParams, rows: int) -> Optional[str]:
     return None if why is None else why.decode()
 
 
+_BLOCK_NORM_INTS = struct.Struct("6i12x2i5q").unpack_from     # fields of BlockNormParams without the three floats: one by one they cost more than the launch
+
+
 def block_norm(x, y, x_out, h, rows: int, bp: BlockNormParams, gate=None, post_w=None, post_b=None, pre_w=None, pre_b=None, stream=None) -> None:
     """Norms after and before a block with its gate and residual addition, per row: ``n = post ? norm(y) * post_w + post_b : y``,
     ``x_out = residual_scale * x + block_scale * act(gate) * n``, ``h = norm(x_out before its rounding) * pre_w + pre_b``. None: no such input or output
     (weights: ones, biases: zeros). x_out and h may be x or y. Asynchronous on ``stream``."""
-    d = bp.d
+    d, _, _, _, _, gate_rows, x_dtype, y_dtype, x_stride, y_stride, out_stride, h_stride, gate_stride = _BLOCK_NORM_INTS(bp)
     _check(lib().efa_block_norm(
-        _matrix("block_norm: x", x, rows, d, bp.x_stride, bp.x_dtype), _matrix("block_norm: y", y, rows, d, bp.y_stride, bp.y_dtype),
-        _matrix("block_norm: gate", gate, rows if bp.gate_rows else 1, d, bp.gate_stride, F16),
+        _matrix("block_norm: x", x, rows, d, x_stride, x_dtype), _matrix("block_norm: y", y, rows, d, y_stride, y_dtype),
+        _matrix("block_norm: gate", gate, rows if gate_rows else 1, d, gate_stride, F16),
         _matrix("block_norm: post_w", post_w, 1, d, 0, F16), _matrix("block_norm: post_b", post_b, 1, d, 0, F16),
         _matrix("block_norm: pre_w", pre_w, 1, d, 0, F16), _matrix("block_norm: pre_b", pre_b, 1, d, 0, F16),
-        _matrix("block_norm: x_out", x_out, rows, d, bp.out_stride, bp.x_dtype), _matrix("block_norm: h", h, rows, d, bp.h_stride, F16),
+        _matrix("block_norm: x_out", x_out, rows, d, out_stride, x_dtype), _matrix("block_norm: h", h, rows, d, h_stride, F16),
         rows, bp, _stream(stream)), "block_norm")
 
 

@@ -1,8 +1,8 @@
 // The pages of a paged cache: taken, shared, given back, moved. All of it goes by device memory: the host knows the sizes only.
 //
-// Which pages are free is a scan over their counts. One cluster of eight blocks does it, a segment of the pages to each block: counts per block, exchanged
-// through the cluster's shared memory, then ranks within the segment; so the lowest free pages are found in one launch, in an order that nothing but the arrays
-// decides. What moves keys is a kernel of its own over all SMs.
+// Which pages are free is a scan over their counts. One block does it, or for large pools and long lists a cluster of eight, a segment of the pages to each block: 512
+// neighbouring pages to a warp, whose votes stay in registers from the counting to the ranking; so the lowest free pages are found in one pass and one launch,
+// in an order that nothing but the arrays decides. What moves keys is a kernel of its own over all SMs.
 //
 // Everything that comes from device memory is brought into range before it is an index; what was out of range is reported in the status word.
 #include "host_util.h"
@@ -18,6 +18,7 @@ namespace efa {
 namespace {
 
 constexpr int PG_CLUSTER = 8, PG_THREADS = 1024, PG_WARPS = PG_THREADS / 32;
+constexpr int PG_VOTES = 16, PG_TILE = PG_THREADS * PG_VOTES;  // of 32 pages to a warp; pages that a block looks at in one pass
 constexpr int PG_MOVE_THREADS = 256, PG_SEGMENT = 32768;       // bytes of a page that a block moves at a time
 enum { SITE_TAKE = 60, SITE_FORK = 61, SITE_FREE = 62, SITE_COMPACT = 63, SITE_COPY = 64 };
 
@@ -40,30 +41,16 @@ __device__ __forceinline__ void report(int* status, int code, int who, int site)
 __device__ __forceinline__ long long capacity(const PoolArgs& p) { return (long long)p.max_pages * p.page_size; }
 
 // Keys of a slot, brought into what its table holds.
-__device__ __forceinline__ int keys_of(const PoolArgs& p, int b, int site)
+__device__ __forceinline__ int keys_in_table(const PoolArgs& p, int kv, int b, int site)
 {
-    const int kv = p.kv_len[b];
     const int cut = (int)min(max((long long)kv, 0ll), min(capacity(p), (long long)INT_MAX));
     if (cut != kv) report(p.status, KS_BAD_LENGTH, b, site);
     return cut;
 }
+__device__ __forceinline__ int keys_of(const PoolArgs& p, int b, int site) { return keys_in_table(p, p.kv_len[b], b, site); }
 __device__ __forceinline__ int pages_of(const PoolArgs& p, int keys) { return (int)(((long long)keys + p.page_size - 1) / p.page_size); }
 
-// Sum over the block; `part` [PG_WARPS] in shared memory.
-__device__ __forceinline__ int block_sum(int v, int* part)
-{
-    #pragma unroll
-    for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = part[threadIdx.x & 31];
-    #pragma unroll
-    for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
-    return v;
-}
-
-// Sum of the values of the threads before this one, and of all of them in `total`.
+// Sum of the values of the threads before this one, and of all of them in `total`; `part` [PG_WARPS] in shared memory.
 __device__ __forceinline__ int block_scan(int v, int* part, int& total)
 {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -86,113 +73,186 @@ __device__ __forceinline__ int block_scan(int v, int* part, int& total)
     return run - v + __shfl_sync(0xffffffffu, all - w, warp);
 }
 
-// Sums over the cluster: of what the blocks before this one, and all of them, put into `mine` (shared memory, one word a block).
-__device__ __forceinline__ int cluster_scan(int v, int* mine, int& total)
+// All blocks of the cluster, or of the one block there is.
+__device__ __forceinline__ void sync_all() { if (gridDim.z > 1) cluster_sync(); else __syncthreads(); }
+__device__ __forceinline__ int rank_of_block() { return gridDim.z > 1 ? (int)cluster_rank() : 0; }
+__device__ __forceinline__ int shared_of(const int* p, int block)
 {
-    if (threadIdx.x == 0) *mine = v;
-    cluster_sync();
-    int before = 0;
-    total = 0;
-    const int rank = (int)cluster_rank();
-    #pragma unroll
-    for (int q = 0; q < PG_CLUSTER; q++) {
-        int x;
-        asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(x) : "r"(cluster_addr(mine, q)));
-        before += q < rank ? x : 0;
-        total += x;
-    }
-    return before;
+    if (gridDim.z == 1) return *p;
+    int x;
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(x) : "r"(cluster_addr(p, (uint32_t)block)));
+    return x;
 }
 
 struct Range { int lo, hi; };
 __device__ __forceinline__ Range segment(int n)
 {
-    const int each = (n + PG_CLUSTER - 1) / PG_CLUSTER, lo = min(n, each * (int)cluster_rank());
-    return Range{lo, min(n, lo + each)};
+    const int each = (int)(((long long)n + gridDim.z - 1) / gridDim.z), lo = (int)min((long long)n, (long long)each * rank_of_block());
+    return Range{lo, (int)min((long long)n, (long long)lo + each)};
 }
 
-// Free pages [lo, hi) get their ranks among all free pages; those below `wanted` go into list[rank] and get a count of 1.
-__device__ __forceinline__ int count_free(const int* refs, Range r, int* part)
+// A warp's pages of the tile at `base`: votes[j] says which of base + warp * 512 + 32 j + (0 .. 31) satisfy the predicate; their number.
+template <class F>
+__device__ __forceinline__ int vote(int base, int hi, uint32_t (&votes)[PG_VOTES], F predicate)
 {
+    const int first = base + (int)(threadIdx.x >> 5) * (32 * PG_VOTES) + (int)(threadIdx.x & 31);
+    bool yes[PG_VOTES];
+    #pragma unroll
+    for (int j = 0; j < PG_VOTES; j++) yes[j] = first + 32 * j < hi && predicate(first + 32 * j);
     int n = 0;
-    for (int p = r.lo + (int)threadIdx.x; p < r.hi; p += PG_THREADS) n += refs[p] <= 0 ? 1 : 0;
-    return block_sum(n, part);
+    #pragma unroll
+    for (int j = 0; j < PG_VOTES; j++) {
+        votes[j] = __ballot_sync(0xffffffffu, yes[j]);
+        n += __popc(votes[j]);
+    }
+    return n;
 }
-__device__ __forceinline__ void list_free(int* refs, Range r, int before, int wanted, int* list, int* part)
+
+// Sums of a warp's numbers over the block: of the warps before, and of all.
+__device__ __forceinline__ int warp_scan(int n, int* part, int& total)
 {
-    for (int base = r.lo; base < r.hi && before < wanted; base += PG_THREADS) {
-        const int p = base + (int)threadIdx.x;
-        const int free = p < r.hi && refs[p] <= 0 ? 1 : 0;
-        int total;
-        const int rank = before + block_scan(free, part, total);
-        if (free && rank < wanted) { list[rank] = p; refs[p] = 1; }
-        before += total;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    __syncthreads();
+    if (lane == 0) part[warp] = n;
+    __syncthreads();
+    const int w = part[lane];
+    int all = w;
+    #pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+        const int o = __shfl_up_sync(0xffffffffu, all, d);
+        if (lane >= d) all += o;
+    }
+    total = __shfl_sync(0xffffffffu, all, 31);
+    return __shfl_sync(0xffffffffu, all - w, warp);
+}
+
+// Calls f(page, rank) for the pages that the votes name; rank: that of the warp's first.
+template <class F>
+__device__ __forceinline__ void ranked(int base, const uint32_t (&votes)[PG_VOTES], int rank, F f)
+{
+    const int lane = threadIdx.x & 31, first = base + (int)(threadIdx.x >> 5) * (32 * PG_VOTES) + lane;
+    #pragma unroll
+    for (int j = 0; j < PG_VOTES; j++) {
+        if (votes[j] >> lane & 1u) f(first + 32 * j, rank + __popc(votes[j] & ((1u << lane) - 1u)));
+        rank += __popc(votes[j]);
     }
 }
 
-// workspace: list [num_pages], then what the kernels say of it.
-struct TakeArgs { PoolArgs p; const int* q_start; int* list; };
+// The numbers that the blocks have put into `mine` (shared memory): what the blocks before have, and all. Ends with everything that was written visible to all.
+__device__ __forceinline__ int over_blocks(int v, int* mine, int& total)
+{
+    if (threadIdx.x == 0) *mine = v;
+    sync_all();
+    int before = 0;
+    total = 0;
+    for (int q = 0; q < (int)gridDim.z; q++) {
+        const int x = shared_of(mine, q);
+        before += q < rank_of_block() ? x : 0;
+        total += x;
+    }
+    return before;
+}
+
+// The free pages of a block's segment: found (their number), and listed: those of a rank below `wanted` go to list[rank] and have a count of 1 from then on.
+struct FreePages {
+    Range own;
+    uint32_t votes[PG_VOTES];            // of the segment's first tile, which is mostly all of it
+    int n;                               // free pages of that, of this warp
+
+    __device__ __forceinline__ int find(const int* refs, int num_pages, int* part)
+    {
+        own = segment(num_pages);
+        const auto free = [&](int p) { return refs[p] <= 0; };
+        n = vote(own.lo, own.hi, votes, free);
+        int total, all;
+        warp_scan(n, part, total);
+        for (int base = own.lo + PG_TILE; base < own.hi; base += PG_TILE) {
+            uint32_t v[PG_VOTES];
+            warp_scan(vote(base, own.hi, v, free), part, all);
+            total += all;
+        }
+        return total;
+    }
+    __device__ __forceinline__ void list(int* refs, int before, int wanted, int* to, int* part)
+    {
+        const auto take = [&](int p, int rank) { if (rank < wanted) { to[rank] = p; refs[p] = 1; } };
+        int total;
+        int rank = before + warp_scan(n, part, total);
+        ranked(own.lo, votes, rank, take);
+        before += total;
+        for (int base = own.lo + PG_TILE; base < own.hi && before < wanted; base += PG_TILE) {
+            uint32_t v[PG_VOTES];
+            const int m = vote(base, own.hi, v, [&](int p) { return refs[p] <= 0; });
+            rank = before + warp_scan(m, part, total);
+            ranked(base, v, rank, take);
+            before += total;
+        }
+    }
+};
+
+// workspace: list [num_pages]; of every slot the pages it has, those it gets, and how many its block's slots before it get.
+struct TakeArgs { PoolArgs p; const int* q_start; int* list; int* have; int* gets; int* rank; };
 
 __global__ void __launch_bounds__(PG_THREADS)
 pages_take_kernel(const TakeArgs a)
 {
-    __shared__ int part[PG_WARPS], mine[2];
-    __shared__ int3 todo[PG_THREADS];
+    __shared__ int part[PG_WARPS], need_of, free_of, need_before[PG_CLUSTER];
     pdl_wait();
     pdl_trigger();
     const PoolArgs& p = a.p;
-    const Range seqs = segment(p.num_seqs), own = segment(p.num_pages);
-
-    // A slot's new length, and the pages that it has and wants.
-    auto grown = [&](int b, int& have, int& want) {
-        const int kv = keys_of(p, b, SITE_TAKE);
-        const long long n = (long long)a.q_start[b + 1] - a.q_start[b];
-        const long long after = min((long long)kv + max(n, 0ll), min(capacity(p), (long long)INT_MAX));
-        if (n < 0 || after != kv + n) report(p.status, KS_BAD_LENGTH, b, SITE_TAKE);
-        have = pages_of(p, kv);
-        want = pages_of(p, (int)after);
-        return (int)after;
-    };
+    const Range seqs = segment(p.num_seqs);
+    FreePages pages;
+    const int found = pages.find(p.refs, p.num_pages, part);
     int need = 0;
-    for (int b = seqs.lo + (int)threadIdx.x; b < seqs.hi; b += PG_THREADS) {
-        int have, want;
-        grown(b, have, want);
-        need += want - have;
-    }
-    need = block_sum(need, part);
-    int wanted, there;
-    int first = cluster_scan(need, &mine[0], wanted);
-    const int before = cluster_scan(count_free(p.refs, own, part), &mine[1], there);
-    list_free(p.refs, own, before, wanted, a.list, part);
-    cluster_sync();
     for (int base = seqs.lo; base < seqs.hi; base += PG_THREADS) {
         const int b = base + (int)threadIdx.x;
-        int have = 0, want = 0, after = 0, total;
-        if (b < seqs.hi) after = grown(b, have, want);
-        const int rank = first + block_scan(want - have, part, total);
-        todo[threadIdx.x] = make_int3(have, want, rank);
-        __syncthreads();
-        for (int i = threadIdx.x >> 5; i < PG_THREADS; i += PG_WARPS) {
-            const int3 d = todo[i];
-            for (int e = d.x + (int)(threadIdx.x & 31); e < d.y; e += 32) {
-                const int r = d.z + e - d.x;
-                p.pages[(long long)(base + i) * p.max_pages + e] = r < there ? a.list[r] : -1;
-                if (r >= there) report(p.status, KS_NO_PAGE, base + i, SITE_TAKE);
-            }
+        int have = 0, gets = 0, total;
+        if (b < seqs.hi) {
+            const int kv = keys_of(p, b, SITE_TAKE);
+            const long long n = (long long)a.q_start[b + 1] - a.q_start[b];
+            const long long after = min((long long)kv + max(n, 0ll), min(capacity(p), (long long)INT_MAX));
+            if (n < 0 || after != kv + n) report(p.status, KS_BAD_LENGTH, b, SITE_TAKE);
+            have = pages_of(p, kv);
+            gets = pages_of(p, (int)after) - have;
+            p.kv_len[b] = (int)after;                          // no other thread looks at it
         }
-        __syncthreads();
-        if (b < seqs.hi) p.kv_len[b] = after;
-        first += total;
+        const int before = block_scan(gets, part, total);
+        if (b < seqs.hi) { a.have[b] = have; a.gets[b] = gets; a.rank[b] = need + before; }
+        need += total;
+    }
+    if (threadIdx.x == 0) { need_of = need; free_of = found; }
+    sync_all();
+    int wanted = 0, there = 0, free_before = 0;
+    for (int q = 0; q < (int)gridDim.z; q++) {
+        const int f = shared_of(&free_of, q);
+        free_before += q < rank_of_block() ? f : 0;
+        there += f;
+        if (threadIdx.x == 0) need_before[q] = wanted;
+        wanted += shared_of(&need_of, q);
+    }
+    pages.list(p.refs, free_before, wanted, a.list, part);
+    sync_all();
+    // Entries, slots to the warps of all blocks in turn.
+    const int each = (int)(((long long)p.num_seqs + gridDim.z - 1) / gridDim.z);
+    for (int b = rank_of_block() + (int)gridDim.z * (int)(threadIdx.x >> 5); b < p.num_seqs; b += (int)gridDim.z * PG_WARPS) {
+        const int gets = a.gets[b];
+        if (gets == 0) continue;
+        const int rank = a.rank[b] + need_before[b / each];
+        int* const to = p.pages + (long long)b * p.max_pages + a.have[b];
+        if ((threadIdx.x & 31) == 0 && rank + gets > there) report(p.status, KS_NO_PAGE, b, SITE_TAKE);
+        #pragma unroll 4
+        for (int e = (int)(threadIdx.x & 31); e < gets; e += 32) to[e] = rank + e < there ? a.list[rank + e] : -1;
     }
 }
 
 // Moves: pairs of pages, whole (keys NULL) or their first keys[i] keys. count: on the device, or NULL for n of them.
 struct MoveArgs {
-    uint8_t* part[4];           // k, v, k_exp, v_exp
-    long long stride[4];        // bytes from a page to the next
-    int head_bytes[4];          // bytes of a head of a page
-    int key_bytes[4];
-    int heads, num_pages;
+    uint8_t* part[2];           // k, v
+    uint8_t* exps[2];           // their exponents, or NULL
+    long long stride;           // bytes from a page to the next
+    int head_bytes, key_bytes;  // bytes of a head of a page, and of a key of it
+    int heads, page_size, num_pages;
+    int segments;               // of a page's k: heads, or pieces of PG_SEGMENT bytes
     const int* src;
     const int* dst;
     const int* keys;
@@ -201,67 +261,136 @@ struct MoveArgs {
     int* status;
 };
 
+// Moves first, first + step, ... of n pairs of pages, by a block.
+__device__ __forceinline__ void move(const MoveArgs& a, int n, long long first, long long step)
+{
+    constexpr int THREADS = PG_MOVE_THREADS;
+    const int thread = threadIdx.x;
+    const int per_page = 2 * a.segments;
+    const long long items = (long long)n * per_page;
+    for (long long item = first; item < items; item += step) {
+        const int i = (int)(item / per_page), of_page = (int)(item % per_page), what = of_page / a.segments, s = of_page % a.segments;
+        const int src = a.src[i], dst = a.dst[i], keys = a.keys ? a.keys[i] : 0;
+        if ((unsigned)src >= (unsigned)a.num_pages || (unsigned)dst >= (unsigned)a.num_pages) {
+            if (thread == 0 && of_page == 0) report(a.status, KS_BAD_PAGE, i, a.site);
+            continue;
+        }
+        // A head's first keys, or a segment of the page; with it the exponents of these keys, or, beside the first segment, all of the page's.
+        const long long at = a.keys ? (long long)s * a.head_bytes : (long long)s * PG_SEGMENT;
+        const int bytes = a.keys ? keys * a.key_bytes : (int)min((long long)PG_SEGMENT, (long long)a.heads * a.head_bytes - at);
+        uint8_t* const part = what ? a.part[1] : a.part[0];
+        uint8_t* const exps = what ? a.exps[1] : a.exps[0];
+        const uint8_t* const from = part + src * a.stride + at;
+        uint8_t* const to = part + dst * a.stride + at;
+        const int chunks = bytes / 16;                         // a key is 16 bytes at least
+        int c = thread;
+        for (; c + 7 * THREADS < chunks; c += 8 * THREADS) {
+            uint4 v[8];
+            #pragma unroll
+            for (int j = 0; j < 8; j++) v[j] = reinterpret_cast<const uint4*>(from)[c + j * THREADS];
+            #pragma unroll
+            for (int j = 0; j < 8; j++) reinterpret_cast<uint4*>(to)[c + j * THREADS] = v[j];
+        }
+        if (c < chunks) {
+            uint4 v[7];
+            #pragma unroll
+            for (int j = 0; j < 7; j++)
+                if (c + j * THREADS < chunks) v[j] = reinterpret_cast<const uint4*>(from)[c + j * THREADS];
+            #pragma unroll
+            for (int j = 0; j < 7; j++)
+                if (c + j * THREADS < chunks) reinterpret_cast<uint4*>(to)[c + j * THREADS] = v[j];
+        }
+        if (exps) {                                            // of a head's keys byte by byte, of a page, beside its first segment, all
+            const long long page = (long long)a.heads * a.page_size;
+            const uint8_t* const es = exps + src * page + (a.keys ? (long long)s * a.page_size : 0);
+            uint8_t* const ed = exps + dst * page + (a.keys ? (long long)s * a.page_size : 0);
+            if (a.keys)
+                for (int k = thread; k < keys; k += THREADS) ed[k] = es[k];
+            else if (s == 0)
+                for (long long l = thread; l * 16 < page; l += THREADS) reinterpret_cast<uint4*>(ed)[l] = reinterpret_cast<const uint4*>(es)[l];
+        }
+    }
+}
+
 // workspace of a fork: list [num_pages], then [num_seqs] each of claim, keys of the child, rank of its page, and the moves: source, target, keys; then their count.
 struct ForkArgs { PoolArgs p; const int* parents; const int* children; int n; int* list; int* claim; int* keys; int* rank; int* src; int* dst; int* rest; int* count; };
+
+constexpr int PG_FEW = 512;             // forks whose children are compared with one another, without the claims' round trip through memory
 
 __global__ void __launch_bounds__(PG_THREADS)
 pages_fork_kernel(const ForkArgs a)
 {
-    __shared__ int part[PG_WARPS], mine[2];
+    __shared__ int part[PG_WARPS], mine[2], named[PG_FEW];
     pdl_wait();
     pdl_trigger();
     const PoolArgs& p = a.p;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const Range forks = segment(a.n), own = segment(p.num_pages);
+    const Range forks = segment(a.n);
     auto slot = [&](int b) { return (unsigned)b < (unsigned)p.num_seqs; };
+    FreePages pages;
+    const int found = pages.find(p.refs, p.num_pages, part);
 
     // The first entry that names a child has it.
-    for (int i = forks.lo + (int)threadIdx.x; i < forks.hi; i += PG_THREADS)
-        if (slot(a.children[i])) a.claim[a.children[i]] = INT_MAX;
-    cluster_sync();
-    for (int i = forks.lo + (int)threadIdx.x; i < forks.hi; i += PG_THREADS)
-        if (slot(a.children[i])) atomicMin(&a.claim[a.children[i]], i);
-    cluster_sync();
-    int need = 0;
-    for (int i = forks.lo + (int)threadIdx.x; i < forks.hi; i += PG_THREADS) {
-        const int c = a.children[i], b = a.parents[i];
-        int keys = -1;
-        if (!slot(c) || !slot(b) || a.claim[c] != i || p.kv_len[c] != 0) report(p.status, KS_BAD_SLOT, slot(c) ? c : i, SITE_FORK);
-        else {
-            keys = keys_of(p, b, SITE_FORK);
-            if (keys % p.page_size) {
-                const int source = p.pages[(long long)b * p.max_pages + keys / p.page_size];
-                if ((unsigned)source < (unsigned)p.num_pages) need++;
-                else report(p.status, KS_BAD_PAGE, b, SITE_FORK);
-            }
-        }
-        a.keys[i] = keys;
+    const bool few = a.n <= PG_FEW;
+    if (few) {
+        if ((int)threadIdx.x < a.n) named[threadIdx.x] = a.children[threadIdx.x];
+        __syncthreads();
+    } else {
+        for (int i = forks.lo + (int)threadIdx.x; i < forks.hi; i += PG_THREADS)
+            if (slot(a.children[i])) a.claim[a.children[i]] = INT_MAX;
+        sync_all();
+        for (int i = forks.lo + (int)threadIdx.x; i < forks.hi; i += PG_THREADS)
+            if (slot(a.children[i])) atomicMin(&a.claim[a.children[i]], i);
+        sync_all();
     }
-    need = block_sum(need, part);
-    int wanted, there;
-    int first = cluster_scan(need, &mine[0], wanted);
-    const int before = cluster_scan(count_free(p.refs, own, part), &mine[1], there);
-    list_free(p.refs, own, before, wanted, a.list, part);
-    if (cluster_rank() == 0 && threadIdx.x == 0) *a.count = min(wanted, there);
-    // Ranks of the children's pages.
+    // Keys of the children (-1: an entry that changes nothing) and the ranks of the pages that they get.
+    int need = 0;
     for (int base = forks.lo; base < forks.hi; base += PG_THREADS) {
         const int i = base + (int)threadIdx.x;
-        int wants = 0, total;
-        if (i < forks.hi && a.keys[i] > 0 && a.keys[i] % p.page_size) {
-            const int source = p.pages[(long long)a.parents[i] * p.max_pages + a.keys[i] / p.page_size];
-            wants = (unsigned)source < (unsigned)p.num_pages ? 1 : 0;
+        int keys = -1, wants = 0, total;
+        if (i < forks.hi) {
+            const int c = a.children[i], b = a.parents[i];
+            const int child_keys = slot(c) ? p.kv_len[c] : 0, parent_keys = slot(b) ? p.kv_len[b] : 0;
+            bool first = true;
+            if (few) {
+                #pragma unroll 8
+                for (int j = 0; j < i; j++) first &= named[j] != c;
+            } else first = slot(c) && a.claim[c] == i;
+            if (!first || !slot(c) || !slot(b) || child_keys != 0) report(p.status, KS_BAD_SLOT, slot(c) ? c : i, SITE_FORK);
+            else {
+                keys = keys_in_table(p, parent_keys, b, SITE_FORK);
+                if (keys % p.page_size) {
+                    const int source = p.pages[(long long)b * p.max_pages + keys / p.page_size];
+                    if ((unsigned)source < (unsigned)p.num_pages) wants = 1;
+                    else report(p.status, KS_BAD_PAGE, b, SITE_FORK);
+                }
+            }
         }
-        const int rank = first + block_scan(wants, part, total);
-        if (i < forks.hi) a.rank[i] = wants ? rank : -1;
-        first += total;
+        const int rank = need + block_scan(wants, part, total);
+        if (i < forks.hi) { a.keys[i] = keys; a.rank[i] = wants ? rank : -1; }
+        need += total;
     }
-    cluster_sync();
-    for (int i = forks.lo + warp; i < forks.hi; i += PG_WARPS) {
+    if (threadIdx.x == 0) mine[1] = found;
+    int wanted, there = 0, before = 0;
+    const int need_before = over_blocks(need, &mine[0], wanted);
+    for (int q = 0; q < (int)gridDim.z; q++) {
+        const int x = shared_of(&mine[1], q);
+        before += q < rank_of_block() ? x : 0;
+        there += x;
+    }
+    if (need_before)
+        for (int i = forks.lo + (int)threadIdx.x; i < forks.hi; i += PG_THREADS)
+            if (a.rank[i] >= 0) a.rank[i] += need_before;
+    pages.list(p.refs, before, wanted, a.list, part);
+    if (rank_of_block() == 0 && threadIdx.x == 0) *a.count = min(wanted, there);
+    sync_all();
+    for (int i = rank_of_block() + (int)gridDim.z * warp; i < a.n; i += (int)gridDim.z * PG_WARPS) {
         const int keys = a.keys[i];
         if (keys < 0) continue;
         const int c = a.children[i], full = keys / p.page_size, rank = a.rank[i];
         const int* const from = p.pages + (long long)a.parents[i] * p.max_pages;
         int* const to = p.pages + (long long)c * p.max_pages;
+        #pragma unroll 4
         for (int e = lane; e < full; e += 32) {
             const int page = from[e];
             const bool good = (unsigned)page < (unsigned)p.num_pages;
@@ -272,10 +401,11 @@ pages_fork_kernel(const ForkArgs a)
         if (lane == 0) {
             if (keys % p.page_size) {
                 const bool got = rank >= 0 && rank < there;
-                to[full] = got ? a.list[rank] : -1;
+                const int page = got ? a.list[rank] : -1;
+                to[full] = page;
                 if (got) {
                     a.src[rank] = from[full];
-                    a.dst[rank] = a.list[rank];
+                    a.dst[rank] = page;
                     a.rest[rank] = keys % p.page_size;
                 } else if (rank >= 0) report(p.status, KS_NO_PAGE, c, SITE_FORK);
             }
@@ -284,28 +414,29 @@ pages_fork_kernel(const ForkArgs a)
     }
 }
 
-__global__ void __launch_bounds__(256)
-pages_free_kernel(const PoolArgs p, const int* seqs, int n)
+constexpr int PG_FREE_THREADS = 128;
+
+__global__ void __launch_bounds__(PG_FREE_THREADS)
+pages_free_kernel(const PoolArgs p, const int* seqs)
 {
+    __shared__ int keys_of_slot;
     pdl_wait();
     pdl_trigger();
-    const int lane = threadIdx.x & 31, i = blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (i >= n) return;
-    const int b = seqs[i];
+    const int i = blockIdx.x, b = seqs[i];
     if ((unsigned)b >= (unsigned)p.num_seqs) {
-        if (lane == 0) report(p.status, KS_BAD_SLOT, i, SITE_FREE);
+        if (threadIdx.x == 0) report(p.status, KS_BAD_SLOT, i, SITE_FREE);
         return;
     }
-    int keys = 0;
-    if (lane == 0) keys = atomicExch(&p.kv_len[b], 0);         // whoever names the slot again finds it empty
-    keys = __shfl_sync(0xffffffffu, keys, 0);
-    const int cut = (int)min(max((long long)keys, 0ll), min(capacity(p), (long long)INT_MAX));
-    if (cut != keys && lane == 0) report(p.status, KS_BAD_LENGTH, b, SITE_FREE);
+    if (threadIdx.x == 0) keys_of_slot = atomicExch(&p.kv_len[b], 0);          // whoever names the slot again finds it empty
+    __syncthreads();
+    const int keys = keys_of_slot, cut = (int)min(max((long long)keys, 0ll), min(capacity(p), (long long)INT_MAX));
+    if (cut != keys && threadIdx.x == 0) report(p.status, KS_BAD_LENGTH, b, SITE_FREE);
     const int held = pages_of(p, cut);
-    for (int e = lane; e < held; e += 32) {
+    #pragma unroll 4
+    for (int e = threadIdx.x; e < held; e += PG_FREE_THREADS) {
         const int page = p.pages[(long long)b * p.max_pages + e];
         if ((unsigned)page >= (unsigned)p.num_pages) {
-            if (page != -1) report(p.status, KS_BAD_PAGE, b, SITE_FREE);     // -1: there was no page to be had
+            if (page != -1) report(p.status, KS_BAD_PAGE, b, SITE_FREE);       // -1: there was no page to be had
         } else if (atomicSub(&p.refs[page], 1) <= 0) {
             atomicAdd(&p.refs[page], 1);
             report(p.status, KS_BAD_PAGE, b, SITE_FREE);
@@ -323,40 +454,70 @@ pages_compact_kernel(const CompactArgs a)
     pdl_wait();
     pdl_trigger();
     const PoolArgs& p = a.p;
-    const Range own = segment(p.num_pages);
-    int n = own.hi - own.lo - count_free(p.refs, own, part), live;
-    int before = cluster_scan(n, &mine[0], live);
-    n = 0;
-    for (int q = own.lo + (int)threadIdx.x; q < min(own.hi, live); q += PG_THREADS) n += p.refs[q] > 0 ? 1 : 0;
-    int stay;                                                  // pages in use before L
-    cluster_scan(block_sum(n, part), &mine[1], stay);
-    for (int base = own.lo; base < own.hi; base += PG_THREADS) {
-        const int q = base + (int)threadIdx.x;
-        const bool used = q < own.hi && p.refs[q] > 0;
-        int total;
-        const int rank = before + block_scan(used ? 1 : 0, part, total);       // pages in use before q
-        if (q < own.hi) {
-            if (used && q >= live) a.from[rank - stay] = q;
-            else a.moved[q] = used ? q : -1;
-            if (!used && q < live) a.to[q - rank] = q;
+    FreePages pages;
+    const int found = pages.find(p.refs, p.num_pages, part);
+    int free_all;
+    const int free_before = over_blocks(found, &mine[0], free_all);
+    const int live = p.num_pages - free_all;
+    // Free pages before L, in this segment: as many as pages in use at or behind L. Rank of a free page before L: of its hole.
+    int rank = free_before, total, holes = 0;
+    auto in_front = [&](int base, const uint32_t (&votes)[PG_VOTES]) {
+        int n = 0;
+        const int first = base + (int)(threadIdx.x >> 5) * (32 * PG_VOTES);
+        #pragma unroll
+        for (int j = 0; j < PG_VOTES; j++) {
+            const int left = live - (first + 32 * j);          // of the 32, those before L
+            n += left >= 32 ? __popc(votes[j]) : left > 0 ? __popc(votes[j] & ((1u << left) - 1u)) : 0;
         }
-        before += total;
+        return n;
+    };
+    auto free = [&](int q) { return p.refs[q] <= 0; };
+    for (int base = pages.own.lo; base < pages.own.hi && base < live; base += PG_TILE) {
+        uint32_t v[PG_VOTES];
+        if (base == pages.own.lo) {
+            #pragma unroll
+            for (int j = 0; j < PG_VOTES; j++) v[j] = pages.votes[j];
+        } else vote(base, pages.own.hi, v, free);
+        warp_scan(in_front(base, v), part, total);
+        holes += total;
     }
-    cluster_sync();
-    if (cluster_rank() == 0 && threadIdx.x == 0) *a.count = live - stay;
-    for (int i = (int)cluster_rank() * PG_THREADS + threadIdx.x; i < live - stay; i += PG_CLUSTER * PG_THREADS) a.moved[a.from[i]] = a.to[i];
+    int moves;
+    over_blocks(holes, &mine[1], moves);
+    for (int base = pages.own.lo; base < pages.own.hi; base += PG_TILE) {
+        uint32_t v[PG_VOTES];
+        int n = pages.n;
+        if (base == pages.own.lo) {
+            #pragma unroll
+            for (int j = 0; j < PG_VOTES; j++) v[j] = pages.votes[j];
+        } else n = vote(base, pages.own.hi, v, free);
+        int at = rank + warp_scan(n, part, total);             // free pages before this warp's
+        const int lane = threadIdx.x & 31, first = base + (int)(threadIdx.x >> 5) * (32 * PG_VOTES) + lane;
+        #pragma unroll
+        for (int j = 0; j < PG_VOTES; j++) {
+            const int q = first + 32 * j, frees = at + __popc(v[j] & ((1u << lane) - 1u));
+            if (q < pages.own.hi) {
+                const bool is_free = v[j] >> lane & 1u;
+                if (!is_free && q >= live) a.from[q - frees - (live - moves)] = q;     // pages in use before q, less those before L
+                else a.moved[q] = is_free ? -1 : q;
+                if (is_free && q < live) a.to[frees] = q;
+            }
+            at += __popc(v[j]);
+        }
+        rank += total;
+    }
+    if (rank_of_block() == 0 && threadIdx.x == 0) *a.count = moves;
+    sync_all();
+    for (int i = rank_of_block() * PG_THREADS + threadIdx.x; i < moves; i += (int)gridDim.z * PG_THREADS) a.moved[a.from[i]] = a.to[i];
 }
 
-// The table and the counts of the pool after the moves.
-__global__ void __launch_bounds__(256)
-pages_rename_kernel(const CompactArgs a)
+// The table and the counts of the pool after the moves, by `blocks` blocks of 256 threads.
+__device__ __forceinline__ void rename(const CompactArgs& a, int block, int blocks)
 {
-    pdl_wait();
-    pdl_trigger();
     const PoolArgs& p = a.p;
-    const int lane = threadIdx.x & 31, warps = gridDim.x * 8, warp = blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31, warps = blocks * 8, warp = block * 8 + (threadIdx.x >> 5);
     for (int b = warp; b < p.num_seqs; b += warps) {
         const int held = pages_of(p, keys_of(p, b, SITE_COMPACT));
+        #pragma unroll 4
         for (int e = lane; e < held; e += 32) {
             const long long at = (long long)b * p.max_pages + e;
             const int page = p.pages[at], to = (unsigned)page < (unsigned)p.num_pages ? a.moved[page] : -1;
@@ -365,81 +526,57 @@ pages_rename_kernel(const CompactArgs a)
         }
     }
     // A place before L that was free is written by the page that moves there, every other by itself.
-    const int moves = *a.count;
+    const int moves = *a.count, last = moves ? a.to[moves - 1] : -1;
     for (int q = warp * 32 + lane; q < p.num_pages; q += warps * 32) {
         const int to = a.moved[q], n = p.refs[q];
         if (to == q) a.refs_out[q] = n;
         else if (to >= 0) { a.refs_out[to] = n; a.refs_out[q] = 0; }
-        else if (moves == 0 || q > a.to[moves - 1]) a.refs_out[q] = 0;      // behind the last free place that is filled
+        else if (q > last) a.refs_out[q] = 0;                  // behind the last free place that is filled
     }
 }
 
+// RENAME: first the table and the counts, by the grid's first `renamers` blocks, which take part in the moves last.
+template <bool RENAME>
 __global__ void __launch_bounds__(PG_MOVE_THREADS)
-pages_move_kernel(const MoveArgs a, int segments /* of a page's k */, int exp_segments)
+pages_move_kernel(const MoveArgs a, const CompactArgs names, int renamers)
 {
     pdl_wait();
     pdl_trigger();
-    const int n = a.count ? min(*a.count, a.n) : a.n;
-    const int per_page = 2 * (segments + exp_segments);
-    for (long long item = blockIdx.x; item < (long long)n * per_page; item += gridDim.x) {
-        const int i = (int)(item / per_page);
-        int s = (int)(item % per_page);
-        const int src = a.src[i], dst = a.dst[i];
-        if ((unsigned)src >= (unsigned)a.num_pages || (unsigned)dst >= (unsigned)a.num_pages) {
-            if (threadIdx.x == 0 && s == 0) report(a.status, KS_BAD_PAGE, i, a.site);
-            continue;
-        }
-        const bool exps = s >= 2 * segments;
-        if (exps) s -= 2 * segments;
-        const int per = exps ? exp_segments : segments, what = (exps ? 2 : 0) + s / per;
-        s %= per;
-        long long at, bytes;
-        if (a.keys) {                                          // a head's first keys
-            at = (long long)s * a.head_bytes[what];
-            bytes = (long long)a.keys[i] * a.key_bytes[what];
-        } else {
-            const long long all = (long long)a.heads * a.head_bytes[what];
-            at = (long long)s * PG_SEGMENT;
-            bytes = min((long long)PG_SEGMENT, all - at);
-        }
-        const uint8_t* const from = a.part[what] + src * a.stride[what] + at;
-        uint8_t* const to = a.part[what] + dst * a.stride[what] + at;
-        const int chunks = (int)(bytes / 16);
-        int c = threadIdx.x;
-        for (; c + 7 * PG_MOVE_THREADS < chunks; c += 8 * PG_MOVE_THREADS) {
-            uint4 v[8];
-            #pragma unroll
-            for (int j = 0; j < 8; j++) v[j] = reinterpret_cast<const uint4*>(from)[c + j * PG_MOVE_THREADS];
-            #pragma unroll
-            for (int j = 0; j < 8; j++) reinterpret_cast<uint4*>(to)[c + j * PG_MOVE_THREADS] = v[j];
-        }
-        for (; c < chunks; c += PG_MOVE_THREADS) reinterpret_cast<uint4*>(to)[c] = reinterpret_cast<const uint4*>(from)[c];
-        for (long long b = (long long)chunks * 16 + threadIdx.x; b < bytes; b += PG_MOVE_THREADS) to[b] = from[b];
-    }
+    if (RENAME && (int)blockIdx.x < renamers) rename(names, blockIdx.x, renamers);
+    move(a, a.count ? min(*a.count, a.n) : a.n, RENAME ? ((int)blockIdx.x + (int)gridDim.x - renamers) % (int)gridDim.x : blockIdx.x, gridDim.x);
 }
 
-int launch_moves(const efa_paged_cache& c, const int* src, const int* dst, const int* keys, const int* count, int n, int site, int* status, cudaStream_t stream)
+MoveArgs move_args(const efa_paged_cache& c, const int* src, const int* dst, const int* keys, const int* count, int n, int site, int* status)
 {
     MoveArgs a{};
     const int elem = c.dtype == EFA_F16 ? 2 : 1;
     const long long dense = (long long)c.H_kv * c.page_size * c.d_h;
     a.part[0] = static_cast<uint8_t*>(c.k); a.part[1] = static_cast<uint8_t*>(c.v);
-    a.part[2] = c.k_exp; a.part[3] = c.v_exp;
-    for (int i = 0; i < 4; i++) {
-        a.key_bytes[i] = i < 2 ? c.d_h * elem : 1;
-        a.head_bytes[i] = a.key_bytes[i] * c.page_size;
-        a.stride[i] = i < 2 ? (c.page_stride ? c.page_stride : dense) * elem : (long long)c.H_kv * c.page_size;
-    }
+    if (c.dtype == EFA_E4M3) { a.exps[0] = c.k_exp; a.exps[1] = c.v_exp; }
+    a.stride = (c.page_stride ? c.page_stride : dense) * elem;
+    a.key_bytes = c.d_h * elem;
+    a.head_bytes = a.key_bytes * c.page_size;
+    a.page_size = c.page_size;
     a.heads = c.H_kv; a.num_pages = c.num_pages;
     a.src = src; a.dst = dst; a.keys = keys; a.count = count;
     a.n = n; a.site = site; a.status = status;
-    const auto pieces = [&](int i) { return keys ? c.H_kv : (int)(((long long)c.H_kv * a.head_bytes[i] + PG_SEGMENT - 1) / PG_SEGMENT); };
-    const int segments = pieces(0), exp_segments = c.dtype == EFA_E4M3 ? pieces(2) : 0;
-    const long long items = (long long)n * 2 * (segments + exp_segments);
-    const unsigned blocks = (unsigned)std::min<long long>(items, 8ll * device_sms());
-    EFA_CUDA(launch_value(pages_move_kernel, dim3(blocks), PG_MOVE_THREADS, 0, stream, a, segments, exp_segments));
+    a.segments = keys ? c.H_kv : (int)(((long long)c.H_kv * a.head_bytes + PG_SEGMENT - 1) / PG_SEGMENT);
+    return a;
+}
+
+int launch_moves(const MoveArgs& a, const CompactArgs* names, cudaStream_t stream)
+{
+    const long long items = (long long)a.n * 2 * a.segments, most = 8ll * device_sms();
+    if (names) {
+        const int work = std::max(names->p.num_seqs, (names->p.num_pages + 31) / 32), renamers = std::min((work + 7) / 8, device_sms());
+        const unsigned blocks = (unsigned)std::max<long long>(renamers, std::min(items, most));
+        EFA_CUDA(launch_value(pages_move_kernel<true>, dim3(blocks), PG_MOVE_THREADS, 0, stream, a, *names, renamers));
+    } else EFA_CUDA(launch_value(pages_move_kernel<false>, dim3((unsigned)std::min(items, most)), PG_MOVE_THREADS, 0, stream, a, CompactArgs{}, 0));
     return 0;
 }
+
+// Blocks of a launch that looks at all pages and at n slots: one while that is little, as eight wait for one another.
+int blocks_of(const efa_page_pool& p, int n) { return p.num_pages > PG_TILE || n > PG_WARPS ? PG_CLUSTER : 1; }
 
 PoolArgs device_pool(const efa_page_pool& p) { return PoolArgs{p.refs, p.pages, p.kv_len, p.num_pages, p.page_size, p.num_seqs, p.max_pages, kernel_status_word()}; }
 
@@ -486,8 +623,10 @@ int pages_take(const efa_page_pool& p, const int* q_start, void* workspace, size
     if (int rc = check_workspace("pages_take", p, workspace, workspace_bytes)) return rc;
     const void* const mem[] = {p.refs, p.pages, p.kv_len, q_start, workspace};
     if (int rc = check_memory("pages_take", mem, 5)) return rc;
-    const TakeArgs a{device_pool(p), q_start, static_cast<int*>(workspace)};
-    EFA_CUDA(launch_value(pages_take_kernel, dim3(1, 1, PG_CLUSTER), PG_THREADS, 0, stream, a));
+    int* const list = static_cast<int*>(workspace);
+    int* const slots = list + words(p.num_pages + 2);
+    const TakeArgs a{device_pool(p), q_start, list, slots, slots + words(p.num_seqs), slots + 2 * words(p.num_seqs)};
+    EFA_CUDA(launch_value(pages_take_kernel, dim3(1, 1, blocks_of(p, p.num_seqs)), PG_THREADS, 0, stream, a));
     return 0;
 }
 
@@ -506,8 +645,8 @@ int pages_fork(const efa_page_pool& p, const efa_paged_cache& c, const int* pare
     a.list = at; at += words(p.num_pages + 2);
     for (int** q : {&a.claim, &a.keys, &a.rank, &a.src, &a.dst, &a.rest}) { *q = at; at += words(p.num_seqs); }
     a.count = at;
-    EFA_CUDA(launch_value(pages_fork_kernel, dim3(1, 1, PG_CLUSTER), PG_THREADS, 0, stream, a));
-    return launch_moves(c, a.src, a.dst, a.rest, a.count, n, SITE_FORK, a.p.status, stream);
+    EFA_CUDA(launch_value(pages_fork_kernel, dim3(1, 1, blocks_of(p, n)), PG_THREADS, 0, stream, a));
+    return launch_moves(move_args(c, a.src, a.dst, a.rest, a.count, n, SITE_FORK, a.p.status), nullptr, stream);
 }
 
 int pages_free(const efa_page_pool& p, const int* seqs, int n, cudaStream_t stream)
@@ -518,7 +657,7 @@ int pages_free(const efa_page_pool& p, const int* seqs, int n, cudaStream_t stre
     if (!seqs) { set_error("pages_free: seqs is null"); return 2; }
     const void* const mem[] = {p.refs, p.pages, p.kv_len, seqs};
     if (int rc = check_memory("pages_free", mem, 4)) return rc;
-    EFA_CUDA(launch_value(pages_free_kernel, dim3((n + 7) / 8), 256, 0, stream, device_pool(p), seqs, n));
+    EFA_CUDA(launch_value(pages_free_kernel, dim3(n), PG_FREE_THREADS, 0, stream, device_pool(p), seqs));
     return 0;
 }
 
@@ -533,10 +672,8 @@ int pages_compact(const efa_page_pool& p, const efa_paged_cache& c, int* pages_o
     const int half = p.num_pages / 2 + 1;                      // no more pages can move than there are free ones before L
     int* const at = static_cast<int*>(workspace);
     const CompactArgs a{device_pool(p), pages_out, refs_out, moved, at, at + half, at + words(p.num_pages + 2)};
-    EFA_CUDA(launch_value(pages_compact_kernel, dim3(1, 1, PG_CLUSTER), PG_THREADS, 0, stream, a));
-    const int work = std::max(p.num_seqs, (p.num_pages + 31) / 32);
-    EFA_CUDA(launch_value(pages_rename_kernel, dim3(std::min((work + 7) / 8, 2 * device_sms())), 256, 0, stream, a));
-    return launch_moves(c, a.from, a.to, nullptr, a.count, half, SITE_COMPACT, a.p.status, stream);
+    EFA_CUDA(launch_value(pages_compact_kernel, dim3(1, 1, blocks_of(p, 0)), PG_THREADS, 0, stream, a));
+    return launch_moves(move_args(c, a.from, a.to, nullptr, a.count, half, SITE_COMPACT, a.p.status), &a, stream);
 }
 
 int pages_copy(const efa_paged_cache& c, const int* src, const int* dst, int n, cudaStream_t stream)
@@ -547,7 +684,7 @@ int pages_copy(const efa_paged_cache& c, const int* src, const int* dst, int n, 
     if (!src || !dst) { set_error("pages_copy: src or dst is null"); return 2; }
     const void* const mem[] = {c.k, src, dst};
     if (int rc = check_memory("pages_copy", mem, 3)) return rc;
-    return launch_moves(c, src, dst, nullptr, nullptr, n, SITE_COPY, kernel_status_word(), stream);
+    return launch_moves(move_args(c, src, dst, nullptr, nullptr, n, SITE_COPY, kernel_status_word()), nullptr, stream);
 }
 
 }  // namespace efa
