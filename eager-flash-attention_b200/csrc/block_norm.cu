@@ -253,97 +253,91 @@ block_norm_kernel(const NormArgs a)
     constexpr int PER_BLOCK = T <= 32 ? 128 / T : 1;
     pdl_wait();
     pdl_trigger();
-    const int lane = threadIdx.x % T, first = blockIdx.x * PER_BLOCK + (T <= 32 ? threadIdx.x / T : 0), step = gridDim.x * PER_BLOCK;
-    int slot = 0;
+    const int lane = threadIdx.x % T, at = blockIdx.x * PER_BLOCK + (T <= 32 ? threadIdx.x / T : 0);
     constexpr int H = MODE == SINGLE ? 8 : 4, W = MODE == SINGLE || WIDE ? 8 : 4;   // words of eight fp16, and of what may be fp32
     const bool x_f32 = WIDE && a.x_f32, y_f32 = WIDE && a.y_f32;
-    // The lanes of a warp go round together: rows behind the last are the last, without a store.
-    const int rounds = (a.rows - blockIdx.x * PER_BLOCK + step - 1) / step;
-    for (int i = 0, at = first; i < rounds; i++, at += step) {
-        const bool there = T > 32 || at < a.rows;
-        const long long row = T > 32 ? at : min(at, a.rows - 1);
-        const char* const xr = static_cast<const char*>(a.x) + row * a.x_stride * (x_f32 ? 4 : 2);
-        const char* const yr = static_cast<const char*>(a.y) + row * a.y_stride * (y_f32 ? 4 : 2);
-        const __half* const gr = a.gate + row * a.gate_stride;
-        constexpr int ENDS = Share<T, MODE>::ENDS;
-        const Share<T, MODE> p(lane, a.d, (unsigned)row * (unsigned)a.x_stride & 7u);
-        float2 v[NC][4];
-        float ends[2] = {0.f, 0.f}, x_ends[2], g_ends[2];
-        Raw<W> x[LAZY ? 1 : NC];
-        Raw<H> g[LAZY ? 1 : NC];
-        {
-            Raw<W> y[NC];
-            #pragma unroll
-            for (int c = 0; c < NC; c++) {
-                if (a.y) load8(y[c], yr, y_f32, p, c);
-                if constexpr (!LAZY) {
-                    if (a.x) load8(x[c], xr, x_f32, p, c);
-                    if (a.gate) a.gate_stride ? load8(g[c], gr, false, p, c) : load8<true>(g[c], gr, false, p, c);
-                }
-            }
-            #pragma unroll
-            for (int k = 0; k < ENDS; k++)
-                if (p.end(k) < a.d) {
-                    if (a.y) ends[k] = element(yr, y_f32, p.end(k));
-                    if (a.x) x_ends[k] = element(xr, x_f32, p.end(k));
-                    if (a.gate) g_ends[k] = __half2float(gr[p.end(k)]);
-                }
-            #pragma unroll
-            for (int c = 0; c < NC; c++) numbers<MODE>(y[c], y_f32, v[c]);
-        }
-        if (a.post) normalise(v, ends, a, p, a.post_w, a.post_b, part, slot);
-        auto gated = [&](float n, float gate) { return a.sigmoid ? __fdividef(n, 1.f + __expf(-gate)) : n * gate; };
-        auto summed = [&](float n, float residual) { return a.y ? fmaf(a.residual_scale, residual, a.block_scale * n) : a.residual_scale * residual; };
-        char* const out = static_cast<char*>(a.x_out) + row * a.out_stride * (x_f32 ? 4 : 2);
+    int slot = 0;
+    // The lanes of a warp go together: rows behind the last are the last, without a store.
+    const bool there = T > 32 || at < a.rows;
+    const long long row = T > 32 ? at : min(at, a.rows - 1);
+    const char* const xr = static_cast<const char*>(a.x) + row * a.x_stride * (x_f32 ? 4 : 2);
+    const char* const yr = static_cast<const char*>(a.y) + row * a.y_stride * (y_f32 ? 4 : 2);
+    const __half* const gr = a.gate + row * a.gate_stride;
+    constexpr int ENDS = Share<T, MODE>::ENDS;
+    const Share<T, MODE> p(lane, a.d, (unsigned)row * (unsigned)a.x_stride & 7u);
+    float2 v[NC][4];
+    float ends[2] = {0.f, 0.f}, x_ends[2], g_ends[2];
+    Raw<W> x[LAZY ? 1 : NC];
+    Raw<H> g[LAZY ? 1 : NC];
+    {
+        Raw<W> y[NC];
         #pragma unroll
         for (int c = 0; c < NC; c++) {
-            float2 n[4];
-            if constexpr (LAZY) {
-                if (a.x) load8(x[0], xr, x_f32, p, c);
-                if (a.gate) a.gate_stride ? load8(g[0], gr, false, p, c) : load8<true>(g[0], gr, false, p, c);
+            if (a.y) load8(y[c], yr, y_f32, p, c);
+            if constexpr (!LAZY) {
+                if (a.x) load8(x[c], xr, x_f32, p, c);
+                if (a.gate) a.gate_stride ? load8(g[c], gr, false, p, c) : load8<true>(g[c], gr, false, p, c);
             }
-            if (a.gate) {
-                numbers<MODE>(g[LAZY ? 0 : c], false, n);
-                #pragma unroll
-                for (int i = 0; i < 4; i++) v[c][i] = a.sigmoid ? make_float2(gated(v[c][i].x, n[i].x), gated(v[c][i].y, n[i].y)) : mul2(v[c][i], n[i]);
-            }
-            if (a.x) {
-                numbers<MODE>(x[LAZY ? 0 : c], x_f32, n);
-                #pragma unroll
-                for (int i = 0; i < 4; i++) v[c][i] = a.y ? fma2(two(a.residual_scale), n[i], mul2(two(a.block_scale), v[c][i])) : mul2(two(a.residual_scale), n[i]);
-            } else {
-                #pragma unroll
-                for (int i = 0; i < 4; i++) v[c][i] = mul2(v[c][i], two(a.block_scale));
-            }
-            if (a.x_out && there) store8(out, x_f32, p, c, v[c]);
         }
         #pragma unroll
-        for (int k = 0; k < ENDS; k++) {
-            if (p.end(k) >= a.d) continue;
-            if (a.gate) ends[k] = gated(ends[k], g_ends[k]);
-            ends[k] = a.x ? summed(ends[k], x_ends[k]) : a.block_scale * ends[k];
-            if (a.x_out && there) store1(out, x_f32, p.end(k), ends[k]);
+        for (int k = 0; k < ENDS; k++)
+            if (p.end(k) < a.d) {
+                if (a.y) ends[k] = element(yr, y_f32, p.end(k));
+                if (a.x) x_ends[k] = element(xr, x_f32, p.end(k));
+                if (a.gate) g_ends[k] = __half2float(gr[p.end(k)]);
+            }
+        #pragma unroll
+        for (int c = 0; c < NC; c++) numbers<MODE>(y[c], y_f32, v[c]);
+    }
+    if (a.post) normalise(v, ends, a, p, a.post_w, a.post_b, part, slot);
+    auto gated = [&](float n, float gate) { return a.sigmoid ? __fdividef(n, 1.f + __expf(-gate)) : n * gate; };
+    auto summed = [&](float n, float residual) { return a.y ? fmaf(a.residual_scale, residual, a.block_scale * n) : a.residual_scale * residual; };
+    char* const out = static_cast<char*>(a.x_out) + row * a.out_stride * (x_f32 ? 4 : 2);
+    #pragma unroll
+    for (int c = 0; c < NC; c++) {
+        float2 n[4];
+        if constexpr (LAZY) {
+            if (a.x) load8(x[0], xr, x_f32, p, c);
+            if (a.gate) a.gate_stride ? load8(g[0], gr, false, p, c) : load8<true>(g[0], gr, false, p, c);
         }
-        if (a.pre) {
-            normalise(v, ends, a, p, a.pre_w, a.pre_b, part, slot);
+        if (a.gate) {
+            numbers<MODE>(g[LAZY ? 0 : c], false, n);
             #pragma unroll
-            for (int c = 0; c < NC; c++)
-                if (there) store8(a.h + row * a.h_stride, false, p, c, v[c]);
-            #pragma unroll
-            for (int k = 0; k < ENDS; k++)
-                if (there && p.end(k) < a.d) store1(a.h + row * a.h_stride, false, p.end(k), ends[k]);
+            for (int i = 0; i < 4; i++) v[c][i] = a.sigmoid ? make_float2(gated(v[c][i].x, n[i].x), gated(v[c][i].y, n[i].y)) : mul2(v[c][i], n[i]);
         }
+        if (a.x) {
+            numbers<MODE>(x[LAZY ? 0 : c], x_f32, n);
+            #pragma unroll
+            for (int i = 0; i < 4; i++) v[c][i] = a.y ? fma2(two(a.residual_scale), n[i], mul2(two(a.block_scale), v[c][i])) : mul2(two(a.residual_scale), n[i]);
+        } else {
+            #pragma unroll
+            for (int i = 0; i < 4; i++) v[c][i] = mul2(v[c][i], two(a.block_scale));
+        }
+        if (a.x_out && there) store8(out, x_f32, p, c, v[c]);
+    }
+    #pragma unroll
+    for (int k = 0; k < ENDS; k++) {
+        if (p.end(k) >= a.d) continue;
+        if (a.gate) ends[k] = gated(ends[k], g_ends[k]);
+        ends[k] = a.x ? summed(ends[k], x_ends[k]) : a.block_scale * ends[k];
+        if (a.x_out && there) store1(out, x_f32, p.end(k), ends[k]);
+    }
+    if (a.pre) {
+        normalise(v, ends, a, p, a.pre_w, a.pre_b, part, slot);
+        #pragma unroll
+        for (int c = 0; c < NC; c++)
+            if (there) store8(a.h + row * a.h_stride, false, p, c, v[c]);
+        #pragma unroll
+        for (int k = 0; k < ENDS; k++)
+            if (there && p.end(k) < a.d) store1(a.h + row * a.h_stride, false, p.end(k), ends[k]);
     }
 }
 
 template <int T, int NC, bool LAZY = false>
 int launch_norm(const NormArgs& a, int mode, cudaStream_t stream)
 {
-    constexpr int PER_BLOCK = T <= 32 ? 128 / T : 1, AT_ONCE = 1024 / (T <= 32 ? 128 : T);     // about as many blocks as an SM holds
-    const long long blocks = ((long long)a.rows + PER_BLOCK - 1) / PER_BLOCK, most = (long long)device_sms() * AT_ONCE;
-    // Many rows: as many blocks as there is room for, with equal numbers of rows. Few: a block to each, which the hardware spreads better.
-    const long long rounds = blocks >= 4 * most ? (blocks + most - 1) / most : 1;
-    const dim3 grid((unsigned)((blocks + rounds - 1) / rounds));
+    constexpr int PER_BLOCK = T <= 32 ? 128 / T : 1;
+    const dim3 grid((unsigned)(((long long)a.rows + PER_BLOCK - 1) / PER_BLOCK));
     const bool wide = a.x_f32 || a.y_f32;
     const auto kernel = mode == ALIGNED ? (wide ? block_norm_kernel<T, NC, ALIGNED, true, LAZY> : block_norm_kernel<T, NC, ALIGNED, false, LAZY>)
                       : mode == SHIFTED ? (wide ? block_norm_kernel<T, NC, SHIFTED, true, LAZY> : block_norm_kernel<T, NC, SHIFTED, false, LAZY>)
