@@ -256,33 +256,18 @@ proj_w4_kernel(const W4Args a, int stages, const __grid_constant__ CUtensorMap c
             #pragma unroll
             for (int i = 0; i < 4; i++) sum[warp * TILE + (8 * n + 2 * t + (i & 1)) * CHANNELS + 16 * m + 8 * (i >> 1) + row] = acc[m][n][i];
     __syncthreads();
-    const int wanted = rows * CHANNELS;
+    for (int e = threadIdx.x; e < rows * CHANNELS; e += blockDim.x) {
+        float v = sum[e];
+        #pragma unroll
+        for (int w = 1; w < warps; w++) v += sum[w * TILE + e];
+        if (parts > 1) sum[e] = v;
+        else store_sum(a, v, m0 + e / CHANNELS, n0 + e % CHANNELS);
+    }
     if (parts > 1) {
-        for (int e = threadIdx.x; e < wanted; e += blockDim.x) {
-            float v = sum[e];
-            for (int w = 1; w < warps; w++) v += sum[w * TILE + e];
-            sum[e] = v;
-        }
         cluster_sync();
+        store_sums(a, sum, rows, CHANNELS, parts, part, m0, n0);
+        cluster_sync();                                        // the others may still read this block's sums
     }
-    for (int e = part * (int)blockDim.x + threadIdx.x; e < wanted; e += parts * blockDim.x) {
-        float v = 0.f;
-        if (parts > 1) {
-            for (int q = 0; q < parts; q++) {
-                float y;
-                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(y) : "r"(cluster_addr(sum + e, q)));
-                v += y;
-            }
-        } else {
-            for (int w = 0; w < warps; w++) v += sum[w * TILE + e];
-        }
-        const int m = m0 + e / CHANNELS, n = n0 + e % CHANNELS;
-        if (n < a.d_out) {
-            if (a.out_f32) static_cast<float*>(a.out)[m * a.out_stride + n] = v;
-            else static_cast<__half*>(a.out)[m * a.out_stride + n] = __float2half_rn(v);
-        }
-    }
-    if (parts > 1) cluster_sync();                             // the others may still read this block's sums
 }
 
 template <int G, int NT>
@@ -350,7 +335,7 @@ int project_w4(const void* X, long long x_stride, const efa_w4& w, void* out, in
     if (int rc = check_memory("project_w4", mem, 5)) return rc;
     const W4Args a{w.codes, static_cast<const __half*>(w.scales), w.zeros, static_cast<const __half*>(X), out, rows, w.d_in, w.d_out,
                    w.code_stride ? w.code_stride : w.d_in / 2, w.scale_stride ? w.scale_stride : w.d_out, w.zero_stride ? w.zero_stride : w.d_out,
-                   x_stride ? x_stride : w.d_in, out_stride ? out_stride : w.d_out, out_dtype == EFA_F32, kernel_status_word()};
+                   x_stride ? x_stride : w.d_in, out_stride ? out_stride : w.d_out, out_dtype == EFA_F32, aligned16(out) && (out_stride ? out_stride : w.d_out) % 4 == 0, kernel_status_word()};
     // Up to eight rows the products of mma.sync are not the time. Beyond, tiles of 16 rows that read the weights again, or tcgen05 with up to 64 rows to a tile, whose start and
     // end cost more: by the work, in weights times tiles of 16. us, tiles of 16 / tcgen05: 16 rows, 4096 x 4096 6.8 / 8.8, 4096 x 6144 13.2 / 10.7, 8192 x 32768 55 / 39;
     // 32 rows, 2048 x 4096 7.9 / 8.2, 8192 x 1024 6.9 / 9.8, 4096 x 4096 9.8 / 10.1; 64 rows, 1024 x 1024 3.4 / 7.3, 1056 x 4163 15 / 12.4, 4096 x 4096 18 / 12.

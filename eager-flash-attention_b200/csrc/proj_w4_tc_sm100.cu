@@ -74,7 +74,23 @@ proj_w4_tc_kernel(const W4Args a, int tile_channels, bool x_blocks, const __grid
     const int units = (a.d_in + W4_UNIT - 1) / W4_UNIT, u0 = (int)((long long)units * part / parts), u1 = (int)((long long)units * (part + 1) / parts);
     const int steps = (u1 - u0) * C::STEPS;
     uint8_t* const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-    if (threadIdx.x == 0) {
+    // Copies of unit u0 + i's codes, and of the X of a unit that begins a copy of it.
+    auto copy_codes = [&](unsigned i) {
+        const unsigned slot = i % C::STAGES;
+        mbar_expect_tx(&full[slot], 2 * tile_channels * 64);
+        tma_load_2d(smem + slot * C::SLOT, &codes_map, &full[slot], (u0 + (int)i) * (W4_UNIT / 2), n0);
+    };
+    auto copy_x = [&](unsigned xi) {
+        const unsigned slot = xi % C::X_STAGES;
+        const int first = 2 * (u0 + (int)xi * C::X_UNITS);     // of the blocks of 64 k
+        uint8_t* const to = smem + C::STAGES * C::SLOT + slot * C::X_SLOT;
+        mbar_expect_tx(&x_full[slot], C::X_SLOT);
+        if (x_blocks) tma_load_3d(to, &x_map, &x_full[slot], 0, m0, first);
+        else
+            for (int j = 0; j < C::X_BLOCKS; j++) tma_load_2d(to + j * C::X_BLOCK, &x_map, &x_full[slot], (first + j) * 64, m0);
+    };
+    const unsigned my_units = (unsigned)(u1 - u0);
+    if (warp == TC_COPY && lane == 0) {
         for (int i = 0; i < C::STAGES; i++) { mbar_init(&full[i], 1); mbar_init(&empty[i], 8); }
         for (int i = 0; i < C::X_STAGES; i++) { mbar_init(&x_full[i], 1); mbar_init(&x_empty[i], 8); }
         for (int i = 0; i < 4; i++) { mbar_init(&a_full[i >> 1][i & 1], 4); mbar_init(&d_full[i >> 1][i & 1], 1); mbar_init(&d_empty[i >> 1][i & 1], 4); }
@@ -83,7 +99,7 @@ proj_w4_tc_kernel(const W4Args a, int tile_channels, bool x_blocks, const __grid
         tma_prefetch_desc(&codes_map);
         tma_prefetch_desc(&x_map);
     }
-    if (warp == TC_COPY) tmem_alloc(&tmem_at, 512);
+    if (warp == TC_COPY + 1) tmem_alloc(&tmem_at, 512);
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
@@ -100,20 +116,14 @@ proj_w4_tc_kernel(const W4Args a, int tile_channels, bool x_blocks, const __grid
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(TC_REGS_REST));
         if (warp == TC_COPY) {
             if (lane == 0) {
-                for (unsigned i = 0; i < (unsigned)(u1 - u0); i++) {
+                for (unsigned i = 0; i < my_units; i++) {
                     if (i % C::X_UNITS == 0) {
-                        const unsigned xi = i / C::X_UNITS, slot = xi % C::X_STAGES, block = 2 * (u0 + i);
-                        if (!mbar_wait(&x_empty[slot], (uint32_t)(xi / C::X_STAGES & 1) ^ 1u, &abort_word, 71)) break;
-                        uint8_t* const to = smem + C::STAGES * C::SLOT + slot * C::X_SLOT;
-                        mbar_expect_tx(&x_full[slot], C::X_SLOT);
-                        if (x_blocks) tma_load_3d(to, &x_map, &x_full[slot], 0, m0, block);
-                        else
-                            for (int j = 0; j < C::X_BLOCKS; j++) tma_load_2d(to + j * C::X_BLOCK, &x_map, &x_full[slot], (block + j) * 64, m0);
+                        const unsigned xi = i / C::X_UNITS;
+                        if (!mbar_wait(&x_empty[xi % C::X_STAGES], (xi / C::X_STAGES & 1) ^ 1u, &abort_word, 71)) break;
+                        copy_x(xi);
                     }
-                    const unsigned slot = i % C::STAGES;
-                    if (!mbar_wait(&empty[slot], (uint32_t)(i / C::STAGES & 1) ^ 1u, &abort_word, 72)) break;
-                    mbar_expect_tx(&full[slot], 2 * tile_channels * 64);
-                    tma_load_2d(smem + slot * C::SLOT, &codes_map, &full[slot], (u0 + i) * (W4_UNIT / 2), n0);
+                    if (!mbar_wait(&empty[i % C::STAGES], (i / C::STAGES & 1) ^ 1u, &abort_word, 72)) break;
+                    copy_codes(i);
                 }
             }
         } else if (warp <= TC_COPY + 2) {
@@ -151,8 +161,8 @@ proj_w4_tc_kernel(const W4Args a, int tile_channels, bool x_blocks, const __grid
         float2 acc[N / 2];
         #pragma unroll
         for (int i = 0; i < N / 2; i++) acc[i] = make_float2(0.f, 0.f);
-        for (int i = 0; i < W4_AHEAD && group0 + i < groups; i++) prefetch_l2(scales + (group0 + i) * a.scale_stride);
         __half next[C::GROUPS] = {};
+        for (int i = 0; i < W4_AHEAD && group0 + i < groups; i++) prefetch_l2(scales + (group0 + i) * a.scale_stride);
         const __half* at = scales + group0 * a.scale_stride;
         int left = groups - group0;                            // groups from there on: a step may end behind the last
         auto ask = [&]() {
@@ -264,24 +274,13 @@ proj_w4_tc_kernel(const W4Args a, int tile_channels, bool x_blocks, const __grid
         }
     }
     __syncthreads();
-    if (warp == TC_COPY) { tc_fence_after_sync(); tmem_dealloc(tmem_at, 512); }
-    if (parts > 1) cluster_sync();
-    for (int e = part * (int)blockDim.x + threadIdx.x; e < rows * block; e += parts * blockDim.x) {
-        float v = 0.f;
-        if (parts > 1) {
-            for (int q = 0; q < parts; q++) {
-                float y;
-                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(y) : "r"(cluster_addr(sum + e, q)));
-                v += y;
-            }
-        } else v = sum[e];
-        const int m = m0 + e / block, n = n0 + e % block;
-        if (n < a.d_out) {
-            if (a.out_f32) static_cast<float*>(a.out)[m * a.out_stride + n] = v;
-            else static_cast<__half*>(a.out)[m * a.out_stride + n] = __float2half_rn(v);
-        }
-    }
-    if (parts > 1) cluster_sync();                             // the others may still read this block's sums
+    if (warp == TC_COPY + 1) { tc_fence_after_sync(); tmem_dealloc(tmem_at, 512); }
+    if (parts > 1) {
+        cluster_sync();
+        store_sums(a, sum, rows, block, parts, part, m0, n0);
+        cluster_sync();                                        // the others may still read this block's sums
+    } else
+        for (int e = 4 * threadIdx.x; e < rows * block; e += 4 * TC_THREADS) store_sum4(a, *reinterpret_cast<const float4*>(sum + e), m0 + e / block, n0 + e % block);
 }
 
 // Clusters of p blocks that the device holds at a time: blocks that have an SM each must find them in one part of the GPU. Asked once.
