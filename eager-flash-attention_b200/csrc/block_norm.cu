@@ -372,9 +372,13 @@ int block_norm(const void* x, const void* y, const void* gate, const void* post_
     if ((p.gate != EFA_GATE_NONE) != (gate != nullptr)) { set_error("block_norm: a gate's values come with its kind, and without one there are none"); return 2; }
     if (!x_out && !h) { set_error("block_norm: x_out and h are null"); return 2; }
     if (h && !p.pre) { set_error("block_norm: h is written by the pre norm only"); return 2; }
+    if (!aligned(x, p.x_dtype == EFA_F32 ? 4 : 2) || !aligned(x_out, p.x_dtype == EFA_F32 ? 4 : 2) || !aligned(y, p.y_dtype == EFA_F32 ? 4 : 2) || !aligned(h, 2) || !aligned(gate, 2) ||
+        !aligned(post_w, 2) || !aligned(post_b, 2) || !aligned(pre_w, 2) || !aligned(pre_b, 2)) {
+        set_error("block_norm: tensors must be aligned to their elements");
+        return 2;
+    }
     const void* const mem[] = {x, y, gate, post_w, post_b, pre_w, pre_b, x_out, h};
-    const void* const looked_at[] = {x, y, gate, post_w ? post_w : post_b, pre_w ? pre_w : pre_b, h ? h : x_out};
-    if (int rc = check_memory("block_norm", looked_at, 6)) return rc;
+    if (int rc = check_memory("block_norm", mem, 9)) return rc;
     const auto stride = [&](int64_t s) { return s ? (long long)s : (long long)p.d; };
     NormArgs a{x, y, static_cast<const __half*>(gate), static_cast<const __half*>(post_w), static_cast<const __half*>(post_b), static_cast<const __half*>(pre_w),
                static_cast<const __half*>(pre_b), x_out, static_cast<__half*>(h), rows, p.d, p.kind == EFA_NORM_LAYER, p.post != 0, h != nullptr, p.gate == EFA_GATE_SIGMOID,

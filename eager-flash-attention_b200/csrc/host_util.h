@@ -70,7 +70,8 @@ bool own_device_memory(const void* p);
 // of each group that belongs together: 0.08 us each, of 4 us that a call takes on the host. Null pointers are passed over.
 int check_memory(const char* what, const void* const* p, int n);
 
-inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+inline bool aligned(const void* p, unsigned bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+inline bool aligned16(const void* p) { return aligned(p, 16); }
 
 #ifdef __CUDACC__
 // A launch whose blocks may start while the kernel before it in the stream still runs, as soon as all blocks of that one have

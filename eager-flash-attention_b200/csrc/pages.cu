@@ -609,6 +609,7 @@ const char* page_pool_check(const efa_page_pool& p)
     if (p.num_seqs < 0) return "pages: negative number of slots";
     if (!p.refs) return "pages: refs must not be null";
     if (p.num_seqs > 0 && (!p.pages || !p.kv_len)) return "pages: pages and kv_len must not be null";
+    if (!aligned(p.refs, 4) || !aligned(p.pages, 4) || !aligned(p.kv_len, 4)) return "pages: arrays must be aligned to their numbers";
     if (p.num_pages > 1 << 30 || p.num_seqs > 1 << 30 || (long long)p.num_seqs * p.max_pages > INT_MAX) return "pages: sizes too large";
     return nullptr;
 }
@@ -619,7 +620,7 @@ int pages_take(const efa_page_pool& p, const int* q_start, void* workspace, size
 {
     if (const char* why = page_pool_check(p)) { set_error("pages_take: %s", why); return 2; }
     if (p.num_seqs == 0) return 0;
-    if (!q_start) { set_error("pages_take: q_start is null"); return 2; }
+    if (!q_start || !aligned(q_start, 4)) { set_error("pages_take: q_start is null or not aligned"); return 2; }
     if (int rc = check_workspace("pages_take", p, workspace, workspace_bytes)) return rc;
     const void* const mem[] = {p.refs, p.pages, p.kv_len, q_start, workspace};
     if (int rc = check_memory("pages_take", mem, 5)) return rc;
@@ -636,7 +637,7 @@ int pages_fork(const efa_page_pool& p, const efa_paged_cache& c, const int* pare
     if (const char* why = check_cache(c, &p)) { set_error("pages_fork: %s", why); return 2; }
     if (n < 0 || n > p.num_seqs) { set_error("pages_fork: n must be from 0 to the number of slots (got %d)", n); return 2; }
     if (n == 0) return 0;
-    if (!parents || !children) { set_error("pages_fork: parents or children is null"); return 2; }
+    if (!parents || !children || !aligned(parents, 4) || !aligned(children, 4)) { set_error("pages_fork: parents or children is null or not aligned"); return 2; }
     if (int rc = check_workspace("pages_fork", p, workspace, workspace_bytes)) return rc;
     const void* const mem[] = {p.refs, p.pages, p.kv_len, c.k, parents, children, workspace};
     if (int rc = check_memory("pages_fork", mem, 7)) return rc;
@@ -654,7 +655,7 @@ int pages_free(const efa_page_pool& p, const int* seqs, int n, cudaStream_t stre
     if (const char* why = page_pool_check(p)) { set_error("pages_free: %s", why); return 2; }
     if (n < 0 || n > 1 << 24) { set_error("pages_free: n must be from 0 to 2^24 (got %d)", n); return 2; }
     if (n == 0) return 0;
-    if (!seqs) { set_error("pages_free: seqs is null"); return 2; }
+    if (!seqs || !aligned(seqs, 4)) { set_error("pages_free: seqs is null or not aligned"); return 2; }
     const void* const mem[] = {p.refs, p.pages, p.kv_len, seqs};
     if (int rc = check_memory("pages_free", mem, 4)) return rc;
     EFA_CUDA(launch_value(pages_free_kernel, dim3(n), PG_FREE_THREADS, 0, stream, device_pool(p), seqs));
@@ -666,6 +667,7 @@ int pages_compact(const efa_page_pool& p, const efa_paged_cache& c, int* pages_o
     if (const char* why = page_pool_check(p)) { set_error("pages_compact: %s", why); return 2; }
     if (const char* why = check_cache(c, &p)) { set_error("pages_compact: %s", why); return 2; }
     if (!refs_out || !moved || (!pages_out && p.num_seqs > 0)) { set_error("pages_compact: pages_out, refs_out or moved is null"); return 2; }
+    if (!aligned(pages_out, 4) || !aligned(refs_out, 4) || !aligned(moved, 4)) { set_error("pages_compact: arrays must be aligned to their numbers"); return 2; }
     if (int rc = check_workspace("pages_compact", p, workspace, workspace_bytes)) return rc;
     const void* const mem[] = {p.refs, p.pages, p.kv_len, c.k, pages_out, refs_out, moved, workspace};
     if (int rc = check_memory("pages_compact", mem, 8)) return rc;
@@ -681,7 +683,7 @@ int pages_copy(const efa_paged_cache& c, const int* src, const int* dst, int n, 
     if (const char* why = check_cache(c, nullptr)) { set_error("pages_copy: %s", why); return 2; }
     if (n < 0 || n > c.num_pages) { set_error("pages_copy: n must be from 0 to the number of pages (got %d)", n); return 2; }
     if (n == 0) return 0;
-    if (!src || !dst) { set_error("pages_copy: src or dst is null"); return 2; }
+    if (!src || !dst || !aligned(src, 4) || !aligned(dst, 4)) { set_error("pages_copy: src or dst is null or not aligned"); return 2; }
     const void* const mem[] = {c.k, src, dst};
     if (int rc = check_memory("pages_copy", mem, 3)) return rc;
     return launch_moves(move_args(c, src, dst, nullptr, nullptr, n, SITE_COPY, kernel_status_word()), nullptr, stream);

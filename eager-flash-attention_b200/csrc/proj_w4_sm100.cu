@@ -314,7 +314,7 @@ const char* w4_check(const efa_w4& w)
     if (w.d_in > 1 << 24 || w.d_out > 1 << 24) return "w4: sizes too large";
     if (!w.codes || !w.scales) return "w4: codes and scales must not be null";
     if (!aligned16(w.codes)) return "w4: codes must be 16-byte aligned";
-    if ((reinterpret_cast<uintptr_t>(w.scales) & 1) != 0) return "w4: scales must be aligned to their elements";
+    if (!aligned(w.scales, 2)) return "w4: scales must be aligned to their elements";
     if (w.code_stride != 0 && (w.code_stride < w.d_in / 2 || w.code_stride % 16)) return "w4: code_stride must be 0 or a multiple of 16 that holds a row";
     if (w.scale_stride != 0 && w.scale_stride < w.d_out) return "w4: scale_stride must be 0 or at least d_out";
     if (w.zero_stride != 0 && w.zero_stride < w.d_out) return "w4: zero_stride must be 0 or at least d_out";
@@ -324,13 +324,13 @@ const char* w4_check(const efa_w4& w)
 int project_w4(const void* X, long long x_stride, const efa_w4& w, void* out, int out_dtype, long long out_stride, int rows, cudaStream_t stream)
 {
     if (const char* why = w4_check(w)) { set_error("project_w4: %s", why); return 2; }
-    if (rows < 0 || rows > 1 << 20) { set_error("project_w4: rows must be from 0 to 2^20 (got %d)", rows); return 2; }
+    if (rows < 0 || rows > 1 << 19) { set_error("project_w4: rows must be from 0 to 2^19 (got %d)", rows); return 2; }
     if (out_dtype != EFA_F16 && out_dtype != EFA_F32) { set_error("project_w4: out must be EFA_F16 or EFA_F32"); return 2; }
     if (x_stride != 0 && (x_stride < w.d_in || x_stride % 8)) { set_error("project_w4: x_stride must be 0 or a multiple of 8 that holds d_in"); return 2; }
     if (out_stride != 0 && out_stride < w.d_out) { set_error("project_w4: out_stride must be 0 or at least d_out"); return 2; }
     if (rows == 0) return 0;
     if (!X || !out) { set_error("project_w4: X or out is null"); return 2; }
-    if (!aligned16(X) || (reinterpret_cast<uintptr_t>(out) & (out_dtype == EFA_F16 ? 1 : 3)) != 0) { set_error("project_w4: X must be 16-byte aligned, out to its elements"); return 2; }
+    if (!aligned16(X) || !aligned(out, out_dtype == EFA_F16 ? 2 : 4)) { set_error("project_w4: X must be 16-byte aligned, out to its elements"); return 2; }
     const void* const mem[] = {X, w.codes, w.scales, w.zeros, out};
     if (int rc = check_memory("project_w4", mem, 5)) return rc;
     const W4Args a{w.codes, static_cast<const __half*>(w.scales), w.zeros, static_cast<const __half*>(X), out, rows, w.d_in, w.d_out,

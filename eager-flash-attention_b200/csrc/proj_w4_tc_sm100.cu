@@ -284,8 +284,8 @@ proj_w4_tc_kernel(const W4Args a, int tile_channels, bool x_blocks, const __grid
 }
 
 // Clusters of p blocks that the device holds at a time: blocks that have an SM each must find them in one part of the GPU. Asked once.
-template <class K>
-int clusters_at_once(K kernel, int p, int smem, int dev)
+template <auto kernel>
+int clusters_at_once(int p, int smem, int dev)
 {
     static int known[64][9] = {};
     if (dev < 64 && known[dev][p]) return known[dev][p];
@@ -324,7 +324,7 @@ int launch_tc(const W4Args& a, cudaStream_t stream)
     int channels = 128, parts = 1;
     double best = 1e30;
     for (int p = 1; p <= std::min(8, units); p++) {
-        const int at_once = clusters_at_once(kernel, p, C::SMEM, dev);
+        const int at_once = clusters_at_once<kernel>(p, C::SMEM, dev);
         for (int c = 128; c >= 96; c -= 16) {
             const long long clusters = (long long)((a.d_out + 2 * c - 1) / (2 * c)) * row_tiles;
             const double time = (double)((clusters + at_once - 1) / at_once) * (4.0 + 0.6 * ((units + p - 1) / p) + (p > 1 ? 1.0 : 0.0));

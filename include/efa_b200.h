@@ -226,10 +226,11 @@ int efa_paged_attention(const void* Q, void* O, const efa_paged_cache* cache, co
  * refs[p]: how many entries of sequences name page p; 0 = free. All zeros is an empty pool; refs may be raised by the caller to keep pages (a shared
  * prefix), and lowered again. Entries behind a sequence's last page are neither read nor written.
  * A page that is not full belongs to one sequence: efa_pages_fork copies it, full pages are shared. So efa_cache_write always writes into pages of one sequence.
- * Calls change the arrays in stream order; a captured graph follows their contents. What is found wrong is reported by efa_kernel_status (site 60
+ * Calls change the arrays in stream order; a captured graph follows their contents. The first call on a device comes before any stream capture. What is found wrong is reported by efa_kernel_status (site 60
  * take, 61 fork, 62 free, 63 compact, 64 copy; sequence or page in place of the block) and the call stays inside its buffers: code 2 a page outside the
  * pool (the entry counts as no page), 3 a length outside the table, 4 no free page (the entry becomes -1, whose keys efa_cache_write does not
- * write and attention reads as zeros), 5 a sequence that may not be named (outside the pool of slots, or a child that is not empty or named twice). */
+ * write and attention reads as zeros), 5 a sequence that may not be named (outside the pool of
+ * slots, where its place in the list is what is reported; or a child that is not empty or named twice). */
 typedef struct efa_page_pool {
     int* refs;              /* [num_pages] */
     int* pages;             /* [num_seqs][max_pages] */
@@ -292,7 +293,8 @@ const char* efa_block_norm_check(const efa_block_norm_params* p, int rows);
 
 /* y NULL: no block output (r = residual_scale * x: the norm before the first block; then neither post nor gate). x NULL: no residual. x_out or h NULL: not
  * wanted (not both). post_w, post_b, pre_w, pre_b: fp16 [d], NULL: ones and zeros. x_out and h may be x or y themselves where type and stride are the same.
- * Any alignment; rows, strides and d that are multiples of 8 with 16-byte aligned tensors go faster. Asynchronous on `stream`. */
+ * Tensors that begin at 16 bytes, with strides that are alike modulo 8 elements (dense ones are), go faster than others. The bits of a row do not depend on the other
+ * rows, nor, if d is a multiple of 8, on its place among them. Asynchronous on `stream`. */
 int efa_block_norm(const void* x, const void* y, const void* gate, const void* post_w, const void* post_b, const void* pre_w, const void* pre_b,
                    void* x_out, void* h, int rows, const efa_block_norm_params* p, void* stream);
 
@@ -313,7 +315,8 @@ const char* efa_w4_check(const efa_w4* w);
 /* out[rows][d_out] = X[rows][d_in] * w: efa_project_f16 for few rows, where reading the weights is all the time (the reference's project, attn_main.cu:262-273, is
  * fp32 throughout). X fp16, 16-byte aligned, x_stride (elements, 0 = dense) a multiple of 8; out fp16 (EFA_F16) or fp32 (EFA_F32), out_stride elements. Codes
  * minus zeros are fp16 numbers exactly; products and sums are fp32, the scales are applied to the sums of their groups: nothing is rounded but the result. Made
- * for up to 64 rows; more go in tiles of 64 that read the weights again. The order of the sum depends on the sizes only. Asynchronous on `stream`. */
+ * for up to 64 rows; more (2^19 at most) go in tiles that read the weights again. out does not overlap X. The order of the sum, and so the bits, depends on the sizes and
+ * the number of SMs only. Asynchronous on `stream`. The first call on a device comes before any stream capture (the status word is allocated then). */
 int efa_project_w4(const void* X, int64_t x_stride, const efa_w4* w, void* out, int out_dtype, int64_t out_stride, int rows, void* stream);
 
 /* Status word written by kernels whose bounded waits ran out, or that found lengths or pages of a paged batch wrong: out4 = {code, block, site, 0};

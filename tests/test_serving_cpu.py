@@ -48,6 +48,11 @@ def test_norm_arguments_that_are_refused(pkg):
         pkg.block_norm(AT, None, AT, AT, 1, pkg.block_norm_params(64, gate=pkg.GATE_PLAIN), gate=AT)
     with pytest.raises(pkg.EfaError, match="pre norm"):
         pkg.block_norm(AT, AT, AT, AT, 1, pkg.block_norm_params(64, pre=False))
+    for at in range(4):
+        with pytest.raises(pkg.EfaError, match="aligned"):
+            pkg.block_norm(*[AT + (i == at) for i in range(4)], 1, bp)
+    with pytest.raises(pkg.EfaError, match="aligned"):
+        pkg.block_norm(AT + 2, AT, AT, AT, 1, pkg.block_norm_params(64, x_dtype=pkg.F32))
     pkg.block_norm(AT, AT, AT, AT, 0, bp)                                   # no rows: nothing is looked at
 
 
@@ -89,7 +94,7 @@ def test_weights_that_are_refused(pkg, change, why):
 
 def test_projections_that_are_refused(pkg):
     w = _w4(pkg)
-    for args, kw, why in (((AT, w, AT, -1), {}, "rows"), ((AT, w, AT, (1 << 20) + 1), {}, "rows"), ((AT, w, AT, 1), dict(out_dtype=2), "EFA_F16 or EFA_F32"),
+    for args, kw, why in (((AT, w, AT, -1), {}, "rows"), ((AT, w, AT, (1 << 19) + 1), {}, "rows"), ((AT, w, AT, 1), dict(out_dtype=2), "EFA_F16 or EFA_F32"),
                           ((AT, w, AT, 1), dict(x_stride=248), "x_stride"), ((AT, w, AT, 1), dict(x_stride=260), "x_stride"), ((AT, w, AT, 1), dict(out_stride=47), "out_stride"),
                           ((None, w, AT, 1), {}, "null"), ((AT, w, None, 1), {}, "null"), ((AT + 8, w, AT, 1), {}, "aligned"), ((AT, w, AT + 1, 1), {}, "aligned"),
                           ((AT, w, AT + 2, 1), dict(out_dtype=0), "aligned")):
@@ -137,7 +142,7 @@ def _calls(pkg, pool, cache, ws=AT, size=1 << 20):
 
 @pytest.mark.parametrize("change,why", [
     (dict(page_size=8), "page_size"), (dict(page_size=48), "page_size"), (dict(num_pages=0), "positive"), (dict(max_pages=0), "positive"), (dict(num_seqs=-1), "negative"),
-    (dict(refs=None), "refs"), (dict(pages=None), "pages and kv_len"), (dict(kv_len=None), "pages and kv_len"), (dict(num_pages=(1 << 30) + 1), "too large"),
+    (dict(refs=None), "refs"), (dict(pages=None), "pages and kv_len"), (dict(kv_len=None), "pages and kv_len"), (dict(num_pages=(1 << 30) + 1), "too large"), (dict(refs=AT + 2), "aligned"), (dict(pages=AT + 1), "aligned"), (dict(kv_len=AT + 3), "aligned"),
     (dict(num_seqs=1 << 20, max_pages=1 << 20), "too large")])
 def test_pools_that_are_refused(pkg, change, why):
     pool = _pool(pkg, **change)
@@ -171,6 +176,10 @@ def test_page_calls_that_are_refused(pkg):
                  lambda: pkg.pages_free(pool, None, n=1), lambda: pkg.pages_copy(cache, AT, None, n=1), lambda: pkg.pages_compact(pool, cache, AT, None, AT, AT, workspace_bytes=need)):
         with pytest.raises(pkg.EfaError, match="null"):
             call()
+    for call in (lambda: pkg.pages_take(pool, AT + 2, AT, workspace_bytes=need), lambda: pkg.pages_fork(pool, cache, AT, AT + 1, AT, n=1, workspace_bytes=need),
+                 lambda: pkg.pages_free(pool, AT + 2, n=1), lambda: pkg.pages_copy(cache, AT + 1, AT, n=1), lambda: pkg.pages_compact(pool, cache, AT, AT, AT + 2, AT, workspace_bytes=need)):
+        with pytest.raises(pkg.EfaError, match="aligned"):
+            call()
     pkg.pages_fork(pool, cache, None, None, AT, n=0, workspace_bytes=need)                  # nothing to do: nothing is looked at
     pkg.pages_free(pool, None, n=0)
     pkg.pages_copy(cache, None, None, n=0)
@@ -203,7 +212,7 @@ def test_page_tensors_that_are_refused(pkg):
 # ---- sources -------------------------------------------------------------------------------------------------------------------------------
 def test_kernels_wait_before_they_read(pkg):
     """They are launched while the kernel ahead of them may still run."""
-    for name, kernels in (("block_norm.cu", 1), ("proj_w4_sm100.cu", 1), ("pages.cu", 6)):
+    for name, kernels in (("block_norm.cu", 1), ("proj_w4_sm100.cu", 1), ("proj_w4_tc_sm100.cu", 1), ("pages.cu", 5)):
         with open(os.path.join(CSRC, name)) as f:
             text = re.sub(r"//[^\n]*", "", f.read())
         bodies = text.split("__global__")[1:]

@@ -131,3 +131,55 @@ def test_no_rows(pkg, torch_cuda):
     pkg.project_w4(X, pkg.w4_weight(codes, scales), out, 0)
     torch.cuda.synchronize()
     assert torch.all(out == 777)
+
+
+def test_many_rows(pkg, torch_cuda):
+    """As many rows as there may be, on both ways."""
+    a = make(1 << 19, 32, 8, 32, True, 9)
+    out = project(pkg, *a)
+    for at in (slice(0, 1000), slice((1 << 18) - 500, (1 << 18) + 500), slice((1 << 19) - 1000, 1 << 19)):
+        check(out[at], *reference(a[0][at], *a[1:], torch.float16))
+    a = make(5000, 1024, 2000, 128, False, 9)
+    check(project(pkg, *a), *reference(*a, torch.float16))
+
+
+def test_a_kind_of_kernel_that_is_first_met_in_a_capture(pkg, torch_cuda):
+    """In a process of its own: one call outside of a capture, then every kind of kernel for the first time within one."""
+    import subprocess
+    import sys
+    code = """
+import sys; sys.path[:0] = ["tests", "."]
+import torch, __graft_entry__ as e
+from test_w4_gpu import make, reference, check
+pkg = e.load_package()
+X, *w = make(1, 128, 64, 128, False, 1)
+out = torch.zeros(1, 64, dtype=torch.float16, device="cuda")
+pkg.project_w4(X, pkg.w4_weight(*w), out, 1)
+cases = [make(r, 2048, 4096, g, True, r + g) for r in (3, 16, 40, 64) for g in (32, 64, 128)] + [make(r, 4096, 6144, 64, False, r) for r in (12, 30)]
+outs = [torch.zeros(a[0].shape[0], a[1].shape[0], dtype=torch.float16, device="cuda") for a in cases]
+side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+weights = [pkg.w4_weight(*a[1:]) for a in cases]
+with torch.cuda.graph(graph, stream=side):
+    for a, w, out in zip(cases, weights, outs):
+        pkg.project_w4(a[0], w, out, a[0].shape[0], stream=side)
+graph.replay()
+torch.cuda.synchronize()
+for a, out in zip(cases, outs):
+    check(out, *reference(*a, torch.float16))
+"""
+    import conftest
+    r = subprocess.run([sys.executable, "-c", code], cwd=conftest.ROOT, capture_output=True, text=True, timeout=200)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
+def test_calls_on_two_streams_at_a_time(pkg, torch_cuda):
+    """Kernels that hold an SM's tensor memory, and others, side by side on one GPU."""
+    cases = [make(64, 4096, 4096, 128, True, 1), make(12, 4096, 6144, 64, False, 2), make(1, 8192, 1024, 128, False, 3), make(40, 2048, 4096, 32, True, 4)]
+    want = [project(pkg, *a) for a in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    weights, outs = [pkg.w4_weight(*a[1:]) for a in cases], [torch.zeros_like(w) for w in want]
+    for _ in range(50):
+        for a, w, out, s in zip(cases, weights, outs, streams):
+            pkg.project_w4(a[0], w, out, a[0].shape[0], stream=s)
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(want, outs)) and pkg.kernel_status()[0] == 0
