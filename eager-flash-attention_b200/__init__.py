@@ -643,13 +643,15 @@ def block_norm(x, y, x_out, h, rows: int, bp: BlockNormParams, gate=None, post_w
     ``x_out = residual_scale * x + block_scale * act(gate) * n``, ``h = norm(x_out before its rounding) * pre_w + pre_b``. None: no such input or output
     (weights: ones, biases: zeros). x_out and h may be x or y. Asynchronous on ``stream``."""
     d, _, _, _, _, gate_rows, x_dtype, y_dtype, x_stride, y_stride, out_stride, h_stride, gate_stride = _BLOCK_NORM_INTS(bp)
-    _check(lib().efa_block_norm(
+    rc = (_lib or lib()).efa_block_norm(
         _matrix("block_norm: x", x, rows, d, x_stride, x_dtype), _matrix("block_norm: y", y, rows, d, y_stride, y_dtype),
         _matrix("block_norm: gate", gate, rows if gate_rows else 1, d, gate_stride, F16),
         _matrix("block_norm: post_w", post_w, 1, d, 0, F16), _matrix("block_norm: post_b", post_b, 1, d, 0, F16),
         _matrix("block_norm: pre_w", pre_w, 1, d, 0, F16), _matrix("block_norm: pre_b", pre_b, 1, d, 0, F16),
         _matrix("block_norm: x_out", x_out, rows, d, out_stride, x_dtype), _matrix("block_norm: h", h, rows, d, h_stride, F16),
-        rows, bp, _stream(stream)), "block_norm")
+        rows, bp, _stream(stream))
+    if rc:
+        _check(rc, "block_norm")
 
 
 def w4_weight(codes, scales, zeros=None) -> W4:
@@ -680,9 +682,13 @@ def project_w4(X, w: W4, out, rows: int, stream=None, x_stride: int = 0, out_str
     """``out[rows][d_out] = X[rows][d_in] @ w``, out fp16 or fp32 (``out_dtype`` where out is an address; strides in elements, 0 = dense). Made for few rows; prompts
     go through ``project`` with fp16 weights. Asynchronous on ``stream``."""
     if out_dtype is None:
-        out_dtype = _dtype("project_w4: out", out) if hasattr(out, "dtype") else F16
-    _check(lib().efa_project_w4(_matrix("project_w4: X", X, rows, w.d_in, x_stride, F16), x_stride, w,
-                                _matrix("project_w4: out", out, rows, w.d_out, out_stride, out_dtype), out_dtype, out_stride, rows, _stream(stream)), "project_w4")
+        out_dtype = _real.get(getattr(out, "dtype", None))
+        if out_dtype is None:
+            out_dtype = _dtype("project_w4: out", out) if hasattr(out, "dtype") else F16
+    rc = (_lib or lib()).efa_project_w4(_matrix("project_w4: X", X, rows, w.d_in, x_stride, F16), x_stride, w,
+                                        _matrix("project_w4: out", out, rows, w.d_out, out_stride, out_dtype), out_dtype, out_stride, rows, _stream(stream))
+    if rc:
+        _check(rc, "project_w4")
 
 
 def kernel_status() -> Sequence[int]:
