@@ -168,7 +168,7 @@ proj_w4_tc_kernel(const W4Args a, int tile_channels, bool x_blocks, const __grid
         auto ask = [&]() {
             #pragma unroll
             for (int i = 0; i < C::GROUPS; i++) {
-                if (G == W4_UNIT || i < left) next[i] = at[i * a.scale_stride];
+                next[i] = G == W4_UNIT || i < left ? at[i * a.scale_stride] : __half(0.f);     // of no group: nothing, where the one before may have infinities
                 if (i + W4_AHEAD < left) prefetch_l2(at + (i + W4_AHEAD) * a.scale_stride);
             }
             at += C::GROUPS * a.scale_stride;
