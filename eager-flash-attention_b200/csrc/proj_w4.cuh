@@ -24,29 +24,6 @@ struct W4Args {
 constexpr int W4_AHEAD = 12;
 __device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" :: "l"(p)); }
 
-// mbar_wait (sm100_ptx.cuh) with a hint that the hardware may hold the thread for that long: many warps wait here beside others that need their issue slots.
-__device__ __forceinline__ bool mbar_wait_idle(uint64_t* bar, uint32_t parity, volatile int* abort_word, int site)
-{
-    unsigned long long t0 = 0;
-    while (true) {
-        uint32_t done;
-        asm volatile(
-            "{\n"
-            ".reg .pred p;\n"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n"
-            "selp.u32 %0, 1, 0, p;\n"
-            "}\n" : "=r"(done) : "r"(smem_u32(bar)), "r"(parity), "r"(20000u) : "memory");
-        if (done) return true;
-        if (*abort_word != 0) return false;
-        const unsigned long long now = globaltimer_ns();
-        if (t0 == 0) t0 = now;
-        else if (now - t0 > kWaitLimitNs) {
-            *abort_word = site;
-            return false;
-        }
-    }
-}
-
 __device__ __forceinline__ void store_sum(const W4Args& a, float v, int m, int n)
 {
     if (n >= a.d_out) return;

@@ -183,3 +183,27 @@ def test_calls_on_two_streams_at_a_time(pkg, torch_cuda):
             pkg.project_w4(a[0], w, out, a[0].shape[0], stream=s)
     torch.cuda.synchronize()
     assert all(torch.equal(x, y) for x, y in zip(want, outs)) and pkg.kernel_status()[0] == 0
+
+
+# More tiles of 32 channels than blocks, by one or by many, whole ones and not; fewer units of k than warps, as many, and more; rows of which little and much is copied.
+@pytest.mark.parametrize("d_in,d_out,group", [(32, 9473, 32), (96, 40001, 32), (1024, 9504, 64), (2080, 12001, 32), (4096, 19000, 128), (8256, 9500, 64), (12288, 9985, 128)])
+@pytest.mark.parametrize("rows", [1, 2, 3, 4, 8])
+def test_blocks_that_go_on_to_another_tile(pkg, torch_cuda, d_in, d_out, group, rows):
+    a = make(rows, d_in, d_out, group, rows % 2 == 1, d_in + rows)
+    out = project(pkg, *a)
+    check(out, *reference(*a, torch.float16))
+    for _ in range(3):
+        assert torch.equal(project(pkg, *a), out)
+    assert pkg.kernel_status()[0] == 0
+
+
+@pytest.mark.parametrize("rows", [4, 16, 32])
+def test_an_infinite_scale_is_its_channels_own(pkg, torch_cuda, rows):
+    """Also in the last group, behind which a step has none."""
+    X, codes, scales, _ = make(rows, 1056, 16200, 32, False, 10)
+    clean = project(pkg, X, codes, scales, None)
+    scales[32, 5], scales[0, 700] = float("inf"), float("inf")
+    got = project(pkg, X, codes, scales, None)
+    assert torch.isinf(got[:, [5, 700]]).all()
+    rest = [n for n in range(16200) if n not in (5, 700)]
+    assert torch.equal(got[:, rest], clean[:, rest])
