@@ -1,6 +1,9 @@
 // The norms after and before a block, its gate and its residual addition in one pass over the rows. A row is held in registers by the threads that share it,
 // in fp32: its sums are taken over what is there already, and nothing is read twice. Layer norms sum the squares of what is left when the mean is
 // taken off, not the squares less the mean's: a mean far above the spread costs no digits.
+//
+// Memory is the floor: x, y, the gate, x_out and h once. 8192 x 4096 with a gate of every row 52.4 us, 6.4 TB/s (98 % of a copy's rate); 16384 x 1024 two layer norms 27.0 (76 %: two passes over
+// registers between barriers), 2000 x 12000 fp32 75.7 (78 %), 1237 x 2049 fp32 8.7 (62 %: little more than a round); one row 3.1, of which the launch is 2.
 #include "host_util.h"
 #include "serving.h"
 #include "sm100_ptx.cuh"
@@ -29,6 +32,7 @@ struct NormArgs {
     bool layer, post, pre, sigmoid, x_f32, y_f32;
     float eps, residual_scale, block_scale, inv_d;
     long long x_stride, y_stride, out_stride, h_stride, gate_stride;
+    int ahead;                           // rows to the one whose inputs a block fetches into the L2
 };
 
 // How a thread has its elements. ALIGNED: chunks of eight neighbours, each 16 bytes of fp16. SHIFTED: rows that begin anywhere, but at the same place within 16
@@ -146,6 +150,13 @@ __device__ __forceinline__ void store8(void* row, bool f32, const Share<T, MODE>
                 make_uint4(pack_f16x2(v[0].x, v[0].y), pack_f16x2(v[1].x, v[1].y), pack_f16x2(v[2].x, v[2].y), pack_f16x2(v[3].x, v[3].y));
         }
     }
+}
+
+// A row (its 16-byte pieces) asked for into the L2.
+__device__ __forceinline__ void prefetch_row(const char* row, unsigned bytes)
+{
+    const unsigned skip = (16u - (unsigned)reinterpret_cast<uintptr_t>(row)) & 15u;
+    if (bytes >= skip + 16) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" :: "l"(row + skip), "r"((bytes - skip) & ~15u) : "memory");
 }
 
 // Sum over the T threads of a row. `slot` alternates: when it comes round again all threads have passed the barrier in between.
@@ -289,7 +300,15 @@ block_norm_kernel(const NormArgs a)
         #pragma unroll
         for (int c = 0; c < NC; c++) numbers<MODE>(y[c], y_f32, v[c]);
     }
-    if (a.post) normalise(v, ends, a, p, a.post_w, a.post_b, part, slot);
+    // While a block has its row, memory would wait: it fetches the row of the block that will have its place, as soon as its own is there (not before, which delays it). us, without / with:
+    // 8192 x 4096 59.1 / 52.4, 512 x 16384 fp32 34.6 / 31.7, 1000 x 5001 fp32 25.5 / 22.6; half as far again 54.1, 33.0, 23.2; several rows to a warp nothing.
+    auto prefetch = [&]() {
+        if (T <= 32 || lane != 0 || a.rows - a.ahead <= at) return;
+        if (a.y) prefetch_row(yr + a.ahead * a.y_stride * (y_f32 ? 4 : 2), a.d * (y_f32 ? 4 : 2));
+        if (a.x) prefetch_row(xr + a.ahead * a.x_stride * (x_f32 ? 4 : 2), a.d * (x_f32 ? 4 : 2));
+        if (a.gate && a.gate_stride) prefetch_row(reinterpret_cast<const char*>(gr + a.ahead * a.gate_stride), a.d * 2);
+    };
+    if (a.post) { normalise(v, ends, a, p, a.post_w, a.post_b, part, slot); prefetch(); }
     auto gated = [&](float n, float gate) { return a.sigmoid ? __fdividef(n, 1.f + __expf(-gate)) : n * gate; };
     auto summed = [&](float n, float residual) { return a.y ? fmaf(a.residual_scale, residual, a.block_scale * n) : a.residual_scale * residual; };
     char* const out = static_cast<char*>(a.x_out) + row * a.out_stride * (x_f32 ? 4 : 2);
@@ -322,6 +341,7 @@ block_norm_kernel(const NormArgs a)
         ends[k] = a.x ? summed(ends[k], x_ends[k]) : a.block_scale * ends[k];
         if (a.x_out && there) store1(out, x_f32, p.end(k), ends[k]);
     }
+    if (!a.post) prefetch();
     if (a.pre) {
         normalise(v, ends, a, p, a.pre_w, a.pre_b, part, slot);
         #pragma unroll
@@ -333,16 +353,15 @@ block_norm_kernel(const NormArgs a)
     }
 }
 
-template <int T, int NC, bool LAZY = false>
+template <int T, int NC, bool WIDE, bool LAZY = false>
 int launch_norm(const NormArgs& a, int mode, cudaStream_t stream)
 {
     constexpr int PER_BLOCK = T <= 32 ? 128 / T : 1;
     const dim3 grid((unsigned)(((long long)a.rows + PER_BLOCK - 1) / PER_BLOCK));
-    const bool wide = a.x_f32 || a.y_f32;
-    const auto kernel = mode == ALIGNED ? (wide ? block_norm_kernel<T, NC, ALIGNED, true, LAZY> : block_norm_kernel<T, NC, ALIGNED, false, LAZY>)
-                      : mode == SHIFTED ? (wide ? block_norm_kernel<T, NC, SHIFTED, true, LAZY> : block_norm_kernel<T, NC, SHIFTED, false, LAZY>)
-                                        : (wide ? block_norm_kernel<T, NC, SINGLE, true, LAZY> : block_norm_kernel<T, NC, SINGLE, false, LAZY>);
-    EFA_CUDA(launch_value(kernel, grid, T <= 32 ? 128 : T, 0, stream, a));
+    const auto kernel = mode == ALIGNED ? block_norm_kernel<T, NC, ALIGNED, WIDE, LAZY> : mode == SHIFTED ? block_norm_kernel<T, NC, SHIFTED, WIDE, LAZY> : block_norm_kernel<T, NC, SINGLE, WIDE, LAZY>;
+    NormArgs b = a;
+    b.ahead = device_sms() * blocks_per_sm(T <= 32 ? 128 : T, NC, mode != SINGLE && !WIDE, LAZY);
+    EFA_CUDA(launch_value(kernel, grid, T <= 32 ? 128 : T, 0, stream, b));
     return 0;
 }
 
@@ -390,21 +409,38 @@ int block_norm(const void* x, const void* y, const void* gate, const void* post_
     for (const long long t : strides) alike = alike && (t - strides[0]) % 8 == 0;
     a.x_stride = strides[0];
     const int mode = !aligned || !alike ? SINGLE : strides[0] % 8 == 0 && p.d % 8 == 0 ? ALIGNED : SHIFTED;
-    // Threads to a row and chunks to a thread by d alone, not by the number of rows.
+    // Threads to a row and chunks to a thread by d and the types alone, not by the number of rows: two chunks where all is fp16, one of fp32 (twice the registers), three where that many
+    // threads would have half a chunk. us, one chunk / two / four: fp16 8192 x 4096 59.4 / 52.7 / 55.9, 16384 x 1024 31.0 / 26.9 / 31.3; fp32 1237 x 4096 13.4 / 14.1 / 16.9, 2000 x 1024
+    // 7.2 / 7.5 / 9.4; one / three: 1000 x 5001 28.9 / 22.7, 2000 x 2560 18.5 / 17.7; two of 1024 threads / three or four of 512: 2000 x 12000 78.2 / 75.7, 512 x 16384 32.4 / 33.6.
     const int d = mode == SINGLE ? p.d : p.d / 8 * 8;          // in chunks; the ends of a row are extra
-    if (d <= 64) return launch_norm<8, 1>(a, mode, stream);
-    if (d <= 128) return launch_norm<16, 1>(a, mode, stream);
-    if (d <= 256) return launch_norm<32, 1>(a, mode, stream);
-    if (d <= 512) return launch_norm<32, 2>(a, mode, stream);
-    if (d <= 1024) return launch_norm<64, 2>(a, mode, stream);
-    if (d <= 2048) return launch_norm<128, 2>(a, mode, stream);
-    if (d <= 128 * 24) return launch_norm<128, 3>(a, mode, stream);
-    if (d <= 4096) return launch_norm<256, 2>(a, mode, stream);
-    if (d <= 256 * 24) return launch_norm<256, 3>(a, mode, stream);
-    if (d <= 8192) return launch_norm<512, 2>(a, mode, stream);
-    if (d <= 512 * 24) return launch_norm<512, 3>(a, mode, stream);
-    if (d <= 16384) return launch_norm<512, 4>(a, mode, stream);
-    return launch_norm<1024, 4, true>(a, mode, stream);
+    if (a.x_f32 || a.y_f32) {
+        if (d <= 64) return launch_norm<8, 1, true>(a, mode, stream);
+        if (d <= 128) return launch_norm<16, 1, true>(a, mode, stream);
+        if (d <= 256) return launch_norm<32, 1, true>(a, mode, stream);
+        if (d <= 512) return launch_norm<64, 1, true>(a, mode, stream);
+        if (d <= 1024) return launch_norm<128, 1, true>(a, mode, stream);
+        if (d <= 2048) return launch_norm<256, 1, true>(a, mode, stream);
+        if (d <= 128 * 3 * 8) return launch_norm<128, 3, true>(a, mode, stream);
+        if (d <= 4096) return launch_norm<512, 1, true>(a, mode, stream);
+        if (d <= 256 * 3 * 8) return launch_norm<256, 3, true>(a, mode, stream);
+        if (d <= 8192) return launch_norm<1024, 1, true>(a, mode, stream);
+        if (d <= 512 * 3 * 8) return launch_norm<512, 3, true>(a, mode, stream);
+        if (d <= 16384) return launch_norm<1024, 2, true>(a, mode, stream);
+        return launch_norm<1024, 4, true, true>(a, mode, stream);
+    }
+    if (d <= 64) return launch_norm<8, 1, false>(a, mode, stream);
+    if (d <= 128) return launch_norm<16, 1, false>(a, mode, stream);
+    if (d <= 256) return launch_norm<32, 1, false>(a, mode, stream);
+    if (d <= 512) return launch_norm<32, 2, false>(a, mode, stream);
+    if (d <= 1024) return launch_norm<64, 2, false>(a, mode, stream);
+    if (d <= 2048) return launch_norm<128, 2, false>(a, mode, stream);
+    if (d <= 128 * 3 * 8) return launch_norm<128, 3, false>(a, mode, stream);
+    if (d <= 4096) return launch_norm<256, 2, false>(a, mode, stream);
+    if (d <= 256 * 3 * 8) return launch_norm<256, 3, false>(a, mode, stream);
+    if (d <= 8192) return launch_norm<512, 2, false>(a, mode, stream);
+    if (d <= 512 * 3 * 8) return launch_norm<512, 3, false>(a, mode, stream);
+    if (d <= 16384) return launch_norm<512, 4, false>(a, mode, stream);
+    return launch_norm<1024, 4, false, true>(a, mode, stream);
 }
 
 }  // namespace efa
