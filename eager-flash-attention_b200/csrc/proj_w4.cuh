@@ -20,7 +20,7 @@ struct W4Args {
     int* status;
 };
 
-// Scales are asked for a step ahead, which is less than memory takes: they are fetched into the L2 this many groups ahead of that.
+// tcgen05: scales are asked for a step ahead, which is less than memory takes: they are fetched into the L2 this many groups ahead of that (8192 x 32768: 74 us without, 60 with).
 constexpr int W4_AHEAD = 12;
 __device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" :: "l"(p)); }
 

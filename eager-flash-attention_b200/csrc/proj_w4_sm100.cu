@@ -8,7 +8,7 @@
 // channel are in one group: 16, 8 or 4 bytes to a lane for groups of 128, 64 or 32.
 //
 // Reading the weights is the floor (a group of 128: 0.516 bytes each). What bounds it: up to some 10 us the way from the launch to the first codes, the sums and the end (one row,
-// 4096 x 4096: 4.5 us of which the bytes are 1.3; 1056 x 4163: 2.9). Beyond, instructions: 624 to a warp's 32 channels x 256 k, of which 320 make fragments and multiply, issued
+// 4096 x 4096: 4.5 us of which the bytes are 1.3; 1056 x 4163: 2.9). Beyond, instructions: 624 to 656 to a warp's 32 channels x 256 k, of which 320 make fragments and multiply, issued
 // at 0.6 to a cycle and scheduler (one row, 8192 x 32768: 33 us, 4.1 TB/s of the 6.5; 2048 x 65536: 21 us; without the scales' part, a tenth of the instructions, a tenth less).
 #include "proj_w4.cuh"
 #include "serving.h"
