@@ -74,9 +74,11 @@ template <int N> __device__ __forceinline__ void load_shared(uint32_t addr, uint
 
 // What a warp keeps in shared memory: stages of codes (128 bytes of each of 16 MT channels), of X (512 bytes of each row), and a unit's scales.
 constexpr int W4_K = 256;               // k of a unit
+template <int WARPS> struct W4Head { uint64_t bars[WARPS][W4_STAGES], full[2], empty[2]; int abort_word; };     // in the first 1024 bytes
 template <int G, int MT, int NT, int WARPS>
 struct W4Cfg {
-    static constexpr int SMEM = WARPS == 16 ? 226 * 1024 : 112 * 1024;         // of the SM's, to a block
+    static constexpr int SMEM = WARPS == 16 ? 227 * 1024 : 113 * 1024;         // of the SM's 228 KB, less one to each block
+    static_assert(sizeof(W4Head<WARPS>) <= 1024, "");
     static constexpr int CHANNELS = 16 * MT, SUBS = W4_K / G;
     static constexpr int CODE_BYTES = CHANNELS * 128, TABLE = SUBS * CHANNELS * (int)sizeof(float2);
     __host__ __device__ static constexpr int copies(int rows, int stages) { return WARPS * (stages * (CODE_BYTES + rows * 512) + TABLE); }
@@ -107,9 +109,10 @@ proj_w4_kernel(const W4Args a, int stages, const __grid_constant__ CUtensorMap c
     using C = W4Cfg<G, MT, NT, WARPS>;
     constexpr int SUBS = C::SUBS, WORDS = G / 32;              // groups of a unit, words of codes of a lane and group
     constexpr int CHANNELS = C::CHANNELS, PER_LANE = (CHANNELS + 31) / 32;
-    extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t bars[WARPS][W4_STAGES], full[2], empty[2];
-    __shared__ int abort_word;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint64_t (&bars)[WARPS][W4_STAGES] = reinterpret_cast<W4Head<WARPS>*>(smem_raw)->bars;
+    uint64_t (&full)[2] = reinterpret_cast<W4Head<WARPS>*>(smem_raw)->full, (&empty)[2] = reinterpret_cast<W4Head<WARPS>*>(smem_raw)->empty;
+    int& abort_word = reinterpret_cast<W4Head<WARPS>*>(smem_raw)->abort_word;
     constexpr int warps = WARPS;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int first = blockIdx.x * CHANNELS, next_tile = gridDim.x * CHANNELS, m0 = blockIdx.y * 8 * NT, rows = min(a.rows - m0, 8 * NT);
@@ -118,7 +121,7 @@ proj_w4_kernel(const W4Args a, int stages, const __grid_constant__ CUtensorMap c
     // Warps take the units of a block in turn, so that what they read at a time is neighbours in the rows of codes.
     const int step = warps, u0 = (int)((long long)units * part / parts) + warp, u1 = (int)((long long)units * (part + 1) / parts);
 
-    uint8_t* const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    uint8_t* const smem = smem_raw + 1024;
     // Codes of all warps first, then X, then the tables.
     uint8_t* const slots = smem + warp * (stages * C::CODE_BYTES);
     const uint32_t x_slots = smem_u32(smem) + warps * (stages * C::CODE_BYTES) + warp * (stages * rows * 512);
@@ -417,10 +420,11 @@ int project_w4(const void* X, long long x_stride, const efa_w4& w, void* out, in
                    w.code_stride ? w.code_stride : w.d_in / 2, w.scale_stride ? w.scale_stride : w.d_out, w.zero_stride ? w.zero_stride : w.d_out,
                    x_stride ? x_stride : w.d_in, out_stride ? out_stride : w.d_out, out_dtype == EFA_F32, aligned16(out) && (out_stride ? out_stride : w.d_out) % 4 == 0, kernel_status_word()};
     // Up to eight rows the products of mma.sync are not the time. Beyond, tiles of 16 rows that read the weights again, or tcgen05 with up to 64 rows to a tile, whose start and
-    // end cost more: by the work, in weights times tiles of 16. us, tiles of 16 / tcgen05: 16 rows, 4096 x 4096 6.7 / 8.8, 4096 x 6144 (groups of 64) 9.6 / 10.6 and (of 32) 14.2 / 11.9,
-    // 2048 x 16384 12.0 / 11.1, 8192 x 8192 16.6 / 15.1; 32 rows, 2048 x 4096 7.9 / 8.2, 4096 x 4096 9.7 / 9.5, 2048 x 8192 11.6 / 9.4; 64 rows, 1024 x 1024 3.4 / 7.3,
-    // 1056 x 4163 15 / 10.8, 4096 x 4096 18 / 11.3.
-    if (rows > 8 && (double)((rows + 15) / 16) * w.d_in * w.d_out > (double)(1 << 24)) return w4_tc_launch(a, w.group, stream);
+    // end cost more, and every group of a row its sums: by the work, in weights times tiles of 16, twice as much where a row has many groups. us, tiles of 16 / tcgen05: 16 rows, 4096 x 4096 6.7 /
+    // 8.8, 2048 x 16384 12.0 / 11.1, 8192 x 8192 16.6 / 15.1; 32 rows, 4096 x 4096 9.7 / 9.5, 2048 x 8192 11.6 / 9.4; 64 rows, 1024 x 1024 3.4 / 7.3, 4096 x 4096 18 / 11.3. Groups of 64:
+    // 12 rows, 4096 x 6144 9.4 / 10.5, 32 rows, 2048 x 6144 9.6 / 8.9; of 32: 16 rows, 4096 x 8192 11.1 / 13.3, 64 rows, 4096 x 2048 10.2 / 14.5, 1056 x 4160 9.8 / 10.7, 4096 x 4096 19.8 / 18.1.
+    const double most = w.d_in >= 64 * w.group ? 1 << 25 : 1 << 24;
+    if (rows > 8 && (double)((rows + 15) / 16) * w.d_in * w.d_out > most) return w4_tc_launch(a, w.group, stream);
     return w.group == 128 ? launch_group<128>(a, stream) : w.group == 64 ? launch_group<64>(a, stream) : launch_group<32>(a, stream);
 }
 

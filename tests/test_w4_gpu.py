@@ -207,3 +207,14 @@ def test_an_infinite_scale_is_its_channels_own(pkg, torch_cuda, rows):
     assert torch.isinf(got[:, [5, 700]]).all()
     rest = [n for n in range(16200) if n not in (5, 700)]
     assert torch.equal(got[:, rest], clean[:, rest])
+
+
+@pytest.mark.parametrize("rows", [9, 16, 17, 32, 33, 64, 80])
+@pytest.mark.parametrize("d_in,group", [(1120, 32), (1088, 64), (1152, 128)])
+@pytest.mark.parametrize("d_out,zeros", [(15503, True), (16000, False)])
+def test_tiles_that_hold_their_sums_in_tensor_memory(pkg, torch_cuda, rows, d_in, group, d_out, zeros):
+    """Every width of these tiles with every group; lengths that end inside a unit of 128."""
+    for dtype in (torch.float16, torch.float32):
+        a = make(rows, d_in, d_out, group, zeros, rows + d_in)
+        check(project(pkg, *a, dtype), *reference(*a, dtype))
+    assert pkg.kernel_status()[0] == 0
