@@ -4,9 +4,9 @@
 // neighbouring pages to a warp, whose votes stay in registers from the counting to the ranking; so the lowest free pages are found in one pass and one launch,
 // in an order that nothing but the arrays decides. What moves keys is a kernel of its own over all SMs.
 //
-// What bounds them, GPU time: the scan is a chain of steps that wait for memory or for one another: arrays, counts, ranks, list, entries (taking for 64 prompts out of 16384 pages 14.0 us, with the
-// votes in memory instead of registers 26.7; forking one sequence 9.8). Moves are memory's: 68.5 us of bytes in 68 at 6.5 TB/s, compaction 76.9 with its
-// plan; 24.2 in 27.4 for copies of 8-bit pages. The table and the counts are renamed beside the moves: after them 83.8.
+// What bounds them, GPU time: the scan is a chain of steps that wait for memory or for one another: arrays, counts, ranks, list, entries (pages of 16 for 180 prompts of up to 2048 tokens taken and
+// given back 13.2 us, with the votes in memory instead of registers 26.7; forking one sequence 9.6). Moves are memory's: 68.5 us of bytes in 68 at 6.5 TB/s, compaction 76.9 with its
+// plan; 24.2 in 27.3 for copies of 8-bit pages. The table and the counts are renamed beside the moves: after them 83.8.
 //
 // Everything that comes from device memory is brought into range before it is an index; what was out of range is reported in the status word.
 #include "host_util.h"
@@ -45,9 +45,10 @@ __device__ __forceinline__ void report(int* status, int code, int who, int site)
 __device__ __forceinline__ long long capacity(const PoolArgs& p) { return (long long)p.max_pages * p.page_size; }
 
 // Keys of a slot, brought into what its table holds.
+__device__ __forceinline__ int keys_that_fit(const PoolArgs& p, int kv) { return (int)min(max((long long)kv, 0ll), min(capacity(p), (long long)INT_MAX)); }
 __device__ __forceinline__ int keys_in_table(const PoolArgs& p, int kv, int b, int site)
 {
-    const int cut = (int)min(max((long long)kv, 0ll), min(capacity(p), (long long)INT_MAX));
+    const int cut = keys_that_fit(p, kv);
     if (cut != kv) report(p.status, KS_BAD_LENGTH, b, site);
     return cut;
 }
@@ -142,19 +143,21 @@ __device__ __forceinline__ void ranked(int base, const uint32_t (&votes)[PG_VOTE
     }
 }
 
-// The numbers that the blocks have put into `mine` (shared memory): what the blocks before have, and all. Ends with everything that was written visible to all.
+// The numbers that the blocks have put into `mine` (shared memory), a block's to a lane, and their sums: of the blocks before, and of all. A word from another SM takes 400 cycles: all at once.
+struct Sums { int own, before, all; };
+__device__ __forceinline__ Sums sums_of(const int* mine)
+{
+    const int lane = threadIdx.x & 31, x = lane < (int)gridDim.z ? shared_of(mine, lane) : 0;
+    return Sums{x, (int)__reduce_add_sync(0xffffffffu, lane < rank_of_block() ? x : 0), (int)__reduce_add_sync(0xffffffffu, x)};
+}
+// The same of v. Ends with everything that was written visible to all.
 __device__ __forceinline__ int over_blocks(int v, int* mine, int& total)
 {
     if (threadIdx.x == 0) *mine = v;
     sync_all();
-    int before = 0;
-    total = 0;
-    for (int q = 0; q < (int)gridDim.z; q++) {
-        const int x = shared_of(mine, q);
-        before += q < rank_of_block() ? x : 0;
-        total += x;
-    }
-    return before;
+    const Sums s = sums_of(mine);
+    total = s.all;
+    return s.before;
 }
 
 // The free pages of a block's segment: found (their number), and listed: those of a rank below `wanted` go to list[rank] and have a count of 1 from then on.
@@ -163,11 +166,23 @@ struct FreePages {
     uint32_t votes[PG_VOTES];            // of the segment's first tile, which is mostly all of it
     int n;                               // free pages of that, of this warp
 
-    __device__ __forceinline__ int find(const int* refs, int num_pages, int* part)
+    // `meanwhile`: what has to be asked for too, while the counts are on their way.
+    template <class F>
+    __device__ __forceinline__ int find(const int* refs, int num_pages, int* part, F meanwhile)
     {
         own = segment(num_pages);
         const auto free = [&](int p) { return refs[p] <= 0; };
-        n = vote(own.lo, own.hi, votes, free);
+        const int first = own.lo + (int)(threadIdx.x >> 5) * (32 * PG_VOTES) + (int)(threadIdx.x & 31);
+        int count[PG_VOTES];
+        #pragma unroll
+        for (int j = 0; j < PG_VOTES; j++) count[j] = first + 32 * j < own.hi ? refs[first + 32 * j] : 1;
+        meanwhile();
+        n = 0;
+        #pragma unroll
+        for (int j = 0; j < PG_VOTES; j++) {
+            votes[j] = __ballot_sync(0xffffffffu, count[j] <= 0);
+            n += __popc(votes[j]);
+        }
         int total, all;
         warp_scan(n, part, total);
         for (int base = own.lo + PG_TILE; base < own.hi; base += PG_TILE) {
@@ -194,55 +209,53 @@ struct FreePages {
     }
 };
 
-// workspace: list [num_pages]; of every slot the pages it has, those it gets, and how many its block's slots before it get.
+// workspace: list [num_pages]; of slots behind a block's first PG_THREADS the pages they have, those they get, and how many the block's slots before them get.
 struct TakeArgs { PoolArgs p; const int* q_start; int* list; int* have; int* gets; int* rank; };
 
 __global__ void __launch_bounds__(PG_THREADS)
 pages_take_kernel(const TakeArgs a)
 {
-    __shared__ int part[PG_WARPS], need_of, free_of, need_before[PG_CLUSTER];
+    __shared__ int part[PG_WARPS], need_of, free_of;
+    __shared__ int have_of[PG_THREADS], gets_of[PG_THREADS], rank_of[PG_THREADS];      // of the block's first slots; of others in the workspace
     pdl_wait();
     pdl_trigger();
     const PoolArgs& p = a.p;
     const Range seqs = segment(p.num_seqs);
     FreePages pages;
-    const int found = pages.find(p.refs, p.num_pages, part);
+    struct Slot { int kv, from, to; } first{0, 0, 0};
+    auto ask = [&](int b) { return b < seqs.hi ? Slot{p.kv_len[b], a.q_start[b], a.q_start[b + 1]} : Slot{0, 0, 0}; };
+    const int found = pages.find(p.refs, p.num_pages, part, [&]() { first = ask(seqs.lo + (int)threadIdx.x); });
     int need = 0;
     for (int base = seqs.lo; base < seqs.hi; base += PG_THREADS) {
         const int b = base + (int)threadIdx.x;
+        const Slot slot = base == seqs.lo ? first : ask(b);
         int have = 0, gets = 0, total;
         if (b < seqs.hi) {
-            const int kv = keys_of(p, b, SITE_TAKE);
-            const long long n = (long long)a.q_start[b + 1] - a.q_start[b];
+            const int kv = keys_in_table(p, slot.kv, b, SITE_TAKE);
+            const long long n = (long long)slot.to - slot.from;
             const long long after = min((long long)kv + max(n, 0ll), min(capacity(p), (long long)INT_MAX));
             if (n < 0 || after != kv + n) report(p.status, KS_BAD_LENGTH, b, SITE_TAKE);
             have = pages_of(p, kv);
             gets = pages_of(p, (int)after) - have;
             p.kv_len[b] = (int)after;                          // no other thread looks at it
         }
-        const int before = block_scan(gets, part, total);
-        if (b < seqs.hi) { a.have[b] = have; a.gets[b] = gets; a.rank[b] = need + before; }
+        const int rank = need + block_scan(gets, part, total);
+        if (base == seqs.lo) { have_of[threadIdx.x] = have; gets_of[threadIdx.x] = gets; rank_of[threadIdx.x] = rank; }
+        else if (b < seqs.hi) { a.have[b] = have; a.gets[b] = gets; a.rank[b] = rank; }
         need += total;
     }
     if (threadIdx.x == 0) { need_of = need; free_of = found; }
     sync_all();
-    int wanted = 0, there = 0, free_before = 0;
-    for (int q = 0; q < (int)gridDim.z; q++) {
-        const int f = shared_of(&free_of, q);
-        free_before += q < rank_of_block() ? f : 0;
-        there += f;
-        if (threadIdx.x == 0) need_before[q] = wanted;
-        wanted += shared_of(&need_of, q);
-    }
-    pages.list(p.refs, free_before, wanted, a.list, part);
+    const Sums needs = sums_of(&need_of), frees = sums_of(&free_of);
+    const int there = frees.all;
+    pages.list(p.refs, frees.before, needs.all, a.list, part);
     sync_all();
-    // Entries, slots to the warps of all blocks in turn.
-    const int each = (int)(((long long)p.num_seqs + gridDim.z - 1) / gridDim.z);
-    for (int b = rank_of_block() + (int)gridDim.z * (int)(threadIdx.x >> 5); b < p.num_seqs; b += (int)gridDim.z * PG_WARPS) {
-        const int gets = a.gets[b];
+    // Entries of the block's slots, in turn to its warps.
+    for (int b = seqs.lo + (int)(threadIdx.x >> 5); b < seqs.hi; b += PG_WARPS) {
+        const int at = b - seqs.lo, gets = at < PG_THREADS ? gets_of[at] : a.gets[b];
         if (gets == 0) continue;
-        const int rank = a.rank[b] + need_before[b / each];
-        int* const to = p.pages + (long long)b * p.max_pages + a.have[b];
+        const int rank = needs.before + (at < PG_THREADS ? rank_of[at] : a.rank[b]);
+        int* const to = p.pages + (long long)b * p.max_pages + (at < PG_THREADS ? have_of[at] : a.have[b]);
         if ((threadIdx.x & 31) == 0 && rank + gets > there) report(p.status, KS_NO_PAGE, b, SITE_TAKE);
         #pragma unroll 4
         for (int e = (int)(threadIdx.x & 31); e < gets; e += 32) to[e] = rank + e < there ? a.list[rank + e] : -1;
@@ -316,7 +329,7 @@ __device__ __forceinline__ void move(const MoveArgs& a, int n, long long first, 
     }
 }
 
-// workspace of a fork: list [num_pages], then [num_seqs] each of claim, keys of the child, rank of its page, and the moves: source, target, keys; then their count.
+// workspace of a fork: list [num_pages], then [num_seqs] each of claim, keys of the child and rank of its page (behind a block's first PG_THREADS), and the moves: source, target, keys; then their count.
 struct ForkArgs { PoolArgs p; const int* parents; const int* children; int n; int* list; int* claim; int* keys; int* rank; int* src; int* dst; int* rest; int* count; };
 
 constexpr int PG_FEW = 512;             // forks whose children are compared with one another, without the claims' round trip through memory
@@ -325,6 +338,7 @@ __global__ void __launch_bounds__(PG_THREADS)
 pages_fork_kernel(const ForkArgs a)
 {
     __shared__ int part[PG_WARPS], mine[2], named[PG_FEW];
+    __shared__ int keys_of_fork[PG_THREADS], rank_of_fork[PG_THREADS];                 // of the block's first forks; of others in the workspace
     pdl_wait();
     pdl_trigger();
     const PoolArgs& p = a.p;
@@ -332,7 +346,22 @@ pages_fork_kernel(const ForkArgs a)
     const Range forks = segment(a.n);
     auto slot = [&](int b) { return (unsigned)b < (unsigned)p.num_seqs; };
     FreePages pages;
-    const int found = pages.find(p.refs, p.num_pages, part);
+    struct Pair { int child, parent, child_keys, parent_keys, source; };
+    // source: the page that is not full, of a parent that has one.
+    auto ask = [&](int i) {
+        Pair x{-1, -1, 0, 0, -1};
+        if (i >= forks.hi) return x;
+        x.child = a.children[i];
+        x.parent = a.parents[i];
+        if (slot(x.child)) x.child_keys = p.kv_len[x.child];
+        if (slot(x.parent)) {
+            x.parent_keys = p.kv_len[x.parent];
+            const int keys = keys_that_fit(p, x.parent_keys);
+            if (keys % p.page_size) x.source = p.pages[(long long)x.parent * p.max_pages + keys / p.page_size];
+        }
+        return x;
+    };
+    const int found = pages.find(p.refs, p.num_pages, part, []() {});
 
     // The first entry that names a child has it.
     const bool few = a.n <= PG_FEW;
@@ -351,47 +380,42 @@ pages_fork_kernel(const ForkArgs a)
     int need = 0;
     for (int base = forks.lo; base < forks.hi; base += PG_THREADS) {
         const int i = base + (int)threadIdx.x;
+        const Pair x = ask(i);
         int keys = -1, wants = 0, total;
         if (i < forks.hi) {
-            const int c = a.children[i], b = a.parents[i];
-            const int child_keys = slot(c) ? p.kv_len[c] : 0, parent_keys = slot(b) ? p.kv_len[b] : 0;
-            bool first = true;
+            const int c = x.child, b = x.parent;
+            bool original = true;
             if (few) {
                 #pragma unroll 8
-                for (int j = 0; j < i; j++) first &= named[j] != c;
-            } else first = slot(c) && a.claim[c] == i;
-            if (!first || !slot(c) || !slot(b) || child_keys != 0) report(p.status, KS_BAD_SLOT, slot(c) ? c : i, SITE_FORK);
+                for (int j = 0; j < i; j++) original &= named[j] != c;
+            } else original = slot(c) && a.claim[c] == i;
+            if (!original || !slot(c) || !slot(b) || x.child_keys != 0) report(p.status, KS_BAD_SLOT, slot(c) ? c : i, SITE_FORK);
             else {
-                keys = keys_in_table(p, parent_keys, b, SITE_FORK);
+                keys = keys_in_table(p, x.parent_keys, b, SITE_FORK);
                 if (keys % p.page_size) {
-                    const int source = p.pages[(long long)b * p.max_pages + keys / p.page_size];
-                    if ((unsigned)source < (unsigned)p.num_pages) wants = 1;
+                    if ((unsigned)x.source < (unsigned)p.num_pages) wants = 1;
                     else report(p.status, KS_BAD_PAGE, b, SITE_FORK);
                 }
             }
         }
-        const int rank = need + block_scan(wants, part, total);
-        if (i < forks.hi) { a.keys[i] = keys; a.rank[i] = wants ? rank : -1; }
+        const int before = need + block_scan(wants, part, total), rank = wants ? before : -1;
+        if (base == forks.lo) { keys_of_fork[threadIdx.x] = keys; rank_of_fork[threadIdx.x] = rank; }
+        else if (i < forks.hi) { a.keys[i] = keys; a.rank[i] = rank; }
         need += total;
     }
     if (threadIdx.x == 0) mine[1] = found;
-    int wanted, there = 0, before = 0;
+    int wanted;
     const int need_before = over_blocks(need, &mine[0], wanted);
-    for (int q = 0; q < (int)gridDim.z; q++) {
-        const int x = shared_of(&mine[1], q);
-        before += q < rank_of_block() ? x : 0;
-        there += x;
-    }
-    if (need_before)
-        for (int i = forks.lo + (int)threadIdx.x; i < forks.hi; i += PG_THREADS)
-            if (a.rank[i] >= 0) a.rank[i] += need_before;
-    pages.list(p.refs, before, wanted, a.list, part);
+    const Sums frees = sums_of(&mine[1]);
+    const int there = frees.all;
+    pages.list(p.refs, frees.before, wanted, a.list, part);
     if (rank_of_block() == 0 && threadIdx.x == 0) *a.count = min(wanted, there);
     sync_all();
-    for (int i = rank_of_block() + (int)gridDim.z * warp; i < a.n; i += (int)gridDim.z * PG_WARPS) {
-        const int keys = a.keys[i];
+    for (int i = forks.lo + warp; i < forks.hi; i += PG_WARPS) {
+        const int at = i - forks.lo, keys = at < PG_THREADS ? keys_of_fork[at] : a.keys[i];
         if (keys < 0) continue;
-        const int c = a.children[i], full = keys / p.page_size, rank = a.rank[i];
+        const int rank_here = at < PG_THREADS ? rank_of_fork[at] : a.rank[i], rank = rank_here < 0 ? -1 : need_before + rank_here;
+        const int c = a.children[i], full = keys / p.page_size;
         const int* const from = p.pages + (long long)a.parents[i] * p.max_pages;
         int* const to = p.pages + (long long)c * p.max_pages;
         #pragma unroll 4
@@ -433,7 +457,7 @@ pages_free_kernel(const PoolArgs p, const int* seqs)
     }
     if (threadIdx.x == 0) keys_of_slot = atomicExch(&p.kv_len[b], 0);          // whoever names the slot again finds it empty
     __syncthreads();
-    const int keys = keys_of_slot, cut = (int)min(max((long long)keys, 0ll), min(capacity(p), (long long)INT_MAX));
+    const int keys = keys_of_slot, cut = keys_that_fit(p, keys);
     if (cut != keys && threadIdx.x == 0) report(p.status, KS_BAD_LENGTH, b, SITE_FREE);
     const int held = pages_of(p, cut);
     #pragma unroll 4
@@ -459,7 +483,7 @@ pages_compact_kernel(const CompactArgs a)
     pdl_trigger();
     const PoolArgs& p = a.p;
     FreePages pages;
-    const int found = pages.find(p.refs, p.num_pages, part);
+    const int found = pages.find(p.refs, p.num_pages, part, []() {});
     int free_all;
     const int free_before = over_blocks(found, &mine[0], free_all);
     const int live = p.num_pages - free_all;
@@ -580,7 +604,7 @@ int launch_moves(const MoveArgs& a, const CompactArgs* names, cudaStream_t strea
 }
 
 // Blocks of a launch that looks at all pages and at n slots: one while that is little, as eight wait for one another. GPU time, us, one / eight: fork of one sequence 9.8 / 12.1, of 192 32.5 /
-// 29.8; pages for 64 prompts 27.3 / 13.9.
+// 29.8; pages for 180 prompts 27.3 / 13.9.
 int blocks_of(const efa_page_pool& p, int n) { return p.num_pages > PG_TILE || n > PG_WARPS ? PG_CLUSTER : 1; }
 
 PoolArgs device_pool(const efa_page_pool& p) { return PoolArgs{p.refs, p.pages, p.kv_len, p.num_pages, p.page_size, p.num_seqs, p.max_pages, kernel_status_word()}; }
