@@ -261,3 +261,27 @@ def test_other_stream_graph_and_host_memory(pkg, torch_cuda):
     check(h, *reference(pkg, pkg.block_norm_params(d), want[0], None, None, None, None, w[2], None)[2:], "h")
     with pytest.raises(pkg.EfaError, match="memory of the host"):
         pkg.block_norm(x.cpu(), y, x_out, h, rows, bp, g, *w)
+
+
+# As many rows as make a block look ahead to others', dense and with gaps, at the widths where the kernels of fp32 change, and odd ones.
+@pytest.mark.parametrize("d,gap", [(500, 0), (512, 8), (1000, 0), (1017, 3), (2049, 0), (2560, 8), (4096, 0), (5001, 0), (6144, 0), (8192, 8), (8200, 0), (12003, 0), (12296, 0), (16384, 0), (16390, 1),
+                                   (20001, 0), (32768, 0)])
+@pytest.mark.parametrize("x_bits,y_bits", [(32, 32), (16, 32), (32, 16), (16, 16)])
+def test_many_rows_of_every_width(pkg, torch_cuda, d, gap, x_bits, y_bits):
+    (xt, xk), (yt, yk) = types(pkg, x_bits), types(pkg, y_bits)
+    rows = 2500 if d < 2000 else 900 if d < 9000 else 310
+    x0, y0, g0, *w = inputs(rows, d, xt, yt, True, d)
+    store = [torch.full(((rows + 1) * (d + gap),), 777.0, dtype=t, device="cuda") for t in (xt, yt, torch.float16, torch.float16)]
+    x, y, g, h = (s[:rows * (d + gap)].view(rows, d + gap)[:, :d] for s in store)
+    x.copy_(x0), y.copy_(y0), g.copy_(g0)
+    s = d + gap if gap else 0
+    bp = pkg.block_norm_params(d, kind=d % 2, eps=1e-5, post=d % 3 > 0, gate=pkg.GATE_SIGMOID, gate_rows=True, residual_scale=0.75, block_scale=0.5, x_dtype=xk, y_dtype=yk,
+                               x_stride=s, y_stride=s, out_stride=s, h_stride=s, gate_stride=s)
+    r, tr, hr, th = reference(pkg, bp, x0, y0, g0, *w)
+    pkg.block_norm(x, y, x, h, rows, bp, g, *w)
+    check(x, r, tr, "x_out")
+    check(h, hr, th, "h")
+    assert torch.equal(y, y0) and torch.equal(g, g0)
+    for view, whole in ((x, store[0]), (h, store[3])):
+        view.fill_(777.0)
+        assert torch.all(whole == 777)
