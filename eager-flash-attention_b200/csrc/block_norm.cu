@@ -2,7 +2,7 @@
 // in fp32: its sums are taken over what is there already, and nothing is read twice. Layer norms sum the squares of what is left when the mean is
 // taken off, not the squares less the mean's: a mean far above the spread costs no digits.
 //
-// Memory is the floor: x, y, the gate, x_out and h once. 8192 x 4096 with a gate of every row 52.4 us, 6.4 TB/s (98 % of a copy's rate); 16384 x 1024 two layer norms 27.0 (76 %: two passes over
+// Memory is the floor: x, y, the gate, x_out and h once. 8192 x 4096 with a gate of every row 54.8 us, 6.1 TB/s (94 % of a copy's rate); 16384 x 1024 two layer norms 27.0 (76 %: two passes over
 // registers between barriers), 2000 x 12000 fp32 75.7 (78 %), 1237 x 2049 fp32 8.7 (62 %: little more than a round); one row 3.1, of which the launch is 2.
 #include "host_util.h"
 #include "serving.h"
@@ -301,7 +301,7 @@ block_norm_kernel(const NormArgs a)
         for (int c = 0; c < NC; c++) numbers<MODE>(y[c], y_f32, v[c]);
     }
     // While a block has its row, memory would wait: it fetches the row of the block that will have its place, as soon as its own is there (not before, which delays it). us, without / with:
-    // 8192 x 4096 59.1 / 52.4, 512 x 16384 fp32 34.6 / 31.7, 1000 x 5001 fp32 25.5 / 22.6; half as far again 54.1, 33.0, 23.2; several rows to a warp nothing.
+    // 8192 x 4096 60.2 / 54.8, 512 x 16384 fp32 34.6 / 31.7, 1000 x 5001 fp32 25.5 / 22.6; half as far again 2 to 4 % more; several rows to a warp nothing.
     auto prefetch = [&]() {
         if (T <= 32 || lane != 0 || a.rows - a.ahead <= at) return;
         if (a.y) prefetch_row(yr + a.ahead * a.y_stride * (y_f32 ? 4 : 2), a.d * (y_f32 ? 4 : 2));
@@ -410,7 +410,7 @@ int block_norm(const void* x, const void* y, const void* gate, const void* post_
     a.x_stride = strides[0];
     const int mode = !aligned || !alike ? SINGLE : strides[0] % 8 == 0 && p.d % 8 == 0 ? ALIGNED : SHIFTED;
     // Threads to a row and chunks to a thread by d and the types alone, not by the number of rows: two chunks where all is fp16, one of fp32 (twice the registers), three where that many
-    // threads would have half a chunk. us, one chunk / two / four: fp16 8192 x 4096 59.4 / 52.7 / 55.9, 16384 x 1024 31.0 / 26.9 / 31.3; fp32 1237 x 4096 13.4 / 14.1 / 16.9, 2000 x 1024
+    // threads would have half a chunk. us, one chunk / two / four: fp16 8192 x 4096 (one set of tensors) 59.4 / 52.7 / 55.9, 16384 x 1024 31.0 / 26.9 / 31.3; fp32 1237 x 4096 13.4 / 14.1 / 16.9, 2000 x 1024
     // 7.2 / 7.5 / 9.4; one / three: 1000 x 5001 28.9 / 22.7, 2000 x 2560 18.5 / 17.7; two of 1024 threads / three or four of 512: 2000 x 12000 78.2 / 75.7, 512 x 16384 32.4 / 33.6.
     const int d = mode == SINGLE ? p.d : p.d / 8 * 8;          // in chunks; the ends of a row are extra
     if (a.x_f32 || a.y_f32) {
