@@ -2,13 +2,13 @@
 //
 // The weights are the operand in tensor memory, whose lanes are channels and so threads: a thread has the codes of its channel, 64 bytes per 128 k from shared memory
 // (TMA), and writes them as fp16. A code c (byte 0 of a half, the other byte 0) is the fp16 number c 2^-24 as it stands: of a word of eight codes two logical
-// operations and a shift make bytes of them, a byte permutation of each two puts neighbouring k into the halves of a register, one subtraction takes the zero point
-// off, exactly. X goes to shared memory as it lies (TMA). A group's sums come back in fp32 and are added up times scale * 2^24, by warps of their own.
+// operations make bytes of them (odd ones 16 times themselves), a byte permutation of each two puts neighbouring k into the halves of a register, one multiplication by (1, 1/16) with an
+// addition takes the zero point off, exactly. X goes to shared memory as it lies (TMA). A group's sums come back in fp32 and are added up times scale * 2^24, by warps of their own.
 //
 // Why not the weights in shared memory: they would be written there and read again by the tensor core, 256 bytes for 64 of codes; in tensor memory the thread that has a channel's codes
-// writes them where they are used. What bounds it (8192 x 32768: 64 rows 44.3 us, 3.2 TB/s, 777 TFLOP/s; 16 rows 39.4): making the operand. A unit of 128 k x 256 channels takes 3440 warp
-// instructions, 896 of them the seven logical ones to a word; 1290 cycles, of which the logical pipe works 54 % and the schedulers issue 67 %. More of the operand made before the wait
-// for its place needs registers that the block does not have (49 us with spills); a tile of 256 channels to an SM leaves 20 of 148 SMs without one. 4096 x 4096, 64 rows: 11.3 us, of which start
+// writes them where they are used. What bounds it (8192 x 32768: 64 rows 44.7 us, 3.2 TB/s, 770 TFLOP/s; 16 rows 37.9): making the operand. A unit of 128 k x 256 channels takes some 3300 warp
+// instructions, 768 of them the six logical ones to a word; of its 1290 cycles the logical pipe worked 57 % and the schedulers issued 71 % with seven (odd codes shifted: 45.8 and 39.4 us). More of the operand made before the wait
+// for its place needs registers that the block does not have (49 us with spills); a tile of 256 channels to an SM leaves 20 of 148 SMs without one. 4096 x 4096, 64 rows: 11.2 us, of which start
 // and sums of the cluster are 5.
 #include "proj_w4.cuh"
 
@@ -42,10 +42,10 @@ __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t s)
     asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(s));
     return r;
 }
-__device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b)
+__device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c)
 {
     uint32_t r;
-    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
     return r;
 }
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
@@ -55,14 +55,16 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
     return *reinterpret_cast<float2*>(&r);
 }
 
-// Eight codes to four registers (k, k + 1) of (code - zero) 2^-24. A selector with its high bit set copies a byte's sign, which is 0 here.
-__device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t zero, uint32_t* f)
+// Eight codes to four registers (k, k + 1) of (code - zero) 2^-24; minus: -zero 2^-24 twice. Odd codes come as 16 times themselves. A selector with its high bit set copies the sign of an even
+// code's byte, which is 0.
+__device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t minus, uint32_t* f)
 {
-    const uint32_t even = w & 0x0f0f0f0fu, odd = (w >> 4) & 0x0f0f0f0fu;
-    f[0] = sub2(prmt(even, odd, 0xc480u), zero);
-    f[1] = sub2(prmt(even, odd, 0xd591u), zero);
-    f[2] = sub2(prmt(even, odd, 0xe6a2u), zero);
-    f[3] = sub2(prmt(even, odd, 0xf7b3u), zero);
+    constexpr uint32_t ONE_SIXTEENTH = 0x2c003c00u;            // 1, 1/16
+    const uint32_t even = w & 0x0f0f0f0fu, odd = w & 0xf0f0f0f0u;
+    f[0] = fma2(prmt(even, odd, 0x8480u), ONE_SIXTEENTH, minus);
+    f[1] = fma2(prmt(even, odd, 0x8581u), ONE_SIXTEENTH, minus);
+    f[2] = fma2(prmt(even, odd, 0x8682u), ONE_SIXTEENTH, minus);
+    f[3] = fma2(prmt(even, odd, 0x8783u), ONE_SIXTEENTH, minus);
 }
 
 template <int G, int N>
@@ -243,9 +245,9 @@ proj_w4_tc_kernel(const W4Args a, int tile_channels, bool x_blocks, const __grid
         if (buf < steps) ask();
         for (unsigned s = buf; s < (unsigned)steps; s += 2) {
             const unsigned in_unit = s % C::STEPS, unit = s / C::STEPS, slot = unit % C::STAGES;
-            uint32_t zero[C::GROUPS];
+            uint32_t minus[C::GROUPS];
             #pragma unroll
-            for (int i = 0; i < C::GROUPS; i++) zero[i] = next[i] | next[i] << 16;
+            for (int i = 0; i < C::GROUPS; i++) minus[i] = (next[i] | next[i] << 16) | 0x80008000u;
             if (s + 2 < (unsigned)steps) ask();
             if (!__all_sync(0xffffffffu, mbar_wait(&full[slot], (uint32_t)(unit / C::STAGES) & 1u, &abort_word, 77))) break;
             constexpr int CHUNKS = C::STEP / 32;               // of 16 bytes
@@ -256,7 +258,7 @@ proj_w4_tc_kernel(const W4Args a, int tile_channels, bool x_blocks, const __grid
                 asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
                              : "r"(my_codes + slot * C::SLOT + (((uint32_t)(in_unit * CHUNKS + c) ^ swizzle) << 4)) : "memory");
                 #pragma unroll
-                for (int i = 0; i < 4; i++) codes_to_f16(w[i], zero[32 * c / G], f + 4 * i);
+                for (int i = 0; i < 4; i++) codes_to_f16(w[i], minus[32 * c / G], f + 4 * i);
                 if (c == 0 && s >= 2) {                        // the operand that was here has been multiplied
                     going = __all_sync(0xffffffffu, mbar_wait(&d_full[tile][buf], (uint32_t)((s >> 1) - 1) & 1u, &abort_word, 78));
                     if (!going) break;
