@@ -218,3 +218,23 @@ def test_tiles_that_hold_their_sums_in_tensor_memory(pkg, torch_cuda, rows, d_in
         a = make(rows, d_in, d_out, group, zeros, rows + d_in)
         check(project(pkg, *a, dtype), *reference(*a, dtype))
     assert pkg.kernel_status()[0] == 0
+
+
+def test_blocks_of_several_tiles_in_graphs_side_by_side(pkg, torch_cuda):
+    """Blocks that stay on their SM for several tiles, two of them and one on tcgen05 at a time, replayed."""
+    cases = [make(1, 2048, 16384, 64, True, 1), make(2, 8192, 12000, 128, False, 2), make(48, 2048, 16384, 128, False, 3)]
+    want = [project(pkg, *a) for a in cases]
+    weights, outs, graphs = [pkg.w4_weight(*a[1:]) for a in cases], [torch.zeros_like(w) for w in want], []
+    streams = [torch.cuda.Stream() for _ in cases]
+    for a, w, out, s in zip(cases, weights, outs, streams):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=s):
+            for _ in range(5):
+                pkg.project_w4(a[0], w, out, a[0].shape[0], stream=s)
+    for _ in range(10):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(want, outs)) and pkg.kernel_status()[0] == 0
+    del graphs
