@@ -230,6 +230,7 @@ proj_w4_kernel(const W4Args a, int stages, const __grid_constant__ CUtensorMap c
             tabulate();
             ask();
             if (!__all_sync(0xffffffffu, mbar_wait(&bar[slot], phase, &abort_word, 70))) break;
+            __syncwarp();                                      // the table is other lanes' writing: a vote orders no memory
             const uint32_t codes = code_base + slot * C::CODE_BYTES;
             #pragma unroll
             for (int s = 0; s < SUBS; s++) {
