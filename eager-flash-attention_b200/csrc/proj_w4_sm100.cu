@@ -14,6 +14,7 @@
 #include "serving.h"
 
 #include <algorithm>
+#include <atomic>
 
 namespace efa {
 
@@ -365,7 +366,7 @@ int launch_w4(const W4Args& a, cudaStream_t stream)
     const int blocks = again ? 16 / WARPS * device_sms() : tiles;
     int stages = W4_STAGES;
     while (stages > 1 && C::smem(rows, stages, again) > C::SMEM) stages--;
-    static bool set[64] = {};
+    static std::atomic<bool> set[64];
     int dev = 0;
     EFA_CUDA(cudaGetDevice(&dev));
     if (dev >= 64 || !set[dev]) {

@@ -11,8 +11,10 @@
 // for its place needs registers that the block does not have (49 us with spills); a tile of 256 channels to an SM leaves 20 of 148 SMs without one. 4096 x 4096, 64 rows: 11.2 us, of which start
 // and sums of the cluster are 5.
 #include "proj_w4.cuh"
+#include "w4_plan.h"
 
 #include <algorithm>
+#include <atomic>
 
 namespace efa {
 
@@ -291,13 +293,14 @@ proj_w4_tc_kernel(const W4Args a, int tile_channels, bool x_blocks, const __grid
         for (int e = 4 * threadIdx.x; e < rows * block; e += 4 * TC_THREADS) store_sum4(a, *reinterpret_cast<const float4*>(sum + e), m0 + e / block, n0 + e % block);
 }
 
-// Clusters of p blocks that the device holds at a time: blocks that have an SM each must find them in one part of the GPU. Asked once.
+// Clusters of p blocks that the device holds at a time: blocks that have an SM each must find them in one part of the GPU. Asked once; a question that failed fails the
+// call, as another division would be another order of the sums.
 template <auto kernel>
-int clusters_at_once(int p, int smem, int dev)
+int clusters_at_once(int p, int smem, int dev, int& n)
 {
-    static int known[64][9] = {};
-    if (dev < 64 && known[dev][p]) return known[dev][p];
-    int n = device_sms() / p;
+    static std::atomic<int> known[64][W4_MAX_PARTS + 1];       // one more than the number, 0: not asked yet
+    if (dev < 64 && (n = known[dev][p].load(std::memory_order_relaxed)) != 0) { n--; return 0; }
+    n = device_sms();
     if (p > 1) {
         cudaLaunchConfig_t cfg{};
         cfg.gridDim = dim3(1, 1, p);
@@ -309,10 +312,10 @@ int clusters_at_once(int p, int smem, int dev)
         attr.val.clusterDim.z = (unsigned)p;
         cfg.attrs = &attr;
         cfg.numAttrs = 1;
-        if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) { (void)cudaGetLastError(); n = 0; }
+        EFA_CUDA(cudaOccupancyMaxActiveClusters(&n, kernel, &cfg));
     }
-    if (dev < 64) known[dev][p] = std::max(n, 1);
-    return std::max(n, 1);
+    if (dev < 64) known[dev][p].store(n + 1, std::memory_order_relaxed);
+    return 0;
 }
 
 template <int G, int N>
@@ -321,24 +324,17 @@ int launch_tc(const W4Args& a, cudaStream_t stream)
     using C = TcCfg<G, N>;
     constexpr auto kernel = proj_w4_tc_kernel<G, N>;
     const int units = (a.d_in + W4_UNIT - 1) / W4_UNIT, row_tiles = (a.rows + 63) / 64;
-    static bool set[64] = {};
+    static std::atomic<bool> set[64];
     int dev = 0;
     EFA_CUDA(cudaGetDevice(&dev));
     if (dev >= 64 || !set[dev]) {
         EFA_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
         if (dev < 64) set[dev] = true;
     }
-    // Channels of a block and parts of k: the fewest rounds, each 4 us and 0.6 us a unit, and 1 us for the sums of several blocks. A block of fewer channels computes as long.
-    int channels = 128, parts = 1;
-    double best = 1e30;
-    for (int p = 1; p <= std::min(8, units); p++) {
-        const int at_once = clusters_at_once<kernel>(p, C::SMEM, dev);
-        for (int c = 128; c >= 96; c -= 16) {
-            const long long clusters = (long long)((a.d_out + 2 * c - 1) / (2 * c)) * row_tiles;
-            const double time = (double)((clusters + at_once - 1) / at_once) * (4.0 + 0.6 * ((units + p - 1) / p) + (p > 1 ? 1.0 : 0.0));
-            if (time < best * 0.999) { best = time; channels = c; parts = p; }
-        }
-    }
+    int at_once[W4_MAX_PARTS + 1] = {};
+    for (int p = 1; p <= std::min(W4_MAX_PARTS, units); p++)
+        if (int rc = clusters_at_once<kernel>(p, C::SMEM, dev, at_once[p])) return rc;
+    const auto [channels, parts] = w4_division(a.d_out, row_tiles, units, at_once);
     CUtensorMap codes, x;
     const unsigned long long code_dims[2] = {(unsigned long long)a.d_in / 2, (unsigned long long)a.d_out}, code_stride[1] = {(unsigned long long)a.code_stride};
     const unsigned code_box[2] = {64, 2 * (unsigned)channels};
