@@ -597,27 +597,60 @@ def _dtype(what: str, x, want: Optional[int] = None) -> int:
     return kind
 
 
+def _rows_of(x, rows: int, width: int, stride: int) -> bool:
+    """Whether a tensor of two dimensions or more has ``rows`` rows of ``width`` elements where a kernel looks for them, ``stride`` apart (0: dense): its last dimensions make
+    a row (with a stride they may be longer), those before them the rows. A dense tensor that is all rows may be cut otherwise."""
+    shape, strides = x.shape, x.stride()
+    k, row = len(shape) - 1, shape[-1]
+    while k > 0 and row < width:
+        k -= 1
+        if shape[k] > 1 and strides[k] != row:
+            return False
+        row *= shape[k]
+    if not stride:
+        return row == width or x.numel() == rows * width
+    if row < width:
+        return False
+    there = 1
+    while k > 0 and there < rows:
+        k -= 1
+        if shape[k] == 1:
+            continue
+        if there == 1 and strides[k] and stride % strides[k] == 0:          # every row, or every n-th
+            there = -(-shape[k] * strides[k] // stride)
+        elif there > 1 and strides[k] == there * stride:
+            there *= shape[k]
+        else:
+            return False
+    return there >= rows
+
+
 def _matrix(what: str, x, rows: int, width: int, stride: int, kind: int) -> Optional[int]:
-    """Address of ``rows`` rows of ``width`` elements, ``stride`` apart (0: dense). A tensor of another type or that ends before them is refused."""
+    """Address of ``rows`` rows of ``width`` elements, ``stride`` apart (0: dense). A tensor of another type, that ends before them or whose own shape is of other rows is refused."""
     if x is None:
         return None
     try:
-        if _real.get(x.dtype) == kind and not stride and x.is_contiguous() and x.numel() >= rows * width:
-            return x.data_ptr()
+        if _real.get(x.dtype) == kind:
+            if not stride:
+                if x.is_contiguous() and ((n := x.numel()) == (need := rows * width) or (n > need and x.shape[-1] == width)):
+                    return x.data_ptr()
+            elif x.stride()[-2:] == (stride, 1) and x.shape[-1] >= width and x.shape[-2] >= rows:
+                return x.data_ptr()
     except AttributeError:
         return _ptr(x)
     _dtype(what, x, kind)
     if rows <= 0:
         return x.data_ptr()
     need = (rows - 1) * (stride or width) + width
-    if x.numel() >= need and x.is_contiguous():
-        return x.data_ptr()
-    if not stride:
-        raise EfaError(f"{what} must be a dense tensor of {need} elements, or its stride be given")
-    if x.stride(-1) != 1 and x.shape[-1] > 1:
-        raise EfaError(f"{what}: the elements of a row must be neighbours")
-    if x.untyped_storage().nbytes() // x.element_size() - x.storage_offset() < need:
-        raise EfaError(f"{what}: rows of this stride end {need} elements behind the tensor's first, beyond its memory")
+    if not (x.numel() >= need and x.is_contiguous()):
+        if not stride:
+            raise EfaError(f"{what} must be a dense tensor of {need} elements, or its stride be given")
+        if x.stride(-1) != 1 and x.shape[-1] > 1:
+            raise EfaError(f"{what}: the elements of a row must be neighbours")
+        if x.untyped_storage().nbytes() // x.element_size() - x.storage_offset() < need:
+            raise EfaError(f"{what}: rows of this stride end {need} elements behind the tensor's first, beyond its memory")
+    if x.dim() > 1 and not _rows_of(x, rows, width, stride):
+        raise EfaError(f"{what}: a tensor of shape {list(x.shape)} is not {rows} rows of {width}" + (f", {stride} apart" if stride else ""))
     return x.data_ptr()
 
 
@@ -646,8 +679,8 @@ def block_norm(x, y, x_out, h, rows: int, bp: BlockNormParams, gate=None, post_w
     rc = (_lib or lib()).efa_block_norm(
         _matrix("block_norm: x", x, rows, d, x_stride, x_dtype), _matrix("block_norm: y", y, rows, d, y_stride, y_dtype),
         _matrix("block_norm: gate", gate, rows if gate_rows else 1, d, gate_stride, F16),
-        _matrix("block_norm: post_w", post_w, 1, d, 0, F16), _matrix("block_norm: post_b", post_b, 1, d, 0, F16),
-        _matrix("block_norm: pre_w", pre_w, 1, d, 0, F16), _matrix("block_norm: pre_b", pre_b, 1, d, 0, F16),
+        post_w if post_w is None else _matrix("block_norm: post_w", post_w, 1, d, 0, F16), post_b if post_b is None else _matrix("block_norm: post_b", post_b, 1, d, 0, F16),
+        pre_w if pre_w is None else _matrix("block_norm: pre_w", pre_w, 1, d, 0, F16), pre_b if pre_b is None else _matrix("block_norm: pre_b", pre_b, 1, d, 0, F16),
         _matrix("block_norm: x_out", x_out, rows, d, out_stride, x_dtype), _matrix("block_norm: h", h, rows, d, h_stride, F16),
         rows, bp, _stream(stream))
     if rc:
