@@ -468,6 +468,15 @@ def cache_read(K, V, cache: PagedCache, batch: PagedBatch, stream=None, head_str
     _check(lib().efa_cache_read(K, V, head_stride, token_stride, cache, batch, _stream(stream)), "cache_read")
 
 
+def _bytes(what: str, workspace) -> int:
+    """Bytes of a workspace: of a dense tensor, as the kernels write what lies between the rows of others, and behind an expanded one."""
+    if workspace is None:
+        return 0
+    if not workspace.is_contiguous():
+        raise EfaError(f"{what}: the workspace must be a dense tensor")
+    return workspace.numel() * workspace.element_size()
+
+
 def paged_attention_workspace(cache: PagedCache, batch: PagedBatch, ap: PagedAttentionParams) -> int:
     """Bytes of workspace that paged_attention needs for these sizes (0: none)."""
     why = paged_check(cache, batch, ap)
@@ -482,7 +491,7 @@ def paged_attention(Q, O, cache: PagedCache, batch: PagedBatch, ap: PagedAttenti
     ``workspace``: a tensor of at least paged_attention_workspace bytes (or an address, with ``workspace_bytes``), not used by any
     other call until this one is done. Asynchronous on ``stream``."""
     if workspace_bytes is None:
-        workspace_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+        workspace_bytes = _bytes("paged_attention", workspace)
     tokens, d_h, by_head, by_token, o_token = batch.tokens, cache.d_h, ap.q_head_stride, ap.q_token_stride, ap.o_token_stride
     width = ap.H_q * d_h
     need = (ap.H_q - 1) * by_head + (tokens - 1) * by_token + d_h if by_head or by_token else width * tokens
@@ -539,23 +548,21 @@ def _pairs(what: str, a, b) -> int:
     return a.numel()
 
 
-def _space(workspace, workspace_bytes: Optional[int]):
-    if workspace_bytes is None:
-        workspace_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
-    return _ptr(workspace), workspace_bytes
+def _space(what: str, workspace, workspace_bytes: Optional[int]):
+    return _ptr(workspace), _bytes(what, workspace) if workspace_bytes is None else workspace_bytes
 
 
 def pages_take(pool: PagePool, q_start, workspace, stream=None, workspace_bytes: Optional[int] = None) -> None:
     """Every slot grows by its new tokens, ``q_start[b + 1] - q_start[b]``, and gets the lowest free pages for them. What the pool cannot give becomes -1 in
     the table and is reported (kernel_status code 4)."""
-    _check(lib().efa_pages_take(pool, _ints("pages_take: q_start", q_start, pool.num_seqs + 1), *_space(workspace, workspace_bytes), _stream(stream)), "pages_take")
+    _check(lib().efa_pages_take(pool, _ints("pages_take: q_start", q_start, pool.num_seqs + 1), *_space("pages_take", workspace, workspace_bytes), _stream(stream)), "pages_take")
 
 
 def pages_fork(pool: PagePool, cache: PagedCache, parents, children, workspace, stream=None, n: Optional[int] = None, workspace_bytes: Optional[int] = None) -> None:
     """Slots ``children`` (empty ones) become copies of slots ``parents``: full pages are shared, a partly filled last page is copied."""
     n = _pairs("pages_fork: parents and children", parents, children) if n is None else n
     _check(lib().efa_pages_fork(pool, cache, _ints("pages_fork: parents", parents, n), _ints("pages_fork: children", children, n), n,
-                                *_space(workspace, workspace_bytes), _stream(stream)), "pages_fork")
+                                *_space("pages_fork", workspace, workspace_bytes), _stream(stream)), "pages_fork")
 
 
 def pages_free(pool: PagePool, seqs, stream=None, n: Optional[int] = None) -> None:
@@ -569,7 +576,7 @@ def pages_compact(pool: PagePool, cache: PagedCache, pages_out, refs_out, moved,
     ``moved [num_pages]`` the new place of each page (-1: a free one)."""
     _check(lib().efa_pages_compact(pool, cache, _ints("pages_compact: pages_out", pages_out, pool.num_seqs * pool.max_pages),
                                    _ints("pages_compact: refs_out", refs_out, pool.num_pages), _ints("pages_compact: moved", moved, pool.num_pages),
-                                   *_space(workspace, workspace_bytes), _stream(stream)), "pages_compact")
+                                   *_space("pages_compact", workspace, workspace_bytes), _stream(stream)), "pages_compact")
 
 
 def pages_copy(cache: PagedCache, src, dst, stream=None, n: Optional[int] = None) -> None:

@@ -69,3 +69,17 @@ def test_a_row_of_one_element(pkg):
     assert "shape" in refusal(pkg, lambda: pkg.block_norm(half(4, 2), None, None, half(4, 1), 4, bp))
     assert "shape" not in refusal(pkg, lambda: pkg.block_norm(half(4, 1), None, None, half(4), 4, bp))
     assert "shape" not in refusal(pkg, lambda: pkg.block_norm(half(2, 2), None, None, half(4, 1), 4, bp))
+
+
+def test_workspaces_that_are_not_dense_are_refused(pkg):
+    """An expanded byte has as many elements as one likes, and one byte of memory; what lies between the rows of a view is not the call's."""
+    ints = lambda *shape: torch.zeros(*shape, dtype=torch.int32)  # noqa: E731
+    pool, cache = pkg.page_pool(ints(10), ints(3, 4), ints(3), 16), pkg.PagedCache(AT, AT, None, None, 10, 16, 8, 128, pkg.F16, 0)
+    batch, ap = pkg.paged_batch(ints(4), ints(3), ints(3, 4), 3, 1, 64), pkg.paged_attention_params(16, 128)
+    for ws in (torch.zeros(1, dtype=torch.uint8).expand(1 << 20), torch.zeros(1 << 12, 1 << 9, dtype=torch.uint8)[:, :256]):
+        for call in (lambda: pkg.pages_take(pool, ints(4), ws), lambda: pkg.pages_fork(pool, cache, ints(1), ints(1), ws),
+                     lambda: pkg.pages_compact(pool, cache, ints(3, 4), ints(10), ints(10), ws), lambda: pkg.paged_attention(AT, AT, cache, batch, ap, ws)):
+            assert "the workspace must be a dense tensor" in refusal(pkg, call)
+    dense = torch.zeros(1 << 20, dtype=torch.uint8)
+    for call in (lambda: pkg.pages_take(pool, ints(4), dense), lambda: pkg.paged_attention(AT, AT, cache, batch, ap, dense)):
+        assert "dense" not in refusal(pkg, call)
