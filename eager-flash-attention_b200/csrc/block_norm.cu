@@ -410,12 +410,25 @@ int block_norm(const void* x, const void* y, const void* gate, const void* post_
         return 2;
     }
     const void* const mem[] = {x, y, gate, post_w, post_b, pre_w, pre_b, x_out, h};
-    if (int rc = check_memory("block_norm", mem, 9)) return rc;
     const auto stride = [&](int64_t s) { return s ? (long long)s : (long long)p.d; };
     NormArgs a{x, y, static_cast<const __half*>(gate), static_cast<const __half*>(post_w), static_cast<const __half*>(post_b), static_cast<const __half*>(pre_w),
                static_cast<const __half*>(pre_b), x_out, static_cast<__half*>(h), rows, p.d, p.kind == EFA_NORM_LAYER, p.post != 0, h != nullptr, p.gate == EFA_GATE_SIGMOID,
                p.x_dtype == EFA_F32, p.y_dtype == EFA_F32, p.eps, p.residual_scale, p.block_scale, (float)(1.0 / p.d),
                stride(p.x_stride), stride(p.y_stride), stride(p.out_stride), stride(p.h_stride), p.gate_rows ? stride(p.gate_stride) : 0};
+    const int x_elem = a.x_f32 ? 4 : 2, y_elem = a.y_f32 ? 4 : 2;
+    const auto span = [&](const void* at, long long n, long long s, int elem) { return RowSpan{at, n, (long long)p.d * elem, s * elem, elem}; };
+    const RowSpan outs[] = {span(x_out, rows, a.out_stride, x_elem), span(h, rows, a.h_stride, 2)};
+    const RowSpan ins[] = {span(x, rows, a.x_stride, x_elem), span(y, rows, a.y_stride, y_elem), a.gate_stride ? span(gate, rows, a.gate_stride, 2) : span(gate, 1, p.d, 2),
+                           span(post_w, 1, p.d, 2), span(post_b, 1, p.d, 2), span(pre_w, 1, p.d, 2), span(pre_b, 1, p.d, 2)};
+    for (int o = 0; o < 2; o++)
+        for (int i = 0; i < 7; i++)
+            if (rows_clash(outs[o], ins[i], i < 3)) {
+                static const char* const names[] = {"x", "y", "gate", "post_w", "post_b", "pre_w", "pre_b"};
+                set_error("block_norm: %s overlaps %s, and is not the same rows of the same type", o ? "h" : "x_out", names[i]);
+                return 2;
+            }
+    if (rows_clash(outs[0], outs[1], true)) { set_error("block_norm: x_out and h overlap"); return 2; }
+    if (int rc = check_memory("block_norm", mem, 9)) return rc;
     bool aligned = true, alike = true;
     for (const void* q : mem) aligned = aligned && aligned16(q);
     const long long strides[] = {x ? a.x_stride : a.y_stride, y ? a.y_stride : a.x_stride, x_out ? a.out_stride : a.x_stride, h ? a.h_stride : a.x_stride, gate && a.gate_stride ? a.gate_stride : a.x_stride};

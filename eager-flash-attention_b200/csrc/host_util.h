@@ -70,6 +70,12 @@ bool own_device_memory(const void* p);
 // of each group that belongs together: 0.08 us each, of 4 us that a call takes on the host. Null pointers are passed over.
 int check_memory(const char* what, const void* const* p, int n);
 
+// Rows of a tensor in memory: `rows` of `width` bytes, `stride` bytes apart, of elements of `elem` bytes.
+struct RowSpan { const void* at; long long rows, width, stride; int elem; };
+// Whether a call that writes `out` and reads `in` row by row would lose what it has to read: they meet, and not as the same rows of the same elements (which a call may allow:
+// in place). Rows of one stride may lie in one another's gaps; of two strides what meets is taken as lost.
+bool rows_clash(const RowSpan& out, const RowSpan& in, bool in_place);
+
 inline bool aligned(const void* p, unsigned bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 inline bool aligned16(const void* p) { return aligned(p, 16); }
 

@@ -416,11 +416,16 @@ int project_w4(const void* X, long long x_stride, const efa_w4& w, void* out, in
     if (rows == 0) return 0;
     if (!X || !out) { set_error("project_w4: X or out is null"); return 2; }
     if (!aligned16(X) || !aligned(out, out_dtype == EFA_F16 ? 2 : 4)) { set_error("project_w4: X must be 16-byte aligned, out to its elements"); return 2; }
-    const void* const mem[] = {X, w.codes, w.scales, w.zeros, out};
-    if (int rc = check_memory("project_w4", mem, 5)) return rc;
     const W4Args a{w.codes, static_cast<const __half*>(w.scales), w.zeros, static_cast<const __half*>(X), out, rows, w.d_in, w.d_out,
                    w.code_stride ? w.code_stride : w.d_in / 2, w.scale_stride ? w.scale_stride : w.d_out, w.zero_stride ? w.zero_stride : w.d_out,
                    x_stride ? x_stride : w.d_in, out_stride ? out_stride : w.d_out, out_dtype == EFA_F32, aligned16(out) && (out_stride ? out_stride : w.d_out) % 4 == 0, kernel_status_word()};
+    const int elem = a.out_f32 ? 4 : 2;
+    if (rows_clash(RowSpan{out, rows, (long long)a.d_out * elem, a.out_stride * elem, elem}, RowSpan{X, rows, 2ll * a.d_in, 2 * a.x_stride, 2}, false)) {
+        set_error("project_w4: out overlaps X");
+        return 2;
+    }
+    const void* const mem[] = {X, w.codes, w.scales, w.zeros, out};
+    if (int rc = check_memory("project_w4", mem, 5)) return rc;
     // Up to eight rows the products of mma.sync are not the time. Beyond, tiles of 16 rows that read the weights again, or tcgen05 with up to 64 rows to a tile, whose start and
     // end cost more, and every group of a row its sums: by the work, in weights times tiles of 16, twice as much where a row has many groups. us, tiles of 16 / tcgen05: 16 rows, 4096 x 4096 6.7 /
     // 8.8, 2048 x 16384 12.0 / 11.1, 8192 x 8192 16.6 / 15.1; 32 rows, 4096 x 4096 9.7 / 9.5, 2048 x 8192 11.6 / 9.4; 64 rows, 1024 x 1024 3.4 / 7.3, 4096 x 4096 18 / 11.3. Groups of 64:

@@ -292,7 +292,8 @@ typedef struct efa_block_norm_params {
 const char* efa_block_norm_check(const efa_block_norm_params* p, int rows);
 
 /* y NULL: no block output (r = residual_scale * x: the norm before the first block; then neither post nor gate). x NULL: no residual. x_out or h NULL: not
- * wanted (not both). post_w, post_b, pre_w, pre_b: fp16 [d], NULL: ones and zeros. x_out and h may be x or y themselves where type and stride are the same.
+ * wanted (not both). post_w, post_b, pre_w, pre_b: fp16 [d], NULL: ones and zeros. x_out and h may be x or y themselves where type and stride are the same; an
+ * output that meets what is read in another way is refused (rows of one stride may lie in one another's gaps).
  * Tensors that begin at 16 bytes, with strides that are alike modulo 8 elements (dense ones are), go faster than others. The bits of a row do not depend on the other
  * rows, nor, if d is a multiple of 8, on its place among them. Asynchronous on `stream`. */
 int efa_block_norm(const void* x, const void* y, const void* gate, const void* post_w, const void* post_b, const void* pre_w, const void* pre_b,
@@ -315,7 +316,7 @@ const char* efa_w4_check(const efa_w4* w);
 /* out[rows][d_out] = X[rows][d_in] * w: efa_project_f16 for few rows, where reading the weights is all the time (the reference's project, attn_main.cu:262-273, is
  * fp32 throughout). X fp16, 16-byte aligned, x_stride (elements, 0 = dense) a multiple of 8; out fp16 (EFA_F16) or fp32 (EFA_F32), out_stride elements. Codes
  * minus zeros are fp16 numbers exactly; products and sums are fp32, the scales are applied to the sums of their groups: nothing is rounded but the result. Made
- * for up to 64 rows; more (2^19 at most) go in tiles that read the weights again. out does not overlap X. The order of the sum, and so the bits, depends on the sizes and
+ * for up to 64 rows; more (2^19 at most) go in tiles that read the weights again. An out that overlaps X is refused (rows of one stride may lie in one another's gaps). The order of the sum, and so the bits, depends on the sizes and
  * the number of SMs only. Asynchronous on `stream`. The first call on a device comes before any stream capture (the status word is allocated then). */
 int efa_project_w4(const void* X, int64_t x_stride, const efa_w4* w, void* out, int out_dtype, int64_t out_stride, int rows, void* stream);
 
