@@ -184,15 +184,12 @@ int check_memory(const char* what, const void* const* p, int n)
     return 0;
 }
 
-bool rows_clash(const RowSpan& out, const RowSpan& in, bool in_place)
+bool rows_meet(const RowSpan& out, const RowSpan& in, bool in_place)
 {
-    if (!out.at || !in.at || out.rows < 1 || in.rows < 1) return false;
-    const intptr_t a = reinterpret_cast<intptr_t>(out.at), b = reinterpret_cast<intptr_t>(in.at);
-    if (a + (out.rows - 1) * out.stride + out.width <= b || b + (in.rows - 1) * in.stride + in.width <= a) return false;
     const bool alike = out.stride == in.stride || (out.rows == 1 && in.rows == 1);
-    if (a == b && alike && out.elem == in.elem && out.width == in.width && out.rows == in.rows) return !in_place;
+    if (out.at == in.at && alike && out.elem == in.elem && out.width == in.width && out.rows == in.rows) return !in_place;
     if (out.stride != in.stride) return true;
-    const long long ahead = ((b - a) % out.stride + out.stride) % out.stride;  // bytes from a row of out to the next row of in
+    const long long ahead = ((in.at - out.at) % out.stride + out.stride) % out.stride;     // bytes from a row of out to the next row of in
     return ahead < out.width || ahead > out.stride - in.width;
 }
 

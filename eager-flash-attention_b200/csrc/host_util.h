@@ -70,11 +70,18 @@ bool own_device_memory(const void* p);
 // of each group that belongs together: 0.08 us each, of 4 us that a call takes on the host. Null pointers are passed over.
 int check_memory(const char* what, const void* const* p, int n);
 
-// Rows of a tensor in memory: `rows` of `width` bytes, `stride` bytes apart, of elements of `elem` bytes.
-struct RowSpan { const void* at; long long rows, width, stride; int elem; };
+// Rows of a tensor in memory: `rows` of `width` bytes, `stride` bytes apart, of elements of `elem` bytes, from `at` to `end`. Without memory: none.
+struct RowSpan {
+    intptr_t at, end;
+    long long rows, width, stride;
+    int elem;
+    RowSpan(const void* p, long long rows_, long long width_, long long stride_, int elem_)
+        : at(reinterpret_cast<intptr_t>(p)), end(p ? at + (rows_ - 1) * stride_ + width_ : at), rows(rows_), width(width_), stride(stride_), elem(elem_) {}
+};
+bool rows_meet(const RowSpan& out, const RowSpan& in, bool in_place);
 // Whether a call that writes `out` and reads `in` row by row would lose what it has to read: they meet, and not as the same rows of the same elements (which a call may allow:
 // in place). Rows of one stride may lie in one another's gaps; of two strides what meets is taken as lost.
-bool rows_clash(const RowSpan& out, const RowSpan& in, bool in_place);
+inline bool rows_clash(const RowSpan& out, const RowSpan& in, bool in_place) { return out.at < in.end && in.at < out.end && rows_meet(out, in, in_place); }
 
 inline bool aligned(const void* p, unsigned bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 inline bool aligned16(const void* p) { return aligned(p, 16); }
