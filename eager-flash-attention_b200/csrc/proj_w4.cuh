@@ -3,6 +3,7 @@
 
 #include "host_util.h"
 #include "sm100_ptx.cuh"
+#include "w4_plan.h"
 
 namespace efa {
 
@@ -65,6 +66,7 @@ __device__ __forceinline__ void store_sums(const W4Args& a, const float* sum, in
 }
 
 // tcgen05 over tiles of up to 64 rows (proj_w4_tc_sm100.cu).
-int w4_tc_launch(const W4Args& a, int group, cudaStream_t stream);
+int w4_tc_plan(const W4Args& a, int group, W4Division& to);
+int w4_tc_launch(const W4Args& a, int group, const W4Division& to, cudaStream_t stream);
 
 }  // namespace efa

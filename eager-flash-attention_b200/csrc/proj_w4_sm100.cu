@@ -351,10 +351,7 @@ int launch_w4(const W4Args& a, cudaStream_t stream)
     using C = W4Cfg<G, W4_MT, NT, WARPS>;
     constexpr auto kernel = proj_w4_kernel<G, W4_MT, NT, WARPS>;
     const int tiles = (a.d_out + C::CHANNELS - 1) / C::CHANNELS, row_tiles = (a.rows + 8 * NT - 1) / (8 * NT), units = (a.d_in + W4_K - 1) / W4_K;
-    // Few tiles: a cluster shares k, as long as every warp has a unit and every block an SM. us in 1 / 2 / 4 parts: 16 rows, 8192 x 1024 10.0 / 7.0 / 5.6,
-    // 4096 x 4096 (one part) 6.8 / 7.2.
-    int parts = 1;
-    while (parts < 8 && 2 * parts * WARPS <= units && (long long)tiles * row_tiles * 2 * parts <= device_sms()) parts *= 2;
+    const int parts = w4_parts((long long)tiles * row_tiles, units, WARPS, device_sms());
     CUtensorMap codes;
     const unsigned long long dims[2] = {(unsigned long long)a.d_in / 2, (unsigned long long)a.d_out}, strides[1] = {(unsigned long long)a.code_stride};
     const unsigned box[2] = {W4_K / 2, C::CHANNELS};
@@ -427,11 +424,12 @@ int project_w4(const void* X, long long x_stride, const efa_w4& w, void* out, in
     const void* const mem[] = {X, w.codes, w.scales, w.zeros, out};
     if (int rc = check_memory("project_w4", mem, 5)) return rc;
     // Up to eight rows the products of mma.sync are not the time. Beyond, tiles of 16 rows that read the weights again, or tcgen05 with up to 64 rows to a tile, whose start and
-    // end cost more, and every group of a row its sums: by the work, in weights times tiles of 16, twice as much where a row has many groups. us, tiles of 16 / tcgen05: 16 rows, 4096 x 4096 6.7 /
-    // 8.8, 2048 x 16384 12.0 / 11.1, 8192 x 8192 16.6 / 15.1; 32 rows, 4096 x 4096 9.7 / 9.5, 2048 x 8192 11.6 / 9.4; 64 rows, 1024 x 1024 3.4 / 7.3, 4096 x 4096 18 / 11.3. Groups of 64:
-    // 12 rows, 4096 x 6144 9.4 / 10.5, 32 rows, 2048 x 6144 9.6 / 8.9; of 32: 16 rows, 4096 x 8192 11.1 / 13.3, 64 rows, 4096 x 2048 10.2 / 14.5, 1056 x 4160 9.8 / 10.7, 4096 x 4096 19.8 / 18.1.
-    const double most = w.d_in >= 64 * w.group ? 1 << 25 : 1 << 24;
-    if (rows > 8 && (double)((rows + 15) / 16) * w.d_in * w.d_out > most) return w4_tc_launch(a, w.group, stream);
+    // end cost more, and every group of a row its sums: by what either takes (w4_plan.h).
+    if (rows > 8) {
+        W4Division to;
+        if (int rc = w4_tc_plan(a, w.group, to)) return rc;
+        if (w4_tc_time(to, w.d_in, w.d_out, rows, w.group) < w4_mma_time(w.d_in, w.d_out, rows, w.group, device_sms())) return w4_tc_launch(a, w.group, to, stream);
+    }
     return w.group == 128 ? launch_group<128>(a, stream) : w.group == 64 ? launch_group<64>(a, stream) : launch_group<32>(a, stream);
 }
 

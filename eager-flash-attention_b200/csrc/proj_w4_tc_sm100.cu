@@ -11,7 +11,6 @@
 // for its place needs registers that the block does not have (49 us with spills); a tile of 256 channels to an SM leaves 20 of 148 SMs without one. 4096 x 4096, 64 rows: 11.2 us, of which start
 // and sums of the cluster are 5.
 #include "proj_w4.cuh"
-#include "w4_plan.h"
 
 #include <algorithm>
 #include <atomic>
@@ -319,11 +318,11 @@ int clusters_at_once(int p, int smem, int dev, int& n)
 }
 
 template <int G, int N>
-int launch_tc(const W4Args& a, cudaStream_t stream)
+int plan_tc(const W4Args& a, W4Division& to)
 {
     using C = TcCfg<G, N>;
     constexpr auto kernel = proj_w4_tc_kernel<G, N>;
-    const int units = (a.d_in + W4_UNIT - 1) / W4_UNIT, row_tiles = (a.rows + 63) / 64;
+    const int units = (a.d_in + W4_UNIT - 1) / W4_UNIT;
     static std::atomic<bool> set[64];
     int dev = 0;
     EFA_CUDA(cudaGetDevice(&dev));
@@ -334,7 +333,16 @@ int launch_tc(const W4Args& a, cudaStream_t stream)
     int at_once[W4_MAX_PARTS + 1] = {};
     for (int p = 1; p <= std::min(W4_MAX_PARTS, units); p++)
         if (int rc = clusters_at_once<kernel>(p, C::SMEM, dev, at_once[p])) return rc;
-    const auto [channels, parts] = w4_division(a.d_out, row_tiles, units, at_once);
+    to = w4_division(a.d_out, (a.rows + 63) / 64, units, at_once);
+    return 0;
+}
+
+template <int G, int N>
+int launch_tc(const W4Args& a, const W4Division& to, cudaStream_t stream)
+{
+    using C = TcCfg<G, N>;
+    constexpr auto kernel = proj_w4_tc_kernel<G, N>;
+    const int channels = to.channels;
     CUtensorMap codes, x;
     const unsigned long long code_dims[2] = {(unsigned long long)a.d_in / 2, (unsigned long long)a.d_out}, code_stride[1] = {(unsigned long long)a.code_stride};
     const unsigned code_box[2] = {64, 2 * (unsigned)channels};
@@ -350,22 +358,30 @@ int launch_tc(const W4Args& a, cudaStream_t stream)
         const unsigned box[2] = {64, N};
         if (make_tmap_f16(&x, a.X, 2, dims, strides, box)) return 1;
     }
-    const dim3 grid((a.d_out + 2 * channels - 1) / (2 * channels), row_tiles, parts);
+    const dim3 grid((a.d_out + 2 * channels - 1) / (2 * channels), (a.rows + 63) / 64, to.parts);
     EFA_CUDA(launch_value(kernel, grid, TC_THREADS, C::SMEM, stream, a, channels, x_blocks, codes, x));
     return 0;
 }
 
 template <int G>
-int launch_rows(const W4Args& a, cudaStream_t stream)
+int plan_rows(const W4Args& a, W4Division& to) { return a.rows <= 16 ? plan_tc<G, 16>(a, to) : a.rows <= 32 ? plan_tc<G, 32>(a, to) : plan_tc<G, 64>(a, to); }
+
+template <int G>
+int launch_rows(const W4Args& a, const W4Division& to, cudaStream_t stream)
 {
-    return a.rows <= 16 ? launch_tc<G, 16>(a, stream) : a.rows <= 32 ? launch_tc<G, 32>(a, stream) : launch_tc<G, 64>(a, stream);
+    return a.rows <= 16 ? launch_tc<G, 16>(a, to, stream) : a.rows <= 32 ? launch_tc<G, 32>(a, to, stream) : launch_tc<G, 64>(a, to, stream);
 }
 
 }  // namespace
 
-int w4_tc_launch(const W4Args& a, int group, cudaStream_t stream)
+int w4_tc_plan(const W4Args& a, int group, W4Division& to)
 {
-    return group == 128 ? launch_rows<128>(a, stream) : group == 64 ? launch_rows<64>(a, stream) : launch_rows<32>(a, stream);
+    return group == 128 ? plan_rows<128>(a, to) : group == 64 ? plan_rows<64>(a, to) : plan_rows<32>(a, to);
+}
+
+int w4_tc_launch(const W4Args& a, int group, const W4Division& to, cudaStream_t stream)
+{
+    return group == 128 ? launch_rows<128>(a, to, stream) : group == 64 ? launch_rows<64>(a, to, stream) : launch_rows<32>(a, to, stream);
 }
 
 }  // namespace efa

@@ -1,4 +1,4 @@
-"""How the products of 4-bit weights are divided among clusters, on the CPU: never into clusters that the device cannot hold."""
+"""Which kernel the products of 4-bit weights take, and how they are divided among clusters, on the CPU: never into clusters that the device cannot hold."""
 import ctypes
 import os
 import subprocess
@@ -12,24 +12,34 @@ SOURCE = """
 extern "C" void divide(int d_out, int row_tiles, int units, const int* at_once, int* out)
 {
     const efa::W4Division to = efa::w4_division(d_out, row_tiles, units, at_once);
-    out[0] = to.channels; out[1] = to.parts;
+    out[0] = to.channels; out[1] = to.parts; out[2] = (int)to.rounds; out[3] = to.units;
+}
+extern "C" int tcgen05(int d_in, int d_out, int rows, int group, const int* at_once)
+{
+    const efa::W4Division to = efa::w4_division(d_out, (rows + 63) / 64, (d_in + 127) / 128, at_once);
+    return efa::w4_tc_time(to, d_in, d_out, rows, group) < efa::w4_mma_time(d_in, d_out, rows, group, 148);
 }
 """
-B200 = [0, 148, 70, 46, 34, 26, 23, 18, 16]           # one block to an SM, clusters within one part of the GPU
+B200 = [0, 148, 74, 45, 33, 26, 22, 15, 15]           # one block to an SM, clusters within one part of the GPU
 
 
 @pytest.fixture(scope="module")
-def divide(tmp_path_factory):
+def library(tmp_path_factory):
     d = tmp_path_factory.mktemp("division")
     (d / "divide.cpp").write_text(SOURCE)
     subprocess.run(["g++", "-O1", "-std=c++17", "-shared", "-fPIC", "-I", os.path.join(ROOT, "eager-flash-attention_b200", "csrc"),
                     str(d / "divide.cpp"), "-o", str(d / "divide.so")], check=True)
-    lib = ctypes.CDLL(str(d / "divide.so"))
+    return ctypes.CDLL(str(d / "divide.so"))
 
+
+@pytest.fixture(scope="module")
+def divide(library):
     def run(d_out, row_tiles, units, at_once):
-        out = (ctypes.c_int * 2)()
-        lib.divide(d_out, row_tiles, units, (ctypes.c_int * 9)(*at_once), out)
-        return tuple(out)
+        out = (ctypes.c_int * 4)()
+        library.divide(d_out, row_tiles, units, (ctypes.c_int * 9)(*at_once), out)
+        c, p, rounds, share = out
+        assert share == -(-units // p) and rounds == -(-(-(-d_out // (2 * c)) * row_tiles) // max(1, at_once[p]))
+        return c, p
     return run
 
 
@@ -56,3 +66,23 @@ def test_clusters_that_do_not_fit_are_no_choice(divide, missing):
 def test_a_block_by_itself_there_always_is(divide):
     for size in SIZES:
         assert divide(*size, [0] * 9)[1] == 1
+
+
+# (d_in, d_out, group, rows): us on mma.sync, on tcgen05, where they are further apart than the figures are off.
+MEASURED = {(1024, 1024, 128, 16): (3.07, 4.91), (4096, 2048, 32, 9): (5.44, 8.16), (16384, 1024, 32, 33): (21.1, 33.9), (16384, 1024, 64, 64): (19.4, 22.6), (8192, 2048, 32, 48): (17.7, 20.9),
+            (4096, 4096, 64, 16): (7.14, 9.16), (8192, 1024, 128, 16): (6.37, 8.88), (6144, 2048, 32, 64): (14.1, 17.8), (5120, 1536, 32, 96): (12.4, 16.0),
+            (512, 8192, 128, 64): (15.5, 8.5), (512, 8192, 32, 64): (16.1, 9.5), (1536, 5120, 128, 32): (8.98, 7.43), (8192, 2048, 128, 17): (11.5, 9.8), (8192, 8192, 128, 16): (18.0, 14.5),
+            (4096, 14336, 64, 12): (17.8, 15.4), (14336, 4096, 128, 9): (19.3, 15.3)}
+
+
+def test_the_kernel_that_was_measured_to_be_faster(library):
+    at_once = (ctypes.c_int * 9)(*B200)
+    for size, (mma, tc) in MEASURED.items():
+        assert library.tcgen05(size[0], size[1], size[3], size[2], at_once) == (tc < mma), size
+
+
+def test_the_largest_sizes_are_counted_without_overflow(library):
+    at_once = (ctypes.c_int * 9)(*B200)
+    for group in (32, 64, 128):
+        assert library.tcgen05(1 << 24, 1 << 24, 1 << 19, group, at_once) == 1
+        assert library.tcgen05(1 << 24, 1, 9, group, at_once) in (0, 1) and library.tcgen05(group, 1 << 24, 1 << 19, group, at_once) in (0, 1)
