@@ -295,7 +295,7 @@ const char* efa_block_norm_check(const efa_block_norm_params* p, int rows);
  * wanted (not both). post_w, post_b, pre_w, pre_b: fp16 [d], NULL: ones and zeros. x_out and h may be x or y themselves where type and stride are the same; an
  * output that meets what is read in another way is refused (rows of one stride may lie in one another's gaps).
  * Tensors that begin at 16 bytes, with strides that are alike modulo 8 elements (dense ones are), go faster than others. The bits of a row do not depend on the other
- * rows, nor, if d is a multiple of 8, on its place among them. Asynchronous on `stream`. */
+ * rows, nor, if d and all strides are multiples of 8, on its place among them. Asynchronous on `stream`. */
 int efa_block_norm(const void* x, const void* y, const void* gate, const void* post_w, const void* post_b, const void* pre_w, const void* pre_b,
                    void* x_out, void* h, int rows, const efa_block_norm_params* p, void* stream);
 
