@@ -228,7 +228,7 @@ int efa_paged_attention(const void* Q, void* O, const efa_paged_cache* cache, co
  * A page that is not full belongs to one sequence: efa_pages_fork copies it, full pages are shared. So efa_cache_write always writes into pages of one sequence.
  * Calls change the arrays in stream order; a captured graph follows their contents. The first call on a device comes before any stream capture. What is found wrong is reported by efa_kernel_status (site 60
  * take, 61 fork, 62 free, 63 compact, 64 copy; sequence or page in place of the block) and the call stays inside its buffers: code 2 a page outside the
- * pool (the entry counts as no page), 3 a length outside the table, 4 no free page (the entry becomes -1, whose keys efa_cache_write does not
+ * pool (the entry counts as no page; -1 is passed over, but for efa_pages_fork, which reports a parent's too), 3 a length outside the table, 4 no free page (the entry becomes -1, whose keys efa_cache_write does not
  * write and attention reads as zeros), 5 a sequence that may not be named (outside the pool of
  * slots, where its place in the list is what is reported; or a child that is not empty or named twice). */
 typedef struct efa_page_pool {
