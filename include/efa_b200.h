@@ -316,8 +316,8 @@ const char* efa_w4_check(const efa_w4* w);
 /* out[rows][d_out] = X[rows][d_in] * w: efa_project_f16 for few rows, where reading the weights is all the time (the reference's project, attn_main.cu:262-273, is
  * fp32 throughout). X fp16, 16-byte aligned, x_stride (elements, 0 = dense) a multiple of 8; out fp16 (EFA_F16) or fp32 (EFA_F32), out_stride elements. Codes
  * minus zeros are fp16 numbers exactly; products and sums are fp32, the scales are applied to the sums of their groups: nothing is rounded but the result. Made
- * for up to 64 rows; more (2^19 at most) go in tiles that read the weights again. An out that overlaps X is refused (rows of one stride may lie in one another's gaps). The order of the sum, and so the bits, depends on the sizes and
- * the number of SMs only. Asynchronous on `stream`. The first call on a device comes before any stream capture (the status word is allocated then). */
+ * for up to 64 rows; more (2^19 at most) go in tiles that read the weights again. An out that overlaps X is refused (rows of one stride may lie in one another's gaps). The order of the sum, and so the bits, depends on the
+ * sizes (rows and group among them) and on the GPU: its SMs, and the clusters that it holds at a time. Asynchronous on `stream`. The first call on a device comes before any stream capture (the status word is allocated then). */
 int efa_project_w4(const void* X, int64_t x_stride, const efa_w4* w, void* out, int out_dtype, int64_t out_stride, int rows, void* stream);
 
 /* Status word written by kernels whose bounded waits ran out, or that found lengths or pages of a paged batch wrong: out4 = {code, block, site, 0};
