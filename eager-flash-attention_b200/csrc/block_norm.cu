@@ -77,9 +77,18 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
 }
 
 // e = exp(-|g|) does not overflow, and e / (1 + e) or 1 / (1 + e) is the sigmoid: 1 / (1 + exp(-g)) is nothing below -87.3, where a large value is not yet small. All
-// of it 2^24 times itself, so that an e down to 2^-150 is a normal number (one gate at a time with subnormals: calls of 8192 x 4096 65.2 us for 63.7).
-__device__ __forceinline__ float2 sigmoid(float2 g)
+// of it 2^24 times itself, so that an e down to 2^-150 is a normal number.
+__device__ __forceinline__ float sigmoid(float g)
 {
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fmaf(g < 0.f ? g : -g, 1.44269504f, 24.f)));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(e + 16777216.f));
+    return (g < 0.f ? e : 16777216.f) * r;
+}
+// v times the sigmoid of g: in pairs where the threads have whole chunks (calls of 8192 x 4096 62.4 us one by one, 62.1 so); elsewhere pairs cost registers that there are not.
+template <bool PAIRS> __device__ __forceinline__ float2 gated(float2 v, float2 g)
+{
+    if constexpr (!PAIRS) return make_float2(v.x * sigmoid(g.x), v.y * sigmoid(g.y));
     const float2 t = fma2(make_float2(fabsf(g.x), fabsf(g.y)), two(-1.44269504f), two(24.f));
     float2 e, r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(t.x));
@@ -87,7 +96,7 @@ __device__ __forceinline__ float2 sigmoid(float2 g)
     const float2 sum = add2(e, two(16777216.f));
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(sum.x));
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(sum.y));
-    return mul2(make_float2(g.x < 0.f ? e.x : 16777216.f, g.y < 0.f ? e.y : 16777216.f), r);
+    return mul2(v, mul2(make_float2(g.x < 0.f ? e.x : 16777216.f, g.y < 0.f ? e.y : 16777216.f), r));
 }
 
 __device__ __forceinline__ float element(const void* row, bool f32, int e) { return f32 ? static_cast<const float*>(row)[e] : __half2float(static_cast<const __half*>(row)[e]); }
@@ -335,7 +344,7 @@ block_norm_kernel(const NormArgs a)
         if (a.gate) {
             numbers<MODE>(g[LAZY ? 0 : c], false, n);
             #pragma unroll
-            for (int i = 0; i < 4; i++) v[c][i] = mul2(v[c][i], a.sigmoid ? sigmoid(n[i]) : n[i]);
+            for (int i = 0; i < 4; i++) v[c][i] = a.sigmoid ? gated<MODE == ALIGNED>(v[c][i], n[i]) : mul2(v[c][i], n[i]);
         }
         if (a.x) {
             numbers<MODE>(x[LAZY ? 0 : c], x_f32, n);
@@ -350,7 +359,7 @@ block_norm_kernel(const NormArgs a)
     #pragma unroll
     for (int k = 0; k < ENDS; k++) {
         if (p.end(k) >= a.d) continue;
-        if (a.gate) ends[k] *= a.sigmoid ? sigmoid(two(g_ends[k])).x : g_ends[k];
+        if (a.gate) ends[k] *= a.sigmoid ? sigmoid(g_ends[k]) : g_ends[k];
         ends[k] = a.x ? summed(ends[k], x_ends[k]) : a.block_scale * ends[k];
         if (a.x_out && there) store1(out, x_f32, p.end(k), ends[k]);
     }
