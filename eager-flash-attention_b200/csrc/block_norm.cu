@@ -2,8 +2,9 @@
 // in fp32: its sums are taken over what is there already, and nothing is read twice. Layer norms sum the squares of what is left when the mean is
 // taken off, not the squares less the mean's: a mean far above the spread costs no digits.
 //
-// Memory is the floor: x, y, the gate, x_out and h once. 8192 x 4096 with a gate of every row 54.8 us, 6.1 TB/s (94 % of a copy's rate); 16384 x 1024 two layer norms 27.0 (76 %: two passes over
-// registers between barriers), 2000 x 12000 fp32 75.7 (78 %), 1237 x 2049 fp32 8.7 (62 %: little more than a round); one row 3.1, of which the launch is 2.
+// Memory is the floor: x, y, the gate, x_out and h once. GPU time in graphs of 30 calls, some milliseconds: 8192 x 4096 with a gate of every row 54.8 us, 6.1 TB/s (94 % of a copy's rate; after a second of such
+// calls, at the power cap, 62, 83 %); 16384 x 1024 two layer norms 27.0 (76 %: two passes over registers between barriers), 2000 x 12000 fp32 75.7 (78 %), 1237 x 2049 fp32 8.7 (62 %: little more than
+// a round); one row 3.1, of which the launch is 2.
 #include "host_util.h"
 #include "serving.h"
 #include "sm100_ptx.cuh"
@@ -270,7 +271,8 @@ __device__ __forceinline__ void normalise(float2 (&v)[NC][4], float (&ends)[2], 
     }
 }
 
-// Blocks that registers are kept free for: 64 to 128 of them to a thread.
+// Blocks that registers are kept free for: 64 to 128 of them to a thread. A kernel that takes fewer may have one block more. Rows above 16384 (1024 threads, four chunks, 64 registers) do not fit
+// whole: five of the six kernels spill 36 to 172 bytes a thread.
 constexpr int blocks_per_sm(int threads, int chunks, bool lean, bool lazy)
 {
     const int registers = chunks == 1 ? 64 : lazy ? 64 : chunks == 2 ? (lean ? 64 : 96) : chunks == 3 ? (lean ? 80 : 112) : 128;
@@ -323,7 +325,8 @@ block_norm_kernel(const NormArgs a)
         #pragma unroll
         for (int c = 0; c < NC; c++) numbers<MODE>(y[c], y_f32, v[c]);
     }
-    // While a block has its row, memory would wait: it fetches the row of the block that will have its place, as soon as its own is there (not before, which delays it). us, without / with:
+    // While a block has its row, memory would wait: it fetches the row of the block that will have its place (or of one of those before it, where more blocks are resident than the launch's bound says: rows
+    // that somebody is reading then), as soon as its own is there (not before, which delays it). us, without / with:
     // 8192 x 4096 60.2 / 54.8, 512 x 16384 fp32 34.6 / 31.7, 1000 x 5001 fp32 25.5 / 22.6; half as far again 2 to 4 % more; several rows to a warp nothing.
     auto prefetch = [&]() {
         if (T <= 32 || lane != 0 || a.rows - a.ahead <= at) return;

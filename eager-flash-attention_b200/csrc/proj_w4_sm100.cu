@@ -4,11 +4,12 @@
 // mma.sync m16n8k16 with the weights as the side of 16 (output channels) and the rows of X as the side of 8: one token uses an eighth of it. The order of k
 // within a group is free as long as both sides agree on it, so codes go from memory to a fragment as they lie: a lane's word is eight neighbouring k of one
 // channel, `(word >> 4 i) & 0x000f000f` is the pair (k + i, k + i + 4) of two products' fragments, and x is paired alike. A code c becomes the fp16 number
-// 1024 + c (or 1024 + 16 c, times 1/16) by one logical operation, and c - zero exactly by one more: nine instructions to eight weights. All four lanes that share a
-// channel are in one group: 16, 8 or 4 bytes to a lane for groups of 128, 64 or 32.
+// 1024 + c (or 1024 + 16 c, times 1/16) by one logical operation, and c - zero exactly by one more: nine instructions to eight weights. (Integers that are put into a float's mantissa below a power of
+// two: the method of Kim et al., "Who Says Elephants Can't Run", 2022, for weights of 4 and 8 bits.) All four lanes that share a channel are in one group: 16, 8 or 4 bytes to a lane for
+// groups of 128, 64 or 32.
 //
 // Reading the weights is the floor (a group of 128: 0.516 bytes each). What bounds it: up to some 10 us the way from the launch to the first codes, the sums and the end (one row,
-// 4096 x 4096: 4.5 us of which the bytes are 1.3; 1056 x 4163: 2.9). Beyond, instructions: 624 to 656 to a warp's 32 channels x 256 k, of which 320 make fragments and multiply, issued
+// 4096 x 4096: 4.1 us of which the bytes are 1.3; 1056 x 4163: 3.0). From six rows on a warp waits for each of its units: there is no room for a second one in flight. Beyond, instructions: 624 to 656 to a warp's 32 channels x 256 k, of which 320 make fragments and multiply, issued
 // at 0.6 to a cycle and scheduler (one row, 8192 x 32768: 33 us, 4.1 TB/s of the 6.5; 2048 x 65536: 21 us; without the scales' part, a tenth of the instructions, a tenth less).
 #include "proj_w4.cuh"
 #include "serving.h"
@@ -20,7 +21,8 @@ namespace efa {
 
 namespace {
 
-// Sixteen warps to an SM, in one block or two: four to a scheduler hide one another's waits. Of up to three stages as many as have room.
+// Sixteen warps to an SM, in one block or two: four to a scheduler hide one another's waits. Of up to three stages as many as have room: two up to five rows (four with groups of 32), one beyond.
+// The kernels of 9 to 16 rows with groups of 64 and 128 spill 24 and 44 bytes a thread at 128 registers.
 constexpr int W4_STAGES = 3;
 constexpr int W4_MT = 2;                // tiles of 16 channels to a warp
 
@@ -102,7 +104,7 @@ template <int G> __device__ __forceinline__ int x_place(int row, int c)
 }
 
 // A block: 16 MT channels, 8 NT rows, all k, its warps (and the blocks of its cluster, along z) taking the units of 256 k in turn, added at the end in shared
-// memory in the order of the warps and blocks. A warp has its own units copied ahead, codes by TMA, X by its lanes: nobody waits for anybody before the sums.
+// memory in the order of the warps and blocks. A warp copies its own units, ahead where there is more than one stage, codes by TMA, X by its lanes: nobody waits for anybody before the sums.
 template <int G, int MT, int NT, int WARPS>
 __global__ void __launch_bounds__(32 * WARPS, 16 / WARPS)
 proj_w4_kernel(const W4Args a, int stages, const __grid_constant__ CUtensorMap codes_map)

@@ -6,7 +6,8 @@
 // addition takes the zero point off, exactly. X goes to shared memory as it lies (TMA). A group's sums come back in fp32 and are added up times scale * 2^24, by warps of their own.
 //
 // Why not the weights in shared memory: they would be written there and read again by the tensor core, 256 bytes for 64 of codes; in tensor memory the thread that has a channel's codes
-// writes them where they are used. What bounds it (8192 x 32768: 64 rows 44.7 us, 3.2 TB/s, 770 TFLOP/s; 16 rows 37.9): making the operand. A unit of 128 k x 256 channels takes some 3300 warp
+// writes them where they are used. What bounds it (8192 x 32768 in graphs of 30 calls: 64 rows 44.7 us, 3.2 TB/s, 770 TFLOP/s; after a second of them, at the power cap, 52,
+// 660 TFLOP/s; 16 rows 37.9): making the operand. A unit of 128 k x 256 channels takes some 3300 warp
 // instructions, 768 of them the six logical ones to a word; of its 1290 cycles the logical pipe worked 57 % and the schedulers issued 71 % with seven (odd codes shifted: 45.8 and 39.4 us). More of the operand made before the wait
 // for its place needs registers that the block does not have (49 us with spills); a tile of 256 channels to an SM leaves 20 of 148 SMs without one. 4096 x 4096, 64 rows: 11.2 us, of which start
 // and sums of the cluster are 5.
