@@ -186,11 +186,12 @@ int check_memory(const char* what, const void* const* p, int n)
 
 bool rows_meet(const RowSpan& out, const RowSpan& in, bool in_place)
 {
-    const bool alike = out.stride == in.stride || (out.rows == 1 && in.rows == 1);
-    if (out.at == in.at && alike && out.elem == in.elem && out.width == in.width && out.rows == in.rows) return !in_place;
-    if (out.stride != in.stride) return true;
-    const long long ahead = ((in.at - out.at) % out.stride + out.stride) % out.stride;     // bytes from a row of out to the next row of in
-    return ahead < out.width || ahead > out.stride - in.width;
+    const bool alone = out.rows == 1 && in.rows == 1;
+    if (out.at == in.at && (alone || out.stride == in.stride) && out.elem == in.elem && out.width == in.width && out.rows == in.rows) return !in_place;
+    if (alone || (out.rows > 1 && in.rows > 1 && out.stride != in.stride)) return true;
+    const long long stride = out.rows > 1 ? out.stride : in.stride;                // one row has none
+    const long long ahead = ((in.at - out.at) % stride + stride) % stride;         // bytes from a row of out to the next row of in
+    return ahead < out.width || ahead > stride - in.width;
 }
 
 static int make_tmap(CUtensorMap* out, CUtensorMapDataType type, unsigned elem_bytes, const void* base, int rank,

@@ -57,3 +57,15 @@ def test_projections(pkg):
     assert "overlap" not in call(AT, AT + 512, 9, x_stride=304, out_stride=304)                     # columns of one tensor
     assert "out overlaps X" in call(AT, AT + 512, 9, x_stride=304, out_stride=304, out_dtype=pkg.F32)
     assert "out overlaps X" in call(AT, AT + 510, 9, x_stride=304, out_stride=304)
+
+
+def test_one_row_between_others(pkg):
+    """A vector in the gaps of strided rows, and one output row in the gaps of what is read."""
+    kw = dict(out_stride=128, h_stride=128)
+    assert "overlap" not in norm(pkg, 9, 64, AT, B, C, None, gate=C + 128, **kw)
+    assert "x_out overlaps gate" in norm(pkg, 9, 64, AT, B, C, None, gate=C + 64, **kw)
+    assert "x_out overlaps gate" in norm(pkg, 9, 64, AT, B, C, None, gate=C + 192, **kw)
+    assert "overlap" not in norm(pkg, 9, 64, AT, B, C, C + 128, pre_w=C + 9 * 256, **kw)
+    assert "h overlaps pre_w" in norm(pkg, 9, 64, AT, B, C, C + 128, pre_w=C + 128 + 256, **kw)
+    assert "x_out and h overlap" in norm(pkg, 1, 64, AT, B, C, C + 64)
+    assert "overlap" not in norm(pkg, 1, 64, AT, B, C, C + 128)
