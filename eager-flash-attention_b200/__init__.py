@@ -468,13 +468,15 @@ def cache_read(K, V, cache: PagedCache, batch: PagedBatch, stream=None, head_str
     _check(lib().efa_cache_read(K, V, head_stride, token_stride, cache, batch, _stream(stream)), "cache_read")
 
 
-def _bytes(what: str, workspace) -> int:
-    """Bytes of a workspace: of a dense tensor, as the kernels write what lies between the rows of others, and behind an expanded one."""
+def _space(what: str, workspace, workspace_bytes: Optional[int]):
+    """Address and bytes of a workspace: of a dense tensor (the kernels would write what lies between the rows of others, and behind an expanded one), or as they are given."""
+    if workspace_bytes is not None:
+        return _ptr(workspace), workspace_bytes
     if workspace is None:
-        return 0
+        return None, 0
     if not workspace.is_contiguous():
         raise EfaError(f"{what}: the workspace must be a dense tensor")
-    return workspace.numel() * workspace.element_size()
+    return workspace.data_ptr(), workspace.nbytes
 
 
 def paged_attention_workspace(cache: PagedCache, batch: PagedBatch, ap: PagedAttentionParams) -> int:
@@ -490,14 +492,13 @@ def paged_attention(Q, O, cache: PagedCache, batch: PagedBatch, ap: PagedAttenti
     """Attention of the batch's chunks over the cache, which holds their own keys already: O ``[tokens][H_q * d_h]`` fp16.
     ``workspace``: a tensor of at least paged_attention_workspace bytes (or an address, with ``workspace_bytes``), not used by any
     other call until this one is done. Asynchronous on ``stream``."""
-    if workspace_bytes is None:
-        workspace_bytes = _bytes("paged_attention", workspace)
+    space, size = _space("paged_attention", workspace, workspace_bytes)
     tokens, d_h, by_head, by_token, o_token = batch.tokens, cache.d_h, ap.q_head_stride, ap.q_token_stride, ap.o_token_stride
     width = ap.H_q * d_h
     need = (ap.H_q - 1) * by_head + (tokens - 1) * by_token + d_h if by_head or by_token else width * tokens
     Q = _rows("paged_attention", Q, batch, need, not (by_head or by_token))
     O = _rows("paged_attention", O, batch, (tokens - 1) * o_token + width if o_token else width * tokens, not o_token)
-    _check(lib().efa_paged_attention(Q, O, cache, batch, ap, _ptr(workspace), workspace_bytes, _stream(stream)), "paged_attention")
+    _check(lib().efa_paged_attention(Q, O, cache, batch, ap, space, size, _stream(stream)), "paged_attention")
 
 
 # ------------------------------------------------------------------------------------------------
@@ -546,10 +547,6 @@ def _pairs(what: str, a, b) -> int:
     if a.numel() != b.numel():
         raise EfaError(f"{what} must be as many")
     return a.numel()
-
-
-def _space(what: str, workspace, workspace_bytes: Optional[int]):
-    return _ptr(workspace), _bytes(what, workspace) if workspace_bytes is None else workspace_bytes
 
 
 def pages_take(pool: PagePool, q_start, workspace, stream=None, workspace_bytes: Optional[int] = None) -> None:
@@ -639,8 +636,10 @@ def _matrix(what: str, x, rows: int, width: int, stride: int, kind: int) -> Opti
     try:
         if _real.get(x.dtype) == kind:
             if not stride:
-                if x.is_contiguous() and ((n := x.numel()) == (need := rows * width) or (n > need and x.shape[-1] == width)):
-                    return x.data_ptr()
+                if x.is_contiguous():
+                    more = x.numel() - rows * width
+                    if not more or (more > 0 and x.shape[-1] == width):
+                        return x.data_ptr()
             elif x.stride()[-2:] == (stride, 1) and x.shape[-1] >= width and x.shape[-2] >= rows:
                 return x.data_ptr()
     except AttributeError:
@@ -659,6 +658,16 @@ def _matrix(what: str, x, rows: int, width: int, stride: int, kind: int) -> Opti
     if x.dim() > 1 and not _rows_of(x, rows, width, stride):
         raise EfaError(f"{what}: a tensor of shape {list(x.shape)} is not {rows} rows of {width}" + (f", {stride} apart" if stride else ""))
     return x.data_ptr()
+
+
+def _vector(what: str, x, width: int) -> Optional[int]:
+    """Address of ``width`` fp16 elements."""
+    try:
+        if _real.get(x.dtype) == F16 and x.numel() == width and x.is_contiguous():
+            return x.data_ptr()
+    except AttributeError:
+        return _ptr(x)
+    return _matrix(what, x, 1, width, 0, F16)
 
 
 def block_norm_params(d: int, kind: int = NORM_RMS, eps: float = 1e-6, post: bool = False, pre: bool = True, gate: int = GATE_NONE, gate_rows: bool = False,
@@ -686,8 +695,8 @@ def block_norm(x, y, x_out, h, rows: int, bp: BlockNormParams, gate=None, post_w
     rc = (_lib or lib()).efa_block_norm(
         _matrix("block_norm: x", x, rows, d, x_stride, x_dtype), _matrix("block_norm: y", y, rows, d, y_stride, y_dtype),
         _matrix("block_norm: gate", gate, rows if gate_rows else 1, d, gate_stride, F16),
-        post_w if post_w is None else _matrix("block_norm: post_w", post_w, 1, d, 0, F16), post_b if post_b is None else _matrix("block_norm: post_b", post_b, 1, d, 0, F16),
-        pre_w if pre_w is None else _matrix("block_norm: pre_w", pre_w, 1, d, 0, F16), pre_b if pre_b is None else _matrix("block_norm: pre_b", pre_b, 1, d, 0, F16),
+        post_w if post_w is None else _vector("block_norm: post_w", post_w, d), post_b if post_b is None else _vector("block_norm: post_b", post_b, d),
+        pre_w if pre_w is None else _vector("block_norm: pre_w", pre_w, d), pre_b if pre_b is None else _vector("block_norm: pre_b", pre_b, d),
         _matrix("block_norm: x_out", x_out, rows, d, out_stride, x_dtype), _matrix("block_norm: h", h, rows, d, h_stride, F16),
         rows, bp, _stream(stream))
     if rc:
@@ -722,8 +731,9 @@ def project_w4(X, w: W4, out, rows: int, stream=None, x_stride: int = 0, out_str
     """``out[rows][d_out] = X[rows][d_in] @ w``, out fp16 or fp32 (``out_dtype`` where out is an address; strides in elements, 0 = dense). Made for few rows; prompts
     go through ``project`` with fp16 weights. Asynchronous on ``stream``."""
     if out_dtype is None:
-        out_dtype = _real.get(getattr(out, "dtype", None))
-        if out_dtype is None:
+        try:
+            out_dtype = _real[out.dtype]
+        except (AttributeError, KeyError):
             out_dtype = _dtype("project_w4: out", out) if hasattr(out, "dtype") else F16
     rc = (_lib or lib()).efa_project_w4(_matrix("project_w4: X", X, rows, w.d_in, x_stride, F16), x_stride, w,
                                         _matrix("project_w4: out", out, rows, w.d_out, out_stride, out_dtype), out_dtype, out_stride, rows, _stream(stream))

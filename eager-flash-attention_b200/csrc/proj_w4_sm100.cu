@@ -348,12 +348,12 @@ proj_w4_kernel(const W4Args a, int stages, const __grid_constant__ CUtensorMap c
 }
 
 template <int G, int NT, int WARPS>
-int launch_w4(const W4Args& a, cudaStream_t stream)
+int launch_w4(const W4Args& a, int sms, cudaStream_t stream)
 {
     using C = W4Cfg<G, W4_MT, NT, WARPS>;
     constexpr auto kernel = proj_w4_kernel<G, W4_MT, NT, WARPS>;
     const int tiles = (a.d_out + C::CHANNELS - 1) / C::CHANNELS, row_tiles = (a.rows + 8 * NT - 1) / (8 * NT), units = (a.d_in + W4_K - 1) / W4_K;
-    const int parts = w4_parts((long long)tiles * row_tiles, units, WARPS, device_sms());
+    const int parts = w4_parts((long long)tiles * row_tiles, units, WARPS, sms);
     CUtensorMap codes;
     const unsigned long long dims[2] = {(unsigned long long)a.d_in / 2, (unsigned long long)a.d_out}, strides[1] = {(unsigned long long)a.code_stride};
     const unsigned box[2] = {W4_K / 2, C::CHANNELS};
@@ -361,8 +361,8 @@ int launch_w4(const W4Args& a, cudaStream_t stream)
     const int rows = std::min(a.rows, 8 * NT);
     // More tiles than blocks at a time: a block goes on to another tile, whose copies are under way before the sums of this one, if there is room for a stage of them beside the one in
     // use. us, blocks of one tile / of several: one row, 2048 x 65536 27.0 / 21.0, 4096 x 28672 25.1 / 19.9; with one stage 8 rows, 8192 x 32768 39.4 / 42.
-    const bool again = NT == 1 && tiles > 16 / WARPS * device_sms() && C::ahead(rows);
-    const int blocks = again ? 16 / WARPS * device_sms() : tiles;
+    const bool again = NT == 1 && tiles > 16 / WARPS * sms && C::ahead(rows);
+    const int blocks = again ? 16 / WARPS * sms : tiles;
     int stages = W4_STAGES;
     while (stages > 1 && C::smem(rows, stages, again) > C::SMEM) stages--;
     static std::atomic<bool> set[64];
@@ -377,15 +377,15 @@ int launch_w4(const W4Args& a, cudaStream_t stream)
 }
 
 template <int G>
-int launch_group(const W4Args& a, cudaStream_t stream)
+int launch_group(const W4Args& a, int sms, cudaStream_t stream)
 {
-    if (a.rows > 8) return launch_w4<G, 2, 8>(a, stream);
+    if (a.rows > 8) return launch_w4<G, 2, 8>(a, sms, stream);
     // One block to an SM has all sixteen warps; and of tiles that go round, those of much k: seven rounds of 148 are less than four of 296. us, two blocks of eight / one of sixteen: 8 rows,
     // 4096 x 4096 5.4 / 4.7, 14336 x 4096 13.8 / 11.7; one row, 8192 x 32768 37.6 / 33.4. Against it: 4096 x 6144 (192 tiles) 7.3 / 10.2, 4096 x 28672 (16 units: one to a
     // warp) 20.0 / 21.6, 8192 x 1024 (a cluster to a tile) 4.2 / 4.8.
-    const int tiles = (a.d_out + 16 * W4_MT - 1) / (16 * W4_MT), units = (a.d_in + W4_K - 1) / W4_K, sms = device_sms();
+    const int tiles = (a.d_out + 16 * W4_MT - 1) / (16 * W4_MT), units = (a.d_in + W4_K - 1) / W4_K;
     const bool sixteen = tiles <= sms ? units >= 16 && 2 * tiles > sms : units >= 32 && tiles > 2 * sms && W4Cfg<G, W4_MT, 1, 16>::ahead(a.rows);
-    return sixteen ? launch_w4<G, 1, 16>(a, stream) : launch_w4<G, 1, 8>(a, stream);
+    return sixteen ? launch_w4<G, 1, 16>(a, sms, stream) : launch_w4<G, 1, 8>(a, sms, stream);
 }
 
 }  // namespace
@@ -427,12 +427,16 @@ int project_w4(const void* X, long long x_stride, const efa_w4& w, void* out, in
     if (int rc = check_memory("project_w4", mem, 5)) return rc;
     // Up to eight rows the products of mma.sync are not the time. Beyond, tiles of 16 rows that read the weights again, or tcgen05 with up to 64 rows to a tile, whose start and
     // end cost more, and every group of a row its sums: by what either takes (w4_plan.h).
+    const int sms = device_sms();
     if (rows > 8) {
-        W4Division to;
-        if (int rc = w4_tc_plan(a, w.group, to)) return rc;
-        if (w4_tc_time(to, w.d_in, w.d_out, rows, w.group) < w4_mma_time(w.d_in, w.d_out, rows, w.group, device_sms())) return w4_tc_launch(a, w.group, to, stream);
+        const double mma = w4_mma_time(w.d_in, w.d_out, rows, w.group, sms);
+        if (w4_tc_least(w.d_in, w.d_out, rows, w.group) < mma) {
+            W4Division to;
+            if (int rc = w4_tc_plan(a, w.group, to)) return rc;
+            if (w4_tc_time(to, w.d_in, w.d_out, rows, w.group) < mma) return w4_tc_launch(a, w.group, to, stream);
+        }
     }
-    return w.group == 128 ? launch_group<128>(a, stream) : w.group == 64 ? launch_group<64>(a, stream) : launch_group<32>(a, stream);
+    return w.group == 128 ? launch_group<128>(a, sms, stream) : w.group == 64 ? launch_group<64>(a, sms, stream) : launch_group<32>(a, sms, stream);
 }
 
 }  // namespace efa

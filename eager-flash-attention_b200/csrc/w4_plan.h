@@ -63,5 +63,10 @@ inline double w4_tc_time(const W4Division& to, int d_in, int d_out, int rows, in
     const W4Tc& c = costs[group == 32 ? 0 : group == 64 ? 1 : 2][rows <= 16 ? 0 : rows <= 32 ? 1 : 2];
     return (double)to.rounds * (c.round + c.round_unit * to.units) + c.weights * ((rows + 15) / 16) * ((double)d_in * d_out / (1 << 24));
 }
+// However the device divides it: one round, k in as many parts as there can be.
+inline double w4_tc_least(int d_in, int d_out, int rows, int group)
+{
+    return w4_tc_time(W4Division{128, W4_MAX_PARTS, 1, ((d_in + 127) / 128 + W4_MAX_PARTS - 1) / W4_MAX_PARTS}, d_in, d_out, rows, group);
+}
 
 }  // namespace efa

@@ -17,6 +17,7 @@ extern "C" void divide(int d_out, int row_tiles, int units, const int* at_once, 
 extern "C" int tcgen05(int d_in, int d_out, int rows, int group, const int* at_once)
 {
     const efa::W4Division to = efa::w4_division(d_out, (rows + 63) / 64, (d_in + 127) / 128, at_once);
+    if (efa::w4_tc_least(d_in, d_out, rows, group) > efa::w4_tc_time(to, d_in, d_out, rows, group)) return -1;
     return efa::w4_tc_time(to, d_in, d_out, rows, group) < efa::w4_mma_time(d_in, d_out, rows, group, 148);
 }
 """
@@ -86,3 +87,12 @@ def test_the_largest_sizes_are_counted_without_overflow(library):
     for group in (32, 64, 128):
         assert library.tcgen05(1 << 24, 1 << 24, 1 << 19, group, at_once) == 1
         assert library.tcgen05(1 << 24, 1, 9, group, at_once) in (0, 1) and library.tcgen05(group, 1 << 24, 1 << 19, group, at_once) in (0, 1)
+
+
+def test_the_least_that_tcgen05_takes_is_no_more_than_it_takes(library):
+    for at_once in (B200, [0, 148] + [0] * 7, [0] * 9):
+        at_once = (ctypes.c_int * 9)(*at_once)
+        for group in (32, 64, 128):
+            for d_out, _, units in SIZES:
+                for rows in (9, 17, 33, 64, 65, 500):
+                    assert library.tcgen05(128 * units, d_out, rows, group, at_once) >= 0
