@@ -217,6 +217,36 @@ def test_compact_with_a_length_outside_the_table(pkg, torch_cuda, slot, wrong, h
     assert refs_out.tolist() == refs and moved.tolist() == list(range(10)) + [-1] * 4
 
 
+# ---- pages that are kept -----------------------------------------------------------------------------------------------------------------
+def test_pages_that_the_caller_keeps(pkg, torch_cuda):
+    """A prefix whose counts are raised outlives its slot, is not given to another, moves with a compaction, and is free when its counts are lowered."""
+    p, refs, pages, kv = pool(pkg)
+    for q in (5, 6):
+        refs[q] += 1
+    p.put(refs)
+    pkg.pages_free(p.pool, p.ints([2, 0]))
+    kv[2] = kv[0] = 0
+    refs = [0, 0, 1, 1, 1, 1, 1, 0, 0, 1, 0, 0, 0, 0]
+    p.expect(refs, pages, kv, 0, FREE)
+    pkg.pages_take(p.pool, p.ints([0, 0, 0, 0, 0, 0, 60]), p.ws)
+    kv[5], pages[5] = 60, [0, 1, 7, 8]
+    for q in pages[5]:
+        refs[q] = 1
+    p.expect(refs, pages, kv, 0, TAKE)
+    pkg.pages_free(p.pool, p.ints([1]))                                               # 2, 3 and 4
+    kv[1] = 0
+    moved = p.ints([0] * 14)
+    pkg.pages_compact(p.pool, p.cache, p.pages, p.refs, moved, p.ws)                  # 7 in use: 0 1 5 6 7 8 9, of which 7, 8, 9 go to 2, 3, 4
+    assert moved.tolist() == [0, 1, -1, -1, -1, 5, 6, 2, 3, 4, -1, -1, -1, -1]
+    refs, pages[5], pages[3][0] = [1] * 7 + [0] * 7, [0, 1, 2, 3], 4
+    p.expect(refs, pages, kv, 0, COMPACT)
+    p.moved([(7, 2, 16), (8, 3, 16), (9, 4, 16)])
+    p.refs[5:7] -= 1
+    pkg.pages_take(p.pool, p.ints([0, 33, 33, 33, 33, 33, 33]), p.ws)
+    kv[0], pages[0], refs[7] = 33, [5, 6, 7, -7], 1
+    p.expect(refs, pages, kv, 0, TAKE)
+
+
 # ---- anything ------------------------------------------------------------------------------------------------------------------------------
 # One block and a cluster of eight, by the pages and by the slots; lists above and below the length where children are compared in shared memory.
 @pytest.mark.parametrize("num_pages,num_seqs,max_pages", [(1, 1, 1), (40, 7, 3), (300, 31, 5), (17000, 33, 9), (2000, 700, 4), (20011, 1100, 3)])

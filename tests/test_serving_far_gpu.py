@@ -75,3 +75,17 @@ def test_pages_gigabytes_apart(pkg, torch_cuda):
     for x, y in zip(parts, want):
         assert torch.equal(x, torch.stack([y[3], y[3], y[0], y[3]]))
     assert refs.tolist() == [1, 0, 0, 0] and pages.tolist() == [[0, -7], [-7, -7]]
+
+
+@pytest.mark.parametrize("d_in,d_out,group,rows", [(1 << 24, 3, 128, 1), (1 << 24, 40, 32, 9), (1 << 23, 300, 64, 17), (32, 1 << 24, 32, 1), (64, (1 << 24) - 5, 64, 9), (128, 1 << 24, 128, 17)])
+def test_projections_of_the_longest_and_widest_matrices(pkg, torch_cuda, d_in, d_out, group, rows):
+    X, *w = make(rows, d_in, d_out, group, rows != 9, rows)
+    out = torch.full((rows, d_out), 777.0, dtype=torch.float32, device="cuda")
+    pkg.project_w4(X, pkg.w4_weight(*w), out, rows)
+    torch.cuda.synchronize()
+    step = max(1, (1 << 26) // d_in)
+    for lo in range(0, d_out, max(step, d_out // 8)):                               # slices of the channels, the first and the last among them
+        at = slice(lo, min(d_out, lo + step)) if lo + max(step, d_out // 8) < d_out else slice(max(0, d_out - step), d_out)
+        part = (w[0][at], w[1][:, at], None if w[2] is None else w[2][:, at])
+        check(out[:, at], *reference(X, *(p if p is None else p.contiguous() for p in part), torch.float32))
+    assert pkg.kernel_status()[0] == 0
